@@ -26,8 +26,9 @@ extern "C" {
 /* 2: lf_row_shrink gained num_adapters, workspace, workspace_bytes and flags,
  * lf_row_expand gained segments (arguments inserted mid-list).
  * 3: lf_lora gained num_slots (appended).
- * 4: lf_row_expand_tiled added. */
-#define LF_ABI_VERSION 4
+ * 4: lf_row_expand_tiled added.
+ * 5: the MXFP4 and expert entry points added. */
+#define LF_ABI_VERSION 5
 #define LF_OK 0
 #define LF_EINVAL 1
 #define LF_EHIP 2
@@ -307,6 +308,78 @@ int lf_nf4_lora_status(const void* workspace, void* stream, int32_t* status);
  * ------------------------------------------------------------------------ */
 int lf_swiglu(const uint16_t* gate_up, int64_t rows, int64_t n, int64_t in_stride, uint16_t* out,
               int64_t out_stride, void* stream);
+
+/* --------------------------------------------------------------------------
+ * MXFP4 (OCP microscaling): blocks of 32 e2m1 codes along k, two a byte (the
+ * low nibble is the even k), and one e8m0 scale byte s a block: a code stands
+ * for level * 2^(s - 127), level in 0, .5, 1, 1.5, 2, 3, 4, 6; s = 255 is NaN.
+ * lf_mxfp4_quantize: x [rows, k] bf16 (fp32 != 0: fp32), k % 32 == 0, rows
+ * 16-byte aligned; codes [rows, k / 2], scales [rows, k / 32]. With m the
+ * block's largest magnitude, s = max(floor(log2 m) - 2 + 127, 0) (0 for a block
+ * of zeros), codes rounded to nearest, ties to even, saturated at 6; a block
+ * that holds infinity or NaN gets s = 255 and zero codes.
+ * lf_mxfp4_dequantize: the bf16 values of `blocks` blocks (exact; s of 253 and
+ * 254, which the quantiser does not make, give infinity past bf16's range).
+ * ------------------------------------------------------------------------ */
+int lf_mxfp4_quantize(const void* x, int32_t fp32, int64_t rows, int64_t k, int64_t x_stride, uint8_t* codes,
+                      uint8_t* scales, void* stream);
+int lf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t blocks, uint16_t* out, void* stream);
+
+/* --------------------------------------------------------------------------
+ * Mixture of experts.
+ * lf_route_experts: logits [tokens, experts] bf16 (fp32 != 0: fp32) with row
+ * stride `stride`. Each token chooses the `top` experts of largest logit (of
+ * equal ones the lowest expert first; -inf: not allowed): chosen int32 [tokens,
+ * top] (-1 where fewer are allowed), weights fp32 [tokens, top] = softmax over
+ * the experts, divided by its sum over the chosen if renormalize (0 beside -1;
+ * NaN for a token whose logits hold NaN or +inf, NaN ranking below all). The
+ * choices sorted by expert, then by token and choice: offsets int32 [experts +
+ * 1], token_of int32 [tokens * top] (the token at each place, -1 from
+ * offsets[experts] on), positions int32 [tokens, top] (the place of each choice,
+ * -1 beside -1). experts 1..1024, top 1..64; the workspace need not be cleared.
+ *
+ * lf_expert_linear: y[p] = x[tokens[p]] w[e]^T (+ bias[e]) for every place p of
+ * offsets[e] .. offsets[e + 1] (tokens NULL: x[p]); fp32 sums, rounded once.
+ * x bf16 [x_rows, k] with row stride x_stride, or packed MXFP4 with x_scales
+ * (contiguous; then w is MXFP4 too); w [experts, n, k] bf16, or packed with
+ * w_scales. k % 32 == 0 with an MXFP4 weight, else k % 8 == 0; x rows and w
+ * 16-byte aligned. offsets NULL: one expert with all `rows` (the dense
+ * product). swiglu: w rows [0, n/2) gate, [n/2, n) up, y = silu(gate) * up in
+ * fp32, n/2 columns. Rows of y that belong to no expert are not written. Bounds
+ * and tokens outside the buffers are clamped to them.
+ *
+ * lf_combine_experts: y[t] = base[t] + sum_j weights[t, j] rows[positions[t, j]]
+ * (base NULL: 0; positions outside the rows are skipped), fp32 in order of j,
+ * rounded once; positions and weights contiguous [tokens, top].
+ * ------------------------------------------------------------------------ */
+int64_t lf_route_experts_workspace_size(int64_t tokens, int32_t experts);
+int lf_route_experts(const void* logits, int32_t fp32, int64_t tokens, int32_t experts, int64_t stride, int32_t top,
+                     int32_t renormalize, float* weights, int32_t* chosen, int32_t* offsets, int32_t* token_of,
+                     int32_t* positions, void* workspace, int64_t workspace_bytes, void* stream);
+
+typedef struct lf_expert_product {
+  const void* x;
+  const uint8_t* x_scales; /* NULL: x is bf16 */
+  int64_t x_stride;        /* elements (bf16 x) */
+  int64_t x_rows;
+  const void* w;
+  const uint8_t* w_scales; /* NULL: w is bf16 */
+  const uint16_t* bias;    /* [experts, n] or NULL */
+  const int32_t* offsets;  /* [experts + 1] or NULL */
+  const int32_t* tokens;   /* [rows] or NULL */
+  uint16_t* y;
+  int64_t y_stride;
+  int64_t rows;
+  int64_t n;
+  int64_t k;
+  int64_t experts;
+  int32_t swiglu;
+} lf_expert_product;
+int lf_expert_linear(const lf_expert_product* product, void* stream);
+
+int lf_combine_experts(const uint16_t* rows, int64_t num_rows, int64_t rows_stride, const int32_t* positions,
+                       const float* weights, int64_t tokens, int32_t top, int64_t n, const uint16_t* base,
+                       int64_t base_stride, uint16_t* y, int64_t y_stride, void* stream);
 
 #ifdef __cplusplus
 }

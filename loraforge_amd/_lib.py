@@ -26,7 +26,7 @@ LF_PLAN_PREFILL = 8
 LF_TEST_WITHHOLD_PARTIALS = 0x100
 LF_KERNEL_DECODE, LF_KERNEL_DECODE_WIDE, LF_KERNEL_DECODE_CHUNKS, LF_KERNEL_PREFILL = range(4)
 NOALLOC_SCRATCH_BYTES = 8 * 1024 * 1024
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 # Per device index, filled by the operators' Python paths: fit for the kernels
 # (gfx950), and compute units.
@@ -79,6 +79,27 @@ class Lora(ctypes.Structure):
 
 class Plan(ctypes.Structure):
     _fields_ = [("kernel", c_int32), ("tile_rows", c_int32), ("z_parts", c_int32), ("z_launch", c_int32)]
+
+
+class ExpertProduct(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("x_scales", c_void_p),
+        ("x_stride", c_int64),
+        ("x_rows", c_int64),
+        ("w", c_void_p),
+        ("w_scales", c_void_p),
+        ("bias", c_void_p),
+        ("offsets", c_void_p),
+        ("tokens", c_void_p),
+        ("y", c_void_p),
+        ("y_stride", c_int64),
+        ("rows", c_int64),
+        ("n", c_int64),
+        ("k", c_int64),
+        ("experts", c_int64),
+        ("swiglu", c_int32),
+    ]
 
 
 _PROTOTYPES = {
@@ -163,6 +184,19 @@ _PROTOTYPES = {
     ),
     "lf_nf4_lora_status": (ctypes.c_int, [c_void_p, c_void_p, ctypes.POINTER(c_int32)]),
     "lf_swiglu": (ctypes.c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "lf_mxfp4_quantize": (ctypes.c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "lf_mxfp4_dequantize": (ctypes.c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "lf_route_experts_workspace_size": (c_int64, [c_int64, c_int32]),
+    "lf_route_experts": (
+        ctypes.c_int,
+        [c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_int32] + [c_void_p] * 6 + [c_int64, c_void_p],
+    ),
+    "lf_expert_linear": (ctypes.c_int, [ctypes.POINTER(ExpertProduct), c_void_p]),
+    "lf_combine_experts": (
+        ctypes.c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+         c_void_p],
+    ),
 }
 
 EXPORTS = tuple(_PROTOTYPES)

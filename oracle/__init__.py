@@ -12,6 +12,8 @@ This package restates, in numpy, the arithmetic of the reference
   chain, decode and segmented prefill, and the SwiGLU MLP chain
   (``src/loraforge/integrations/_sglang_nf4_linear.py``,
   ``benchmarks/qwen35_prefill_fused.py``, ``benchmarks/qwen35_decode_silu.py``).
+* ``oracle.experts`` -- the MXFP4 format and mixture-of-experts operators, which
+  the reference does not have.
 * ``oracle.cpu_path`` -- the PyTorch-CPU restatement of the reference serving
   path that ``bench.py`` times as the CPU baseline.
 

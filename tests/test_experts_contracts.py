@@ -1,0 +1,109 @@
+"""What the MXFP4 and expert operators refuse, without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from loraforge_amd import _lib
+from loraforge_amd.ops import (
+    MXFP4Tensor,
+    combine_experts,
+    dequantize_mxfp4,
+    expert_linear,
+    mxfp4_linear,
+    quantize_mxfp4,
+    route_experts,
+)
+
+BF16 = torch.bfloat16
+
+
+def mx(*shape):
+    return MXFP4Tensor(torch.zeros(*shape[:-1], shape[-1] // 2, dtype=torch.uint8),
+                       torch.zeros(*shape[:-1], shape[-1] // 32, dtype=torch.uint8))
+
+
+def test_python_checks():
+    x = torch.zeros(4, 64, dtype=BF16)
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        quantize_mxfp4([1.0])
+    with pytest.raises(ValueError, match="dtype"):
+        quantize_mxfp4(x.half())
+    with pytest.raises(ValueError, match="same CUDA"):
+        quantize_mxfp4(x)
+    with pytest.raises(TypeError, match="MXFP4Tensor"):
+        dequantize_mxfp4(x)
+    with pytest.raises(ValueError, match="same CUDA"):
+        dequantize_mxfp4(mx(4, 64))
+    with pytest.raises(TypeError, match="MXFP4Tensor"):
+        mxfp4_linear(x, x)
+    with pytest.raises(ValueError, match="same CUDA"):
+        mxfp4_linear(x, mx(8, 64))
+    with pytest.raises(ValueError, match="3D"):
+        expert_linear(x, x, None)
+    with pytest.raises(TypeError, match="weight"):
+        expert_linear(x, None, None)
+    with pytest.raises(ValueError, match="same CUDA"):
+        route_experts(torch.zeros(2, 4), 2)
+    with pytest.raises(ValueError, match="dtype"):
+        route_experts(torch.zeros(2, 4, dtype=torch.int32), 2)
+    with pytest.raises(ValueError, match="same CUDA"):
+        combine_experts(x, torch.zeros(4, 1, dtype=torch.int32), torch.zeros(4, 1))
+    assert mx(3, 5, 64).shape == (3, 5, 64)
+
+
+def refused(match, status):
+    with pytest.raises(ValueError, match=match):
+        _lib.check(status)
+
+
+def test_c_entry_points_refuse_without_device_work():
+    lib = _lib.library()
+    p = ctypes.c_void_p(16)
+    refused("multiple of 32", lib.lf_mxfp4_quantize(p, 0, 1, 48, 48, p, p, None))
+    refused("x_stride", lib.lf_mxfp4_quantize(p, 0, 2, 64, 32, p, p, None))
+    refused("16-byte", lib.lf_mxfp4_quantize(ctypes.c_void_p(8), 0, 1, 64, 64, p, p, None))
+    refused("16-byte", lib.lf_mxfp4_quantize(p, 0, 2, 64, 68, p, p, None))
+    refused("null", lib.lf_mxfp4_dequantize(p, None, 4, p, None))
+    refused("16-byte", lib.lf_mxfp4_dequantize(p, p, 4, ctypes.c_void_p(2), None))
+    assert lib.lf_mxfp4_quantize(None, 0, 0, 64, 64, None, None, None) == _lib.LF_OK
+    route = lambda experts=8, top=2, stride=8, tokens=3, ws=None, size=0: lib.lf_route_experts(  # noqa: E731
+        p, 0, tokens, experts, stride, top, 1, p, p, p, p, p, ws, size, None)
+    refused("1..1024", route(experts=1025))
+    refused("top_k", route(top=9))
+    refused("top_k", route(experts=100, top=65, stride=100))
+    refused("stride", route(stride=7))
+    refused("int32", route(tokens=2**30))
+    refused("workspace", route(tokens=65))
+    assert lib.lf_route_experts_workspace_size(64, 8) == 0
+    assert lib.lf_route_experts_workspace_size(65, 8) >= 5 * 8 * 4
+    assert lib.lf_route_experts_workspace_size(10, 2000) == -1
+    refused("cover n", lib.lf_combine_experts(p, 4, 7, p, p, 2, 1, 8, None, 0, p, 8, None))
+    refused("null", lib.lf_combine_experts(p, 4, 8, None, p, 2, 1, 8, None, 0, p, 8, None))
+
+
+@pytest.mark.parametrize(
+    "change,match",
+    [
+        (dict(k=40), "multiple of 32"),
+        (dict(w_scales=None, k=36), "or 8"),
+        (dict(w_scales=None, x_scales=16), "needs an MXFP4 weight"),
+        (dict(n=33, swiglu=1), "equal number"),
+        (dict(experts=2), "offsets required"),
+        (dict(tokens=16), "offsets required"),
+        (dict(x=8), "16-byte"),
+        (dict(w=4), "16-byte"),
+        (dict(x_stride=68), "16-byte"),
+        (dict(y_stride=31), "y_stride"),
+        (dict(x_rows=1), "each row"),
+        (dict(y=None), "null"),
+        (dict(rows=2**31), "int32"),
+        (dict(n=0), "positive"),
+    ],
+)
+def test_c_product_refusals(change, match):
+    a = _lib.ExpertProduct(x=16, w=16, w_scales=16, y=16, x_stride=64, x_rows=2, rows=2, n=32, k=64, experts=1, y_stride=32)
+    for name, value in change.items():
+        setattr(a, name, value)
+    refused(match, _lib.library().lf_expert_linear(ctypes.byref(a), None))
