@@ -357,6 +357,17 @@ int lf_route_experts(const void* logits, int32_t fp32, int64_t tokens, int32_t e
                      int32_t renormalize, float* weights, int32_t* chosen, int32_t* offsets, int32_t* token_of,
                      int32_t* positions, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Kernel of a product: the weight stream (few rows per expert; `columns` weight rows
+ * a workgroup: 16, 32 or 64), or MFMA tiles of at most `rows` (64, 128, 192, 256) x
+ * `columns` weight rows (64, 128, 256; with SwiGLU 128 or 256). */
+#define LF_EXPERT_STREAM 0
+#define LF_EXPERT_TILE 1
+typedef struct lf_expert_plan {
+  int32_t kernel;
+  int32_t rows;
+  int32_t columns;
+} lf_expert_plan;
+
 typedef struct lf_expert_product {
   const void* x;
   const uint8_t* x_scales; /* NULL: x is bf16 */
@@ -374,8 +385,12 @@ typedef struct lf_expert_product {
   int64_t k;
   int64_t experts;
   int32_t swiglu;
+  const lf_expert_plan* plan; /* NULL: the library chooses */
 } lf_expert_product;
 int lf_expert_linear(const lf_expert_product* product, void* stream);
+/* The plan that the library chooses for a product of these sizes, types (whether
+ * x_scales, w_scales and offsets are given) and swiglu: host arithmetic. */
+int lf_expert_linear_plan(const lf_expert_product* product, lf_expert_plan* plan);
 
 int lf_combine_experts(const uint16_t* rows, int64_t num_rows, int64_t rows_stride, const int32_t* positions,
                        const float* weights, int64_t tokens, int32_t top, int64_t n, const uint16_t* base,

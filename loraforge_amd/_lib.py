@@ -81,6 +81,13 @@ class Plan(ctypes.Structure):
     _fields_ = [("kernel", c_int32), ("tile_rows", c_int32), ("z_parts", c_int32), ("z_launch", c_int32)]
 
 
+LF_EXPERT_STREAM, LF_EXPERT_TILE = range(2)
+
+
+class ExpertPlan(ctypes.Structure):
+    _fields_ = [("kernel", c_int32), ("rows", c_int32), ("columns", c_int32)]
+
+
 class ExpertProduct(ctypes.Structure):
     _fields_ = [
         ("x", c_void_p),
@@ -99,6 +106,7 @@ class ExpertProduct(ctypes.Structure):
         ("k", c_int64),
         ("experts", c_int64),
         ("swiglu", c_int32),
+        ("plan", ctypes.POINTER(ExpertPlan)),
     ]
 
 
@@ -191,6 +199,7 @@ _PROTOTYPES = {
         ctypes.c_int,
         [c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_int32] + [c_void_p] * 6 + [c_int64, c_void_p],
     ),
+    "lf_expert_linear_plan": (ctypes.c_int, [ctypes.POINTER(ExpertProduct), ctypes.POINTER(ExpertPlan)]),
     "lf_expert_linear": (ctypes.c_int, [ctypes.POINTER(ExpertProduct), c_void_p]),
     "lf_combine_experts": (
         ctypes.c_int,

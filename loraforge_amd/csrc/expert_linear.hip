@@ -1,6 +1,39 @@
 // C entry point of the products with bf16 or MXFP4 weights: checks and choice of kernel.
+#include <algorithm>
+
 #include "expert_params.h"
 #include "../../include/loraforge_amd.h"
+
+namespace lf {
+namespace expert {
+namespace {
+
+// What the tile kernel can take: scale rows within 32-bit offsets, four blocks of MXFP4 x.
+bool tiles_fit(const lf_expert_product& a) {
+  const int64_t blocks = a.k / mx::kBlock, most = int64_t(1) << 31;
+  return (!a.w_scales || a.n * blocks < most) && (!a.x_scales || (a.x_rows * blocks < most && a.k >= 128));
+}
+
+lf_expert_plan plan_of(const lf_expert_product& a) {
+  const int64_t used = a.offsets ? std::min(a.experts, a.rows) : 1;
+  const int64_t width = a.swiglu ? a.n / 2 : a.n;
+  const int64_t each = (a.rows + used - 1) / used;  // rows of an expert, on average
+  lf_expert_plan plan{};
+  if (each > 32 && tiles_fit(a)) {
+    plan.kernel = LF_EXPERT_TILE;
+    plan.rows = int32_t(std::min<int64_t>(256, (each + 63) / 64 * 64));
+    plan.columns = 256;
+    return plan;
+  }
+  plan.kernel = LF_EXPERT_STREAM;
+  const int64_t groups = (width + (a.swiglu ? 7 : 15)) / (a.swiglu ? 8 : 16) * used;
+  plan.columns = groups >= 4 * 512 ? 64 : groups >= 2 * 512 ? 32 : 16;
+  return plan;
+}
+
+}  // namespace
+}  // namespace expert
+}  // namespace lf
 
 extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   LF_REQUIRE(a != nullptr, "null pointer argument");
@@ -38,5 +71,25 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   p.experts = int(a->experts);
   p.width = int(width);
   p.swiglu = a->swiglu ? 1 : 0;
-  return lf::expert::launch_stream(p, static_cast<hipStream_t>(stream));
+  p.y_vec = lf::aligned16(a->y) && a->y_stride % 8 == 0;
+  const lf_expert_plan plan = a->plan ? *a->plan : lf::expert::plan_of(*a);
+  auto s = static_cast<hipStream_t>(stream);
+  if (plan.kernel == LF_EXPERT_STREAM) {
+    LF_REQUIRE(plan.columns == 16 || plan.columns == 32 || plan.columns == 64, "stream plan: 16, 32 or 64 columns");
+    return lf::expert::launch_stream(p, plan.columns / 16, s);
+  }
+  LF_REQUIRE(plan.kernel == LF_EXPERT_TILE && lf::expert::tiles_fit(*a), "this product cannot run in tiles");
+  LF_REQUIRE(plan.rows >= 64 && plan.rows <= 256 && plan.rows % 64 == 0, "tile plan: 64, 128, 192 or 256 rows");
+  LF_REQUIRE(plan.columns == 128 || plan.columns == 256 || (plan.columns == 64 && !a->swiglu),
+             "tile plan: 64 (not with SwiGLU), 128 or 256 columns");
+  if (x_mx) return lf::expert::launch_tiles_mx(p, plan.rows, plan.columns, s);
+  return w_mx ? lf::expert::launch_tiles_mxw(p, plan.rows, plan.columns, s)
+              : lf::expert::launch_tiles_bf16(p, plan.rows, plan.columns, s);
+}
+
+extern "C" int lf_expert_linear_plan(const lf_expert_product* a, lf_expert_plan* plan) {
+  LF_REQUIRE(a != nullptr && plan != nullptr, "null pointer argument");
+  LF_REQUIRE(a->rows >= 1 && a->n >= 1 && a->k >= 8 && a->experts >= 1, "sizes must be positive");
+  *plan = lf::expert::plan_of(*a);
+  return lf::kOk;
 }

@@ -25,6 +25,7 @@ struct Params {
   int64_t y_stride;
   int rows, x_rows, n, k, experts;
   int width;   // output columns: n, or n / 2 with SwiGLU
+  int y_vec;   // rows of y are 16-byte aligned
   int swiglu;  // w rows [gate | up]: y = silu(gate) * up
 };
 
@@ -79,7 +80,12 @@ __device__ __forceinline__ int64_t x_row_of(const Params& p, int pos) {
 // SwiGLU in fp32: g / (1 + e^-g) * u, nothing rounded.
 __device__ __forceinline__ float silu_mul_f32(float g, float u) { return silu_f32(g) * u; }
 
-int launch_stream(const Params& p, hipStream_t stream);
+// `groups`: 16-row groups of weight rows per workgroup (1, 2 or 4).
+int launch_stream(const Params& p, int groups, hipStream_t stream);
+// Tiles of at most `cap` rows x `columns` weight rows (one translation unit per pair of types).
+int launch_tiles_bf16(const Params& p, int cap, int columns, hipStream_t stream);
+int launch_tiles_mxw(const Params& p, int cap, int columns, hipStream_t stream);
+int launch_tiles_mx(const Params& p, int cap, int columns, hipStream_t stream);
 
 }  // namespace expert
 }  // namespace lf

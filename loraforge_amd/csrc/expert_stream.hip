@@ -188,16 +188,13 @@ __global__ __launch_bounds__(kThreads, 4) void stream_kernel(Params p) {
 }
 
 template <bool kXMx, bool kWMx>
-int launch_types(const Params& p, hipStream_t stream) {
+int launch_types(const Params& p, int groups, hipStream_t stream) {
   const int segments = p.offsets ? (p.experts < p.rows ? p.experts : p.rows) : 1;
-  const int out = p.swiglu ? 8 : 16;
-  // Fewer columns per workgroup where the grid would not fill the device twice.
-  const int64_t blocks = (p.width + out - 1) / out;
-  const int f = blocks * segments >= 4 * 512 ? 4 : blocks * segments >= 2 * 512 ? 2 : 1;
-  const dim3 grid(unsigned((blocks + f - 1) / f), unsigned(segments)), threads(kThreads);
-  if (f == 4)
+  const int64_t columns = (p.swiglu ? 8 : 16) * groups;
+  const dim3 grid(unsigned((p.width + columns - 1) / columns), unsigned(segments)), threads(kThreads);
+  if (groups == 4)
     hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 4>), grid, threads, 0, stream, p);
-  else if (f == 2)
+  else if (groups == 2)
     hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 2>), grid, threads, 0, stream, p);
   else
     hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 1>), grid, threads, 0, stream, p);
@@ -207,9 +204,9 @@ int launch_types(const Params& p, hipStream_t stream) {
 
 }  // namespace
 
-int launch_stream(const Params& p, hipStream_t stream) {
-  if (p.xs) return launch_types<true, true>(p, stream);
-  return p.ws ? launch_types<false, true>(p, stream) : launch_types<false, false>(p, stream);
+int launch_stream(const Params& p, int groups, hipStream_t stream) {
+  if (p.xs) return launch_types<true, true>(p, groups, stream);
+  return p.ws ? launch_types<false, true>(p, groups, stream) : launch_types<false, false>(p, groups, stream);
 }
 
 }  // namespace expert

@@ -1,0 +1,466 @@
+// Products of many rows (prefill): MFMA tiles of up to 256 rows x 64 kJ weight rows.
+//
+// Four waves, one per SIMD, in a 2 x 2 arrangement: a wave owns 32 kI rows x
+// 32 kJ weight rows (v_mfma_f32_32x32x16_bf16, or v_mfma_scale_f32_32x32x64_f8f6f4
+// where both operands are MXFP4; the weight is the A operand). Both operands
+// go through LDS by direct copies, in stages of 128 bytes of every x row (64 k in
+// bf16, 256 k in MXFP4); a ring of kSlots stages, the copies of a stage
+// issued as soon as its slot is free. A stage is four sub-steps; the operands
+// of a sub-step are read while the one before it is multiplied. MXFP4 weights
+// beside bf16 x are decoded in registers (four conversions per eight weights,
+// exact), so they cost a quarter of the copies and no pass of their own.
+//
+// The order of k within a stage is free as long as both operands agree: lane
+// half h of sub-step s takes unit 4 h + s (16 bytes), so that an MXFP4 lane's
+// blocks of a stage are consecutive and its scales one dword (byte s for
+// sub-step s), and beside bf16 x a lane's 32 weights of a stage are one block.
+//
+// An expert's rows are cut into tiles of equal height (a multiple of 64, up to
+// 256), so an expert with few rows costs as much as they need: the body is chosen
+// by the tile's rows.
+#pragma once
+
+#include "expert_params.h"
+#include "lds_pipeline.h"
+
+namespace lf {
+namespace expert {
+namespace tile {
+
+constexpr int kThreads = 256;
+constexpr int kLds = 160 * 1024;
+constexpr int kSubSteps = 4;
+constexpr int kXRow = 128;  // bytes of an x row per stage
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <bool kXMx, bool kWMx, int kI, int kJ>
+struct Shape {
+  static constexpr bool kDecode = kWMx && !kXMx;           // MXFP4 weights for bf16 x
+  static constexpr int kStageK = kXMx ? 256 : 64;
+  static constexpr int kWRow = kDecode ? 32 : 128;         // bytes of a weight row per stage
+  // (A copy per wave at least: 64 rows of 32 bytes go twice.)
+  static constexpr int kXBytes = 64 * kI * kXRow, kWBytes = 64 * kJ * kWRow < 4096 ? 4096 : 64 * kJ * kWRow;
+  static constexpr int kStage = kXBytes + kWBytes;
+  static constexpr int kSlots = kLds / kStage >= 4 ? 4 : kLds / kStage;
+  static_assert(kSlots >= 2, "two stages have to fit");
+  static constexpr int kXCopies = kXBytes / 4096, kWCopies = kWBytes / 4096;  // per wave
+  static constexpr int kScaleLoads = kXMx ? kI + kJ : kDecode ? kJ : 0;
+  static constexpr int kLoads = kXCopies + kWCopies;
+};
+
+struct Scales {
+  uint32_t x[4], w[4];
+};
+
+// The operands of one sub-step.
+template <int kI, int kJ>
+struct Frags {
+  u32x4 x[kI], w[kJ];
+};
+
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
+
+template <bool kXMx, bool kWMx, int kI, int kJ>
+struct Body {
+  using S = Shape<kXMx, kWMx, kI, kJ>;
+  const Params& p;
+  int lane, wave, h;        // h: lane half
+  int stages;
+  // Copies: the lane's 16-byte unit of each row it copies, and where it starts.
+  const char* xsrc[S::kXCopies];
+  const char* wsrc[S::kWCopies];
+  int xleft, wleft;         // bytes of the row from the lane's unit on
+  // Operand reads: byte offsets in a slot of sub-step s = 0, row of fragment 0.
+  int xread, wread, xmask, wmask;
+  // Scale rows: byte offsets from p.xs and from the expert's first row (below 2 GiB).
+  const uint8_t* wbase;
+  uint32_t xscale[kXMx ? kI : 1], wscale[kWMx ? kJ : 1];
+  f32x16 acc[kI][kJ];
+
+  __device__ __forceinline__ Body(const Params& p_) : p(p_) {}
+
+  __device__ __forceinline__ int weight_row(int nt, int r) const {
+    if (!p.swiglu) return min(nt * 64 * kJ + r, p.n - 1);
+    // A wave's fragments are gate and up rows of the same columns in turn.
+    const int column = nt * 32 * kJ + (r / (32 * kJ)) * 16 * kJ + (r / 64 % (kJ > 1 ? kJ / 2 : 1)) * 32 + r % 32;
+    return min(column, p.width - 1) + (r / 32 % 2 ? p.width : 0);
+  }
+
+  // Copies of index first .. last - 1 of the next stage into a slot. Past the end
+  // of k (in the last stage and the stages after it) they copy zeros.
+  __device__ __forceinline__ void copy(char* slot, int first, int last) {
+    const char* zeros = reinterpret_cast<const char*>(&kZeros);
+#pragma unroll
+    for (int d = 0; d < S::kXCopies; ++d)
+      if (d >= first && d < last) {
+        copy16(xleft > 0 ? xsrc[d] : zeros, slot + (d * 4 + wave) * 1024);
+        xsrc[d] += kXRow;
+      }
+#pragma unroll
+    for (int d = 0; d < S::kWCopies; ++d)
+      if (d + S::kXCopies >= first && d + S::kXCopies < last) {
+        copy16(wleft > 0 ? wsrc[d] : zeros, slot + S::kXBytes + (d * 4 + wave) * 1024);
+        wsrc[d] += S::kWRow;
+      }
+    if (last == S::kLoads) {
+      xleft -= kXRow;
+      wleft -= S::kWRow;
+    }
+  }
+
+  // Scales of stage st: with MXFP4 x the lane's four blocks of every fragment row
+  // (one load of any alignment, not past the row; k >= 128), beside bf16 x its one
+  // block. Loads are never skipped: the waits count them. What they load is put
+  // in place when it is used (used_scales), with zeros past the end of k.
+  __device__ __forceinline__ int scale_block(int st) const { return (kXMx ? 8 : 2) * st + (kXMx ? 4 : 1) * h; }
+  __device__ __forceinline__ void load_scales(int st, Scales& s) const {
+    typedef uint32_t u32u __attribute__((aligned(1)));
+    if constexpr (kXMx) {
+      const uint32_t from = uint32_t(min(scale_block(st), p.k / mx::kBlock - 4));
+#pragma unroll
+      for (int i = 0; i < kI; ++i) s.x[i] = *reinterpret_cast<const u32u*>(p.xs + (xscale[i] + from));
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const u32u*>(wbase + (wscale[j] + from));
+    } else if constexpr (kWMx) {
+      const uint32_t from = uint32_t(min(scale_block(st), p.k / mx::kBlock - 1));
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) s.w[j] = wbase[wscale[j] + from];
+    }
+  }
+  __device__ __forceinline__ void used_scales(int st, const Scales& s, Scales& u) const {
+    if constexpr (kXMx) {
+      const int shift = 8 * min(max(scale_block(st) + 4 - p.k / mx::kBlock, 0), 4);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) u.x[i] = uint32_t(uint64_t(s.x[i]) >> shift);
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) u.w[j] = uint32_t(uint64_t(s.w[j]) >> shift);
+    } else if constexpr (kWMx) {
+      const uint32_t mask = scale_block(st) < p.k / mx::kBlock ? 0xffu : 0u;
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) u.w[j] = s.w[j] & mask;
+    }
+  }
+
+  // Operands of sub-step s. (MXFP4 weights beside bf16 x are read once per stage.)
+  __device__ __forceinline__ void read(const char* slot, int s, Frags<kI, kJ>& f) const {
+    const int unit = (4 * h + s) * 16;
+#pragma unroll
+    for (int i = 0; i < kI; ++i) f.x[i] = *reinterpret_cast<const u32x4*>(slot + xread + i * 64 * kXRow + (unit ^ xmask));
+    if constexpr (!S::kDecode) {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+        f.w[j] = *reinterpret_cast<const u32x4*>(slot + S::kXBytes + wread + j * 32 * kXRow + (unit ^ wmask));
+    }
+  }
+  __device__ __forceinline__ void read_codes(const char* slot, u32x4 (&codes)[kJ]) const {
+    if constexpr (S::kDecode) {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+        codes[j] = *reinterpret_cast<const u32x4*>(slot + S::kXBytes + wread + j * 32 * S::kWRow + h * 16);
+    }
+  }
+
+  template <int kS>
+  __device__ __forceinline__ void multiply(const Frags<kI, kJ>& f, const Scales& sc, int i, int j) {
+    if constexpr (kXMx) {
+      const i32x8 a{int(f.w[j].x), int(f.w[j].y), int(f.w[j].z), int(f.w[j].w), 0, 0, 0, 0};
+      const i32x8 b{int(f.x[i].x), int(f.x[i].y), int(f.x[i].z), int(f.x[i].w), 0, 0, 0, 0};
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc[i][j], 4, 4, kS, int(sc.w[j]), kS, int(sc.x[i]));
+    } else {
+      acc[i][j] = mfma32(vec_bf16x8(f.w[j]), vec_bf16x8(f.x[i]), acc[i][j]);
+    }
+  }
+
+  // One sub-step: reads (and decodes) the next one's operands, multiplies its own,
+  // with `extra(n)` behind the n-th of its kI kJ instructions.
+  template <int kS, class Extra>
+  __device__ __forceinline__ void sub_step(const Frags<kI, kJ>& f, const Scales& sc, Extra&& extra) {
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        multiply<kS>(f, sc, i, j);
+        extra(j * kI + i);
+        pin();
+      }
+  }
+
+  // The stage in `cur`, whose first operands are in `f` and scales in `sc`; `next`
+  // holds the one after it (its scales loaded in `ahead`), and on return `f`, `sc`
+  // and `codes` are that stage's. `ahead` then loads a later stage's.
+  __device__ __forceinline__ void stage(char* cur, const char* next, int st, Frags<kI, kJ>& f, u32x4 (&codes)[kJ],
+                                        Scales& sc, Scales& ahead) {
+    constexpr int kM = kI * kJ;
+    Frags<kI, kJ> g;
+    auto decode = [&](Frags<kI, kJ>& to, const u32x4 (&from)[kJ], const Scales& s, int sub, int n) {
+      // Fragment j's conversions behind instruction j kI (all of them early enough for the next sub-step).
+      if constexpr (S::kDecode)
+        if (n % kI == 0) to.w[n / kI] = mx::decode8(from[n / kI][sub], mx::scale_f32(s.w[n / kI]));
+    };
+    read(cur, 1, g);
+    pin();
+    sub_step<0>(f, sc, [&](int n) { decode(g, codes, sc, 1, n); });
+    read(cur, 2, f);
+    pin();
+    sub_step<1>(g, sc, [&](int n) { decode(f, codes, sc, 2, n); });
+    read(cur, 3, g);
+    pin();
+    sub_step<2>(f, sc, [&](int n) { decode(g, codes, sc, 3, n); });
+    // Every wave has read all of `cur`, and `next` and `ahead` have arrived.
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    wait_vm<(S::kSlots - 2) * (S::kLoads + S::kScaleLoads)>();
+    barrier_only();
+    Scales su;
+    used_scales(st + 1, ahead, su);
+    read(next, 0, f);
+    u32x4 codes_next[kJ];
+    read_codes(next, codes_next);
+    load_scales(st + S::kSlots + 1, ahead);
+    pin();
+    sub_step<3>(g, sc, [&](int n) {
+      copy(cur, n * S::kLoads / kM, (n + 1) * S::kLoads / kM);
+      decode(f, codes_next, su, 0, n);
+    });
+    sc = su;
+    if constexpr (S::kDecode) {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) codes[j] = codes_next[j];
+    }
+  }
+
+  // All stages. The slots are separate arguments so that the compiler knows
+  // that reads of one do not depend on the copies into another (it would wait
+  // for every copy in flight before each read).
+  __device__ __forceinline__ void ring(char* __restrict__ s0, char* __restrict__ s1, char* __restrict__ s2,
+                                       char* __restrict__ s3) {
+    constexpr int kN = S::kSlots;
+    // Loads in order: scales 0, then for each stage n of the ring scales n + 1 and copies n.
+    Scales first, ahead[kN], sc;
+    load_scales(0, first);
+    auto start = [&](char* slot, int n) {
+      load_scales(n + 1, ahead[n]);
+      pin();
+      copy(slot, 0, S::kLoads);
+      pin();
+    };
+    start(s0, 0);
+    start(s1, 1);
+    if constexpr (kN > 2) start(s2, 2);
+    if constexpr (kN > 3) start(s3, 3);
+    wait_vm<(kN - 1) * (S::kLoads + S::kScaleLoads)>();
+    barrier_only();
+    used_scales(0, first, sc);
+    Frags<kI, kJ> f;
+    u32x4 codes[kJ];
+    read(s0, 0, f);
+    read_codes(s0, codes);
+    if constexpr (S::kDecode) {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) f.w[j] = mx::decode8(codes[j].x, mx::scale_f32(sc.w[j]));
+    }
+    // (The tall tiles run whole rounds of the ring, stages past the end on zeros: with
+    // more than one way out of the loop the compiler moves their sums through scratch.)
+    constexpr bool kWhole = kI >= 2 && kI * kJ >= 8;
+    for (int st = 0; st < stages; st += kN) {
+      stage(s0, s1, st, f, codes, sc, ahead[0]);
+      if (!kWhole && st + 1 >= stages) break;
+      stage(s1, kN == 2 ? s0 : s2, st + 1, f, codes, sc, ahead[1]);
+      if constexpr (kN > 2) {
+        if (!kWhole && st + 2 >= stages) break;
+        stage(s2, kN == 3 ? s0 : s3, st + 2, f, codes, sc, ahead[2]);
+      }
+      if constexpr (kN > 3) {
+        if (!kWhole && st + 3 >= stages) break;
+        stage(s3, s0, st + 3, f, codes, sc, ahead[3]);
+      }
+    }
+  }
+
+  // The tile of `count` rows from `first` on, weight rows of column tile nt.
+  __device__ __forceinline__ void run(char* lds, const Segment& seg, int first, int count, int nt) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    h = lane >> 5;
+    const int wm = wave & 1, wn = wave >> 1, c = lane & 31;
+    const int blocks = p.k / mx::kBlock;
+    const int row_bytes_x = kXMx ? p.k / 2 : p.k * 2, row_bytes_w = kWMx ? p.k / 2 : p.k * 2;
+    stages = (p.k + S::kStageK - 1) / S::kStageK;
+    const int last = first + count - 1;
+
+    // A copy covers eight rows of 128 bytes (of 32 bytes: 32 rows); row r's unit u
+    // sits at u ^ (r & 7), so that reads of one unit of consecutive rows meet no bank twice.
+    const int r8 = lane >> 3;
+    const int xunit = ((lane & 7) ^ r8) * 16;
+#pragma unroll
+    for (int d = 0; d < S::kXCopies; ++d)
+      xsrc[d] = p.x + x_row_of(p, min(first + 8 * (d * 4 + wave) + r8, last)) * p.x_row + xunit;
+    const int64_t w0 = int64_t(seg.expert) * p.n;
+    const int wr = S::kWRow == 128 ? r8 : lane >> 1;
+    const int wunit = S::kWRow == 128 ? xunit : (lane & 1) * 16;
+#pragma unroll
+    for (int d = 0; d < S::kWCopies; ++d)
+      wsrc[d] = p.w + (w0 + weight_row(nt, ((d * 4 + wave) * (1024 / S::kWRow) + wr) % (64 * kJ))) * row_bytes_w + wunit;
+
+    xleft = row_bytes_x - xunit;
+    wleft = row_bytes_w - wunit;
+
+    xread = (32 * wm + c) * kXRow;  // fragment i: rows 64 i + 32 wm ..
+    xmask = (c & 7) * 16;
+    wread = (32 * kJ * wn + c) * S::kWRow;
+    wmask = xmask;
+    if constexpr (kXMx) {
+#pragma unroll
+      for (int i = 0; i < kI; ++i) xscale[i] = uint32_t(x_row_of(p, min(first + 64 * i + 32 * wm + c, last))) * blocks;
+    }
+    if constexpr (kWMx) {
+      wbase = p.ws + w0 * blocks;
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) wscale[j] = uint32_t(weight_row(nt, 32 * kJ * wn + 32 * j + c)) * blocks;
+    }
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    ring(lds, lds + S::kStage, lds + (S::kSlots > 2 ? 2 : 0) * S::kStage, lds + (S::kSlots > 3 ? 3 : 0) * S::kStage);
+
+    // acc[i][j][4 g + e]: row 64 i + 32 wm + c of the tile, weight row 8 g + 4 h + e of fragment j.
+    const uint16_t* bias = p.bias ? p.bias + w0 : nullptr;
+    const int base = nt * 64 * kJ + 32 * kJ * wn;
+    if (p.swiglu) {
+      if constexpr (kJ >= 2) {
+#pragma unroll
+        for (int j = 0; j < kJ; j += 2) {
+          const int col = base / 2 + 16 * j;
+          if (bias) {
+            add_bias(bias, col, j);
+            add_bias(bias + p.width, col, j + 1);
+          }
+#pragma unroll
+          for (int i = 0; i < kI; ++i) {
+            uint32_t o[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              o[r] = pack_bf16x2(silu_mul_f32(acc[i][j][2 * r], acc[i][j + 1][2 * r]),
+                                 silu_mul_f32(acc[i][j][2 * r + 1], acc[i][j + 1][2 * r + 1]));
+            store(o, lds, first + 64 * i + 32 * wm + c, last, col);
+            pin();
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+        const int col = base + 32 * j;
+        if (bias) add_bias(bias, col, j);
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {
+          uint32_t o[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) o[r] = pack_bf16x2(acc[i][j][2 * r], acc[i][j][2 * r + 1]);
+          store(o, lds, first + 64 * i + 32 * wm + c, last, col);
+          pin();
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void add_bias(const uint16_t* bias, int col, int j) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float b = bf16_to_f32(bias[min(col + 8 * (r >> 2) + 4 * h + (r & 3), p.width - 1)]);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) acc[i][j][r] += b;
+    }
+  }
+
+  // 32 columns of one row, as pairs: o[2 g + e] holds columns 8 g + 4 h + 2 e and the
+  // next. The lane halves swap so that each holds eight consecutive columns; at the
+  // edges the values go one by one, through LDS of the lane's own.
+  __device__ __forceinline__ void store(const uint32_t (&o)[8], char* lds, int row, int last, int col) const {
+    uint16_t* y = p.y + int64_t(row) * p.y_stride;
+    if (p.y_vec && col + 32 <= p.width) {
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        const auto a = __builtin_amdgcn_permlane32_swap(o[2 * g], o[2 * g + 2], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(o[2 * g + 1], o[2 * g + 3], false, false);
+        if (row <= last)
+          *reinterpret_cast<u32x4*>(y + col + 8 * (g + h)) = u32x4{uint32_t(a[0]), uint32_t(b[0]), uint32_t(a[1]), uint32_t(b[1])};
+      }
+      return;
+    }
+    uint16_t* mine = reinterpret_cast<uint16_t*>(lds + threadIdx.x * 32);
+    *reinterpret_cast<u32x4*>(mine) = u32x4{o[0], o[1], o[2], o[3]};
+    *reinterpret_cast<u32x4*>(mine + 8) = u32x4{o[4], o[5], o[6], o[7]};
+    if (row > last) return;
+#pragma unroll 1
+    for (int r = 0; r < 16; ++r) {
+      const int at = col + 8 * (r >> 2) + 4 * h + (r & 3);
+      if (at < p.width) y[at] = mine[r];
+    }
+  }
+};
+
+// Where a workgroup's tile is. Tiles are numbered by expert, within an expert in
+// groups of kGroup row tiles, column by column, and dealt to the XCDs (workgroup
+// number modulo 8) in contiguous ranges: an XCD's workgroups share few row and
+// column tiles at a time in its L2, and an expert's weights go to few XCDs.
+constexpr int kGroup = 4;
+constexpr int kXcds = 8;
+
+__device__ __forceinline__ int tiles_of(const Segment& s, int cap) { return (s.end - s.begin + cap - 1) / cap; }
+
+__device__ __forceinline__ int total_tiles(const Params& p, int cap) {
+  if (!p.offsets) return (p.rows + cap - 1) / cap;
+  int sum = 0;
+  for (int e = threadIdx.x & 63; e < p.experts; e += 64) sum += tiles_of(segment_of(p, e), cap);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+  return __builtin_amdgcn_readfirstlane(sum);
+}
+
+template <bool kXMx, bool kWMx, int kJ>
+__global__ __launch_bounds__(kThreads, 1) void tile_kernel(Params p, int cap, int column_tiles) {
+  extern __shared__ char lds[];
+  const int items = total_tiles(p, cap) * column_tiles;
+  const int share = (items + kXcds - 1) / kXcds, local = blockIdx.x / kXcds;
+  int index = int(blockIdx.x % kXcds) * share + local;
+  if (local >= share || index >= items) return;
+  const Segment seg = find_segment(p, index, [&](const Segment& s) { return tiles_of(s, cap) * column_tiles; });
+  const int rows = seg.end - seg.begin, tiles = tiles_of(seg, cap);
+  if (rows <= 0) return;
+  const int group = index / (kGroup * column_tiles), in_group = index - group * kGroup * column_tiles;
+  const int group_tiles = min(kGroup, tiles - group * kGroup);
+  const int mt = group * kGroup + in_group % group_tiles, nt = in_group / group_tiles;
+  const int height = ((rows + tiles - 1) / tiles + 63) / 64 * 64;
+  const int first = seg.begin + mt * height, count = min(height, seg.end - first);
+  if (count <= 0) return;
+  switch ((count + 63) / 64) {
+    case 1: Body<kXMx, kWMx, 1, kJ>(p).run(lds, seg, first, count, nt); break;
+    case 2: Body<kXMx, kWMx, 2, kJ>(p).run(lds, seg, first, count, nt); break;
+    case 3: Body<kXMx, kWMx, 3, kJ>(p).run(lds, seg, first, count, nt); break;
+    default: Body<kXMx, kWMx, 4, kJ>(p).run(lds, seg, first, count, nt); break;
+  }
+}
+
+// Launches tiles of at most `cap` rows (64, 128, 192 or 256) x 64 kJ weight rows.
+template <bool kXMx, bool kWMx, int kJ>
+int launch(const Params& p, int cap, hipStream_t stream) {
+  const int64_t columns = p.swiglu ? 32 * kJ : 64 * kJ;
+  const int64_t column_tiles = (p.width + columns - 1) / columns;
+  // At most: a tile more than whole ones for every expert that has a row.
+  const int64_t used = p.offsets ? (p.experts < p.rows ? p.experts : p.rows) : 1;
+  const int64_t row_tiles = (p.rows + used * (cap - 1)) / cap;
+  LF_REQUIRE(row_tiles * column_tiles < (int64_t(1) << 30), "too many tiles");
+  const unsigned grid = unsigned((row_tiles * column_tiles + kXcds - 1) / kXcds * kXcds);
+  hipLaunchKernelGGL((tile_kernel<kXMx, kWMx, kJ>), dim3(grid), dim3(kThreads), kLds, stream, p, cap, int(column_tiles));
+  LF_HIP(hipGetLastError());
+  return kOk;
+}
+
+}  // namespace tile
+}  // namespace expert
+}  // namespace lf

@@ -128,8 +128,11 @@ def dequantize_mxfp4(t: MXFP4Tensor, *, out=None):
     return out
 
 
-def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out):
-    """The product that ``mxfp4_linear`` and ``expert_linear`` share; ``experts`` is None for the dense one."""
+def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out, plan=None):
+    """The product that ``mxfp4_linear`` and ``expert_linear`` share; ``experts`` is None for the dense one.
+
+    ``plan`` (``_lib.ExpertPlan``) forces a kernel; by default the library chooses.
+    """
     import torch
 
     grouped = experts is not None
@@ -198,6 +201,8 @@ def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out):
     a.w = weights[0].data_ptr()
     a.w_scales = weights[1].data_ptr() if quantised else None
     a.y, a.y_stride, a.swiglu = out.data_ptr(), out.stride(0) if rows > 1 else width, swiglu
+    if plan is not None:
+        a.plan = ctypes.pointer(plan)
     with torch.cuda.device(device):
         _lib.check(_lib.library().lf_expert_linear(ctypes.byref(a), _lib.stream_of(device)))
     return out

@@ -9,7 +9,9 @@ import numpy as np
 import pytest
 import torch
 
+from loraforge_amd import _lib
 from loraforge_amd.ops import MXFP4Tensor, dequantize_mxfp4, expert_linear, mxfp4_linear, quantize_mxfp4
+from loraforge_amd.ops.mxfp4 import product
 from oracle import experts as ox
 
 pytestmark = pytest.mark.gpu
@@ -288,3 +290,105 @@ def test_products_on_a_side_stream_and_in_a_graph(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, mxfp4_linear(quantize_mxfp4(x), w))
+
+
+# --------------------------------------------------------------------------
+# Every kernel and tile, forced
+# --------------------------------------------------------------------------
+
+TYPES = [("bf16", "bf16"), ("bf16", "mxfp4"), ("mxfp4", "mxfp4")]
+PLANS = [(_lib.LF_EXPERT_STREAM, 0, c) for c in (16, 32, 64)] + [
+    (_lib.LF_EXPERT_TILE, r, c) for r in (64, 128, 192, 256) for c in (64, 128, 256)]
+
+
+def forced(x, w, plan, **options):
+    arguments = dict(experts=None, offsets=None, tokens=None, bias=None, swiglu=False, out=None)
+    return product(x, w, **{**arguments, **options}, plan=_lib.ExpertPlan(*plan))
+
+
+@pytest.mark.parametrize("types", TYPES, ids="-".join)
+@pytest.mark.parametrize("plan", PLANS, ids=lambda p: "-".join(map(str, p)))
+@pytest.mark.parametrize("k", [128, 416, 2880])
+def test_every_plan(types, plan, k, device):
+    """Ragged experts on one kernel: tile heights of one to four 64-row steps, ends of k inside a stage, edge columns."""
+    act, weight = types
+    counts = [130, 0, 1, 64, 257, 33, 190]
+    n = 328
+    rows = sum(counts)
+    x, xv = operand(randn(k, rows, k), act, device)
+    w, wv = operand(randn(k + 1, len(counts), n, k, std=0.05), weight, device)
+    b = randn(k + 2, len(counts), n)
+    y = forced(x, w, plan, experts=len(counts), offsets=segments(counts).to(device), bias=b.to(device))
+    start = 0
+    for e, count in enumerate(counts):
+        if count:
+            close(y[start : start + count], *ox.product(xv[start : start + count], wv[e], b[e].double().numpy()))
+        start += count
+
+
+@pytest.mark.parametrize("types", TYPES, ids="-".join)
+@pytest.mark.parametrize("plan", [p for p in PLANS if p[2] > 64 or p[0] == _lib.LF_EXPERT_STREAM], ids=lambda p: "-".join(map(str, p)))
+@pytest.mark.parametrize("n", [512, 776, 88])
+def test_every_plan_swiglu(types, plan, n, device):
+    act, weight = types
+    k, counts = 544, [70, 3, 200]
+    x, xv = operand(randn(n, sum(counts), k), act, device)
+    w, wv = operand(randn(n + 1, len(counts), n, k, std=0.05), weight, device)
+    b = randn(n + 2, len(counts), n)
+    y = forced(x, w, plan, experts=len(counts), offsets=segments(counts).to(device), bias=b.to(device), swiglu=True)
+    start = 0
+    for e, count in enumerate(counts):
+        close(y[start : start + count], *ox.product(xv[start : start + count], wv[e], b[e].double().numpy(), True))
+        start += count
+
+
+@pytest.mark.parametrize("types", TYPES, ids="-".join)
+@pytest.mark.parametrize("columns", [64, 128, 256])
+def test_tiles_of_one_dense_product(types, columns, device):
+    """Several row and column tiles of one segment, on every workgroup order; results do not depend on the tile."""
+    act, weight = types
+    m, n, k = 1300, 700, 512
+    x, xv = operand(randn(40, m, k), act, device)
+    w, wv = operand(randn(41, 1, n, k, std=0.05), weight, device)
+    whole = segments([m]).to(device)
+    y = forced(x, w, (_lib.LF_EXPERT_TILE, 256, columns), experts=1, offsets=whole)
+    close(y, *ox.product(xv, wv[0]))
+    for rows in (64, 128, 192):
+        assert torch.equal(forced(x, w, (_lib.LF_EXPERT_TILE, rows, columns), experts=1, offsets=whole), y)
+
+
+@pytest.mark.parametrize("plan", [(_lib.LF_EXPERT_STREAM, 0, 32), (_lib.LF_EXPERT_TILE, 256, 256)], ids=str)
+def test_output_rows_of_any_alignment(plan, device):
+    m, n, k = 200, 256, 256
+    x, xv = operand(randn(42, m, k), "bf16", device)
+    w, wv = operand(randn(43, n, k, std=0.05), "mxfp4", device)
+    expected = ox.product(xv, wv)
+    for pad, at in ((0, 0), (8, 8), (3, 1), (8, 4)):
+        store = torch.zeros(m, n + pad, dtype=torch.bfloat16, device=device)
+        out = store[:, at : at + n]
+        forced(x, w, plan, out=out)
+        close(out, *expected)
+        assert not store[:, :at].any() and not store[:, at + n :].any()
+
+
+@pytest.mark.parametrize("types", TYPES, ids="-".join)
+def test_scales_and_rows_at_odd_addresses(types, device):
+    """Scale bytes at any address; x rows gathered from a larger store, backwards."""
+    act, weight = types
+    m, n, k = 150, 192, 288
+    x, xv = operand(randn(44, m, k), act, device)
+    w, wv = operand(randn(45, 1, n, k, std=0.05), weight, device)
+
+    def shifted(t):
+        store = torch.zeros(t.numel() + 3, dtype=torch.uint8, device=device)
+        store[3:] = t.reshape(-1)
+        return store[3:].reshape(t.shape)
+
+    if act == "mxfp4":
+        x = MXFP4Tensor(x.codes, shifted(x.scales))
+    if weight == "mxfp4":
+        w = MXFP4Tensor(w.codes, shifted(w.scales))
+    tokens = torch.arange(m - 1, -1, -1, dtype=torch.int32, device=device)
+    for plan in PLANS[2], PLANS[-1], PLANS[3]:
+        y = forced(x, w, plan, experts=1, offsets=segments([m]).to(device), tokens=tokens)
+        close(y, *ox.product(xv[::-1], wv[0]))
