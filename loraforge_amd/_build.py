@@ -44,8 +44,10 @@ HIP_FLAGS = [
 
 # Sources whose kernels must not use scratch: the decode and prefill kernels
 # issue loads the compiler does not track (waited for explicitly), and a
-# register spill of such a result would store it before the load returned.
-NO_SCRATCH = {"nf4_gemv.hip", "nf4_decode_wide.hip", "row_ops.hip"} | {f"nf4_prefill_rows_{part}.hip" for part in "abcd"}
+# register spill of such a result would store it before the load returned. (In the
+# expert tiles a spill in the loop would wait for every copy in flight.)
+NO_SCRATCH = {"nf4_gemv.hip", "nf4_decode_wide.hip", "row_ops.hip"} | {
+    f"nf4_prefill_rows_{part}.hip" for part in "abcd"} | {f"expert_tile_{types}.hip" for types in ("bf16", "mxw", "mx")}
 
 
 def hipcc() -> str:

@@ -261,7 +261,7 @@ struct Body {
     }
     // (The tall tiles run whole rounds of the ring, stages past the end on zeros: with
     // more than one way out of the loop the compiler moves their sums through scratch.)
-    constexpr bool kWhole = kI >= 2 && kI * kJ >= 8;
+    constexpr bool kWhole = kI * kJ > 4;
     for (int st = 0; st < stages; st += kN) {
       stage(s0, s1, st, f, codes, sc, ahead[0]);
       if (!kWhole && st + 1 >= stages) break;
@@ -327,79 +327,81 @@ struct Body {
 
     ring(lds, lds + S::kStage, lds + (S::kSlots > 2 ? 2 : 0) * S::kStage, lds + (S::kSlots > 3 ? 3 : 0) * S::kStage);
 
-    // acc[i][j][4 g + e]: row 64 i + 32 wm + c of the tile, weight row 8 g + 4 h + e of fragment j.
-    const uint16_t* bias = p.bias ? p.bias + w0 : nullptr;
-    const int base = nt * 64 * kJ + 32 * kJ * wn;
-    if (p.swiglu) {
-      if constexpr (kJ >= 2) {
-#pragma unroll
-        for (int j = 0; j < kJ; j += 2) {
-          const int col = base / 2 + 16 * j;
-          if (bias) {
-            add_bias(bias, col, j);
-            add_bias(bias + p.width, col, j + 1);
-          }
-#pragma unroll
-          for (int i = 0; i < kI; ++i) {
-            uint32_t o[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-              o[r] = pack_bf16x2(silu_mul_f32(acc[i][j][2 * r], acc[i][j + 1][2 * r]),
-                                 silu_mul_f32(acc[i][j][2 * r + 1], acc[i][j + 1][2 * r + 1]));
-            store(o, lds, first + 64 * i + 32 * wm + c, last, col);
-            pin();
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        const int col = base + 32 * j;
-        if (bias) add_bias(bias, col, j);
-#pragma unroll
-        for (int i = 0; i < kI; ++i) {
-          uint32_t o[8];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) o[r] = pack_bf16x2(acc[i][j][2 * r], acc[i][j][2 * r + 1]);
-          store(o, lds, first + 64 * i + 32 * wm + c, last, col);
-          pin();
-        }
-      }
-    }
+    // Copies of zeros for stages past the end are still on their way, and other
+    // waves read their last operands.
+    wait_vm<0>();
+    lds_barrier();
+    if (p.swiglu)
+      finish<true>(lds, seg.expert, first, count, nt);
+    else
+      finish<false>(lds, seg.expert, first, count, nt);
   }
 
-  __device__ __forceinline__ void add_bias(const uint16_t* bias, int col, int j) {
+  // Bias, activation, rounding and stores. Each wave passes its sums through LDS of
+  // its own, two fragment rows (64 rows of the tile) at a time: acc[i][j][4 g + e] is
+  // row c of fragment row i and weight row 8 g + 4 h + e of fragment j, and in LDS a
+  // row's columns follow each other, so that eight lanes or more store whole cache
+  // lines and the code is short (an unrolled epilogue straight from the
+  // registers took longer to fetch than to run).
+  template <bool kSwiglu>
+  __device__ __forceinline__ void finish(char* lds, int expert, int first, int count, int nt) {
+    if constexpr (!kSwiglu || kJ >= 2) {
+      constexpr int kRowBytes = 32 * kJ * 4 + 16;             // (padded: rows start at other banks)
+      constexpr int kColumns = kSwiglu ? 16 * kJ : 32 * kJ;   // output columns of the wave
+      constexpr int kLanes = kColumns / 8, kRows = 64 / kLanes;
+      char* mine = lds + wave * 64 * kRowBytes;
+      const int wm = wave & 1, wn = wave >> 1, c = lane & 31;
+      const int part = lane % kLanes, in_row = lane / kLanes;
+      // With SwiGLU eight columns lie in 32 of a gate fragment, their up values one fragment on.
+      const int local = kSwiglu ? part / 4 * 64 + part % 4 * 8 : part * 8;
+      const int col = (nt * 2 + wn) * kColumns + part * 8;
+      float add[8], add_up[8];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float b = bf16_to_f32(bias[min(col + 8 * (r >> 2) + 4 * h + (r & 3), p.width - 1)]);
-#pragma unroll
-      for (int i = 0; i < kI; ++i) acc[i][j][r] += b;
-    }
-  }
-
-  // 32 columns of one row, as pairs: o[2 g + e] holds columns 8 g + 4 h + 2 e and the
-  // next. The lane halves swap so that each holds eight consecutive columns; at the
-  // edges the values go one by one, through LDS of the lane's own.
-  __device__ __forceinline__ void store(const uint32_t (&o)[8], char* lds, int row, int last, int col) const {
-    uint16_t* y = p.y + int64_t(row) * p.y_stride;
-    if (p.y_vec && col + 32 <= p.width) {
-#pragma unroll
-      for (int g = 0; g < 4; g += 2) {
-        const auto a = __builtin_amdgcn_permlane32_swap(o[2 * g], o[2 * g + 2], false, false);
-        const auto b = __builtin_amdgcn_permlane32_swap(o[2 * g + 1], o[2 * g + 3], false, false);
-        if (row <= last)
-          *reinterpret_cast<u32x4*>(y + col + 8 * (g + h)) = u32x4{uint32_t(a[0]), uint32_t(b[0]), uint32_t(a[1]), uint32_t(b[1])};
+      for (int e = 0; e < 8; ++e) {
+        add[e] = add_up[e] = 0.f;
+        if (p.bias) {
+          const uint16_t* bias = p.bias + int64_t(expert) * p.n + min(col + e, p.width - 1);
+          add[e] = bf16_to_f32(bias[0]);
+          if (kSwiglu) add_up[e] = bf16_to_f32(bias[p.width]);
+        }
       }
-      return;
-    }
-    uint16_t* mine = reinterpret_cast<uint16_t*>(lds + threadIdx.x * 32);
-    *reinterpret_cast<u32x4*>(mine) = u32x4{o[0], o[1], o[2], o[3]};
-    *reinterpret_cast<u32x4*>(mine + 8) = u32x4{o[4], o[5], o[6], o[7]};
-    if (row > last) return;
+#pragma unroll
+      for (int pair = 0; pair < (kI + 1) / 2; ++pair) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              if (2 * pair + i < kI) {
+                const f32x16& a = acc[2 * pair + i][j];
+                *reinterpret_cast<f32x4*>(mine + (32 * i + c) * kRowBytes + (32 * j + 8 * g + 4 * h) * 4) =
+                    f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+              }
+        const int staged = min(2, kI - 2 * pair) * 32;
 #pragma unroll 1
-    for (int r = 0; r < 16; ++r) {
-      const int at = col + 8 * (r >> 2) + 4 * h + (r & 3);
-      if (at < p.width) y[at] = mine[r];
+        for (int r0 = 0; r0 < staged; r0 += kRows) {
+          const int r = r0 + in_row;
+          const int row = (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31);
+          const float* v = reinterpret_cast<const float*>(mine + r * kRowBytes) + local;
+          float o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            o[e] = v[e] + add[e];
+            if (kSwiglu) o[e] = silu_mul_f32(o[e], v[32 + e] + add_up[e]);
+          }
+          if (row >= count) continue;
+          uint16_t* y = p.y + int64_t(first + row) * p.y_stride + col;
+          const u32x4 packed{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])};
+          if (p.y_vec && col + 8 <= p.width) {
+            *reinterpret_cast<u32x4*>(y) = packed;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (col + e < p.width) y[e] = uint16_t(packed[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+      }
     }
   }
 };
