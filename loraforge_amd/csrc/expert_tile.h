@@ -42,13 +42,18 @@ struct Shape {
   // (A copy per wave at least: 64 rows of 32 bytes go twice.)
   static constexpr int kXBytes = 64 * kI * kXRow, kWBytes = 64 * kJ * kWRow < 4096 ? 4096 : 64 * kJ * kWRow;
   static constexpr int kStage = kXBytes + kWBytes;
-  static constexpr int kSlots = kLds / kStage >= 4 ? 4 : kLds / kStage;
+  // Scales go through LDS in units of 16 bytes (512 k) of every row that needs them, two buffers.
+  static constexpr int kUnitStages = 512 / kStageK;
+  static constexpr int kScaleRows = (kXMx ? 64 * kI : 0) + (kWMx ? 64 * kJ : 0);
+  static constexpr int kScaleBytes = 2 * 16 * kScaleRows;
+  static constexpr int kSlots = (kLds - kScaleBytes) / kStage >= 4 ? 4 : (kLds - kScaleBytes) / kStage;
   static_assert(kSlots >= 2, "two stages have to fit");
   static constexpr int kXCopies = kXBytes / 4096, kWCopies = kWBytes / 4096;  // per wave
-  static constexpr int kScaleLoads = kXMx ? kI + kJ : kDecode ? kJ : 0;
   static constexpr int kLoads = kXCopies + kWCopies;
 };
 
+// Scales of one stage: with MXFP4 x the lane's four blocks of every fragment row,
+// beside bf16 x its one block.
 struct Scales {
   uint32_t x[4], w[4];
 };
@@ -73,9 +78,10 @@ struct Body {
   int xleft, wleft;         // bytes of the row from the lane's unit on
   // Operand reads: byte offsets in a slot of sub-step s = 0, row of fragment 0.
   int xread, wread, xmask, wmask;
-  // Scale rows: byte offsets from p.xs and from the expert's first row (below 2 GiB).
-  const uint8_t* wbase;
-  uint32_t xscale[kXMx ? kI : 1], wscale[kWMx ? kJ : 1];
+  // Scales: the rows this thread loads, their next unit, and where it reads fragment 0's.
+  const uint8_t *xscale, *wscale;
+  u32x4 xunit, wunit;
+  int xsread, wsread;
   f32x16 acc[kI][kJ];
 
   __device__ __forceinline__ Body(const Params& p_) : p(p_) {}
@@ -103,42 +109,59 @@ struct Body {
         copy16(wleft > 0 ? wsrc[d] : zeros, slot + S::kXBytes + (d * 4 + wave) * 1024);
         wsrc[d] += S::kWRow;
       }
-    if (last == S::kLoads) {
+    if (first < last && last == S::kLoads) {
       xleft -= kXRow;
       wleft -= S::kWRow;
     }
   }
 
-  // Scales of stage st: with MXFP4 x the lane's four blocks of every fragment row
-  // (one load of any alignment, not past the row; k >= 128), beside bf16 x its one
-  // block. Loads are never skipped: the waits count them. What they load is put
-  // in place when it is used (used_scales), with zeros past the end of k.
-  __device__ __forceinline__ int scale_block(int st) const { return (kXMx ? 8 : 2) * st + (kXMx ? 4 : 1) * h; }
-  __device__ __forceinline__ void load_scales(int st, Scales& s) const {
+  // 16 scale bytes of a row from block 16 u on, at any alignment; zeros past the
+  // end of k (codes are zero there) and nothing read past it.
+  __device__ __forceinline__ u32x4 load_unit(const uint8_t* row, int u) const {
+    typedef u32x4 u32x4u __attribute__((aligned(1)));
     typedef uint32_t u32u __attribute__((aligned(1)));
-    if constexpr (kXMx) {
-      const uint32_t from = uint32_t(min(scale_block(st), p.k / mx::kBlock - 4));
+    const int left = p.k / mx::kBlock - 16 * u;
+    row += 16 * u;
+    if (left >= 16) return *reinterpret_cast<const u32x4u*>(row);
+    u32x4 v{0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int i = 0; i < kI; ++i) s.x[i] = *reinterpret_cast<const u32u*>(p.xs + (xscale[i] + from));
+    for (int d = 0; d < 4; ++d) {
+      if (left >= 4 * d + 4) {
+        v[d] = *reinterpret_cast<const u32u*>(row + 4 * d);
+      } else {
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const u32u*>(wbase + (wscale[j] + from));
-    } else if constexpr (kWMx) {
-      const uint32_t from = uint32_t(min(scale_block(st), p.k / mx::kBlock - 1));
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) s.w[j] = wbase[wscale[j] + from];
+        for (int e = 0; e < 3; ++e)
+          if (left > 4 * d + e) v[d] |= uint32_t(row[4 * d + e]) << (8 * e);
+      }
     }
+    return v;
   }
-  __device__ __forceinline__ void used_scales(int st, const Scales& s, Scales& u) const {
-    if constexpr (kXMx) {
-      const int shift = 8 * min(max(scale_block(st) + 4 - p.k / mx::kBlock, 0), 4);
+  __device__ __forceinline__ void load_units(int u) {
+    if constexpr (kXMx)
+      if (threadIdx.x < 64 * kI) xunit = load_unit(xscale, u);
+    if constexpr (kWMx)
+      if (threadIdx.x < 64 * kJ) wunit = load_unit(wscale, u);
+  }
+  __device__ __forceinline__ void write_units(char* scales, int u) const {
+    char* to = scales + (u & 1) * (S::kScaleBytes / 2) + threadIdx.x * 16;
+    if constexpr (kXMx)
+      if (threadIdx.x < 64 * kI) *reinterpret_cast<u32x4*>(to) = xunit;
+    if constexpr (kWMx)
+      if (threadIdx.x < 64 * kJ) *reinterpret_cast<u32x4*>(to + (kXMx ? 64 * kI * 16 : 0)) = wunit;
+  }
+  __device__ __forceinline__ void read_scales(const char* scales, int st, Scales& s) const {
+    if constexpr (kWMx) {
+      const char* from = scales + (st / S::kUnitStages & 1) * (S::kScaleBytes / 2);
+      const int in_unit = st % S::kUnitStages;
+      if constexpr (kXMx) {
 #pragma unroll
-      for (int i = 0; i < kI; ++i) u.x[i] = uint32_t(uint64_t(s.x[i]) >> shift);
+        for (int i = 0; i < kI; ++i) s.x[i] = *reinterpret_cast<const uint32_t*>(from + xsread + i * 64 * 16 + in_unit * 8);
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) u.w[j] = uint32_t(uint64_t(s.w[j]) >> shift);
-    } else if constexpr (kWMx) {
-      const uint32_t mask = scale_block(st) < p.k / mx::kBlock ? 0xffu : 0u;
+        for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const uint32_t*>(from + wsread + j * 32 * 16 + in_unit * 8);
+      } else {
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) u.w[j] = s.w[j] & mask;
+        for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const uint8_t*>(from + wsread + j * 32 * 16 + in_unit * 2);
+      }
     }
   }
 
@@ -186,11 +209,17 @@ struct Body {
       }
   }
 
+  // Copies of a stage go out behind two sub-steps' instructions, half from the
+  // sub-step on that frees their slot, half in the one after (all at once they
+  // fill the memory pipe and hold the matrix instructions back: 8192 x 8192 x 8192
+  // in bf16 8 % slower; over three or four sub-steps the last arrive too late).
+  static constexpr int kFirst = S::kLoads / 2;
+
   // The stage in `cur`, whose first operands are in `f` and scales in `sc`; `next`
-  // holds the one after it (its scales loaded in `ahead`), and on return `f`, `sc`
-  // and `codes` are that stage's. `ahead` then loads a later stage's.
-  __device__ __forceinline__ void stage(char* cur, const char* next, int st, Frags<kI, kJ>& f, u32x4 (&codes)[kJ],
-                                        Scales& sc, Scales& ahead) {
+  // holds the one after it, and on return `f`, `sc` and `codes` are that stage's.
+  // `prev` is the slot whose last reader was the stage before.
+  __device__ __forceinline__ void stage(char* prev, char* cur, const char* next, char* scales, int st, Frags<kI, kJ>& f,
+                                        u32x4 (&codes)[kJ], Scales& sc) {
     constexpr int kM = kI * kJ;
     Frags<kI, kJ> g;
     auto decode = [&](Frags<kI, kJ>& to, const u32x4 (&from)[kJ], const Scales& s, int sub, int n) {
@@ -198,28 +227,40 @@ struct Body {
       if constexpr (S::kDecode)
         if (n % kI == 0) to.w[n / kI] = mx::decode8(from[n / kI][sub], mx::scale_f32(s.w[n / kI]));
     };
+    auto copies = [&](char* slot, int first, int last, int n) {
+      copy(slot, first + n * (last - first) / kM, first + (n + 1) * (last - first) / kM);
+    };
+    if constexpr (kWMx) {
+      if (st % S::kUnitStages == 0) {
+        write_units(scales, st / S::kUnitStages + 1);
+        load_units(st / S::kUnitStages + 2);
+      }
+    }
     read(cur, 1, g);
     pin();
-    sub_step<0>(f, sc, [&](int n) { decode(g, codes, sc, 1, n); });
+    sub_step<0>(f, sc, [&](int n) {
+      decode(g, codes, sc, 1, n);
+      copies(prev, kFirst, S::kLoads, n);
+    });
     read(cur, 2, f);
     pin();
     sub_step<1>(g, sc, [&](int n) { decode(f, codes, sc, 2, n); });
     read(cur, 3, g);
     pin();
     sub_step<2>(f, sc, [&](int n) { decode(g, codes, sc, 3, n); });
-    // Every wave has read all of `cur`, and `next` and `ahead` have arrived.
+    // Every wave has read all of `cur`, and `next` has arrived: at most the copies
+    // of the stages after it are still on their way.
     __builtin_amdgcn_s_waitcnt(0xC07F);
-    wait_vm<(S::kSlots - 2) * (S::kLoads + S::kScaleLoads)>();
+    wait_vm<(S::kSlots - 2) * S::kLoads>();
     barrier_only();
     Scales su;
-    used_scales(st + 1, ahead, su);
+    read_scales(scales, st + 1, su);
     read(next, 0, f);
     u32x4 codes_next[kJ];
     read_codes(next, codes_next);
-    load_scales(st + S::kSlots + 1, ahead);
     pin();
     sub_step<3>(g, sc, [&](int n) {
-      copy(cur, n * S::kLoads / kM, (n + 1) * S::kLoads / kM);
+      copies(cur, 0, kFirst, n);
       decode(f, codes_next, su, 0, n);
     });
     sc = su;
@@ -233,24 +274,23 @@ struct Body {
   // that reads of one do not depend on the copies into another (it would wait
   // for every copy in flight before each read).
   __device__ __forceinline__ void ring(char* __restrict__ s0, char* __restrict__ s1, char* __restrict__ s2,
-                                       char* __restrict__ s3) {
+                                       char* __restrict__ s3, char* __restrict__ scales) {
     constexpr int kN = S::kSlots;
-    // Loads in order: scales 0, then for each stage n of the ring scales n + 1 and copies n.
-    Scales first, ahead[kN], sc;
-    load_scales(0, first);
-    auto start = [&](char* slot, int n) {
-      load_scales(n + 1, ahead[n]);
-      pin();
-      copy(slot, 0, S::kLoads);
-      pin();
-    };
-    start(s0, 0);
-    start(s1, 1);
-    if constexpr (kN > 2) start(s2, 2);
-    if constexpr (kN > 3) start(s3, 3);
-    wait_vm<(kN - 1) * (S::kLoads + S::kScaleLoads)>();
-    barrier_only();
-    used_scales(0, first, sc);
+    load_units(0);
+    pin();
+    copy(s0, 0, S::kLoads);
+    pin();
+    if constexpr (kWMx) write_units(scales, 0);
+    load_units(1);
+    pin();
+    if constexpr (kN > 2) copy(s1, 0, S::kLoads);
+    if constexpr (kN > 3) copy(s2, 0, S::kLoads);
+    copy(kN == 2 ? s1 : kN == 3 ? s2 : s3, 0, kFirst);
+    pin();
+    wait_vm<(kN - 2) * S::kLoads + kFirst>();
+    lds_barrier();
+    Scales sc;
+    read_scales(scales, 0, sc);
     Frags<kI, kJ> f;
     u32x4 codes[kJ];
     read(s0, 0, f);
@@ -262,17 +302,18 @@ struct Body {
     // (The tall tiles run whole rounds of the ring, stages past the end on zeros: with
     // more than one way out of the loop the compiler moves their sums through scratch.)
     constexpr bool kWhole = kI * kJ > 4;
+    char* const last = kN == 2 ? s1 : kN == 3 ? s2 : s3;
     for (int st = 0; st < stages; st += kN) {
-      stage(s0, s1, st, f, codes, sc, ahead[0]);
+      stage(last, s0, s1, scales, st, f, codes, sc);
       if (!kWhole && st + 1 >= stages) break;
-      stage(s1, kN == 2 ? s0 : s2, st + 1, f, codes, sc, ahead[1]);
+      stage(s0, s1, kN == 2 ? s0 : s2, scales, st + 1, f, codes, sc);
       if constexpr (kN > 2) {
         if (!kWhole && st + 2 >= stages) break;
-        stage(s2, kN == 3 ? s0 : s3, st + 2, f, codes, sc, ahead[2]);
+        stage(s1, s2, kN == 3 ? s0 : s3, scales, st + 2, f, codes, sc);
       }
       if constexpr (kN > 3) {
         if (!kWhole && st + 3 >= stages) break;
-        stage(s3, s0, st + 3, f, codes, sc, ahead[3]);
+        stage(s2, s3, s0, scales, st + 3, f, codes, sc);
       }
     }
   }
@@ -291,32 +332,32 @@ struct Body {
     // A copy covers eight rows of 128 bytes (of 32 bytes: 32 rows); row r's unit u
     // sits at u ^ (r & 7), so that reads of one unit of consecutive rows meet no bank twice.
     const int r8 = lane >> 3;
-    const int xunit = ((lane & 7) ^ r8) * 16;
+    const int xat = ((lane & 7) ^ r8) * 16;
 #pragma unroll
     for (int d = 0; d < S::kXCopies; ++d)
-      xsrc[d] = p.x + x_row_of(p, min(first + 8 * (d * 4 + wave) + r8, last)) * p.x_row + xunit;
+      xsrc[d] = p.x + x_row_of(p, min(first + 8 * (d * 4 + wave) + r8, last)) * p.x_row + xat;
     const int64_t w0 = int64_t(seg.expert) * p.n;
     const int wr = S::kWRow == 128 ? r8 : lane >> 1;
-    const int wunit = S::kWRow == 128 ? xunit : (lane & 1) * 16;
+    const int wat = S::kWRow == 128 ? xat : (lane & 1) * 16;
 #pragma unroll
     for (int d = 0; d < S::kWCopies; ++d)
-      wsrc[d] = p.w + (w0 + weight_row(nt, ((d * 4 + wave) * (1024 / S::kWRow) + wr) % (64 * kJ))) * row_bytes_w + wunit;
+      wsrc[d] = p.w + (w0 + weight_row(nt, ((d * 4 + wave) * (1024 / S::kWRow) + wr) % (64 * kJ))) * row_bytes_w + wat;
 
-    xleft = row_bytes_x - xunit;
-    wleft = row_bytes_w - wunit;
+    xleft = row_bytes_x - xat;
+    wleft = row_bytes_w - wat;
 
     xread = (32 * wm + c) * kXRow;  // fragment i: rows 64 i + 32 wm ..
     xmask = (c & 7) * 16;
     wread = (32 * kJ * wn + c) * S::kWRow;
     wmask = xmask;
+    const int t = threadIdx.x;
     if constexpr (kXMx) {
-#pragma unroll
-      for (int i = 0; i < kI; ++i) xscale[i] = uint32_t(x_row_of(p, min(first + 64 * i + 32 * wm + c, last))) * blocks;
+      xscale = p.xs + x_row_of(p, min(first + t, last)) * blocks;
+      xsread = (32 * wm + c) * 16 + 4 * h;
     }
     if constexpr (kWMx) {
-      wbase = p.ws + w0 * blocks;
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) wscale[j] = uint32_t(weight_row(nt, 32 * kJ * wn + 32 * j + c)) * blocks;
+      wscale = p.ws + (w0 + weight_row(nt, t % (64 * kJ))) * blocks;
+      wsread = (kXMx ? 64 * kI * 16 : 0) + (32 * kJ * wn + c) * 16 + (kXMx ? 4 : 1) * h;
     }
 #pragma unroll
     for (int i = 0; i < kI; ++i)
@@ -325,7 +366,8 @@ struct Body {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    ring(lds, lds + S::kStage, lds + (S::kSlots > 2 ? 2 : 0) * S::kStage, lds + (S::kSlots > 3 ? 3 : 0) * S::kStage);
+    ring(lds, lds + S::kStage, lds + (S::kSlots > 2 ? 2 : 0) * S::kStage, lds + (S::kSlots > 3 ? 3 : 0) * S::kStage,
+         lds + S::kSlots * S::kStage);
 
     // Copies of zeros for stages past the end are still on their way, and other
     // waves read their last operands.
@@ -379,7 +421,7 @@ struct Body {
                     f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
               }
         const int staged = min(2, kI - 2 * pair) * 32;
-#pragma unroll 1
+#pragma unroll 4
         for (int r0 = 0; r0 < staged; r0 += kRows) {
           const int r = r0 + in_row;
           const int row = (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31);
