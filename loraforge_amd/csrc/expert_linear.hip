@@ -8,12 +8,19 @@ namespace lf {
 namespace expert {
 namespace {
 
+// What the tile kernel can take: MXFP4 x with 16 scales a row and, as an expert's
+// weights beside it, within 32-bit offsets; four scales a row beside bf16 x.
+bool tiles_fit(const lf_expert_product& a) {
+  if (a.x_scales) return a.k >= 512 && std::max(a.x_rows, a.n) * (a.k / 2) < (int64_t(1) << 32);
+  return !a.w_scales || a.k >= 128;
+}
+
 lf_expert_plan plan_of(const lf_expert_product& a) {
   const int64_t used = a.offsets ? std::min(a.experts, a.rows) : 1;
   const int64_t width = a.swiglu ? a.n / 2 : a.n;
   const int64_t each = (a.rows + used - 1) / used;  // rows of an expert, on average
   lf_expert_plan plan{};
-  if (each > 32) {
+  if (each > 32 && tiles_fit(a)) {
     plan.kernel = LF_EXPERT_TILE;
     plan.rows = int32_t(std::min<int64_t>(256, (each + 63) / 64 * 64));
     plan.columns = 256;
@@ -72,7 +79,7 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
     LF_REQUIRE(plan.columns == 16 || plan.columns == 32 || plan.columns == 64, "stream plan: 16, 32 or 64 columns");
     return lf::expert::launch_stream(p, plan.columns / 16, s);
   }
-  LF_REQUIRE(plan.kernel == LF_EXPERT_TILE, "unknown kernel in the plan");
+  LF_REQUIRE(plan.kernel == LF_EXPERT_TILE && lf::expert::tiles_fit(*a), "this product cannot run in tiles");
   LF_REQUIRE(plan.rows >= 64 && plan.rows <= 256 && plan.rows % 64 == 0, "tile plan: 64, 128, 192 or 256 rows");
   LF_REQUIRE(plan.columns == 128 || plan.columns == 256 || (plan.columns == 64 && !a->swiglu),
              "tile plan: 64 (not with SwiGLU), 128 or 256 columns");

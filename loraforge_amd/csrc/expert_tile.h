@@ -42,20 +42,21 @@ struct Shape {
   // (A copy per wave at least: 64 rows of 32 bytes go twice.)
   static constexpr int kXBytes = 64 * kI * kXRow, kWBytes = 64 * kJ * kWRow < 4096 ? 4096 : 64 * kJ * kWRow;
   static constexpr int kStage = kXBytes + kWBytes;
-  // Scales go through LDS in units of 16 bytes (512 k) of every row that needs them, two buffers.
-  static constexpr int kUnitStages = 512 / kStageK;
+  // Scales go through LDS in units of one round of the ring, two buffers. MXFP4 x:
+  // 16 bytes (two stages) of every x and weight row; beside bf16 x 8 of every weight row.
   static constexpr int kScaleRows = (kXMx ? 64 * kI : 0) + (kWMx ? 64 * kJ : 0);
-  static constexpr int kScaleBytes = 2 * 16 * kScaleRows;
-  static constexpr int kSlots = (kLds - kScaleBytes) / kStage >= 4 ? 4 : (kLds - kScaleBytes) / kStage;
-  static_assert(kSlots >= 2, "two stages have to fit");
+  static constexpr int kUnitBytes = kXMx ? 16 : 8;
+  static constexpr int kScaleBytes = 2 * kUnitBytes * kScaleRows;
+  static constexpr int kFit = (kLds - kScaleBytes) / kStage;
+  static constexpr int kSlots = kXMx ? 2 : kFit >= 4 ? 4 : kFit;
+  static_assert(kFit >= kSlots && kSlots >= 2, "two stages have to fit");
   static constexpr int kXCopies = kXBytes / 4096, kWCopies = kWBytes / 4096;  // per wave
   static constexpr int kLoads = kXCopies + kWCopies;
 };
 
-// Scales of one stage: with MXFP4 x the lane's four blocks of every fragment row,
-// beside bf16 x its one block.
+// A lane's scales: with MXFP4 x its four blocks of every fragment row, beside bf16 x its one block.
 struct Scales {
-  uint32_t x[4], w[4];
+  u32x2 x[4], w[4];  // MXFP4 x: of both stages of a unit
 };
 
 // The operands of one sub-step.
@@ -64,6 +65,7 @@ struct Frags {
   u32x4 x[kI], w[kJ];
 };
 
+__device__ __forceinline__ void reads_done() { __builtin_amdgcn_s_waitcnt(0xC07F); }  // lgkmcnt(0), which the compiler sees
 __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 
 template <bool kXMx, bool kWMx, int kI, int kJ>
@@ -72,15 +74,23 @@ struct Body {
   const Params& p;
   int lane, wave, h;        // h: lane half
   int stages;
-  // Copies: the lane's 16-byte unit of each row it copies, and where it starts.
-  const char* xsrc[S::kXCopies];
-  const char* wsrc[S::kWCopies];
-  int xleft, wleft;         // bytes of the row from the lane's unit on
+  // Copies: where the lane's 16-byte unit of each row that it copies is, and how
+  // many bytes of the row are left from there on. bf16 x: addresses, with zeros in the
+  // place of what lies past the end of k. MXFP4 x: row offsets (below 4 GiB) from a
+  // common base; past the end the row's last unit again, as there both scale bytes are 0
+  // and 2^-254 vanishes whatever the codes.
+  const char* xsrc[kXMx ? 1 : S::kXCopies];
+  const char* wsrc[kXMx ? 1 : S::kWCopies];
+  uint32_t xrow[kXMx ? S::kXCopies : 1], wrow[kXMx ? S::kWCopies : 1];
+  uint32_t at, row_last;
+  const char* wfirst;
+  int xleft, wleft;
   // Operand reads: byte offsets in a slot of sub-step s = 0, row of fragment 0.
   int xread, wread, xmask, wmask;
   // Scales: the rows this thread loads, their next unit, and where it reads fragment 0's.
   const uint8_t *xscale, *wscale;
   u32x4 xunit, wunit;
+  int unit_skip;
   int xsread, wsread;
   f32x16 acc[kI][kJ];
 
@@ -93,75 +103,94 @@ struct Body {
     return min(column, p.width - 1) + (r / 32 % 2 ? p.width : 0);
   }
 
-  // Copies of index first .. last - 1 of the next stage into a slot. Past the end
-  // of k (in the last stage and the stages after it) they copy zeros.
+  // Copies of index first .. last - 1 of the next stage into a slot.
   __device__ __forceinline__ void copy(char* slot, int first, int last) {
-    const char* zeros = reinterpret_cast<const char*>(&kZeros);
+    if constexpr (kXMx) {
+      const uint32_t from = min(at, row_last);
 #pragma unroll
-    for (int d = 0; d < S::kXCopies; ++d)
-      if (d >= first && d < last) {
-        copy16(xleft > 0 ? xsrc[d] : zeros, slot + (d * 4 + wave) * 1024);
-        xsrc[d] += kXRow;
-      }
+      for (int d = 0; d < S::kXCopies; ++d)
+        if (d >= first && d < last) copy16(p.x + (xrow[d] + from), slot + (d * 4 + wave) * 1024);
 #pragma unroll
-    for (int d = 0; d < S::kWCopies; ++d)
-      if (d + S::kXCopies >= first && d + S::kXCopies < last) {
-        copy16(wleft > 0 ? wsrc[d] : zeros, slot + S::kXBytes + (d * 4 + wave) * 1024);
-        wsrc[d] += S::kWRow;
+      for (int d = 0; d < S::kWCopies; ++d)
+        if (d + S::kXCopies >= first && d + S::kXCopies < last)
+          copy16(wfirst + (wrow[d] + from), slot + S::kXBytes + (d * 4 + wave) * 1024);
+      if (first < last && last == S::kLoads) at += kXRow;
+    } else {
+      const char* zeros = reinterpret_cast<const char*>(&kZeros);
+#pragma unroll
+      for (int d = 0; d < S::kXCopies; ++d)
+        if (d >= first && d < last) {
+          copy16(xleft > 0 ? xsrc[d] : zeros, slot + (d * 4 + wave) * 1024);
+          xsrc[d] += kXRow;
+        }
+#pragma unroll
+      for (int d = 0; d < S::kWCopies; ++d)
+        if (d + S::kXCopies >= first && d + S::kXCopies < last) {
+          copy16(wleft > 0 ? wsrc[d] : zeros, slot + S::kXBytes + (d * 4 + wave) * 1024);
+          wsrc[d] += S::kWRow;
+        }
+      if (first < last && last == S::kLoads) {
+        xleft -= kXRow;
+        wleft -= S::kWRow;
       }
-    if (first < last && last == S::kLoads) {
-      xleft -= kXRow;
-      wleft -= S::kWRow;
     }
   }
 
-  // 16 scale bytes of a row from block 16 u on, at any alignment; zeros past the
-  // end of k (codes are zero there) and nothing read past it.
-  __device__ __forceinline__ u32x4 load_unit(const uint8_t* row, int u) const {
+  // Loads the scales of round u (at any alignment): blocks 16 u .. of the thread's x
+  // and weight row (k >= 512), or 2 kSlots u .. of its weight row (k >= 128). Nothing
+  // past the row is read: towards its end the last bytes that can be, and
+  // write_units moves them into place, with zeros past the end of k. No
+  // branches: matrix instructions sink past them out of their order.
+  __device__ __forceinline__ void load_units(int u) {
     typedef u32x4 u32x4u __attribute__((aligned(1)));
     typedef uint32_t u32u __attribute__((aligned(1)));
-    const int left = p.k / mx::kBlock - 16 * u;
-    row += 16 * u;
-    if (left >= 16) return *reinterpret_cast<const u32x4u*>(row);
-    u32x4 v{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      if (left >= 4 * d + 4) {
-        v[d] = *reinterpret_cast<const u32u*>(row + 4 * d);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (left > 4 * d + e) v[d] |= uint32_t(row[4 * d + e]) << (8 * e);
-      }
+    const int blocks = p.k / mx::kBlock;
+    if constexpr (kXMx) {
+      const int from = min(16 * u, blocks - 16);
+      unit_skip = min(16 * u - from, 16);
+      if (kI == 4 || threadIdx.x < 64 * kI) xunit = *reinterpret_cast<const u32x4u*>(xscale + from);
+      if (kJ == 4 || threadIdx.x < 64 * kJ) wunit = *reinterpret_cast<const u32x4u*>(wscale + from);
+    } else if constexpr (kWMx) {
+      const int want = 2 * S::kSlots * u, lo = min(want, blocks - 4), hi = min(want + 4, blocks - 4);
+      wunit.x = *reinterpret_cast<const u32u*>(wscale + lo);
+      wunit.y = *reinterpret_cast<const u32u*>(wscale + hi);
+      wunit.z = uint32_t(min(want - lo, 4));
+      wunit.w = uint32_t(min(want + 4 - hi, 4));
     }
-    return v;
   }
-  __device__ __forceinline__ void load_units(int u) {
-    if constexpr (kXMx)
-      if (threadIdx.x < 64 * kI) xunit = load_unit(xscale, u);
-    if constexpr (kWMx)
-      if (threadIdx.x < 64 * kJ) wunit = load_unit(wscale, u);
+  // v without its first `bytes` (0 .. 16), zeros behind.
+  static __device__ __forceinline__ u32x4 drop_bytes(u32x4 v, int bytes) {
+    if (bytes & 16) v = u32x4{0u, 0u, 0u, 0u};
+    v = bytes & 8 ? u32x4{v.z, v.w, 0u, 0u} : v;
+    v = bytes & 4 ? u32x4{v.y, v.z, v.w, 0u} : v;
+    const int b = bytes & 3;
+    return u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, b), __builtin_amdgcn_alignbyte(v.z, v.y, b),
+                 __builtin_amdgcn_alignbyte(v.w, v.z, b), __builtin_amdgcn_alignbyte(0u, v.w, b)};
   }
   __device__ __forceinline__ void write_units(char* scales, int u) const {
-    char* to = scales + (u & 1) * (S::kScaleBytes / 2) + threadIdx.x * 16;
-    if constexpr (kXMx)
-      if (threadIdx.x < 64 * kI) *reinterpret_cast<u32x4*>(to) = xunit;
-    if constexpr (kWMx)
-      if (threadIdx.x < 64 * kJ) *reinterpret_cast<u32x4*>(to + (kXMx ? 64 * kI * 16 : 0)) = wunit;
+    char* to = scales + (u & 1) * (S::kScaleBytes / 2) + threadIdx.x * S::kUnitBytes;
+    if constexpr (kXMx) {
+      // (The two stages' dwords of a lane half side by side.)
+      const u32x4 x = drop_bytes(xunit, unit_skip), w = drop_bytes(wunit, unit_skip);
+      if (kI == 4 || threadIdx.x < 64 * kI) *reinterpret_cast<u32x4*>(to) = u32x4{x.x, x.z, x.y, x.w};
+      if (kJ == 4 || threadIdx.x < 64 * kJ) *reinterpret_cast<u32x4*>(to + 64 * kI * 16) = u32x4{w.x, w.z, w.y, w.w};
+    } else if constexpr (kWMx) {
+      if (kJ == 4 || threadIdx.x < 64 * kJ)
+        *reinterpret_cast<u32x2*>(to) = u32x2{uint32_t(uint64_t(wunit.x) >> (8 * wunit.z)), uint32_t(uint64_t(wunit.y) >> (8 * wunit.w))};
+    }
   }
-  __device__ __forceinline__ void read_scales(const char* scales, int st, Scales& s) const {
-    if constexpr (kWMx) {
-      const char* from = scales + (st / S::kUnitStages & 1) * (S::kScaleBytes / 2);
-      const int in_unit = st % S::kUnitStages;
-      if constexpr (kXMx) {
+  // Scales of stage kPos of round u. MXFP4 x: both stages' at once (kPos 0).
+  template <int kPos>
+  __device__ __forceinline__ void read_scales(const char* scales, int u, Scales& s) const {
+    const char* from = scales + (u & 1) * (S::kScaleBytes / 2);
+    if constexpr (kXMx) {
 #pragma unroll
-        for (int i = 0; i < kI; ++i) s.x[i] = *reinterpret_cast<const uint32_t*>(from + xsread + i * 64 * 16 + in_unit * 8);
+      for (int i = 0; i < kI; ++i) s.x[i] = *reinterpret_cast<const u32x2*>(from + xsread + i * 64 * 16);
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const uint32_t*>(from + wsread + j * 32 * 16 + in_unit * 8);
-      } else {
+      for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const u32x2*>(from + wsread + j * 32 * 16);
+    } else if constexpr (kWMx) {
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const uint8_t*>(from + wsread + j * 32 * 16 + in_unit * 2);
-      }
+      for (int j = 0; j < kJ; ++j) s.w[j].x = *reinterpret_cast<const uint8_t*>(from + wsread + j * 32 * 8 + kPos * 2);
     }
   }
 
@@ -184,26 +213,25 @@ struct Body {
     }
   }
 
-  template <int kS>
+  template <int kPos, int kS>
   __device__ __forceinline__ void multiply(const Frags<kI, kJ>& f, const Scales& sc, int i, int j) {
     if constexpr (kXMx) {
       const i32x8 a{int(f.w[j].x), int(f.w[j].y), int(f.w[j].z), int(f.w[j].w), 0, 0, 0, 0};
       const i32x8 b{int(f.x[i].x), int(f.x[i].y), int(f.x[i].z), int(f.x[i].w), 0, 0, 0, 0};
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc[i][j], 4, 4, kS, int(sc.w[j]), kS, int(sc.x[i]));
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc[i][j], 4, 4, kS, int(sc.w[j][kPos]), kS, int(sc.x[i][kPos]));
     } else {
       acc[i][j] = mfma32(vec_bf16x8(f.w[j]), vec_bf16x8(f.x[i]), acc[i][j]);
     }
   }
 
-  // One sub-step: reads (and decodes) the next one's operands, multiplies its own,
-  // with `extra(n)` behind the n-th of its kI kJ instructions.
-  template <int kS, class Extra>
+  // One sub-step's kI kJ instructions, with `extra(n)` behind the n-th.
+  template <int kPos, int kS, class Extra>
   __device__ __forceinline__ void sub_step(const Frags<kI, kJ>& f, const Scales& sc, Extra&& extra) {
 #pragma unroll
     for (int j = 0; j < kJ; ++j)
 #pragma unroll
       for (int i = 0; i < kI; ++i) {
-        multiply<kS>(f, sc, i, j);
+        multiply<kPos, kS>(f, sc, i, j);
         extra(j * kI + i);
         pin();
       }
@@ -215,56 +243,62 @@ struct Body {
   // in bf16 8 % slower; over three or four sub-steps the last arrive too late).
   static constexpr int kFirst = S::kLoads / 2;
 
-  // The stage in `cur`, whose first operands are in `f` and scales in `sc`; `next`
-  // holds the one after it, and on return `f`, `sc` and `codes` are that stage's.
-  // `prev` is the slot whose last reader was the stage before.
-  __device__ __forceinline__ void stage(char* prev, char* cur, const char* next, char* scales, int st, Frags<kI, kJ>& f,
-                                        u32x4 (&codes)[kJ], Scales& sc) {
+  // Stage kPos of round u, in `cur`; its first operands are in `f`, its scales in `sc`.
+  // `next` holds the stage after it, and on return `f`, `sc` and `codes` are that
+  // stage's. `prev` is the slot whose last reader was the stage before.
+  template <int kPos>
+  __device__ __forceinline__ void stage(char* prev, char* cur, const char* next, const char* scales, int u,
+                                        Frags<kI, kJ>& f, u32x4 (&codes)[kJ], Scales& sc) {
     constexpr int kM = kI * kJ;
+    constexpr bool kLast = kPos == S::kSlots - 1;
+    constexpr int kNext = kLast ? 0 : kPos + 1;
+    const int u_next = kLast ? u + 1 : u;
     Frags<kI, kJ> g;
     auto decode = [&](Frags<kI, kJ>& to, const u32x4 (&from)[kJ], const Scales& s, int sub, int n) {
       // Fragment j's conversions behind instruction j kI (all of them early enough for the next sub-step).
       if constexpr (S::kDecode)
-        if (n % kI == 0) to.w[n / kI] = mx::decode8(from[n / kI][sub], mx::scale_f32(s.w[n / kI]));
+        if (n % kI == 0) to.w[n / kI] = mx::decode8(from[n / kI][sub], mx::scale_f32(s.w[n / kI].x));
     };
     auto copies = [&](char* slot, int first, int last, int n) {
       copy(slot, first + n * (last - first) / kM, first + (n + 1) * (last - first) / kM);
     };
-    if constexpr (kWMx) {
-      if (st % S::kUnitStages == 0) {
-        write_units(scales, st / S::kUnitStages + 1);
-        load_units(st / S::kUnitStages + 2);
-      }
-    }
+    // (Before each round of reads a wait for the last one, which has long arrived:
+    // the compiler would otherwise wait behind the new reads, for them too.)
+    reads_done();
     read(cur, 1, g);
     pin();
-    sub_step<0>(f, sc, [&](int n) {
+    sub_step<kPos, 0>(f, sc, [&](int n) {
       decode(g, codes, sc, 1, n);
       copies(prev, kFirst, S::kLoads, n);
     });
+    reads_done();
     read(cur, 2, f);
     pin();
-    sub_step<1>(g, sc, [&](int n) { decode(f, codes, sc, 2, n); });
+    sub_step<kPos, 1>(g, sc, [&](int n) { decode(f, codes, sc, 2, n); });
+    reads_done();
     read(cur, 3, g);
     pin();
-    sub_step<2>(f, sc, [&](int n) { decode(g, codes, sc, 3, n); });
+    sub_step<kPos, 2>(f, sc, [&](int n) { decode(g, codes, sc, 3, n); });
     // Every wave has read all of `cur`, and `next` has arrived: at most the copies
     // of the stages after it are still on their way.
-    __builtin_amdgcn_s_waitcnt(0xC07F);
+    reads_done();
     wait_vm<(S::kSlots - 2) * S::kLoads>();
     barrier_only();
     Scales su;
-    read_scales(scales, st + 1, su);
+    if constexpr (S::kDecode) read_scales<kNext>(scales, u_next, su);
     read(next, 0, f);
     u32x4 codes_next[kJ];
     read_codes(next, codes_next);
     pin();
-    sub_step<3>(g, sc, [&](int n) {
+    sub_step<kPos, 3>(g, sc, [&](int n) {
       copies(cur, 0, kFirst, n);
       decode(f, codes_next, su, 0, n);
     });
-    sc = su;
+    // (MXFP4 x: the next round's scales take the place of these, which the last
+    // instruction has read; the next one waits for LDS once a round.)
+    if constexpr (kXMx && kLast) read_scales<0>(scales, u_next, sc);
     if constexpr (S::kDecode) {
+      sc = su;
 #pragma unroll
       for (int j = 0; j < kJ; ++j) codes[j] = codes_next[j];
     }
@@ -279,41 +313,44 @@ struct Body {
     load_units(0);
     pin();
     copy(s0, 0, S::kLoads);
-    pin();
-    if constexpr (kWMx) write_units(scales, 0);
-    load_units(1);
-    pin();
     if constexpr (kN > 2) copy(s1, 0, S::kLoads);
     if constexpr (kN > 3) copy(s2, 0, S::kLoads);
     copy(kN == 2 ? s1 : kN == 3 ? s2 : s3, 0, kFirst);
     pin();
+    if constexpr (kWMx) write_units(scales, 0);
+    load_units(1);
     wait_vm<(kN - 2) * S::kLoads + kFirst>();
     lds_barrier();
     Scales sc;
-    read_scales(scales, 0, sc);
+    read_scales<0>(scales, 0, sc);
     Frags<kI, kJ> f;
     u32x4 codes[kJ];
     read(s0, 0, f);
     read_codes(s0, codes);
     if constexpr (S::kDecode) {
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) f.w[j] = mx::decode8(codes[j].x, mx::scale_f32(sc.w[j]));
+      for (int j = 0; j < kJ; ++j) f.w[j] = mx::decode8(codes[j].x, mx::scale_f32(sc.w[j].x));
     }
     // (The tall tiles run whole rounds of the ring, stages past the end on zeros: with
     // more than one way out of the loop the compiler moves their sums through scratch.)
     constexpr bool kWhole = kI * kJ > 4;
     char* const last = kN == 2 ? s1 : kN == 3 ? s2 : s3;
-    for (int st = 0; st < stages; st += kN) {
-      stage(last, s0, s1, scales, st, f, codes, sc);
+    for (int st = 0, u = 0; st < stages; st += kN, ++u) {
+      // The next round's scales, loaded a round ago, go to the other buffer (its last
+      // readers are behind the last barrier) and the loads of the one after it start.
+      if constexpr (kWMx) write_units(scales, u + 1);
+      load_units(u + 2);
+      pin();
+      stage<0>(last, s0, s1, scales, u, f, codes, sc);
       if (!kWhole && st + 1 >= stages) break;
-      stage(s0, s1, kN == 2 ? s0 : s2, scales, st + 1, f, codes, sc);
+      stage<1>(s0, s1, kN == 2 ? s0 : s2, scales, u, f, codes, sc);
       if constexpr (kN > 2) {
         if (!kWhole && st + 2 >= stages) break;
-        stage(s1, s2, kN == 3 ? s0 : s3, scales, st + 2, f, codes, sc);
+        stage<2>(s1, s2, kN == 3 ? s0 : s3, scales, u, f, codes, sc);
       }
       if constexpr (kN > 3) {
         if (!kWhole && st + 3 >= stages) break;
-        stage(s2, s3, s0, scales, st + 3, f, codes, sc);
+        stage<3>(s2, s3, s0, scales, u, f, codes, sc);
       }
     }
   }
@@ -333,16 +370,28 @@ struct Body {
     // sits at u ^ (r & 7), so that reads of one unit of consecutive rows meet no bank twice.
     const int r8 = lane >> 3;
     const int xat = ((lane & 7) ^ r8) * 16;
-#pragma unroll
-    for (int d = 0; d < S::kXCopies; ++d)
-      xsrc[d] = p.x + x_row_of(p, min(first + 8 * (d * 4 + wave) + r8, last)) * p.x_row + xat;
     const int64_t w0 = int64_t(seg.expert) * p.n;
     const int wr = S::kWRow == 128 ? r8 : lane >> 1;
     const int wat = S::kWRow == 128 ? xat : (lane & 1) * 16;
 #pragma unroll
-    for (int d = 0; d < S::kWCopies; ++d)
-      wsrc[d] = p.w + (w0 + weight_row(nt, ((d * 4 + wave) * (1024 / S::kWRow) + wr) % (64 * kJ))) * row_bytes_w + wat;
-
+    for (int d = 0; d < S::kXCopies; ++d) {
+      const int64_t row = x_row_of(p, min(first + 8 * (d * 4 + wave) + r8, last));
+      if constexpr (kXMx)
+        xrow[d] = uint32_t(row * p.x_row);
+      else
+        xsrc[d] = p.x + row * p.x_row + xat;
+    }
+#pragma unroll
+    for (int d = 0; d < S::kWCopies; ++d) {
+      const int row = weight_row(nt, ((d * 4 + wave) * (1024 / S::kWRow) + wr) % (64 * kJ));
+      if constexpr (kXMx)
+        wrow[d] = uint32_t(row) * uint32_t(row_bytes_w);
+      else
+        wsrc[d] = p.w + (w0 + row) * row_bytes_w + wat;
+    }
+    wfirst = p.w + w0 * row_bytes_w;
+    at = uint32_t(xat);
+    row_last = uint32_t(row_bytes_x) - 16;
     xleft = row_bytes_x - xat;
     wleft = row_bytes_w - wat;
 
@@ -353,11 +402,11 @@ struct Body {
     const int t = threadIdx.x;
     if constexpr (kXMx) {
       xscale = p.xs + x_row_of(p, min(first + t, last)) * blocks;
-      xsread = (32 * wm + c) * 16 + 4 * h;
+      xsread = (32 * wm + c) * 16 + 8 * h;
     }
     if constexpr (kWMx) {
       wscale = p.ws + (w0 + weight_row(nt, t % (64 * kJ))) * blocks;
-      wsread = (kXMx ? 64 * kI * 16 : 0) + (32 * kJ * wn + c) * 16 + (kXMx ? 4 : 1) * h;
+      wsread = (kXMx ? 64 * kI * 16 : 0) + (32 * kJ * wn + c) * S::kUnitBytes + (kXMx ? 8 : 1) * h;
     }
 #pragma unroll
     for (int i = 0; i < kI; ++i)

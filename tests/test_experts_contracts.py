@@ -107,3 +107,34 @@ def test_c_product_refusals(change, match):
     for name, value in change.items():
         setattr(a, name, value)
     refused(match, _lib.library().lf_expert_linear(ctypes.byref(a), None))
+
+
+def plan(**sizes):
+    a = _lib.ExpertProduct(**{**dict(x=16, w=16, y=16, x_rows=64, rows=64, n=4096, k=4096, experts=1), **sizes})
+    p = _lib.ExpertPlan()
+    _lib.check(_lib.library().lf_expert_linear_plan(ctypes.byref(a), ctypes.byref(p)))
+    return p
+
+
+def test_plans():
+    """Few rows stream the weights, many run in tiles, and what the tiles cannot take does not."""
+    for rows in (1, 8, 16):
+        assert plan(rows=rows, x_rows=rows, w_scales=16).kernel == _lib.LF_EXPERT_STREAM
+    for types in ({}, dict(w_scales=16), dict(w_scales=16, x_scales=16)):
+        p = plan(rows=4096, x_rows=4096, **types)
+        assert (p.kernel, p.rows, p.columns) == (_lib.LF_EXPERT_TILE, 256, 256)
+        spread = plan(rows=512, x_rows=512, experts=128, offsets=16, **types)
+        assert spread.kernel == _lib.LF_EXPERT_STREAM
+    assert plan(rows=4096, k=480, w_scales=16, x_scales=16).kernel == _lib.LF_EXPERT_STREAM
+    assert plan(rows=4096, k=96, w_scales=16).kernel == _lib.LF_EXPERT_STREAM
+    assert plan(rows=4096, x_rows=2**22, w_scales=16, x_scales=16).kernel == _lib.LF_EXPERT_STREAM
+    forced = _lib.ExpertPlan(_lib.LF_EXPERT_TILE, 256, 256)
+    a = _lib.ExpertProduct(x=16, x_scales=16, w=16, w_scales=16, y=16, x_rows=2, rows=2, n=32, k=480, experts=1, y_stride=32)
+    for p, match in ((forced, "cannot run in tiles"), (_lib.ExpertPlan(_lib.LF_EXPERT_TILE, 96, 256), "64, 128, 192 or 256 rows"),
+                     (_lib.ExpertPlan(_lib.LF_EXPERT_TILE, 64, 96), "columns"), (_lib.ExpertPlan(_lib.LF_EXPERT_STREAM, 0, 48), "columns"),
+                     (_lib.ExpertPlan(7, 64, 64), "tiles")):
+        a.k = 480 if p is forced else 512
+        a.plan = ctypes.pointer(p)
+        refused(match, _lib.library().lf_expert_linear(ctypes.byref(a), None))
+    a.plan, a.swiglu = ctypes.pointer(_lib.ExpertPlan(_lib.LF_EXPERT_TILE, 64, 64)), 1
+    refused("columns", _lib.library().lf_expert_linear(ctypes.byref(a), None))
