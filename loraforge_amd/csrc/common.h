@@ -65,7 +65,8 @@ __device__ __forceinline__ uint32_t f32_to_bf16(float a) { return pack_bf16x2(a,
 // fp32 -> nearest bf16 value, returned as fp32.
 __device__ __forceinline__ float round_bf16(float a) { return bf16_to_f32(f32_to_bf16(a)); }
 
-// silu(g) = g / (1 + e^-g) in fp32, as the reference's activation
+// bf16(silu(g)) * u in fp32 (the caller's store rounds the product to bf16),
+// silu(g) = g / (1 + e^-g) as the reference's activation
 // (benchmarks/qwen35_decode_silu.py:60-61), in about 13 instructions instead
 // of about 30 for expf and an IEEE division:
 //  - e^-g = 2^(t + lo) = 2^t (1 + lo ln 2) with t = fl(-c log2 e) and lo the
@@ -79,7 +80,10 @@ __device__ __forceinline__ float round_bf16(float a) { return bf16_to_f32(f32_to
 //    to d near 2^128), skipped where 1 + e^-g overflowed (g below about
 //    -88.7: silu -0, as g / inf) or the quotient is infinite; silu has the
 //    sign of g, which also keeps -0 for g = -0.
-__device__ __forceinline__ float silu_f32(float g) {
+// Every SwiGLU path (lf_swiglu and the fused decode and prefill epilogues)
+// uses this one function, so a fused activation and the linear followed by
+// lf_swiglu give identical bits.
+__device__ __forceinline__ float silu_times(float g, float u) {
   constexpr float kNegLog2eHi = -1.44269502162933349609375f;    // -log2(e) rounded to fp32
   constexpr float kNegLog2eLo = -1.925963033500011079e-08f;      // -log2(e) - kNegLog2eHi
   constexpr float kLn2 = 0.693147180559945309f;
@@ -93,14 +97,9 @@ __device__ __forceinline__ float silu_f32(float g) {
   const float r = __builtin_amdgcn_rcpf(ds);
   const float q = g * r;  // g / d / sc
   const bool refine = d < __builtin_huge_valf() && __builtin_fabsf(q) < __builtin_huge_valf();
-  return __builtin_copysignf((refine ? fmaf(fmaf(-q, ds, g), r, q) : q) * sc, g);
+  const float act = __builtin_copysignf((refine ? fmaf(fmaf(-q, ds, g), r, q) : q) * sc, g);
+  return round_bf16(act) * u;
 }
-
-// bf16(silu(g)) * u in fp32 (the caller's store rounds the product to bf16).
-// Every SwiGLU path of the NF4 linears (lf_swiglu and the fused decode and
-// prefill epilogues) uses this one function, so a fused activation and the
-// linear followed by lf_swiglu give identical bits.
-__device__ __forceinline__ float silu_times(float g, float u) { return round_bf16(silu_f32(g)) * u; }
 
 // One 16x16x32 bf16 MFMA step: acc[i = 4*(lane/16) + r][j = lane%16] +=
 // sum_k a[i][k] * b[k][j], where lane l supplies a[l%16][8*(l/16) .. +8)

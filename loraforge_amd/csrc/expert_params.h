@@ -77,8 +77,15 @@ __device__ __forceinline__ int64_t x_row_of(const Params& p, int pos) {
   return p.tokens ? min(max(p.tokens[pos], 0), p.x_rows - 1) : pos;
 }
 
-// SwiGLU in fp32: g / (1 + e^-g) * u, nothing rounded.
-__device__ __forceinline__ float silu_mul_f32(float g, float u) { return silu_f32(g) * u; }
+// SwiGLU in fp32: g / (1 + e^-g) * u from the hardware exp2 and reciprocal (1 ulp
+// each). The rounding of the exponent is worth |g| 2^-24 of the result, and past
+// g = -87.3 the reciprocal gives 0 for less than 1e-36: nothing beside the
+// rounding to bf16 that follows, at a third of the instructions of a correctly
+// rounded quotient (a 256 x 256 tile's epilogue 21.9k -> 12.5k cycles).
+__device__ __forceinline__ float silu_mul_f32(float g, float u) {
+  const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896341f);
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
 
 // `groups`: 16-row groups of weight rows per workgroup (1, 2 or 4).
 int launch_stream(const Params& p, int groups, hipStream_t stream);

@@ -448,14 +448,36 @@ struct Body {
       const int col = (nt * 2 + wn) * kColumns + part * 8;
       float add[8], add_up[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        add[e] = add_up[e] = 0.f;
-        if (p.bias) {
-          const uint16_t* bias = p.bias + int64_t(expert) * p.n + min(col + e, p.width - 1);
-          add[e] = bf16_to_f32(bias[0]);
-          if (kSwiglu) add_up[e] = bf16_to_f32(bias[p.width]);
+      for (int e = 0; e < 8; ++e) add[e] = add_up[e] = 0.f;
+      if (p.bias) {
+        const uint16_t* bias = p.bias + int64_t(expert) * p.n;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at = min(col + e, p.width - 1);
+          add[e] = bf16_to_f32(bias[at]);
+          if (kSwiglu) add_up[e] = bf16_to_f32(bias[at + p.width]);
         }
       }
+      const bool vec = p.y_vec && col + 8 <= p.width;
+      const bool all_vec = __ballot(!vec) == 0;
+      // Eight output columns of staged row r.
+      auto output = [&](int r) {
+        const f32x4* v = reinterpret_cast<const f32x4*>(mine + r * kRowBytes + local * 4);
+        const f32x4 half[2] = {v[0], v[1]};
+        f32x4 up[2];
+        if (kSwiglu) up[0] = v[8], up[1] = v[9];
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float a = half[e >> 1][(e & 1) * 2] + add[2 * e], b = half[e >> 1][(e & 1) * 2 + 1] + add[2 * e + 1];
+          if (kSwiglu) {
+            a = silu_mul_f32(a, up[e >> 1][(e & 1) * 2] + add_up[2 * e]);
+            b = silu_mul_f32(b, up[e >> 1][(e & 1) * 2 + 1] + add_up[2 * e + 1]);
+          }
+          o[e] = pack_bf16x2(a, b);
+        }
+        return u32x4{o[0], o[1], o[2], o[3]};
+      };
 #pragma unroll
       for (int pair = 0; pair < (kI + 1) / 2; ++pair) {
 #pragma unroll
@@ -470,26 +492,29 @@ struct Body {
                     f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
               }
         const int staged = min(2, kI - 2 * pair) * 32;
-#pragma unroll 4
-        for (int r0 = 0; r0 < staged; r0 += kRows) {
-          const int r = r0 + in_row;
-          const int row = (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31);
-          const float* v = reinterpret_cast<const float*>(mine + r * kRowBytes) + local;
-          float o[8];
+        auto place = [&](int r) { return (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31); };
+        if (all_vec) {
+          constexpr int kTogether = 32 / kRows < 4 ? 32 / kRows : 4;  // rows whose reads go out together
+#pragma unroll 1
+          for (int r0 = in_row; r0 < staged; r0 += kTogether * kRows) {
+            u32x4 o[kTogether];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            o[e] = v[e] + add[e];
-            if (kSwiglu) o[e] = silu_mul_f32(o[e], v[32 + e] + add_up[e]);
+            for (int k = 0; k < kTogether; ++k) o[k] = output(r0 + k * kRows);
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k) {
+              const int row = place(r0 + k * kRows);
+              if (row < count) *reinterpret_cast<u32x4*>(p.y + int64_t(first + row) * p.y_stride + col) = o[k];
+            }
           }
-          if (row >= count) continue;
-          uint16_t* y = p.y + int64_t(first + row) * p.y_stride + col;
-          const u32x4 packed{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])};
-          if (p.y_vec && col + 8 <= p.width) {
-            *reinterpret_cast<u32x4*>(y) = packed;
-          } else {
+        } else {
+#pragma unroll 1
+          for (int r = in_row; r < staged; r += kRows) {
+            const u32x4 o = output(r);
+            uint16_t* y = p.y + int64_t(first + place(r)) * p.y_stride + col;
+            if (place(r) >= count) continue;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (col + e < p.width) y[e] = uint16_t(packed[e >> 1] >> (16 * (e & 1)));
+              if (col + e < p.width) y[e] = uint16_t(o[e >> 1] >> (16 * (e & 1)));
           }
         }
       }
