@@ -249,6 +249,12 @@ _BOUND = (
     "lf_nf4_dequant",
     "lf_nf4_dequant_dq_checked",
     "lf_last_error",
+    "lf_mxfp4_quantize",
+    "lf_mxfp4_dequantize",
+    "lf_route_experts_workspace_size",
+    "lf_route_experts",
+    "lf_expert_linear",
+    "lf_combine_experts",
 )
 
 
@@ -257,12 +263,13 @@ def bind(module, **replaced) -> None:
     import torch
 
     from .ops.fused import LoraBatch
+    from .ops.mxfp4 import MXFP4Tensor
 
     stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
     device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
     lib = library()
     addresses = tuple(replaced.get(name) or ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _BOUND)
-    module.init(addresses, stream, device, ARCH_OK, WORKSPACES, COMPUTE_UNITS, LoraBatch)
+    module.init(addresses, stream, device, ARCH_OK, WORKSPACES, COMPUTE_UNITS, LoraBatch, MXFP4Tensor)
 
 
 def binding():

@@ -36,6 +36,12 @@ decltype(&lf_row_expand) g_expand;
 decltype(&lf_nf4_dequant) g_dequant;
 decltype(&lf_nf4_dequant_dq_checked) g_dequant_dq;
 decltype(&lf_last_error) g_last_error;
+decltype(&lf_mxfp4_quantize) g_mx_quantize;
+decltype(&lf_mxfp4_dequantize) g_mx_dequantize;
+decltype(&lf_route_experts_workspace_size) g_route_ws;
+decltype(&lf_route_experts) g_route;
+decltype(&lf_expert_linear) g_product;
+decltype(&lf_combine_experts) g_combine;
 
 PyObject* g_raw_stream;   // torch._C._cuda_getCurrentRawStream
 PyObject* g_get_device;   // torch._C._cuda_getDevice
@@ -43,11 +49,12 @@ PyObject* g_arch_ok;      // device index -> whether the kernels run there
 PyObject* g_workspaces;   // the operators' workspace cache
 PyObject* g_multi_cus;    // device index -> compute units
 PyObject* g_lora_batch;   // ops.fused.LoraBatch
+PyObject* g_mx_tensor;    // ops.mxfp4.MXFP4Tensor
 
 #define NAMES(X)                                                                                                     \
   X(absmax) X(shape) X(code) X(blocksize) X(quant_type) X(offset) X(state2) X(nested) X(_lf_prepared_scales)         \
   X(a_store) X(a_offsets) X(b_store) X(b_offsets) X(b_strides) X(ranks) X(scales) X(token_slots) X(slice_offsets)    \
-  X(max_rank) X(rows)
+  X(max_rank) X(rows) X(codes)
 #define DECL(n) PyObject* s_##n;
 NAMES(DECL)
 #undef DECL
@@ -598,16 +605,244 @@ PyObject* dequant_nested(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return THPVariable_Wrap(out);
 }
 
-// init(addresses, raw_stream, get_device, arch_ok, workspaces, compute_units, lora_batch)
+// ---- MXFP4 and experts ------------------------------------------------------
+
+constexpr int64_t kMxBlock = 32;
+
+// The tensors of an MXFP4Tensor (ops.mxfp4.packed's checks); k is its last dimension.
+struct MxArg {
+  PyObject* held[2] = {};
+  const at::Tensor* codes = nullptr;
+  const at::Tensor* scales = nullptr;
+  int64_t k = 0;
+  ~MxArg() {
+    for (PyObject* o : held) Py_XDECREF(o);
+  }
+  bool take(PyObject* o, int64_t dims = -1) {
+    if (reinterpret_cast<PyObject*>(Py_TYPE(o)) != g_mx_tensor) return false;
+    if (!(held[0] = PyObject_GetAttr(o, s_codes)) || !(held[1] = PyObject_GetAttr(o, s_scales))) return false;
+    codes = plain(held[0]);
+    scales = plain(held[1]);
+    if (!codes || !scales || codes->scalar_type() != at::kByte || scales->scalar_type() != at::kByte ||
+        codes->device() != scales->device() || codes->dim() < 1 || codes->dim() != scales->dim() ||
+        (dims >= 0 && codes->dim() != dims) || !codes->is_contiguous() || !scales->is_contiguous() || !aligned16(*codes))
+      return false;
+    k = codes->size(-1) * 2;
+    if (k == 0 || k % kMxBlock || scales->size(-1) != k / kMxBlock) return false;
+    for (int64_t d = 0; d < codes->dim(); ++d)
+      if (codes->size(d) >= (int64_t(1) << 31) || (d + 1 < codes->dim() && codes->size(d) != scales->size(d))) return false;
+    return true;
+  }
+};
+
+PyObject* pair_of(at::Tensor&& a, at::Tensor&& b) {
+  Ref x(THPVariable_Wrap(std::move(a))), y(THPVariable_Wrap(std::move(b)));
+  return x && y ? PyTuple_Pack(2, x.p, y.p) : nullptr;
+}
+
+// mx_quantize(x) -> (codes, scales) or None
+PyObject* mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 1) return decline();
+  const at::Tensor* x = plain(args[0]);
+  if (!x || x->dim() < 1 || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kFloat)) return decline();
+  const bool fp32 = x->scalar_type() == at::kFloat;
+  const int64_t k = x->size(-1);
+  if (k == 0 || k % kMxBlock || (x->dim() != 2 && !x->is_contiguous())) return decline();
+  const int64_t rows = x->numel() / k, stride = x->dim() == 2 && rows > 1 ? x->stride(0) : k;
+  if (rows == 0 || x->stride(-1) != 1 || stride < k || stride % (fp32 ? 4 : 8) || !aligned16(*x)) return decline();
+  void* stream;
+  if (!current(x->device(), &stream)) return decline();
+  std::vector<int64_t> sizes(x->sizes().begin(), x->sizes().end());
+  sizes.back() = k / 2;
+  at::Tensor codes = at::empty(sizes, x->options().dtype(at::kByte));
+  sizes.back() = k / kMxBlock;
+  at::Tensor scales = at::empty(sizes, x->options().dtype(at::kByte));
+  if (!on_gpu(codes) || !on_gpu(scales)) return decline();
+  const int rc = unlocked([&] {
+    return g_mx_quantize(x->data_ptr(), fp32, rows, k, stride, ptr<uint8_t>(&codes), ptr<uint8_t>(&scales), stream);
+  });
+  if (rc == LF_EINVAL) return decline();
+  if (rc != LF_OK) return failed();
+  return pair_of(std::move(codes), std::move(scales));
+}
+
+// mx_dequantize(t) -> values or None
+PyObject* mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  MxArg t;
+  if (nargs != 1 || !t.take(args[0]) || t.codes->numel() == 0) return decline();
+  void* stream;
+  if (!current(t.codes->device(), &stream)) return decline();
+  std::vector<int64_t> sizes(t.codes->sizes().begin(), t.codes->sizes().end());
+  sizes.back() = t.k;
+  at::Tensor out = at::empty(sizes, t.codes->options().dtype(at::kBFloat16));
+  if (!on_gpu(out)) return decline();
+  const int rc = unlocked([&] {
+    return g_mx_dequantize(ptr<uint8_t>(t.codes), ptr<uint8_t>(t.scales), out.numel() / kMxBlock, ptr<uint16_t>(&out), stream);
+  });
+  if (rc == LF_EINVAL) return decline();
+  if (rc != LF_OK) return failed();
+  return THPVariable_Wrap(std::move(out));
+}
+
+// product(x, weight, offsets or None, tokens or None, bias or None, swiglu) -> out or None:
+// mxfp4_linear (offsets None) and expert_linear with a fresh output.
+PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 6 || (args[5] != Py_True && args[5] != Py_False)) return decline();
+  const bool grouped = args[2] != Py_None, swiglu = args[5] == Py_True;
+  lf_expert_product a{};
+  MxArg wm, xm;
+  const at::Tensor* w = nullptr;
+  int64_t k;
+  if (reinterpret_cast<PyObject*>(Py_TYPE(args[1])) == g_mx_tensor) {
+    if (!wm.take(args[1], grouped ? 3 : 2)) return decline();
+    w = wm.codes;
+    k = wm.k;
+    a.w_scales = ptr<uint8_t>(wm.scales);
+  } else {
+    w = plain(args[1]);
+    if (!grouped || !w || w->dim() != 3 || w->scalar_type() != at::kBFloat16 || !w->is_contiguous() || !aligned16(*w))
+      return decline();
+    k = w->size(2);
+  }
+  const at::Device dev = w->device();
+  const int64_t experts = grouped ? w->size(0) : 1, n = w->size(-2);
+  if (n == 0 || k == 0 || experts == 0 || (swiglu && n % 2)) return decline();
+  const at::Tensor* x;
+  if (reinterpret_cast<PyObject*>(Py_TYPE(args[0])) == g_mx_tensor) {
+    if (!a.w_scales || !xm.take(args[0], 2) || xm.codes->device() != dev || xm.k != k) return decline();
+    x = xm.codes;
+    a.x_scales = ptr<uint8_t>(xm.scales);
+  } else {
+    x = matrix(args[0], dev);
+    if (!x || x->size(1) != k) return decline();
+    a.x_stride = x->size(0) > 1 ? x->stride(0) : k;
+    if (k % 8 || x->stride(1) != 1 || a.x_stride < k || a.x_stride % 8 || !aligned16(*x)) return decline();
+  }
+  a.x_rows = a.rows = x->size(0);
+  if (grouped) {
+    const at::Tensor* offsets = vec(args[2], at::kInt, dev, experts + 1);
+    if (!offsets) return decline();
+    a.offsets = ptr<int32_t>(offsets);
+    if (args[3] != Py_None) {
+      const at::Tensor* tokens = vec(args[3], at::kInt, dev);
+      if (!tokens) return decline();
+      a.tokens = ptr<int32_t>(tokens);
+      a.rows = tokens->numel();
+    }
+  } else if (args[3] != Py_None) {
+    return decline();
+  }
+  if (a.rows == 0 || a.x_rows == 0) return decline();
+  if (args[4] != Py_None) {
+    const at::Tensor* bias = plain(args[4]);
+    if (!bias || bias->scalar_type() != at::kBFloat16 || bias->device() != dev || !bias->is_contiguous() ||
+        bias->dim() != (grouped ? 2 : 1) || bias->size(-1) != n || (grouped && bias->size(0) != experts))
+      return decline();
+    a.bias = ptr<uint16_t>(bias);
+  }
+  void* stream;
+  if (!current(dev, &stream)) return decline();
+  const int64_t width = swiglu ? n / 2 : n;
+  at::Tensor out = at::empty({a.rows, width}, w->options().dtype(at::kBFloat16));
+  if (!on_gpu(out)) return decline();
+  a.x = x->data_ptr();
+  a.w = w->data_ptr();
+  a.y = ptr<uint16_t>(&out);
+  a.y_stride = width;
+  a.n = n;
+  a.k = k;
+  a.experts = experts;
+  a.swiglu = swiglu;
+  const int rc = unlocked([&] { return g_product(&a, stream); });
+  if (rc == LF_EINVAL) return decline();
+  if (rc != LF_OK) return failed();
+  return THPVariable_Wrap(std::move(out));
+}
+
+// route(logits, top_k, renormalize) -> (weights, experts, offsets, tokens, positions) or None
+PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 3 || (args[2] != Py_True && args[2] != Py_False)) return decline();
+  const at::Tensor* x = plain(args[0]);
+  if (!x || x->dim() != 2 || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kFloat)) return decline();
+  const int64_t count = x->size(0), experts = x->size(1);
+  long top;
+  if (experts < 1 || experts > 1024 || !small_int(args[1], 1, experts < 64 ? long(experts) : 64, &top)) return decline();
+  if (count == 0 || count * top >= (int64_t(1) << 31) - (int64_t(1) << 16) || x->stride(1) != 1) return decline();
+  const int64_t stride = count > 1 ? x->stride(0) : experts;
+  if (stride < experts) return decline();
+  void* stream;
+  if (!current(x->device(), &stream)) return decline();
+  const auto ints = x->options().dtype(at::kInt);
+  at::Tensor weights = at::empty({count, top}, x->options().dtype(at::kFloat));
+  at::Tensor chosen = at::empty({count, top}, ints), offsets = at::empty({experts + 1}, ints);
+  at::Tensor tokens = at::empty({count * top}, ints), positions = at::empty({count, top}, ints);
+  const int64_t need = g_route_ws(count, int32_t(experts));
+  at::Tensor scratch;
+  if (need) scratch = at::empty({need}, x->options().dtype(at::kByte));
+  for (const at::Tensor* t : {&weights, &chosen, &offsets, &tokens, &positions})
+    if (!on_gpu(*t)) return decline();
+  if (need && !on_gpu(scratch)) return decline();
+  const int rc = unlocked([&] {
+    return g_route(x->data_ptr(), x->scalar_type() == at::kFloat, count, int32_t(experts), stride, int32_t(top),
+                   args[2] == Py_True, ptr<float>(&weights), ptr<int32_t>(&chosen), ptr<int32_t>(&offsets),
+                   ptr<int32_t>(&tokens), ptr<int32_t>(&positions), need ? scratch.data_ptr() : nullptr, need, stream);
+  });
+  if (rc == LF_EINVAL) return decline();
+  if (rc != LF_OK) return failed();
+  Ref a(THPVariable_Wrap(std::move(weights))), b(THPVariable_Wrap(std::move(chosen))), c(THPVariable_Wrap(std::move(offsets)));
+  Ref d(THPVariable_Wrap(std::move(tokens))), e(THPVariable_Wrap(std::move(positions)));
+  return a && b && c && d && e ? PyTuple_Pack(5, a.p, b.p, c.p, d.p, e.p) : nullptr;
+}
+
+// combine(rows, positions, weights, base or None) -> out or None
+PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 4) return decline();
+  const at::Tensor* rows = plain(args[0]);
+  if (!rows) return decline();
+  const at::Device dev = rows->device();
+  rows = matrix(args[0], dev);
+  const at::Tensor* positions = plain(args[1]);
+  const at::Tensor* weights = plain(args[2]);
+  if (!rows || !positions || !weights || positions->dim() != 2 || positions->scalar_type() != at::kInt ||
+      weights->scalar_type() != at::kFloat || positions->device() != dev || weights->device() != dev ||
+      positions->sizes() != weights->sizes() || !positions->is_contiguous() || !weights->is_contiguous())
+    return decline();
+  const int64_t count = positions->size(0), top = positions->size(1), n = rows->size(1);
+  if (count == 0 || top < 1 || n < 1 || count >= (int64_t(1) << 31) || top >= (int64_t(1) << 31) || rows->numel() == 0)
+    return decline();
+  const int64_t rows_stride = rows->size(0) > 1 ? rows->stride(0) : n;
+  if (rows->stride(1) != 1 || rows_stride < n) return decline();
+  const at::Tensor* base = nullptr;
+  int64_t base_stride = 0;
+  if (args[3] != Py_None) {
+    base = matrix(args[3], dev);
+    if (!base || base->size(0) != count || base->size(1) != n || base->stride(1) != 1) return decline();
+    base_stride = count > 1 ? base->stride(0) : n;
+    if (base_stride < n) return decline();
+  }
+  void* stream;
+  if (!current(dev, &stream)) return decline();
+  at::Tensor out = at::empty({count, n}, rows->options());
+  if (!on_gpu(out)) return decline();
+  const int rc = unlocked([&] {
+    return g_combine(ptr<uint16_t>(rows), rows->size(0), rows_stride, ptr<int32_t>(positions), ptr<float>(weights), count,
+                     int32_t(top), n, ptr<uint16_t>(base), base_stride, ptr<uint16_t>(&out), n, stream);
+  });
+  if (rc == LF_EINVAL) return decline();
+  if (rc != LF_OK) return failed();
+  return THPVariable_Wrap(std::move(out));
+}
+
+// init(addresses, raw_stream, get_device, arch_ok, workspaces, compute_units, lora_batch, mx_tensor)
 PyObject* init(PyObject*, PyObject* args) {
-  PyObject *addresses, *raw, *dev, *arch, *ws, *cus, *batch;
-  if (!PyArg_ParseTuple(args, "O!OOO!O!O!O!", &PyTuple_Type, &addresses, &raw, &dev, &PyDict_Type, &arch, &PyDict_Type, &ws,
-                        &PyDict_Type, &cus, &PyType_Type, &batch))
+  PyObject *addresses, *raw, *dev, *arch, *ws, *cus, *batch, *packed;
+  if (!PyArg_ParseTuple(args, "O!OOO!O!O!O!O!", &PyTuple_Type, &addresses, &raw, &dev, &PyDict_Type, &arch, &PyDict_Type, &ws,
+                        &PyDict_Type, &cus, &PyType_Type, &batch, &PyType_Type, &packed))
     return nullptr;
-  constexpr int kEntries = 9;
+  constexpr int kEntries = 15;
   void* a[kEntries];
   if (PyTuple_GET_SIZE(addresses) != kEntries) {
-    PyErr_SetString(PyExc_ValueError, "nine entry points expected");
+    PyErr_SetString(PyExc_ValueError, "fifteen entry points expected");
     return nullptr;
   }
   for (int i = 0; i < kEntries; ++i)
@@ -624,13 +859,19 @@ PyObject* init(PyObject*, PyObject* args) {
   g_dequant = reinterpret_cast<decltype(g_dequant)>(a[6]);
   g_dequant_dq = reinterpret_cast<decltype(g_dequant_dq)>(a[7]);
   g_last_error = reinterpret_cast<decltype(g_last_error)>(a[8]);
+  g_mx_quantize = reinterpret_cast<decltype(g_mx_quantize)>(a[9]);
+  g_mx_dequantize = reinterpret_cast<decltype(g_mx_dequantize)>(a[10]);
+  g_route_ws = reinterpret_cast<decltype(g_route_ws)>(a[11]);
+  g_route = reinterpret_cast<decltype(g_route)>(a[12]);
+  g_product = reinterpret_cast<decltype(g_product)>(a[13]);
+  g_combine = reinterpret_cast<decltype(g_combine)>(a[14]);
 #define INTERN(n) \
   if (!s_##n && !(s_##n = PyUnicode_InternFromString(#n))) return nullptr;
   NAMES(INTERN)
 #undef INTERN
-  PyObject** slot[6] = {&g_raw_stream, &g_get_device, &g_arch_ok, &g_workspaces, &g_multi_cus, &g_lora_batch};
-  PyObject* value[6] = {raw, dev, arch, ws, cus, batch};
-  for (int i = 0; i < 6; ++i) {
+  PyObject** slot[7] = {&g_raw_stream, &g_get_device, &g_arch_ok, &g_workspaces, &g_multi_cus, &g_lora_batch, &g_mx_tensor};
+  PyObject* value[7] = {raw, dev, arch, ws, cus, batch, packed};
+  for (int i = 0; i < 7; ++i) {
     Py_INCREF(value[i]);
     Py_XDECREF(*slot[i]);
     *slot[i] = value[i];
@@ -654,6 +895,11 @@ PyMethodDef methods[] = {
     {"expand", reinterpret_cast<PyCFunction>(guarded<expand>), METH_FASTCALL, nullptr},
     {"dequant_nested", reinterpret_cast<PyCFunction>(guarded<dequant_nested>), METH_FASTCALL, nullptr},
     {"dequant", reinterpret_cast<PyCFunction>(guarded<dequant>), METH_FASTCALL, nullptr},
+    {"mx_quantize", reinterpret_cast<PyCFunction>(guarded<mx_quantize>), METH_FASTCALL, nullptr},
+    {"mx_dequantize", reinterpret_cast<PyCFunction>(guarded<mx_dequantize>), METH_FASTCALL, nullptr},
+    {"product", reinterpret_cast<PyCFunction>(guarded<product>), METH_FASTCALL, nullptr},
+    {"route", reinterpret_cast<PyCFunction>(guarded<route>), METH_FASTCALL, nullptr},
+    {"combine", reinterpret_cast<PyCFunction>(guarded<combine>), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

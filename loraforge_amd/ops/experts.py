@@ -56,6 +56,10 @@ def route_experts(logits, top_k: int, *, renormalize: bool = True) -> ExpertRout
     """
     import torch
 
+    if getattr(logits, "is_cuda", False):
+        done = _lib.binding().route(logits, top_k, renormalize)
+        if done is not None:
+            return ExpertRouting(*done)
     if not isinstance(logits, torch.Tensor):
         raise TypeError("logits must be a torch.Tensor")
     if logits.dtype not in (torch.bfloat16, torch.float32):
@@ -125,6 +129,10 @@ def combine_experts(rows, positions, weights, *, base=None, out=None):
     """
     import torch
 
+    if out is None and getattr(rows, "is_cuda", False):
+        done = _lib.binding().combine(rows, positions, weights, base)
+        if done is not None:
+            return done
     tensor(rows, "rows", 2, torch.bfloat16)
     tensor(positions, "positions", 2, torch.int32, rows.device)
     tensor(weights, "weights", 2, torch.float32, rows.device)

@@ -73,6 +73,10 @@ def quantize_mxfp4(x) -> MXFP4Tensor:
     """
     import torch
 
+    if getattr(x, "is_cuda", False):
+        done = _lib.binding().mx_quantize(x)
+        if done is not None:
+            return MXFP4Tensor(*done)
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a torch.Tensor")
     if x.ndim < 1 or x.dtype not in (torch.bfloat16, torch.float32):
@@ -112,6 +116,10 @@ def dequantize_mxfp4(t: MXFP4Tensor, *, out=None):
 
     if not isinstance(t, MXFP4Tensor):
         raise TypeError("t must be an MXFP4Tensor")
+    if out is None and getattr(t.codes, "is_cuda", False):
+        done = _lib.binding().mx_dequantize(t)
+        if done is not None:
+            return done
     shape = packed(t, "t", t.ndim)
     if out is None:
         out = torch.empty(shape, dtype=torch.bfloat16, device=t.device)
@@ -137,6 +145,10 @@ def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out, plan=None
 
     grouped = experts is not None
     quantised = isinstance(weight, MXFP4Tensor)
+    if out is None and plan is None and (offsets is not None) == grouped and getattr(weight.codes if quantised else weight, "is_cuda", False):
+        done = _lib.binding().product(x, weight, offsets, tokens, bias, swiglu)
+        if done is not None:
+            return done
     if quantised:
         shape = packed(weight, "weight", 3 if grouped else 2)
         device = weight.device
