@@ -81,7 +81,7 @@ class Plan(ctypes.Structure):
     _fields_ = [("kernel", c_int32), ("tile_rows", c_int32), ("z_parts", c_int32), ("z_launch", c_int32)]
 
 
-LF_EXPERT_STREAM, LF_EXPERT_TILE = range(2)
+LF_EXPERT_STREAM, LF_EXPERT_TILE, LF_EXPERT_ROWS = range(3)
 
 
 class ExpertPlan(ctypes.Structure):

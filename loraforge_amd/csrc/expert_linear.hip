@@ -15,6 +15,9 @@ bool tiles_fit(const lf_expert_product& a) {
   return !a.w_scales || a.k >= 128;
 }
 
+// Scales are loaded 16 at a time.
+bool rows_fit(const lf_expert_product& a) { return !a.w_scales || a.k >= 512; }
+
 lf_expert_plan plan_of(const lf_expert_product& a) {
   const int64_t used = a.offsets ? std::min(a.experts, a.rows) : 1;
   const int64_t width = a.swiglu ? a.n / 2 : a.n;
@@ -78,6 +81,10 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   if (plan.kernel == LF_EXPERT_STREAM) {
     LF_REQUIRE(plan.columns == 16 || plan.columns == 32 || plan.columns == 64, "stream plan: 16, 32 or 64 columns");
     return lf::expert::launch_stream(p, plan.columns / 16, s);
+  }
+  if (plan.kernel == LF_EXPERT_ROWS) {
+    LF_REQUIRE(lf::expert::rows_fit(*a), "this product cannot run with a wave for 16 weight rows");
+    return lf::expert::launch_rows(p, s);
   }
   LF_REQUIRE(plan.kernel == LF_EXPERT_TILE && lf::expert::tiles_fit(*a), "this product cannot run in tiles");
   LF_REQUIRE(plan.rows >= 64 && plan.rows <= 256 && plan.rows % 64 == 0, "tile plan: 64, 128, 192 or 256 rows");

@@ -158,20 +158,11 @@ struct Body {
       wunit.w = uint32_t(min(want + 4 - hi, 4));
     }
   }
-  // v without its first `bytes` (0 .. 16), zeros behind.
-  static __device__ __forceinline__ u32x4 drop_bytes(u32x4 v, int bytes) {
-    if (bytes & 16) v = u32x4{0u, 0u, 0u, 0u};
-    v = bytes & 8 ? u32x4{v.z, v.w, 0u, 0u} : v;
-    v = bytes & 4 ? u32x4{v.y, v.z, v.w, 0u} : v;
-    const int b = bytes & 3;
-    return u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, b), __builtin_amdgcn_alignbyte(v.z, v.y, b),
-                 __builtin_amdgcn_alignbyte(v.w, v.z, b), __builtin_amdgcn_alignbyte(0u, v.w, b)};
-  }
   __device__ __forceinline__ void write_units(char* scales, int u) const {
     char* to = scales + (u & 1) * (S::kScaleBytes / 2) + threadIdx.x * S::kUnitBytes;
     if constexpr (kXMx) {
       // (The two stages' dwords of a lane half side by side.)
-      const u32x4 x = drop_bytes(xunit, unit_skip), w = drop_bytes(wunit, unit_skip);
+      const u32x4 x = mx::drop_bytes(xunit, unit_skip), w = mx::drop_bytes(wunit, unit_skip);
       if (kI == 4 || threadIdx.x < 64 * kI) *reinterpret_cast<u32x4*>(to) = u32x4{x.x, x.z, x.y, x.w};
       if (kJ == 4 || threadIdx.x < 64 * kJ) *reinterpret_cast<u32x4*>(to + 64 * kI * 16) = u32x4{w.x, w.z, w.y, w.w};
     } else if constexpr (kWMx) {

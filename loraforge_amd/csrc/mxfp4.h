@@ -39,5 +39,15 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t magnitude) {
   return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
 }
 
+// v without its first `bytes` (0 .. 16), zeros behind.
+__device__ __forceinline__ u32x4 drop_bytes(u32x4 v, int bytes) {
+  if (bytes & 16) v = u32x4{0u, 0u, 0u, 0u};
+  v = bytes & 8 ? u32x4{v.z, v.w, 0u, 0u} : v;
+  v = bytes & 4 ? u32x4{v.y, v.z, v.w, 0u} : v;
+  const int b = bytes & 3;
+  return u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, b), __builtin_amdgcn_alignbyte(v.z, v.y, b),
+               __builtin_amdgcn_alignbyte(v.w, v.z, b), __builtin_amdgcn_alignbyte(0u, v.w, b)};
+}
+
 }  // namespace mx
 }  // namespace lf

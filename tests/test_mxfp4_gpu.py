@@ -297,7 +297,7 @@ def test_products_on_a_side_stream_and_in_a_graph(device):
 # --------------------------------------------------------------------------
 
 TYPES = [("bf16", "bf16"), ("bf16", "mxfp4"), ("mxfp4", "mxfp4")]
-PLANS = [(_lib.LF_EXPERT_STREAM, 0, c) for c in (16, 32, 64)] + [
+PLANS = [(_lib.LF_EXPERT_STREAM, 0, c) for c in (16, 32, 64)] + [(_lib.LF_EXPERT_ROWS, 0, 128)] + [
     (_lib.LF_EXPERT_TILE, r, c) for r in (64, 128, 192, 256) for c in (64, 128, 256)]
 
 
@@ -312,8 +312,8 @@ def forced(x, w, plan, **options):
 def test_every_plan(types, plan, k, device):
     """Ragged experts on one kernel: tile heights of one to four 64-row steps, ends of k inside a stage, edge columns."""
     act, weight = types
-    if act == "mxfp4" and plan[0] == _lib.LF_EXPERT_TILE and k < 512:
-        k += 512  # (the tiles take MXFP4 x from 512 on)
+    if k < 512 and ((act == "mxfp4" and plan[0] == _lib.LF_EXPERT_TILE) or (weight == "mxfp4" and plan[0] == _lib.LF_EXPERT_ROWS)):
+        k += 512  # (what these kernels take begins there)
     counts = [130, 0, 1, 64, 257, 33, 190]
     n = 328
     rows = sum(counts)
@@ -329,7 +329,7 @@ def test_every_plan(types, plan, k, device):
 
 
 @pytest.mark.parametrize("types", TYPES, ids="-".join)
-@pytest.mark.parametrize("plan", [p for p in PLANS if p[2] > 64 or p[0] == _lib.LF_EXPERT_STREAM], ids=lambda p: "-".join(map(str, p)))
+@pytest.mark.parametrize("plan", [p for p in PLANS if p[2] > 64 or p[0] != _lib.LF_EXPERT_TILE], ids=lambda p: "-".join(map(str, p)))
 @pytest.mark.parametrize("n", [512, 776, 88])
 def test_every_plan_swiglu(types, plan, n, device):
     act, weight = types
@@ -359,9 +359,9 @@ def test_tiles_of_one_dense_product(types, columns, device):
         assert torch.equal(forced(x, w, (_lib.LF_EXPERT_TILE, rows, columns), experts=1, offsets=whole), y)
 
 
-@pytest.mark.parametrize("plan", [(_lib.LF_EXPERT_STREAM, 0, 32), (_lib.LF_EXPERT_TILE, 256, 256)], ids=str)
+@pytest.mark.parametrize("plan", [(_lib.LF_EXPERT_STREAM, 0, 32), (_lib.LF_EXPERT_ROWS, 0, 128), (_lib.LF_EXPERT_TILE, 256, 256)], ids=str)
 def test_output_rows_of_any_alignment(plan, device):
-    m, n, k = 200, 256, 256
+    m, n, k = 200, 256, 576
     x, xv = operand(randn(42, m, k), "bf16", device)
     w, wv = operand(randn(43, n, k, std=0.05), "mxfp4", device)
     expected = ox.product(xv, wv)
@@ -391,6 +391,6 @@ def test_scales_and_rows_at_odd_addresses(types, device):
     if weight == "mxfp4":
         w = MXFP4Tensor(w.codes, shifted(w.scales))
     tokens = torch.arange(m - 1, -1, -1, dtype=torch.int32, device=device)
-    for plan in PLANS[2], PLANS[-1], PLANS[3]:
+    for plan in PLANS[2], PLANS[-1], PLANS[3], PLANS[4]:
         y = forced(x, w, plan, experts=1, offsets=segments([m]).to(device), tokens=tokens)
         close(y, *ox.product(xv[::-1], wv[0]))
