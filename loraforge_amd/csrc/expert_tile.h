@@ -42,14 +42,18 @@ struct Shape {
   // (A copy per wave at least: 64 rows of 32 bytes go twice.)
   static constexpr int kXBytes = 64 * kI * kXRow, kWBytes = 64 * kJ * kWRow < 4096 ? 4096 : 64 * kJ * kWRow;
   static constexpr int kStage = kXBytes + kWBytes;
-  // Scales go through LDS in units of one round of the ring, two buffers. MXFP4 x:
-  // 16 bytes (two stages) of every x and weight row; beside bf16 x 8 of every weight row.
+  // (Deeper for small tiles of MXFP4 x, whose two stages a unit of scales are soon
+  // through: 1024 tokens over 64 experts 4096 x 2048 in 64 x 128 tiles 165 -> 140 us;
+  // bf16 x gains nothing, its small tiles wait for LDS reads.)
+  static constexpr int kMost = kXMx && kI * kJ <= 3 ? 8 : 4;
+  // Scales go through LDS in units, two buffers. MXFP4 x: 16 bytes (two stages) of
+  // every x and weight row; beside bf16 x a round of the ring, up to 8 bytes of every weight row.
   static constexpr int kScaleRows = (kXMx ? 64 * kI : 0) + (kWMx ? 64 * kJ : 0);
   static constexpr int kUnitBytes = kXMx ? 16 : 8;
   static constexpr int kScaleBytes = 2 * kUnitBytes * kScaleRows;
-  static constexpr int kFit = (kLds - kScaleBytes) / kStage;
-  static constexpr int kSlots = kXMx ? 2 : kFit >= 4 ? 4 : kFit;
-  static_assert(kFit >= kSlots && kSlots >= 2, "two stages have to fit");
+  static constexpr int kFit = (kLds - kScaleBytes) / kStage < kMost ? (kLds - kScaleBytes) / kStage : kMost;
+  static constexpr int kSlots = kXMx ? kFit / 2 * 2 : kFit;
+  static_assert(kSlots >= 2, "two stages have to fit");
   static constexpr int kXCopies = kXBytes / 4096, kWCopies = kWBytes / 4096;  // per wave
   static constexpr int kLoads = kXCopies + kWCopies;
 };
@@ -90,7 +94,7 @@ struct Body {
   // Scales: the rows this thread loads, their next unit, and where it reads fragment 0's.
   const uint8_t *xscale, *wscale;
   u32x4 xunit, wunit;
-  int unit_skip;
+  int unit_skip, skips[2];
   int xsread, wsread;
   f32x16 acc[kI][kJ];
 
@@ -136,7 +140,7 @@ struct Body {
     }
   }
 
-  // Loads the scales of round u (at any alignment): blocks 16 u .. of the thread's x
+  // Loads the scales of unit u (at any alignment): blocks 16 u .. of the thread's x
   // and weight row (k >= 512), or 2 kSlots u .. of its weight row (k >= 128). Nothing
   // past the row is read: towards its end the last bytes that can be, and
   // write_units moves them into place, with zeros past the end of k. No
@@ -151,11 +155,12 @@ struct Body {
       if (kI == 4 || threadIdx.x < 64 * kI) xunit = *reinterpret_cast<const u32x4u*>(xscale + from);
       if (kJ == 4 || threadIdx.x < 64 * kJ) wunit = *reinterpret_cast<const u32x4u*>(wscale + from);
     } else if constexpr (kWMx) {
-      const int want = 2 * S::kSlots * u, lo = min(want, blocks - 4), hi = min(want + 4, blocks - 4);
-      wunit.x = *reinterpret_cast<const u32u*>(wscale + lo);
-      wunit.y = *reinterpret_cast<const u32u*>(wscale + hi);
-      wunit.z = uint32_t(min(want - lo, 4));
-      wunit.w = uint32_t(min(want + 4 - hi, 4));
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const int want = 2 * S::kSlots * u + 4 * d, from = min(want, blocks - 4);
+        wunit[d] = *reinterpret_cast<const u32u*>(wscale + from);
+        skips[d] = min(want - from, 4);
+      }
     }
   }
   __device__ __forceinline__ void write_units(char* scales, int u) const {
@@ -167,10 +172,11 @@ struct Body {
       if (kJ == 4 || threadIdx.x < 64 * kJ) *reinterpret_cast<u32x4*>(to + 64 * kI * 16) = u32x4{w.x, w.z, w.y, w.w};
     } else if constexpr (kWMx) {
       if (kJ == 4 || threadIdx.x < 64 * kJ)
-        *reinterpret_cast<u32x2*>(to) = u32x2{uint32_t(uint64_t(wunit.x) >> (8 * wunit.z)), uint32_t(uint64_t(wunit.y) >> (8 * wunit.w))};
+        *reinterpret_cast<u32x2*>(to) =
+            u32x2{uint32_t(uint64_t(wunit.x) >> (8 * skips[0])), uint32_t(uint64_t(wunit.y) >> (8 * skips[1]))};
     }
   }
-  // Scales of stage kPos of round u. MXFP4 x: both stages' at once (kPos 0).
+  // Scales of a stage at place kPos of unit u. MXFP4 x: both stages' of the unit at once (kPos 0).
   template <int kPos>
   __device__ __forceinline__ void read_scales(const char* scales, int u, Scales& s) const {
     const char* from = scales + (u & 1) * (S::kScaleBytes / 2);
@@ -181,7 +187,7 @@ struct Body {
       for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const u32x2*>(from + wsread + j * 32 * 16);
     } else if constexpr (kWMx) {
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) s.w[j].x = *reinterpret_cast<const uint8_t*>(from + wsread + j * 32 * 8 + kPos * 2);
+      for (int j = 0; j < kJ; ++j) s.w[j].x = *reinterpret_cast<const uint8_t*>(from + wsread + j * 32 * S::kUnitBytes + kPos * 2);
     }
   }
 
@@ -209,7 +215,7 @@ struct Body {
     if constexpr (kXMx) {
       const i32x8 a{int(f.w[j].x), int(f.w[j].y), int(f.w[j].z), int(f.w[j].w), 0, 0, 0, 0};
       const i32x8 b{int(f.x[i].x), int(f.x[i].y), int(f.x[i].z), int(f.x[i].w), 0, 0, 0, 0};
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc[i][j], 4, 4, kS, int(sc.w[j][kPos]), kS, int(sc.x[i][kPos]));
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc[i][j], 4, 4, kS, int(sc.w[j][kPos & 1]), kS, int(sc.x[i][kPos & 1]));
     } else {
       acc[i][j] = mfma32(vec_bf16x8(f.w[j]), vec_bf16x8(f.x[i]), acc[i][j]);
     }
@@ -238,12 +244,20 @@ struct Body {
   // `next` holds the stage after it, and on return `f`, `sc` and `codes` are that
   // stage's. `prev` is the slot whose last reader was the stage before.
   template <int kPos>
-  __device__ __forceinline__ void stage(char* prev, char* cur, const char* next, const char* scales, int u,
+  __device__ __forceinline__ void stage(char* prev, char* cur, const char* next, char* scales, int u,
                                         Frags<kI, kJ>& f, u32x4 (&codes)[kJ], Scales& sc) {
     constexpr int kM = kI * kJ;
     constexpr bool kLast = kPos == S::kSlots - 1;
     constexpr int kNext = kLast ? 0 : kPos + 1;
     const int u_next = kLast ? u + 1 : u;
+    // At the start of a unit the next one's scales, loaded a unit ago, go to the other
+    // buffer (its last readers are behind the last barrier) and the loads of the one after it start.
+    if constexpr (kWMx && (kXMx ? kPos % 2 == 0 : kPos == 0)) {
+      const int unit = kXMx ? u * (S::kSlots / 2) + kPos / 2 : u;
+      write_units(scales, unit + 1);
+      load_units(unit + 2);
+      pin();
+    }
     Frags<kI, kJ> g;
     auto decode = [&](Frags<kI, kJ>& to, const u32x4 (&from)[kJ], const Scales& s, int sub, int n) {
       // Fragment j's conversions behind instruction j kI (all of them early enough for the next sub-step).
@@ -287,7 +301,7 @@ struct Body {
     });
     // (MXFP4 x: the next round's scales take the place of these, which the last
     // instruction has read; the next one waits for LDS once a round.)
-    if constexpr (kXMx && kLast) read_scales<0>(scales, u_next, sc);
+    if constexpr (kXMx && kPos % 2 == 1) read_scales<0>(scales, u * (S::kSlots / 2) + kPos / 2 + 1, sc);
     if constexpr (S::kDecode) {
       sc = su;
 #pragma unroll
@@ -299,14 +313,15 @@ struct Body {
   // that reads of one do not depend on the copies into another (it would wait
   // for every copy in flight before each read).
   __device__ __forceinline__ void ring(char* __restrict__ s0, char* __restrict__ s1, char* __restrict__ s2,
-                                       char* __restrict__ s3, char* __restrict__ scales) {
+                                       char* __restrict__ s3, char* __restrict__ s4, char* __restrict__ s5,
+                                       char* __restrict__ s6, char* __restrict__ s7, char* __restrict__ scales) {
     constexpr int kN = S::kSlots;
+    char* const slot[8] = {s0, s1, s2, s3, s4, s5, s6, s7};
     load_units(0);
     pin();
-    copy(s0, 0, S::kLoads);
-    if constexpr (kN > 2) copy(s1, 0, S::kLoads);
-    if constexpr (kN > 3) copy(s2, 0, S::kLoads);
-    copy(kN == 2 ? s1 : kN == 3 ? s2 : s3, 0, kFirst);
+#pragma unroll
+    for (int n = 0; n < kN - 1; ++n) copy(slot[n], 0, S::kLoads);
+    copy(slot[kN - 1], 0, kFirst);
     pin();
     if constexpr (kWMx) write_units(scales, 0);
     load_units(1);
@@ -322,27 +337,24 @@ struct Body {
 #pragma unroll
       for (int j = 0; j < kJ; ++j) f.w[j] = mx::decode8(codes[j].x, mx::scale_f32(sc.w[j].x));
     }
-    // (The tall tiles run whole rounds of the ring, stages past the end on zeros: with
+    // (The larger tiles run whole rounds of the ring, stages past the end on zeros: with
     // more than one way out of the loop the compiler moves their sums through scratch.)
-    constexpr bool kWhole = kI * kJ > 4;
-    char* const last = kN == 2 ? s1 : kN == 3 ? s2 : s3;
+    constexpr bool kWhole = kI * kJ > 3;
     for (int st = 0, u = 0; st < stages; st += kN, ++u) {
-      // The next round's scales, loaded a round ago, go to the other buffer (its last
-      // readers are behind the last barrier) and the loads of the one after it start.
-      if constexpr (kWMx) write_units(scales, u + 1);
-      load_units(u + 2);
-      pin();
-      stage<0>(last, s0, s1, scales, u, f, codes, sc);
-      if (!kWhole && st + 1 >= stages) break;
-      stage<1>(s0, s1, kN == 2 ? s0 : s2, scales, u, f, codes, sc);
-      if constexpr (kN > 2) {
-        if (!kWhole && st + 2 >= stages) break;
-        stage<2>(s1, s2, kN == 3 ? s0 : s3, scales, u, f, codes, sc);
-      }
-      if constexpr (kN > 3) {
-        if (!kWhole && st + 3 >= stages) break;
-        stage<3>(s2, s3, s0, scales, u, f, codes, sc);
-      }
+#define LF_STAGE(n)                                                                                                  \
+  if constexpr (kN > n) {                                                                                            \
+    if (!kWhole && n > 0 && st + n >= stages) break;                                                                  \
+    stage<n>(slot[(n + kN - 1) % kN], slot[n], slot[(n + 1) % kN], scales, u, f, codes, sc);                          \
+  }
+      LF_STAGE(0)
+      LF_STAGE(1)
+      LF_STAGE(2)
+      LF_STAGE(3)
+      LF_STAGE(4)
+      LF_STAGE(5)
+      LF_STAGE(6)
+      LF_STAGE(7)
+#undef LF_STAGE
     }
   }
 
@@ -406,8 +418,8 @@ struct Body {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    ring(lds, lds + S::kStage, lds + (S::kSlots > 2 ? 2 : 0) * S::kStage, lds + (S::kSlots > 3 ? 3 : 0) * S::kStage,
-         lds + S::kSlots * S::kStage);
+    auto slot = [&](int n) { return lds + (n < S::kSlots ? n : 0) * S::kStage; };
+    ring(slot(0), slot(1), slot(2), slot(3), slot(4), slot(5), slot(6), slot(7), lds + S::kSlots * S::kStage);
 
     // Copies of zeros for stages past the end are still on their way, and other
     // waves read their last operands.
