@@ -1,5 +1,7 @@
 // C entry point of the products with bf16 or MXFP4 weights: checks and choice of kernel.
 #include <algorithm>
+#include <cmath>
+#include <limits>
 
 #include "expert_params.h"
 #include "../../include/loraforge_amd.h"
@@ -18,21 +20,113 @@ bool tiles_fit(const lf_expert_product& a) {
 // Scales are loaded 16 at a time.
 bool rows_fit(const lf_expert_product& a) { return !a.w_scales || a.k >= 512; }
 
+// Times of the kernels in us, fitted to 2319 products (dense ones of 1..4096 rows,
+// n 1024..24576, k 1024..8192; 8..128 experts, 1..8192 tokens), every plan of each.
+struct Costs {
+  struct Tile {
+    float fixed, stage, busy;  // of a tile, of a stage (64 k; 256 k of MXFP4 x), and what all CUs at work add to a stage
+  } tile[4][3];                // [rows / 64 - 1][64, 128, 256 columns]
+  struct Rows {
+    float fixed, pass, k, k_busy;  // of the launch, of a pass of 16 rows, of 1024 k of it, and what two workgroups on every CU add
+  } rows;
+  struct Stream {
+    float fixed, pass, k, k_tile, k_busy, k_tile_busy;  // the same, with a part for each 16-row tile of a pass (at most 64 rows)
+  } stream[2];                                           // [16, 32 columns]
+};
+constexpr Costs kCosts[3] = {
+    // bf16 x and weights
+    {{
+         {{4.51f, 0.241f, 0.084f}, {5.23f, 0.315f, 0.187f}, {5.56f, 0.439f, 0.293f}},
+         {{5.37f, 0.326f, 0.083f}, {6.07f, 0.313f, 0.230f}, {8.41f, 0.597f, 0.318f}},
+         {{6.18f, 0.413f, 0.089f}, {7.58f, 0.421f, 0.238f}, {8.21f, 0.881f, 0.421f}},
+         {{6.67f, 0.406f, 0.152f}, {9.83f, 0.545f, 0.310f}, {10.18f, 1.077f, 0.564f}}},
+     {1.86f, 0.45f, 3.02f, 18.43f},
+     {{1.35f, 1.97f, 0.24f, 0.78f, 0.78f, 1.02f},
+      {2.56f, 0.00f, 0.75f, 1.03f, 5.86f, 0.41f}}},
+    // bf16 x, MXFP4 weights
+    {{
+         {{4.65f, 0.287f, 0.045f}, {5.16f, 0.378f, 0.050f}, {5.71f, 0.478f, 0.132f}},
+         {{5.43f, 0.375f, 0.047f}, {5.81f, 0.442f, 0.082f}, {7.62f, 0.694f, 0.151f}},
+         {{6.45f, 0.466f, 0.058f}, {7.21f, 0.577f, 0.092f}, {9.59f, 0.928f, 0.136f}},
+         {{6.82f, 0.525f, 0.100f}, {8.83f, 0.705f, 0.150f}, {13.41f, 1.165f, 0.259f}}},
+     {1.60f, 1.88f, 1.90f, 4.12f},
+     {{1.54f, 1.51f, 0.00f, 0.74f, 0.00f, 1.06f},
+      {1.39f, 2.12f, 0.21f, 0.84f, 0.18f, 1.30f}}},
+    // MXFP4 x and weights
+    {{
+         {{5.11f, 0.295f, 0.171f}, {5.50f, 0.459f, 0.318f}, {4.96f, 0.661f, 0.642f}},
+         {{5.76f, 0.452f, 0.222f}, {6.43f, 0.477f, 0.245f}, {6.77f, 0.800f, 0.566f}},
+         {{6.04f, 0.588f, 0.217f}, {6.06f, 0.789f, 0.394f}, {8.63f, 1.022f, 0.416f}},
+         {{5.10f, 0.707f, 0.381f}, {6.93f, 0.862f, 0.424f}, {10.53f, 1.254f, 0.562f}}},
+     {2.31f, 1.60f, 1.06f, 4.09f},
+     {{1.52f, 1.76f, 0.09f, 0.36f, 0.37f, 0.48f},
+      {1.40f, 2.14f, 0.34f, 0.45f, 0.83f, 0.49f}}},
+};
+
+constexpr double kCus = 256;
+
+// Passes that rows take `cap` at a time: of a dense product, or of experts whose rows
+// are spread about their average as popularity spreads them (exponentially).
+double passes(double each, double cap, bool grouped) {
+  return grouped ? 1.0 / (1.0 - std::exp(-cap / each)) : std::ceil(each / cap);
+}
+
+double tile_us(const Costs& c, int rows, int columns, double each, double used, bool grouped, double width, double stages) {
+  const double per = passes(each, rows, grouped);
+  const double height = std::min(rows / 64.0, std::max(1.0, grouped ? each / per / 64.0 + 0.5 : std::ceil(std::ceil(each / per) / 64.0)));
+  const int low = std::min(3, int(height)), high = std::min(4, low + 1), j = columns == 64 ? 0 : columns == 128 ? 1 : 2;
+  const double part = height - low;
+  auto mix = [&](float Costs::Tile::*m) { return (1.0 - part) * (c.tile[low - 1][j].*m) + part * (c.tile[high - 1][j].*m); };
+  const double fixed = mix(&Costs::Tile::fixed), stage = mix(&Costs::Tile::stage), busy = mix(&Costs::Tile::busy);
+  const double tiles = used * per * std::ceil(width / columns);
+  if (tiles <= kCus) return fixed + stages * (stage + busy * tiles / kCus);
+  constexpr double kLaunch = 3.0;
+  const double round = fixed - kLaunch + stages * (stage + busy);
+  if (grouped) return kLaunch + (tiles / kCus + 0.5) * round;
+  const double full = std::floor(tiles / kCus), rest = tiles / kCus - full;
+  return kLaunch + full * round + (rest > 0 ? fixed - kLaunch + stages * (stage + busy * rest) : 0.0);
+}
+
+// The plan of least time. (Against the fastest plan of each of those products: 1.4 to
+// 2.9 % slower on average by type, 58 % at most: 64 experts of 512 tokens, n and k 1024.)
 lf_expert_plan plan_of(const lf_expert_product& a) {
-  const int64_t used = a.offsets ? std::min(a.experts, a.rows) : 1;
-  const int64_t width = a.swiglu ? a.n / 2 : a.n;
-  const int64_t each = (a.rows + used - 1) / used;  // rows of an expert, on average
-  lf_expert_plan plan{};
-  if (each > 32 && tiles_fit(a)) {
-    plan.kernel = LF_EXPERT_TILE;
-    plan.rows = int32_t(std::min<int64_t>(256, (each + 63) / 64 * 64));
-    plan.columns = 256;
-    return plan;
+  const Costs& c = kCosts[a.x_scales ? 2 : a.w_scales ? 1 : 0];
+  const bool grouped = a.offsets != nullptr && a.experts > 1;
+  const double rows = double(a.rows), experts = double(a.experts);
+  const double used = grouped ? experts * (1.0 - std::pow(1.0 - 1.0 / experts, rows)) : 1.0;
+  const double each = rows / used;  // rows of an expert that has any, on average
+  const double n = double(a.n), k = double(a.k) / 1024.0;
+  lf_expert_plan best{LF_EXPERT_STREAM, 0, 16};
+  double least = std::numeric_limits<double>::infinity();
+  // (No plan is faster than the used weights through HBM; of those that are at it, the one with less work.
+  // bf16 weights of few rows come at 4.3 TB/s in tiles, 4.9 a wave for 16 of them, 5.5 streamed.)
+  const double hbm = used * n * double(a.k) * (a.w_scales ? 17.0 / 32.0 : 2.0) * 1e-6;
+  auto offer = [&](double us, lf_expert_plan plan) {
+    const double rate = a.w_scales || plan.kernel == LF_EXPERT_STREAM ? 5.5 : plan.kernel == LF_EXPERT_ROWS ? 4.9 : 4.3;
+    us = std::max(us, hbm / rate) + 0.1 * us;
+    if (us < least) least = us, best = plan;
+  };
+  for (int i = 0; i < 2; ++i) {
+    const Costs::Stream& s = c.stream[i];
+    const double groups = std::ceil(n / (16 << i)) * used / 512.0, busy = std::min(1.0, groups);
+    const double tiles = std::min(4.0, grouped ? std::max(1.0, each / 16.0 + 0.5) : each <= 16 ? 1.0 : each <= 32 ? 2.0 : 4.0);
+    offer(s.fixed + passes(each, 64, grouped) * (s.pass + k * (s.k + s.k_tile * tiles + (s.k_busy + s.k_tile_busy * tiles) * busy)) *
+                        std::max(1.0, groups),
+          {LF_EXPERT_STREAM, 0, 16 << i});
   }
-  plan.kernel = LF_EXPERT_STREAM;
-  const int64_t groups = (width + (a.swiglu ? 7 : 15)) / (a.swiglu ? 8 : 16) * used;
-  plan.columns = groups >= 4 * 512 ? 64 : groups >= 2 * 512 ? 32 : 16;
-  return plan;
+  if (rows_fit(a)) {
+    const double groups = std::ceil(n / 128.0) * used / 512.0;
+    offer(c.rows.fixed + passes(each, 16, grouped) * (c.rows.pass + k * (c.rows.k + c.rows.k_busy * std::min(1.0, groups))) *
+                             std::max(1.0, groups),
+          {LF_EXPERT_ROWS, 0, 128});
+  }
+  if (tiles_fit(a)) {
+    const double stage_k = a.x_scales ? 256.0 : 64.0;
+    for (int height = 64; height <= 256; height += 64)
+      for (int columns = a.swiglu ? 128 : 64; columns <= 256; columns *= 2)
+        offer(tile_us(c, height, columns, each, used, grouped, n, std::ceil(double(a.k) / stage_k)), {LF_EXPERT_TILE, height, columns});
+  }
+  return best;
 }
 
 }  // namespace
@@ -79,7 +173,7 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   const lf_expert_plan plan = a->plan ? *a->plan : lf::expert::plan_of(*a);
   auto s = static_cast<hipStream_t>(stream);
   if (plan.kernel == LF_EXPERT_STREAM) {
-    LF_REQUIRE(plan.columns == 16 || plan.columns == 32 || plan.columns == 64, "stream plan: 16, 32 or 64 columns");
+    LF_REQUIRE(plan.columns == 16 || plan.columns == 32, "stream plan: 16 or 32 columns");
     return lf::expert::launch_stream(p, plan.columns / 16, s);
   }
   if (plan.kernel == LF_EXPERT_ROWS) {

@@ -87,7 +87,7 @@ __device__ __forceinline__ float silu_mul_f32(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
-// `groups`: 16-row groups of weight rows per workgroup (1, 2 or 4).
+// `groups`: 16-row groups of weight rows per workgroup (1 or 2).
 int launch_stream(const Params& p, int groups, hipStream_t stream);
 int launch_rows(const Params& p, hipStream_t stream);
 // Tiles of at most `cap` rows x `columns` weight rows (one translation unit per pair of types).

@@ -6,7 +6,7 @@
 // whole 128-byte row pieces: fragments loaded straight into the operand layout
 // (16 rows, one per lane) take the address unit 64 cycles a load, four times a copy's, and
 // bounded the kernel that splits k over its waves (expert_stream.hip) at 3.9 TB/s (24
-// tokens over 64 experts, top 4, 4096 x 4096 with SwiGLU: 114 us); this one takes 88.
+// tokens over 64 experts, top 4, 4096 x 4096 with SwiGLU: 114 us); this one takes 72.
 //
 // Each wave streams its weights through a ring of three stages (16 rows x 128 bytes:
 // 256 k in MXFP4, 64 in bf16) without meeting the others; x comes in chunks of 8 KiB
@@ -29,10 +29,6 @@ constexpr int kXBytes = 8192;         // bytes of an x chunk
 constexpr int kScaleStages = 8;       // stages per unit of scales (2048 k, 64 bytes of a row)
 constexpr int kScaleUnit = 16 * 64;   // bytes of a unit of 16 rows
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ i32x8 fp4_operand(const u32x4& v) {
-  return i32x8{int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
-}
 
 // LDS accesses of the stage loop, each block with its own wait: the compiler would
 // wait for every copy in flight before an LDS access of its own.
@@ -187,8 +183,8 @@ struct Rows {
         const uint32_t at[4] = {slot + wread[0], slot + wread[1], x_base + xread[0][0], x_base + xread[1][0]};
         lds_four(v, at, 0);
         if constexpr (kXMx) {
-          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(v[0]), fp4_operand(v[2]), acc, 4, 4, 0, wscale, 0, xscale);
-          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(v[1]), fp4_operand(v[3]), acc, 4, 4, 1, wscale, 1, xscale);
+          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx::operand(v[0]), mx::operand(v[2]), acc, 4, 4, 0, wscale, 0, xscale);
+          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx::operand(v[1]), mx::operand(v[3]), acc, 4, 4, 1, wscale, 1, xscale);
         } else {
           acc = mfma16(vec_bf16x8(v[0]), vec_bf16x8(v[2]), acc);
           acc = mfma16(vec_bf16x8(v[1]), vec_bf16x8(v[3]), acc);

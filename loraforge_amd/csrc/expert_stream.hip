@@ -21,12 +21,8 @@ namespace {
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kStep = 128;   // k per step
-constexpr int kTiles = 8;    // most 16 x 16 tiles of a workgroup's pass: 64 KiB of partial sums
+constexpr int kRowTiles = 4;  // most 16-row tiles of a pass
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ i32x8 fp4_operand(const u32x4& v) {
-  return i32x8{int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
-}
 
 __device__ __forceinline__ u32x4 load16(const char* p) { return *reinterpret_cast<const u32x4*>(p); }
 
@@ -80,7 +76,7 @@ __device__ __forceinline__ void contract(const Rows<kWMx, kF>& w, const Rows<kXM
     if constexpr (kXMx) {
 #pragma unroll
       for (int t = 0; t < kT; ++t)
-        acc[f][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(w.v[f][0]), fp4_operand(x.v[t][0]), acc[f][t],
+        acc[f][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx::operand(w.v[f][0]), mx::operand(x.v[t][0]), acc[f][t],
                                                                      4, 4, 0, w.scale[f], 0, x.scale[t]);
     } else {
 #pragma unroll
@@ -122,9 +118,10 @@ __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg,
 #pragma unroll
     for (int t = 0; t < kT; ++t) acc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Steps requested together: as many as 64 registers hold.
-  constexpr int kRegs = (kWMx ? 5 : 16) * kF + (kXMx ? 5 : 16) * kT;
-  constexpr int kDepth = kRegs <= 16 ? 4 : kRegs <= 32 ? 2 : 1;
+  // Steps requested together: as many as fit 128 registers, two workgroups a CU (an
+  // MXFP4 row takes nine with its scale and addresses).
+  constexpr int kRegs = (kWMx ? 9 : 16) * kF + (kXMx ? 9 : 16) * kT;
+  constexpr int kDepth = kRegs <= 18 ? 4 : kRegs <= 36 ? 2 : 1;
   const int steps = (p.k + kStep - 1) / kStep;
   for (int s = wave; s < steps; s += kDepth * kWaves) {
     Rows<kWMx, kF> wr[kDepth];
@@ -172,18 +169,17 @@ __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg,
 // Grid: column blocks x experts that have rows.
 template <bool kXMx, bool kWMx, int kF>
 __global__ __launch_bounds__(kThreads, 4) void stream_kernel(Params p) {
-  __shared__ float red[kWaves * kTiles * 256];
+  __shared__ float red[kWaves * kF * kRowTiles * 256];
   int index = blockIdx.y;
   const Segment seg = find_segment(p, index, [](const Segment& s) { return s.end > s.begin ? 1 : 0; });
   const int rows = seg.end - seg.begin;
   if (rows <= 0) return;
   if (rows <= 16) {
     stream_rows<kXMx, kWMx, kF, 1>(p, seg, seg.begin, blockIdx.x, red);
-  } else if (kF == 4 || rows <= 32) {
-    for (int first = seg.begin; first < seg.end; first += 32) stream_rows<kXMx, kWMx, kF, 2>(p, seg, first, blockIdx.x, red);
+  } else if (rows <= 32) {
+    stream_rows<kXMx, kWMx, kF, 2>(p, seg, seg.begin, blockIdx.x, red);
   } else {
-    for (int first = seg.begin; first < seg.end; first += 64)
-      stream_rows<kXMx, kWMx, kF, kF == 4 ? 2 : 4>(p, seg, first, blockIdx.x, red);
+    for (int first = seg.begin; first < seg.end; first += 64) stream_rows<kXMx, kWMx, kF, 4>(p, seg, first, blockIdx.x, red);
   }
 }
 
@@ -192,9 +188,7 @@ int launch_types(const Params& p, int groups, hipStream_t stream) {
   const int segments = p.offsets ? (p.experts < p.rows ? p.experts : p.rows) : 1;
   const int64_t columns = (p.swiglu ? 8 : 16) * groups;
   const dim3 grid(unsigned((p.width + columns - 1) / columns), unsigned(segments)), threads(kThreads);
-  if (groups == 4)
-    hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 4>), grid, threads, 0, stream, p);
-  else if (groups == 2)
+  if (groups == 2)
     hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 2>), grid, threads, 0, stream, p);
   else
     hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 1>), grid, threads, 0, stream, p);

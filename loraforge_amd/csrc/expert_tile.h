@@ -32,8 +32,6 @@ constexpr int kLds = 160 * 1024;
 constexpr int kSubSteps = 4;
 constexpr int kXRow = 128;  // bytes of an x row per stage
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
 template <bool kXMx, bool kWMx, int kI, int kJ>
 struct Shape {
   static constexpr bool kDecode = kWMx && !kXMx;           // MXFP4 weights for bf16 x
@@ -213,9 +211,8 @@ struct Body {
   template <int kPos, int kS>
   __device__ __forceinline__ void multiply(const Frags<kI, kJ>& f, const Scales& sc, int i, int j) {
     if constexpr (kXMx) {
-      const i32x8 a{int(f.w[j].x), int(f.w[j].y), int(f.w[j].z), int(f.w[j].w), 0, 0, 0, 0};
-      const i32x8 b{int(f.x[i].x), int(f.x[i].y), int(f.x[i].z), int(f.x[i].w), 0, 0, 0, 0};
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc[i][j], 4, 4, kS, int(sc.w[j][kPos & 1]), kS, int(sc.x[i][kPos & 1]));
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx::operand(f.w[j]), mx::operand(f.x[i]), acc[i][j], 4, 4, kS,
+                                                                    int(sc.w[j][kPos & 1]), kS, int(sc.x[i][kPos & 1]));
     } else {
       acc[i][j] = mfma32(vec_bf16x8(f.w[j]), vec_bf16x8(f.x[i]), acc[i][j]);
     }

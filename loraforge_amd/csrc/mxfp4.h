@@ -26,6 +26,14 @@ __device__ __forceinline__ uint32_t decode2(uint32_t codes, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, kSel));
 }
 
+// 32 packed codes as an operand of the scaled matrix instructions (of 4-bit operands they read four registers).
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ i32x8 operand(const u32x4& codes) {
+  const i32x4 v = __builtin_bit_cast(i32x4, codes);
+  return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+}
+
 // Eight packed codes as eight bf16 values.
 __device__ __forceinline__ u32x4 decode8(uint32_t codes, float scale) {
   return u32x4{decode2<0>(codes, scale), decode2<1>(codes, scale), decode2<2>(codes, scale), decode2<3>(codes, scale)};
