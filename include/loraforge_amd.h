@@ -336,7 +336,8 @@ int lf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t blo
  * choices sorted by expert, then by token and choice: offsets int32 [experts +
  * 1], token_of int32 [tokens * top] (the token at each place, -1 from
  * offsets[experts] on), positions int32 [tokens, top] (the place of each choice,
- * -1 beside -1). experts 1..1024, top 1..64; the workspace need not be cleared.
+ * -1 beside -1). experts 1..1024, top 1..64; the workspace is 16-byte aligned and
+ * need not be cleared.
  *
  * lf_expert_linear: y[p] = x[tokens[p]] w[e]^T (+ bias[e]) for every place p of
  * offsets[e] .. offsets[e + 1] (tokens NULL: x[p]); fp32 sums, rounded once.

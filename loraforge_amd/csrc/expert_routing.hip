@@ -16,6 +16,7 @@
 namespace lf {
 namespace {
 
+constexpr int kSmallThreads = 1024;   // a few tokens, all in one workgroup
 constexpr int kChooseThreads = 512;
 constexpr int kOrderThreads = 1024;
 constexpr int kMaxExperts = 1024;
@@ -30,148 +31,143 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k); }
 
-template <int kCtrl, int kRows>
-__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
-  return max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), kCtrl, kRows, 0xf, false)));
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), kCtrl, 0xf, 0xf, false));
 }
-// Largest value over the wave, uniform.
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-  v = dpp_max<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: lane 15 of each row holds its maximum
-  v = dpp_max<0x112, 0xf>(v);
-  v = dpp_max<0x114, 0xf>(v);
-  v = dpp_max<0x118, 0xf>(v);
-  v = dpp_max<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
-  v = dpp_max<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
-  return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
+// `op` over the kLanes lanes that share a token (16 or 64), the result in each of
+// them: rotations within a row of 16 lanes, then the four rows, in a fixed order.
+template <int kLanes, class Op>
+__device__ __forceinline__ uint32_t across(uint32_t v, Op op) {
+  v = op(v, dpp<0x128>(v));
+  v = op(v, dpp<0x124>(v));
+  v = op(v, dpp<0x122>(v));
+  v = op(v, dpp<0x121>(v));
+  if constexpr (kLanes == 64) {
+    auto row = [&](int lane) { return uint32_t(__builtin_amdgcn_readlane(int(v), lane)); };
+    v = op(op(row(0), row(16)), op(row(32), row(48)));
+  }
+  return v;
+}
+template <int kLanes>
+__device__ __forceinline__ uint32_t max_across(uint32_t v) {
+  return across<kLanes>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+template <int kLanes>
+__device__ __forceinline__ float sum_across(float v) {
+  return __uint_as_float(across<kLanes>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
 }
 
 struct RouteParams {
   const void* logits;
   int64_t stride;
   int32_t fp32, tokens, experts, top, renormalize;
-  int32_t chunk;   // tokens per chunk
+  int32_t chunk;     // tokens per chunk
   int32_t chunks;
+  int32_t row;       // counts of a chunk, a multiple of four
   float* weights;    // [tokens, top]
   int32_t* chosen;   // [tokens, top]
   int32_t* offsets;  // [experts + 1]
   int32_t* token_of; // [tokens * top]
   int32_t* positions;// [tokens, top]
-  int32_t* counts;   // [chunks, experts]
+  int32_t* counts;   // [chunks, row]
 };
 
-// The choices of one token, by one wave: lane l holds experts [l kPer, (l + 1) kPer).
-template <int kPer>
-__device__ __forceinline__ void choose_token(const RouteParams& p, int t, int* hist) {
-  const int lane = threadIdx.x & 63;
+// The choices of the token of these kLanes lanes; lane l of them holds experts l,
+// l + kLanes, ... and at the end choice l (-1: none), whose weight it stores.
+// k rounds of a maximum over keys in the order of the logits. A bf16 key leaves 16 bits
+// for the expert (lowest first), so one maximum finds both; fp32 takes a second one.
+template <bool kFp32, int kLanes, int kPer>
+__device__ __forceinline__ int choose(const RouteParams& p, int t, bool live) {
+  const int lane = threadIdx.x & (kLanes - 1);
   uint32_t key[kPer];
   float value[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = lane + i * kLanes;
+    const int64_t at = int64_t(t) * p.stride + e;
+    value[i] = -__builtin_huge_valf();
+    if (live && e < p.experts)
+      value[i] = kFp32 ? static_cast<const float*>(p.logits)[at] : bf16_to_f32(static_cast<const uint16_t*>(p.logits)[at]);
+  }
   bool odd = false;  // NaN or +inf
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int e = lane * kPer + i;
-    float v = -__builtin_huge_valf();
-    if (e < p.experts)
-      v = p.fp32 ? static_cast<const float*>(p.logits)[int64_t(t) * p.stride + e]
-                 : bf16_to_f32(static_cast<const uint16_t*>(p.logits)[int64_t(t) * p.stride + e]);
-    value[i] = v;
-    key[i] = order_key(v);
-    odd |= !(v < __builtin_huge_valf());
+    key[i] = order_key(value[i]);
+    if (!kFp32 && key[i]) key[i] = (key[i] & 0xffff0000u) | uint32_t(0xffff - (lane + i * kLanes));
+    odd |= !(value[i] < __builtin_huge_valf());
   }
-  const bool bad = __ballot(odd) != 0;
-  uint32_t best = 0;
-  int at = 0;
+  const uint64_t odd_lanes = __ballot(odd);
+  const bool bad = (kLanes == 64 ? odd_lanes : (odd_lanes >> (threadIdx.x & 48)) & 0xffff) != 0;
+  uint32_t my_key = 0, top_key = 0;
   int my_expert = -1;
-  uint32_t my_key = 0;
-  uint32_t top_key = 0;
   for (int j = 0; j < p.top; ++j) {
-    best = key[0];
-    at = 0;
+    uint32_t best = key[0];
 #pragma unroll
-    for (int i = 1; i < kPer; ++i)
-      if (key[i] > best) best = key[i], at = i;
-    const uint32_t m = wave_max(best);
-    if (m == 0) break;  // nothing allowed is left
-    if (j == 0) top_key = m;
-    const int owner = __builtin_ctzll(__ballot(best == m));
-    const int e = owner * kPer + __builtin_amdgcn_readlane(at, owner);
-    if (lane == j) my_expert = e, my_key = m;
-    if (lane == owner) {
+    for (int i = 1; i < kPer; ++i) best = max(best, key[i]);
+    best = max_across<kLanes>(best);
+    int e = 0xffff - int(best & 0xffff);
+    if constexpr (kFp32) {
+      uint32_t last = 0;  // of the experts that have it, the lowest: ~e largest
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i == at) key[i] = 0;
+      for (int i = 0; i < kPer; ++i) last = max(last, key[i] == best ? ~uint32_t(lane + i * kLanes) : 0u);
+      e = int(~max_across<kLanes>(last));
     }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (kFp32 ? e - lane == i * kLanes : key[i] == best) key[i] = 0;
+    if (!kFp32) best = best >> 31 ? best & 0xffff0000u : best | (best ? 0xffffu : 0u);
+    if (j == 0) top_key = best;
+    if (lane == j && best) my_expert = e, my_key = best;
   }
   const float peak = key_value(top_key);
   float share = my_expert >= 0 ? expf(key_value(my_key) - peak) : 0.0f;
-  float total = 0.0f;
-  if (p.renormalize) {
-    total = wave_sum(share);
-  } else {
+  float total = share;
+  if (!p.renormalize) {
+    total = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) total += value[i] > -__builtin_huge_valf() ? expf(value[i] - peak) : 0.0f;
-    total = wave_sum(total);
   }
-  if (lane < p.top) {
+  total = sum_across<kLanes>(total);
+  if (live && lane < p.top) {
     float w = my_expert >= 0 ? share / total : 0.0f;
     if (bad && my_expert >= 0) w = __builtin_nanf("");
     p.weights[int64_t(t) * p.top + lane] = w;
     p.chosen[int64_t(t) * p.top + lane] = my_expert;
-    if (my_expert >= 0) atomicAdd(&hist[my_expert], 1);
   }
+  return my_expert;
 }
 
-__device__ __forceinline__ void choose_chunk(const RouteParams& p, int first, int last, int* hist) {
-  const int waves = blockDim.x >> 6;
-  for (int t = first + int(threadIdx.x >> 6); t < last; t += waves) {
-    if (p.experts <= 64) choose_token<1>(p, t, hist);
-    else if (p.experts <= 128) choose_token<2>(p, t, hist);
-    else if (p.experts <= 256) choose_token<4>(p, t, hist);
-    else choose_token<16>(p, t, hist);
-  }
-}
-
-// Places of a chunk's choices: base[e] is the place of the chunk's first choice of
-// expert e. 1024 choices a pass, in order: a wave finds the earlier choices of the
-// same expert among its 64 by comparing the experts' bits, and adds the counts of
-// the waves before it.
-__device__ __forceinline__ void place_chunk(const RouteParams& p, int first, int last, int* base, int* wave_counts) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int begin = first * p.top, end = last * p.top;
-  for (int at = begin; at < end; at += blockDim.x) {
-    for (int i = threadIdx.x; i < waves * p.experts; i += blockDim.x) wave_counts[i] = 0;
+// Chooses for tokens [first, last), as many at once as the workgroup has lanes for (64 at most),
+// and hands place(token, choice, expert, earlier) each choice with the count of earlier
+// tokens of [first, last) that have the same expert (-1, 0: none). A token chooses an expert
+// once, so a pass' choices of an expert are a mask of its tokens: no order of atomics shows.
+// run[e] counts an expert's choices so far.
+template <bool kFp32, int kLanes, int kPer, class Place>
+__device__ __forceinline__ void choose_range(const RouteParams& p, int first, int last, unsigned long long* mask, int* run, Place place) {
+  constexpr int kMost = 64;  // tokens of a mask
+  const int slot = threadIdx.x / kLanes, slots = min(kMost, int(blockDim.x) / kLanes);
+  const int lane = threadIdx.x & (kLanes - 1);
+  for (int at = first; at < last; at += slots) {
+    for (int e = threadIdx.x; e < p.experts; e += blockDim.x) mask[e] = 0;
     __syncthreads();
-    const int i = at + int(threadIdx.x);
-    const int e = i < end ? p.chosen[i] : -1;
-    uint64_t same = __ballot(e >= 0);
-    for (int bit = 1; bit < p.experts; bit <<= 1) {
-      const uint64_t has = __ballot((e & bit) != 0);
-      same &= (e & bit) ? has : ~has;
-    }
-    const int before = __popcll(same & ((uint64_t(1) << lane) - 1));
-    if (e >= 0 && before == 0) wave_counts[wave * p.experts + e] = __popcll(same);
+    const int t = at + slot;
+    const bool live = slot < slots && t < last;
+    int e = -1;
+    if (at + int(threadIdx.x & ~63u) / kLanes < last) e = choose<kFp32, kLanes, kPer>(p, t, live);  // (a wave as a whole)
+    if (live && e >= 0) atomicOr(&mask[e], 1ull << slot);
     __syncthreads();
-    if (i < end) {
-      int place = -1;
-      if (e >= 0) {
-        place = base[e] + before;
-        for (int w = 0; w < wave; ++w) place += wave_counts[w * p.experts + e];
-        p.token_of[place] = i / p.top;
-      }
-      p.positions[i] = place;
-    }
+    if (live && lane < p.top) place(t, lane, e, e >= 0 ? run[e] + __popcll(mask[e] & ((1ull << slot) - 1)) : 0);
     __syncthreads();
-    for (int x = threadIdx.x; x < p.experts; x += blockDim.x) {
-      int sum = 0;
-      for (int w = 0; w < waves; ++w) sum += wave_counts[w * p.experts + x];
-      base[x] += sum;
-    }
+    for (int x = threadIdx.x; x < p.experts; x += blockDim.x) run[x] += __popcll(mask[x]);
     __syncthreads();
   }
 }
 
-// Exclusive sums of count[0 .. n) in LDS, in place; returns the total.
-__device__ int scan_counts(int* count, int n) {
-  __shared__ int wave_total[kOrderThreads / 64];
+// Exclusive sums of count[0 .. n), n <= the threads, in place; returns the total.
+__device__ int scan_counts(int* count, int n, int* wave_total) {
   const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
   const int mine = i < n ? count[i] : 0;
   int sum = mine;
@@ -183,7 +179,7 @@ __device__ int scan_counts(int* count, int n) {
   if (lane == 63) wave_total[wave] = sum;
   __syncthreads();
   int before = 0, total = 0;
-  for (int w = 0; w < int(blockDim.x >> 6); ++w) {
+  for (int w = 0; w < (n + 63) >> 6; ++w) {
     if (w < wave) before += wave_total[w];
     total += wave_total[w];
   }
@@ -192,78 +188,117 @@ __device__ int scan_counts(int* count, int n) {
   return total;
 }
 
-__device__ __forceinline__ void fill_rest(const RouteParams& p, int total, int part, int parts) {
-  const int64_t end = int64_t(p.tokens) * p.top;
-  for (int64_t i = total + int64_t(part) * blockDim.x + threadIdx.x; i < end; i += int64_t(parts) * blockDim.x) p.token_of[i] = -1;
-}
-
-// A few tokens: the whole routing in one workgroup.
-__global__ __launch_bounds__(kOrderThreads) void route_small_kernel(RouteParams p) {
-  extern __shared__ int lds[];
-  int* base = lds;                        // [experts]
-  int* wave_counts = lds + p.experts;     // [16, experts]
-  for (int e = threadIdx.x; e < p.experts; e += kOrderThreads) base[e] = 0;
-  __syncthreads();
-  choose_chunk(p, 0, p.tokens, base);
-  __syncthreads();
-  const int total = scan_counts(base, p.experts);
-  for (int e = threadIdx.x; e < p.experts; e += kOrderThreads) p.offsets[e] = base[e];
-  if (threadIdx.x == 0) p.offsets[p.experts] = total;
-  fill_rest(p, total, 0, 1);
-  __syncthreads();  // (place_chunk reads choices that other waves of this workgroup stored)
-  place_chunk(p, 0, p.tokens, base, wave_counts);
-}
-
-__global__ __launch_bounds__(kChooseThreads) void route_choose_kernel(RouteParams p) {
-  extern __shared__ int lds[];
-  for (int e = threadIdx.x; e < p.experts; e += kChooseThreads) lds[e] = 0;
-  __syncthreads();
-  const int first = blockIdx.x * p.chunk;
-  choose_chunk(p, first, min(first + p.chunk, p.tokens), lds);
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.experts; e += kChooseThreads) p.counts[int64_t(blockIdx.x) * p.experts + e] = lds[e];
-}
-
-__global__ __launch_bounds__(kOrderThreads) void route_order_kernel(RouteParams p) {
-  extern __shared__ int lds[];
-  int* base = lds;                      // [experts]: all choices of an expert, then its first place
-  int* mine = lds + p.experts;          // [experts]: those of the chunks before this one
-  int* wave_counts = lds + 2 * p.experts;
-  for (int e = threadIdx.x; e < 2 * p.experts; e += kOrderThreads) lds[e] = 0;
-  __syncthreads();
-  // A thread sums some chunks of one expert.
-  const int parts = max(1, kOrderThreads / p.experts);
-  for (int i = threadIdx.x; i < p.experts * parts; i += kOrderThreads) {
-    const int e = i % p.experts, part = i / p.experts;
-    int all = 0, before = 0;
-    for (int c = part; c < p.chunks; c += parts) {
-      const int v = p.counts[int64_t(c) * p.experts + e];
-      all += v;
-      before += c < int(blockIdx.x) ? v : 0;
-    }
-    atomicAdd(&base[e], all);
-    atomicAdd(&mine[e], before);
-  }
-  __syncthreads();
-  const int total = scan_counts(base, p.experts);
-  if (blockIdx.x == 0) {
-    for (int e = threadIdx.x; e < p.experts; e += kOrderThreads) p.offsets[e] = base[e];
-    if (threadIdx.x == 0) p.offsets[p.experts] = total;
-  }
-  fill_rest(p, total, blockIdx.x, gridDim.x);
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.experts; e += kOrderThreads) base[e] += mine[e];
-  __syncthreads();
-  const int first = blockIdx.x * p.chunk;
-  place_chunk(p, first, min(first + p.chunk, p.tokens), base, wave_counts);
-}
-
 // Tokens that one workgroup routes by itself.
 constexpr int kSmallTokens = 64;
 
+// A few tokens: the whole routing in one workgroup, in one pass where 16 lanes hold a token's experts.
+template <bool kFp32, int kLanes, int kPer>
+__global__ __launch_bounds__(kSmallThreads) void route_small_kernel(RouteParams p) {
+  __shared__ unsigned long long mask[kMaxExperts];
+  __shared__ int run[kMaxExperts], wave_total[kSmallThreads / 64];
+  __shared__ int choice[kSmallTokens * kMaxTop];  // expert, and above 16 bits the earlier choices of it; or -1
+  for (int e = threadIdx.x; e < p.experts; e += kSmallThreads) run[e] = 0;
+  choose_range<kFp32, kLanes, kPer>(p, 0, p.tokens, mask, run, [&](int t, int j, int e, int earlier) {
+    choice[t * p.top + j] = e >= 0 ? e | earlier << 16 : -1;
+  });
+  const int total = scan_counts(run, p.experts, wave_total);
+  for (int e = threadIdx.x; e < p.experts; e += kSmallThreads) p.offsets[e] = run[e];
+  if (threadIdx.x == 0) p.offsets[p.experts] = total;
+  for (int i = threadIdx.x; i < p.tokens * p.top; i += kSmallThreads) {
+    const int c = choice[i];
+    const int place = c >= 0 ? run[c & 0xffff] + (c >> 16) : -1;
+    p.positions[i] = place;
+    if (c >= 0) p.token_of[place] = i / p.top;
+    if (i >= total) p.token_of[i] = -1;
+  }
+}
+
+// Choices of a chunk, their places among the chunk's choices of the same expert, and the chunk's counts.
+template <bool kFp32, int kLanes, int kPer>
+__global__ __launch_bounds__(kChooseThreads) void route_choose_kernel(RouteParams p) {
+  __shared__ unsigned long long mask[kMaxExperts];
+  __shared__ int run[kMaxExperts];
+  for (int e = threadIdx.x; e < p.row; e += kChooseThreads) run[e] = 0;
+  const int first = blockIdx.x * p.chunk;
+  choose_range<kFp32, kLanes, kPer>(p, first, min(first + p.chunk, p.tokens), mask, run, [&](int t, int j, int e, int earlier) {
+    p.positions[int64_t(t) * p.top + j] = e >= 0 ? earlier : -1;
+  });
+  for (int e = threadIdx.x; e < p.row; e += kChooseThreads) p.counts[int64_t(blockIdx.x) * p.row + e] = run[e];
+}
+
+// Places of a chunk's choices: those of smaller experts, of the same expert in earlier chunks, and before it in its own.
+__global__ __launch_bounds__(kOrderThreads) void route_order_kernel(RouteParams p) {
+  __shared__ int base[kMaxExperts];  // all choices of an expert, then its first place
+  __shared__ int mine[kMaxExperts];  // those of the chunks before this one
+  __shared__ int wave_total[kOrderThreads / 64];
+  for (int e = threadIdx.x; e < p.experts; e += kOrderThreads) base[e] = mine[e] = 0;
+  const int first = int(blockIdx.x) * p.chunk * p.top;
+  const int last = min(int(blockIdx.x) * p.chunk + p.chunk, p.tokens) * p.top;
+  int at = first + int(threadIdx.x);
+  int e = -1, place = 0;
+  if (at < last) e = p.chosen[at], place = p.positions[at];
+  __syncthreads();
+  // A thread sums some chunks of four experts.
+  const int quads = p.row / 4, parts = kOrderThreads / quads;
+  const int quad = int(threadIdx.x) % quads, part = int(threadIdx.x) / quads;
+  if (part < parts) {
+    int4 all = make_int4(0, 0, 0, 0), before = make_int4(0, 0, 0, 0);
+    const int4* counts = reinterpret_cast<const int4*>(p.counts) + quad;
+#pragma unroll 8
+    for (int c = part; c < p.chunks; c += parts) {
+      const int4 v = counts[int64_t(c) * quads];
+      all.x += v.x, all.y += v.y, all.z += v.z, all.w += v.w;
+      if (c < int(blockIdx.x)) before.x += v.x, before.y += v.y, before.z += v.z, before.w += v.w;
+    }
+    auto add = [&](int x, int a, int b) {
+      if (x < p.experts) atomicAdd(&base[x], a), atomicAdd(&mine[x], b);
+    };
+    add(quad * 4, all.x, before.x), add(quad * 4 + 1, all.y, before.y);
+    add(quad * 4 + 2, all.z, before.z), add(quad * 4 + 3, all.w, before.w);
+  }
+  __syncthreads();
+  const int total = scan_counts(base, p.experts, wave_total);
+  if (blockIdx.x == 0) {
+    for (int x = threadIdx.x; x < p.experts; x += kOrderThreads) p.offsets[x] = base[x];
+    if (threadIdx.x == 0) p.offsets[p.experts] = total;
+  }
+  for (int64_t i = total + int64_t(blockIdx.x) * kOrderThreads + threadIdx.x; i < int64_t(p.tokens) * p.top;
+       i += int64_t(gridDim.x) * kOrderThreads)
+    p.token_of[i] = -1;  // (choices that fell away)
+  while (at < last) {
+    if (e >= 0) {
+      place += base[e] + mine[e];
+      p.positions[at] = place;
+      p.token_of[place] = at / p.top;
+    }
+    at += kOrderThreads;
+    if (at < last) e = p.chosen[at], place = p.positions[at];
+  }
+}
+
 int chunk_tokens(int64_t tokens) {
   const int64_t c = (tokens + kMaxChunks - 1) / kMaxChunks;
-  return int(c < 16 ? 16 : c);
+  return int(c < 32 ? 32 : c);
+}
+int count_row(int32_t experts) { return (experts + 3) / 4 * 4; }
+
+template <bool kFp32, int kLanes, int kPer>
+void launch_route(const RouteParams& p, hipStream_t s) {
+  if (p.chunks == 0) {
+    hipLaunchKernelGGL((route_small_kernel<kFp32, kLanes, kPer>), dim3(1), dim3(kSmallThreads), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((route_choose_kernel<kFp32, kLanes, kPer>), dim3(p.chunks), dim3(kChooseThreads), 0, s, p);
+    hipLaunchKernelGGL(route_order_kernel, dim3(p.chunks), dim3(kOrderThreads), 0, s, p);
+  }
+}
+
+// A token takes 16 lanes where its choices and at most 16 experts a lane fit.
+template <bool kFp32>
+void launch_route(const RouteParams& p, hipStream_t s) {
+  if (p.top > 16 || p.experts > 256) launch_route<kFp32, 64, 16>(p, s);
+  else if (p.experts > 128) launch_route<kFp32, 16, 16>(p, s);
+  else if (p.experts > 64) launch_route<kFp32, 16, 8>(p, s);
+  else launch_route<kFp32, 16, 4>(p, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -329,7 +364,7 @@ extern "C" int64_t lf_route_experts_workspace_size(int64_t tokens, int32_t exper
   if (tokens < 0 || tokens >= (int64_t(1) << 31) || experts < 1 || experts > lf::kMaxExperts) return -1;
   if (tokens <= lf::kSmallTokens) return 0;
   const int chunk = lf::chunk_tokens(tokens);
-  return (tokens + chunk - 1) / chunk * experts * int64_t(sizeof(int32_t));
+  return (tokens + chunk - 1) / chunk * lf::count_row(experts) * int64_t(sizeof(int32_t));
 }
 
 extern "C" int lf_route_experts(const void* logits, int32_t fp32, int64_t tokens, int32_t experts, int64_t stride,
@@ -345,19 +380,16 @@ extern "C" int lf_route_experts(const void* logits, int32_t fp32, int64_t tokens
   const int64_t need = lf_route_experts_workspace_size(tokens, experts);
   LF_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace of %lld bytes required",
              static_cast<long long>(need));
-  lf::RouteParams p{logits, stride, fp32, int32_t(tokens), experts, top, renormalize, 0, 0, weights, chosen, offsets,
-                    token_of, positions, static_cast<int32_t*>(workspace)};
-  auto s = static_cast<hipStream_t>(stream);
-  const unsigned place_lds = unsigned(1 + lf::kOrderThreads / 64) * experts * sizeof(int);
-  if (tokens <= lf::kSmallTokens) {
-    hipLaunchKernelGGL(lf::route_small_kernel, dim3(1), dim3(lf::kOrderThreads), place_lds, s, p);
-  } else {
+  LF_REQUIRE(need == 0 || lf::aligned16(workspace), "the workspace must be 16-byte aligned");
+  lf::RouteParams p{logits, stride, fp32, int32_t(tokens), experts, top, renormalize, 0, 0, lf::count_row(experts), weights,
+                    chosen, offsets, token_of, positions, static_cast<int32_t*>(workspace)};
+  if (tokens > lf::kSmallTokens) {
     p.chunk = lf::chunk_tokens(tokens);
     p.chunks = int32_t((tokens + p.chunk - 1) / p.chunk);
-    hipLaunchKernelGGL(lf::route_choose_kernel, dim3(p.chunks), dim3(lf::kChooseThreads), experts * sizeof(int), s, p);
-    hipLaunchKernelGGL(lf::route_order_kernel, dim3(p.chunks), dim3(lf::kOrderThreads),
-                       place_lds + experts * sizeof(int), s, p);
   }
+  auto s = static_cast<hipStream_t>(stream);
+  if (fp32) lf::launch_route<true>(p, s);
+  else lf::launch_route<false>(p, s);
   LF_HIP(hipGetLastError());
   return lf::kOk;
 }
