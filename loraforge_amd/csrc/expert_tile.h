@@ -189,15 +189,19 @@ struct Body {
     }
   }
 
-  // Operands of sub-step s. (MXFP4 weights beside bf16 x are read once per stage.)
-  __device__ __forceinline__ void read(const char* slot, int s, Frags<kI, kJ>& f) const {
+  // Operands first .. last - 1 of sub-step s: x fragments, then weight fragments.
+  // (MXFP4 weights beside bf16 x are read once per stage.)
+  static constexpr int kReads = kI + (S::kDecode ? 0 : kJ);
+  __device__ __forceinline__ void read(const char* slot, int s, Frags<kI, kJ>& f, int first = 0, int last = kReads) const {
     const int unit = (4 * h + s) * 16;
 #pragma unroll
-    for (int i = 0; i < kI; ++i) f.x[i] = *reinterpret_cast<const u32x4*>(slot + xread + i * 64 * kXRow + (unit ^ xmask));
+    for (int i = 0; i < kI; ++i)
+      if (i >= first && i < last) f.x[i] = *reinterpret_cast<const u32x4*>(slot + xread + i * 64 * kXRow + (unit ^ xmask));
     if constexpr (!S::kDecode) {
 #pragma unroll
       for (int j = 0; j < kJ; ++j)
-        f.w[j] = *reinterpret_cast<const u32x4*>(slot + S::kXBytes + wread + j * 32 * kXRow + (unit ^ wmask));
+        if (j + kI >= first && j + kI < last)
+          f.w[j] = *reinterpret_cast<const u32x4*>(slot + S::kXBytes + wread + j * 32 * kXRow + (unit ^ wmask));
     }
   }
   __device__ __forceinline__ void read_codes(const char* slot, u32x4 (&codes)[kJ]) const {
@@ -236,6 +240,8 @@ struct Body {
   // fill the memory pipe and hold the matrix instructions back: 8192 x 8192 x 8192
   // in bf16 8 % slower; over three or four sub-steps the last arrive too late).
   static constexpr int kFirst = S::kLoads / 2;
+  // A sub-step's reads go out one behind each instruction where there are enough of them.
+  static constexpr bool kSpread = kI * kJ >= kReads;
 
   // Stage kPos of round u, in `cur`; its first operands are in `f`, its scales in `sc`.
   // `next` holds the stage after it, and on return `f`, `sc` and `codes` are that
@@ -266,21 +272,31 @@ struct Body {
     };
     // (Before each round of reads a wait for the last one, which has long arrived:
     // the compiler would otherwise wait behind the new reads, for them too.)
+    auto reads = [&](const char* slot, int sub, Frags<kI, kJ>& to, int n) {
+      if (kSpread) read(slot, sub, to, n, n + 1);
+    };
     reads_done();
-    read(cur, 1, g);
+    if (!kSpread) read(cur, 1, g);
     pin();
     sub_step<kPos, 0>(f, sc, [&](int n) {
+      reads(cur, 1, g, n);
       decode(g, codes, sc, 1, n);
       copies(prev, kFirst, S::kLoads, n);
     });
     reads_done();
-    read(cur, 2, f);
+    if (!kSpread) read(cur, 2, f);
     pin();
-    sub_step<kPos, 1>(g, sc, [&](int n) { decode(f, codes, sc, 2, n); });
+    sub_step<kPos, 1>(g, sc, [&](int n) {
+      reads(cur, 2, f, n);
+      decode(f, codes, sc, 2, n);
+    });
     reads_done();
-    read(cur, 3, g);
+    if (!kSpread) read(cur, 3, g);
     pin();
-    sub_step<kPos, 2>(f, sc, [&](int n) { decode(g, codes, sc, 3, n); });
+    sub_step<kPos, 2>(f, sc, [&](int n) {
+      reads(cur, 3, g, n);
+      decode(g, codes, sc, 3, n);
+    });
     // Every wave has read all of `cur`, and `next` has arrived: at most the copies
     // of the stages after it are still on their way.
     reads_done();
@@ -288,11 +304,12 @@ struct Body {
     barrier_only();
     Scales su;
     if constexpr (S::kDecode) read_scales<kNext>(scales, u_next, su);
-    read(next, 0, f);
     u32x4 codes_next[kJ];
     read_codes(next, codes_next);
+    if (!kSpread) read(next, 0, f);
     pin();
     sub_step<kPos, 3>(g, sc, [&](int n) {
+      reads(next, 0, f, n);
       copies(cur, 0, kFirst, n);
       decode(f, codes_next, su, 0, n);
     });
