@@ -44,11 +44,13 @@ struct Shape {
   // through: 1024 tokens over 64 experts 4096 x 2048 in 64 x 128 tiles 165 -> 140 us;
   // bf16 x gains nothing, its small tiles wait for LDS reads.)
   static constexpr int kMost = kXMx && kI * kJ <= 3 ? 8 : 4;
-  // Scales go through LDS in units, two buffers. MXFP4 x: 16 bytes (two stages) of
-  // every x and weight row; beside bf16 x a round of the ring, up to 8 bytes of every weight row.
-  static constexpr int kScaleRows = (kXMx ? 64 * kI : 0) + (kWMx ? 64 * kJ : 0);
+  // Scales go through LDS in units. MXFP4 x: 16 bytes (two stages) of every x and weight
+  // row; beside bf16 x a round of the ring, up to 8 bytes of every weight row, two buffers.
+  // (A place for each thread's row, also where there are fewer rows:
+  // a condition around the store costs more than the store, above all among matrix instructions.)
   static constexpr int kUnitBytes = kXMx ? 16 : 8;
-  static constexpr int kScaleBytes = 2 * kUnitBytes * kScaleRows;
+  static constexpr int kXUnits = kThreads * 16;  // bytes
+  static constexpr int kScaleBytes = kXMx ? 2 * kXUnits : kWMx ? 2 * kUnitBytes * kThreads : 0;
   static constexpr int kFit = (kLds - kScaleBytes) / kStage < kMost ? (kLds - kScaleBytes) / kStage : kMost;
   static constexpr int kSlots = kXMx ? kFit / 2 * 2 : kFit;
   static_assert(kSlots >= 2, "two stages have to fit");
@@ -143,6 +145,8 @@ struct Body {
   // past the row is read: towards its end the last bytes that can be, and
   // write_units moves them into place, with zeros past the end of k. No
   // branches: matrix instructions sink past them out of their order.
+  // (MXFP4 x: every thread loads, so that each wave has as many loads on their way; kX, kW: which of them.)
+  template <bool kX = true, bool kW = true>
   __device__ __forceinline__ void load_units(int u) {
     typedef u32x4 u32x4u __attribute__((aligned(1)));
     typedef uint32_t u32u __attribute__((aligned(1)));
@@ -150,8 +154,8 @@ struct Body {
     if constexpr (kXMx) {
       const int from = min(16 * u, blocks - 16);
       unit_skip = min(16 * u - from, 16);
-      if (kI == 4 || threadIdx.x < 64 * kI) xunit = *reinterpret_cast<const u32x4u*>(xscale + from);
-      if (kJ == 4 || threadIdx.x < 64 * kJ) wunit = *reinterpret_cast<const u32x4u*>(wscale + from);
+      if constexpr (kX) xunit = *reinterpret_cast<const u32x4u*>(xscale + from);
+      if constexpr (kW) wunit = *reinterpret_cast<const u32x4u*>(wscale + from);
     } else if constexpr (kWMx) {
 #pragma unroll
       for (int d = 0; d < 2; ++d) {
@@ -161,28 +165,36 @@ struct Body {
       }
     }
   }
+  template <bool kX = true, bool kW = true>
   __device__ __forceinline__ void write_units(char* scales, int u) const {
-    char* to = scales + (u & 1) * (S::kScaleBytes / 2) + threadIdx.x * S::kUnitBytes;
+    char* to = scales + (kXMx ? 0 : (u & 1) * (S::kScaleBytes / 2)) + threadIdx.x * S::kUnitBytes;
     if constexpr (kXMx) {
       // (The two stages' dwords of a lane half side by side.)
-      const u32x4 x = mx::drop_bytes(xunit, unit_skip), w = mx::drop_bytes(wunit, unit_skip);
-      if (kI == 4 || threadIdx.x < 64 * kI) *reinterpret_cast<u32x4*>(to) = u32x4{x.x, x.z, x.y, x.w};
-      if (kJ == 4 || threadIdx.x < 64 * kJ) *reinterpret_cast<u32x4*>(to + 64 * kI * 16) = u32x4{w.x, w.z, w.y, w.w};
+      if constexpr (kX) {
+        const u32x4 x = mx::drop_bytes(xunit, unit_skip);
+        *reinterpret_cast<u32x4*>(to) = u32x4{x.x, x.z, x.y, x.w};
+      }
+      if constexpr (kW) {
+        const u32x4 w = mx::drop_bytes(wunit, unit_skip);
+        *reinterpret_cast<u32x4*>(to + S::kXUnits) = u32x4{w.x, w.z, w.y, w.w};
+      }
     } else if constexpr (kWMx) {
-      if (kJ == 4 || threadIdx.x < 64 * kJ)
-        *reinterpret_cast<u32x2*>(to) =
-            u32x2{uint32_t(uint64_t(wunit.x) >> (8 * skips[0])), uint32_t(uint64_t(wunit.y) >> (8 * skips[1]))};
+      *reinterpret_cast<u32x2*>(to) =
+          u32x2{uint32_t(uint64_t(wunit.x) >> (8 * skips[0])), uint32_t(uint64_t(wunit.y) >> (8 * skips[1]))};
     }
   }
-  // Scales of a stage at place kPos of unit u. MXFP4 x: both stages' of the unit at once (kPos 0).
+  // Scales of a stage at place kPos of unit u. MXFP4 x: fragments first .. last - 1
+  // (x, then weights) of both stages of the unit.
   template <int kPos>
-  __device__ __forceinline__ void read_scales(const char* scales, int u, Scales& s) const {
-    const char* from = scales + (u & 1) * (S::kScaleBytes / 2);
+  __device__ __forceinline__ void read_scales(const char* scales, int u, Scales& s, int first = 0, int last = kI + kJ) const {
+    const char* from = scales + (kXMx ? 0 : (u & 1) * (S::kScaleBytes / 2));
     if constexpr (kXMx) {
 #pragma unroll
-      for (int i = 0; i < kI; ++i) s.x[i] = *reinterpret_cast<const u32x2*>(from + xsread + i * 64 * 16);
+      for (int i = 0; i < kI; ++i)
+        if (i >= first && i < last) s.x[i] = *reinterpret_cast<const u32x2*>(from + xsread + i * 64 * 16);
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) s.w[j] = *reinterpret_cast<const u32x2*>(from + wsread + j * 32 * 16);
+      for (int j = 0; j < kJ; ++j)
+        if (j + kI >= first && j + kI < last) s.w[j] = *reinterpret_cast<const u32x2*>(from + wsread + j * 32 * 16);
     } else if constexpr (kWMx) {
 #pragma unroll
       for (int j = 0; j < kJ; ++j) s.w[j].x = *reinterpret_cast<const uint8_t*>(from + wsread + j * 32 * S::kUnitBytes + kPos * 2);
@@ -253,14 +265,30 @@ struct Body {
     constexpr bool kLast = kPos == S::kSlots - 1;
     constexpr int kNext = kLast ? 0 : kPos + 1;
     const int u_next = kLast ? u + 1 : u;
-    // At the start of a unit the next one's scales, loaded a unit ago, go to the other
-    // buffer (its last readers are behind the last barrier) and the loads of the one after it start.
-    if constexpr (kWMx && (kXMx ? kPos % 2 == 0 : kPos == 0)) {
-      const int unit = kXMx ? u * (S::kSlots / 2) + kPos / 2 : u;
-      write_units(scales, unit + 1);
-      load_units(unit + 2);
+    // Beside bf16 x, at the start of a unit the next one's scales, loaded a unit ago, go to the
+    // other buffer (its last readers are behind the last barrier) and the loads of the one after it start.
+    if constexpr (S::kDecode && kPos == 0) {
+      write_units(scales, u + 1);
+      load_units(u + 2);
       pin();
     }
+    // MXFP4 x: a unit's scales are in registers from its first stage on, so the next one's,
+    // written in its second stage behind the first one's barrier, take their place. With two slots
+    // their loads go out behind the first stage's copies, apart (a load of 64 rows' scales takes
+    // the address unit four times as long as a copy), else as soon as their registers are free.
+    const int unit = u * (S::kSlots / 2) + kPos / 2;
+    constexpr bool kLateLoads = kXMx && kPos % 2 == 0 && S::kSlots == 2;
+    auto next_scales = [&](int n) {
+      if constexpr (kXMx && kPos % 2 == 1) {
+        if (n == 0) write_units<true, false>(scales, unit + 1);
+        if (n == kM / 2) write_units<false, true>(scales, unit + 1);
+        if (n == kM / 2 && S::kSlots > 2) load_units(unit + 2);
+      }
+      if constexpr (kLateLoads) {
+        if (n == 0) load_units<true, false>(unit + 1);
+        if (n == kM / 2) load_units<false, true>(unit + 1);
+      }
+    };
     Frags<kI, kJ> g;
     auto decode = [&](Frags<kI, kJ>& to, const u32x4 (&from)[kJ], const Scales& s, int sub, int n) {
       // Fragment j's conversions behind instruction j kI (all of them early enough for the next sub-step).
@@ -289,6 +317,7 @@ struct Body {
     sub_step<kPos, 1>(g, sc, [&](int n) {
       reads(cur, 2, f, n);
       decode(f, codes, sc, 2, n);
+      next_scales(n);
     });
     reads_done();
     if (!kSpread) read(cur, 3, g);
@@ -298,24 +327,24 @@ struct Body {
       decode(g, codes, sc, 3, n);
     });
     // Every wave has read all of `cur`, and `next` has arrived: at most the copies
-    // of the stages after it are still on their way.
+    // of the stages after it, and the two loads of scales behind them, are still on their way.
     reads_done();
-    wait_vm<(S::kSlots - 2) * S::kLoads>();
+    wait_vm<(S::kSlots - 2) * S::kLoads + (kLateLoads ? 2 : 0)>();
     barrier_only();
     Scales su;
     if constexpr (S::kDecode) read_scales<kNext>(scales, u_next, su);
     u32x4 codes_next[kJ];
     read_codes(next, codes_next);
     if (!kSpread) read(next, 0, f);
+    if constexpr (kXMx && kPos % 2 == 1 && !kSpread) read_scales<0>(scales, unit + 1, su);
     pin();
     sub_step<kPos, 3>(g, sc, [&](int n) {
       reads(next, 0, f, n);
+      if constexpr (kXMx && kPos % 2 == 1 && kSpread) read_scales<0>(scales, unit + 1, su, n, n + 1);
       copies(cur, 0, kFirst, n);
       decode(f, codes_next, su, 0, n);
     });
-    // (MXFP4 x: the next round's scales take the place of these, which the last
-    // instruction has read; the next one waits for LDS once a round.)
-    if constexpr (kXMx && kPos % 2 == 1) read_scales<0>(scales, u * (S::kSlots / 2) + kPos / 2 + 1, sc);
+    if constexpr (kXMx && kPos % 2 == 1) sc = su;
     if constexpr (S::kDecode) {
       sc = su;
 #pragma unroll
@@ -338,7 +367,7 @@ struct Body {
     copy(slot[kN - 1], 0, kFirst);
     pin();
     if constexpr (kWMx) write_units(scales, 0);
-    load_units(1);
+    if constexpr (!kXMx || S::kSlots > 2) load_units(1);
     wait_vm<(kN - 2) * S::kLoads + kFirst>();
     lds_barrier();
     Scales sc;
@@ -423,7 +452,7 @@ struct Body {
     }
     if constexpr (kWMx) {
       wscale = p.ws + (w0 + weight_row(nt, t % (64 * kJ))) * blocks;
-      wsread = (kXMx ? 64 * kI * 16 : 0) + (32 * kJ * wn + c) * S::kUnitBytes + (kXMx ? 8 : 1) * h;
+      wsread = (kXMx ? S::kXUnits : 0) + (32 * kJ * wn + c) * S::kUnitBytes + (kXMx ? 8 : 1) * h;
     }
 #pragma unroll
     for (int i = 0; i < kI; ++i)
