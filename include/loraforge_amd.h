@@ -361,8 +361,7 @@ int lf_route_experts(const void* logits, int32_t fp32, int64_t tokens, int32_t e
 /* Kernel of a product: the weight stream with k split over the waves of a workgroup
  * (few rows and weights; `columns` weight rows a workgroup: 16 or 32), the one
  * with a wave for 16 weight rows (few rows per expert, many weights), or MFMA tiles
- * of at most `rows` (64, 128, 192, 256) x `columns` weight rows (64, 128, 256; with
- * SwiGLU 128 or 256). */
+ * of at most `rows` x `columns` weight rows (each 64, 128, 192 or 256). */
 #define LF_EXPERT_STREAM 0
 #define LF_EXPERT_TILE 1
 #define LF_EXPERT_ROWS 2

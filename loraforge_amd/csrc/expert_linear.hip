@@ -20,12 +20,12 @@ bool tiles_fit(const lf_expert_product& a) {
 // Scales are loaded 16 at a time.
 bool rows_fit(const lf_expert_product& a) { return !a.w_scales || a.k >= 512; }
 
-// Times of the kernels in us, fitted to 2319 products (dense ones of 1..4096 rows,
+// Times of the kernels in us, fitted to 2586 products (dense ones of 1..4096 rows,
 // n 1024..24576, k 1024..8192; 8..128 experts, 1..8192 tokens), every plan of each.
 struct Costs {
   struct Tile {
     float fixed, stage, busy;  // of a tile, of a stage (64 k; 256 k of MXFP4 x), and what all CUs at work add to a stage
-  } tile[4][3];                // [rows / 64 - 1][64, 128, 256 columns]
+  } tile[4][4];                // [rows / 64 - 1][columns / 64 - 1]
   struct Rows {
     float fixed, pass, k, k_busy;  // of the launch, of a pass of 16 rows, of 1024 k of it, and what two workgroups on every CU add
   } rows;
@@ -36,31 +36,31 @@ struct Costs {
 constexpr Costs kCosts[3] = {
     // bf16 x and weights
     {{
-         {{4.51f, 0.241f, 0.084f}, {5.23f, 0.315f, 0.187f}, {5.56f, 0.439f, 0.293f}},
-         {{5.37f, 0.326f, 0.083f}, {6.07f, 0.313f, 0.230f}, {8.41f, 0.597f, 0.318f}},
-         {{6.18f, 0.413f, 0.089f}, {7.58f, 0.421f, 0.238f}, {8.21f, 0.881f, 0.421f}},
-         {{6.67f, 0.406f, 0.152f}, {9.83f, 0.545f, 0.310f}, {10.18f, 1.077f, 0.564f}}},
-     {1.86f, 0.45f, 3.02f, 18.43f},
-     {{1.35f, 1.97f, 0.24f, 0.78f, 0.78f, 1.02f},
-      {2.56f, 0.00f, 0.75f, 1.03f, 5.86f, 0.41f}}},
+         {{4.63f, 0.241f, 0.077f}, {5.00f, 0.323f, 0.171f}, {6.31f, 0.415f, 0.214f}, {5.61f, 0.433f, 0.265f}},
+         {{5.61f, 0.321f, 0.076f}, {6.02f, 0.367f, 0.181f}, {8.71f, 0.437f, 0.249f}, {8.34f, 0.541f, 0.324f}},
+         {{6.27f, 0.423f, 0.074f}, {7.25f, 0.418f, 0.212f}, {12.50f, 0.546f, 0.267f}, {7.93f, 0.773f, 0.428f}},
+         {{6.92f, 0.401f, 0.152f}, {9.45f, 0.494f, 0.321f}, {12.35f, 0.729f, 0.438f}, {10.18f, 0.934f, 0.588f}}},
+     {1.74f, 0.49f, 3.02f, 18.08f},
+     {{1.55f, 1.81f, 0.20f, 0.80f, 0.84f, 1.04f},
+      {2.39f, 0.00f, 0.81f, 1.00f, 5.77f, 0.45f}}},
     // bf16 x, MXFP4 weights
     {{
-         {{4.65f, 0.287f, 0.045f}, {5.16f, 0.378f, 0.050f}, {5.71f, 0.478f, 0.132f}},
-         {{5.43f, 0.375f, 0.047f}, {5.81f, 0.442f, 0.082f}, {7.62f, 0.694f, 0.151f}},
-         {{6.45f, 0.466f, 0.058f}, {7.21f, 0.577f, 0.092f}, {9.59f, 0.928f, 0.136f}},
-         {{6.82f, 0.525f, 0.100f}, {8.83f, 0.705f, 0.150f}, {13.41f, 1.165f, 0.259f}}},
-     {1.60f, 1.88f, 1.90f, 4.12f},
-     {{1.54f, 1.51f, 0.00f, 0.74f, 0.00f, 1.06f},
-      {1.39f, 2.12f, 0.21f, 0.84f, 0.18f, 1.30f}}},
+         {{4.62f, 0.311f, 0.051f}, {4.83f, 0.363f, 0.076f}, {6.19f, 0.456f, 0.085f}, {5.67f, 0.474f, 0.134f}},
+         {{5.27f, 0.431f, 0.047f}, {5.73f, 0.445f, 0.079f}, {8.63f, 0.570f, 0.082f}, {7.56f, 0.686f, 0.152f}},
+         {{6.12f, 0.527f, 0.058f}, {7.12f, 0.562f, 0.097f}, {11.34f, 0.721f, 0.116f}, {9.36f, 0.904f, 0.145f}},
+         {{6.75f, 0.512f, 0.106f}, {8.74f, 0.661f, 0.172f}, {15.07f, 0.922f, 0.138f}, {13.36f, 1.136f, 0.275f}}},
+     {1.57f, 1.91f, 1.90f, 4.11f},
+     {{1.70f, 1.40f, 0.00f, 0.73f, 0.00f, 1.11f},
+      {1.48f, 2.02f, 0.20f, 0.84f, 0.24f, 1.30f}}},
     // MXFP4 x and weights
     {{
-         {{5.11f, 0.295f, 0.171f}, {5.50f, 0.459f, 0.318f}, {4.96f, 0.661f, 0.642f}},
-         {{5.76f, 0.452f, 0.222f}, {6.43f, 0.477f, 0.245f}, {6.77f, 0.800f, 0.566f}},
-         {{6.04f, 0.588f, 0.217f}, {6.06f, 0.789f, 0.394f}, {8.63f, 1.022f, 0.416f}},
-         {{5.10f, 0.707f, 0.381f}, {6.93f, 0.862f, 0.424f}, {10.53f, 1.254f, 0.562f}}},
-     {2.31f, 1.60f, 1.06f, 4.09f},
-     {{1.52f, 1.76f, 0.09f, 0.36f, 0.37f, 0.48f},
-      {1.40f, 2.14f, 0.34f, 0.45f, 0.83f, 0.49f}}},
+         {{5.03f, 0.339f, 0.198f}, {5.43f, 0.431f, 0.301f}, {6.33f, 0.542f, 0.361f}, {5.39f, 0.630f, 0.524f}},
+         {{5.73f, 0.432f, 0.220f}, {6.25f, 0.501f, 0.296f}, {8.10f, 0.637f, 0.370f}, {7.04f, 0.731f, 0.541f}},
+         {{5.87f, 0.555f, 0.242f}, {6.32f, 0.685f, 0.375f}, {10.43f, 0.744f, 0.354f}, {8.60f, 0.937f, 0.430f}},
+         {{5.46f, 0.695f, 0.306f}, {7.15f, 0.788f, 0.441f}, {12.95f, 0.882f, 0.373f}, {10.37f, 1.087f, 0.625f}}},
+     {2.30f, 1.56f, 1.06f, 4.08f},
+     {{1.62f, 1.70f, 0.08f, 0.38f, 0.40f, 0.48f},
+      {1.44f, 2.08f, 0.35f, 0.45f, 0.86f, 0.49f}}},
 };
 
 constexpr double kCus = 256;
@@ -74,7 +74,7 @@ double passes(double each, double cap, bool grouped) {
 double tile_us(const Costs& c, int rows, int columns, double each, double used, bool grouped, double width, double stages) {
   const double per = passes(each, rows, grouped);
   const double height = std::min(rows / 64.0, std::max(1.0, grouped ? each / per / 64.0 + 0.5 : std::ceil(std::ceil(each / per) / 64.0)));
-  const int low = std::min(3, int(height)), high = std::min(4, low + 1), j = columns == 64 ? 0 : columns == 128 ? 1 : 2;
+  const int low = std::min(3, int(height)), high = std::min(4, low + 1), j = columns / 64 - 1;
   const double part = height - low;
   auto mix = [&](float Costs::Tile::*m) { return (1.0 - part) * (c.tile[low - 1][j].*m) + part * (c.tile[high - 1][j].*m); };
   const double fixed = mix(&Costs::Tile::fixed), stage = mix(&Costs::Tile::stage), busy = mix(&Costs::Tile::busy);
@@ -87,8 +87,8 @@ double tile_us(const Costs& c, int rows, int columns, double each, double used, 
   return kLaunch + full * round + (rest > 0 ? fixed - kLaunch + stages * (stage + busy * rest) : 0.0);
 }
 
-// The plan of least time. (Against the fastest plan of each of those products: 1.4 to
-// 2.9 % slower on average by type, 58 % at most: 64 experts of 512 tokens, n and k 1024.)
+// The plan of least time. (Against the fastest plan of each of those products: 1.8 to
+// 4.7 % slower on average by type, 61 % at most: 3 rows, n and k 1024, 7.1 and 4.4 us.)
 lf_expert_plan plan_of(const lf_expert_product& a) {
   const Costs& c = kCosts[a.x_scales ? 2 : a.w_scales ? 1 : 0];
   const bool grouped = a.offsets != nullptr && a.experts > 1;
@@ -123,7 +123,7 @@ lf_expert_plan plan_of(const lf_expert_product& a) {
   if (tiles_fit(a)) {
     const double stage_k = a.x_scales ? 256.0 : 64.0;
     for (int height = 64; height <= 256; height += 64)
-      for (int columns = a.swiglu ? 128 : 64; columns <= 256; columns *= 2)
+      for (int columns = 64; columns <= 256; columns += 64)
         offer(tile_us(c, height, columns, each, used, grouped, n, std::ceil(double(a.k) / stage_k)), {LF_EXPERT_TILE, height, columns});
   }
   return best;
@@ -182,8 +182,7 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   }
   LF_REQUIRE(plan.kernel == LF_EXPERT_TILE && lf::expert::tiles_fit(*a), "this product cannot run in tiles");
   LF_REQUIRE(plan.rows >= 64 && plan.rows <= 256 && plan.rows % 64 == 0, "tile plan: 64, 128, 192 or 256 rows");
-  LF_REQUIRE(plan.columns == 128 || plan.columns == 256 || (plan.columns == 64 && !a->swiglu),
-             "tile plan: 64 (not with SwiGLU), 128 or 256 columns");
+  LF_REQUIRE(plan.columns >= 64 && plan.columns <= 256 && plan.columns % 64 == 0, "tile plan: 64, 128, 192 or 256 columns");
   if (x_mx) return lf::expert::launch_tiles_mx(p, plan.rows, plan.columns, s);
   return w_mx ? lf::expert::launch_tiles_mxw(p, plan.rows, plan.columns, s)
               : lf::expert::launch_tiles_bf16(p, plan.rows, plan.columns, s);

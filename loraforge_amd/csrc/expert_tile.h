@@ -37,8 +37,8 @@ struct Shape {
   static constexpr bool kDecode = kWMx && !kXMx;           // MXFP4 weights for bf16 x
   static constexpr int kStageK = kXMx ? 256 : 64;
   static constexpr int kWRow = kDecode ? 32 : 128;         // bytes of a weight row per stage
-  // (A copy per wave at least: 64 rows of 32 bytes go twice.)
-  static constexpr int kXBytes = 64 * kI * kXRow, kWBytes = 64 * kJ * kWRow < 4096 ? 4096 : 64 * kJ * kWRow;
+  // (Whole copies of all waves: of 64 or 192 rows of 32 bytes 64 go twice.)
+  static constexpr int kXBytes = 64 * kI * kXRow, kWBytes = (64 * kJ * kWRow + 4095) / 4096 * 4096;
   static constexpr int kStage = kXBytes + kWBytes;
   // (Deeper for small tiles of MXFP4 x, whose two stages a unit of scales are soon
   // through: 1024 tokens over 64 experts 4096 x 2048 in 64 x 128 tiles 165 -> 140 us;
@@ -102,9 +102,9 @@ struct Body {
 
   __device__ __forceinline__ int weight_row(int nt, int r) const {
     if (!p.swiglu) return min(nt * 64 * kJ + r, p.n - 1);
-    // A wave's fragments are gate and up rows of the same columns in turn.
-    const int column = nt * 32 * kJ + (r / (32 * kJ)) * 16 * kJ + (r / 64 % (kJ > 1 ? kJ / 2 : 1)) * 32 + r % 32;
-    return min(column, p.width - 1) + (r / 32 % 2 ? p.width : 0);
+    // Half a fragment are gate rows, half up rows of the same columns.
+    const int column = nt * 32 * kJ + r / 32 * 16 + r % 16;
+    return min(column, p.width - 1) + (r / 16 % 2 ? p.width : 0);
   }
 
   // Copies of index first .. last - 1 of the next stage into a slot.
@@ -482,86 +482,86 @@ struct Body {
   // registers took longer to fetch than to run).
   template <bool kSwiglu>
   __device__ __forceinline__ void finish(char* lds, int expert, int first, int count, int nt) {
-    if constexpr (!kSwiglu || kJ >= 2) {
-      constexpr int kRowBytes = 32 * kJ * 4 + 16;             // (padded: rows start at other banks)
-      constexpr int kColumns = kSwiglu ? 16 * kJ : 32 * kJ;   // output columns of the wave
-      constexpr int kLanes = kColumns / 8, kRows = 64 / kLanes;
-      char* mine = lds + wave * 64 * kRowBytes;
-      const int wm = wave & 1, wn = wave >> 1, c = lane & 31;
-      const int part = lane % kLanes, in_row = lane / kLanes;
-      // With SwiGLU eight columns lie in 32 of a gate fragment, their up values one fragment on.
-      const int local = kSwiglu ? part / 4 * 64 + part % 4 * 8 : part * 8;
-      const int col = (nt * 2 + wn) * kColumns + part * 8;
-      float add[8], add_up[8];
+    constexpr int kRowBytes = 32 * kJ * 4 + 16;             // (padded: rows start at other banks)
+    constexpr int kColumns = kSwiglu ? 16 * kJ : 32 * kJ;   // output columns of the wave
+    constexpr int kParts = kColumns / 8;  // lanes that share a row (of kLanes, a power of two)
+    constexpr int kLanes = kParts <= 2 ? 2 : kParts <= 4 ? 4 : kParts <= 8 ? 8 : 16, kRows = 64 / kLanes;
+    char* mine = lds + wave * 64 * kRowBytes;
+    const int wm = wave & 1, wn = wave >> 1, c = lane & 31;
+    const bool idle = lane % kLanes >= kParts;
+    const int part = idle ? 0 : lane % kLanes, in_row = lane / kLanes;
+    // With SwiGLU eight columns are half of a fragment's gate values, their up values 16 on.
+    const int local = kSwiglu ? part / 2 * 32 + part % 2 * 8 : part * 8;
+    const int col = (nt * 2 + wn) * kColumns + part * 8;
+    float add[8], add_up[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) add[e] = add_up[e] = 0.f;
-      if (p.bias) {
-        const uint16_t* bias = p.bias + int64_t(expert) * p.n;
+    for (int e = 0; e < 8; ++e) add[e] = add_up[e] = 0.f;
+    if (p.bias) {
+      const uint16_t* bias = p.bias + int64_t(expert) * p.n;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int at = min(col + e, p.width - 1);
-          add[e] = bf16_to_f32(bias[at]);
-          if (kSwiglu) add_up[e] = bf16_to_f32(bias[at + p.width]);
-        }
+      for (int e = 0; e < 8; ++e) {
+        const int at = min(col + e, p.width - 1);
+        add[e] = bf16_to_f32(bias[at]);
+        if (kSwiglu) add_up[e] = bf16_to_f32(bias[at + p.width]);
       }
-      const bool vec = p.y_vec && col + 8 <= p.width;
-      const bool all_vec = __ballot(!vec) == 0;
-      // Eight output columns of staged row r.
-      auto output = [&](int r) {
-        const f32x4* v = reinterpret_cast<const f32x4*>(mine + r * kRowBytes + local * 4);
-        const f32x4 half[2] = {v[0], v[1]};
-        f32x4 up[2];
-        if (kSwiglu) up[0] = v[8], up[1] = v[9];
-        uint32_t o[4];
+    }
+    const bool vec = p.y_vec && col + 8 <= p.width;
+    const bool all_vec = __ballot(!vec) == 0;
+    // Eight output columns of staged row r.
+    auto output = [&](int r) {
+      const f32x4* v = reinterpret_cast<const f32x4*>(mine + r * kRowBytes + local * 4);
+      const f32x4 half[2] = {v[0], v[1]};
+      f32x4 up[2];
+      if (kSwiglu) up[0] = v[4], up[1] = v[5];
+      uint32_t o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a = half[e >> 1][(e & 1) * 2] + add[2 * e], b = half[e >> 1][(e & 1) * 2 + 1] + add[2 * e + 1];
-          if (kSwiglu) {
-            a = silu_mul_f32(a, up[e >> 1][(e & 1) * 2] + add_up[2 * e]);
-            b = silu_mul_f32(b, up[e >> 1][(e & 1) * 2 + 1] + add_up[2 * e + 1]);
-          }
-          o[e] = pack_bf16x2(a, b);
+      for (int e = 0; e < 4; ++e) {
+        float a = half[e >> 1][(e & 1) * 2] + add[2 * e], b = half[e >> 1][(e & 1) * 2 + 1] + add[2 * e + 1];
+        if (kSwiglu) {
+          a = silu_mul_f32(a, up[e >> 1][(e & 1) * 2] + add_up[2 * e]);
+          b = silu_mul_f32(b, up[e >> 1][(e & 1) * 2 + 1] + add_up[2 * e + 1]);
         }
-        return u32x4{o[0], o[1], o[2], o[3]};
-      };
+        o[e] = pack_bf16x2(a, b);
+      }
+      return u32x4{o[0], o[1], o[2], o[3]};
+    };
 #pragma unroll
-      for (int pair = 0; pair < (kI + 1) / 2; ++pair) {
+    for (int pair = 0; pair < (kI + 1) / 2; ++pair) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < kJ; ++j)
+        for (int j = 0; j < kJ; ++j)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-              if (2 * pair + i < kI) {
-                const f32x16& a = acc[2 * pair + i][j];
-                *reinterpret_cast<f32x4*>(mine + (32 * i + c) * kRowBytes + (32 * j + 8 * g + 4 * h) * 4) =
-                    f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
-              }
-        const int staged = min(2, kI - 2 * pair) * 32;
-        auto place = [&](int r) { return (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31); };
-        if (all_vec) {
-          constexpr int kTogether = 32 / kRows < 4 ? 32 / kRows : 4;  // rows whose reads go out together
-#pragma unroll 1
-          for (int r0 = in_row; r0 < staged; r0 += kTogether * kRows) {
-            u32x4 o[kTogether];
-#pragma unroll
-            for (int k = 0; k < kTogether; ++k) o[k] = output(r0 + k * kRows);
-#pragma unroll
-            for (int k = 0; k < kTogether; ++k) {
-              const int row = place(r0 + k * kRows);
-              if (row < count) *reinterpret_cast<u32x4*>(p.y + int64_t(first + row) * p.y_stride + col) = o[k];
+          for (int g = 0; g < 4; ++g)
+            if (2 * pair + i < kI) {
+              const f32x16& a = acc[2 * pair + i][j];
+              *reinterpret_cast<f32x4*>(mine + (32 * i + c) * kRowBytes + (32 * j + 8 * g + 4 * h) * 4) =
+                  f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
             }
-          }
-        } else {
+      const int staged = min(2, kI - 2 * pair) * 32;
+      auto place = [&](int r) { return (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31); };
+      if (all_vec) {
+        constexpr int kTogether = 32 / kRows < 4 ? 32 / kRows : 4;  // rows whose reads go out together
 #pragma unroll 1
-          for (int r = in_row; r < staged; r += kRows) {
-            const u32x4 o = output(r);
-            uint16_t* y = p.y + int64_t(first + place(r)) * p.y_stride + col;
-            if (place(r) >= count) continue;
+        for (int r0 = in_row; r0 < staged; r0 += kTogether * kRows) {
+          u32x4 o[kTogether];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (col + e < p.width) y[e] = uint16_t(o[e >> 1] >> (16 * (e & 1)));
+          for (int k = 0; k < kTogether; ++k) o[k] = output(r0 + k * kRows);
+#pragma unroll
+          for (int k = 0; k < kTogether; ++k) {
+            const int row = place(r0 + k * kRows);
+            if (row < count && !idle) *reinterpret_cast<u32x4*>(p.y + int64_t(first + row) * p.y_stride + col) = o[k];
           }
+        }
+      } else {
+#pragma unroll 1
+        for (int r = in_row; r < staged; r += kRows) {
+          const u32x4 o = output(r);
+          uint16_t* y = p.y + int64_t(first + place(r)) * p.y_stride + col;
+          if (place(r) >= count || idle) continue;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e < p.width) y[e] = uint16_t(o[e >> 1] >> (16 * (e & 1)));
         }
       }
     }

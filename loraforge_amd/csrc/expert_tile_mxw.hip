@@ -8,6 +8,7 @@ int launch_tiles_mxw(const Params& p, int cap, int columns, hipStream_t stream) 
   switch (columns) {
     case 64: return tile::launch<false, true, 1>(p, cap, stream);
     case 128: return tile::launch<false, true, 2>(p, cap, stream);
+    case 192: return tile::launch<false, true, 3>(p, cap, stream);
     default: return tile::launch<false, true, 4>(p, cap, stream);
   }
 }

@@ -136,5 +136,3 @@ def test_plans():
         a.k = 480 if p is forced else 512
         a.plan = ctypes.pointer(p)
         refused(match, _lib.library().lf_expert_linear(ctypes.byref(a), None))
-    a.plan, a.swiglu = ctypes.pointer(_lib.ExpertPlan(_lib.LF_EXPERT_TILE, 64, 64)), 1
-    refused("columns", _lib.library().lf_expert_linear(ctypes.byref(a), None))

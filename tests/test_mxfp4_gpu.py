@@ -298,7 +298,7 @@ def test_products_on_a_side_stream_and_in_a_graph(device):
 
 TYPES = [("bf16", "bf16"), ("bf16", "mxfp4"), ("mxfp4", "mxfp4")]
 PLANS = [(_lib.LF_EXPERT_STREAM, 0, c) for c in (16, 32)] + [(_lib.LF_EXPERT_ROWS, 0, 128)] + [
-    (_lib.LF_EXPERT_TILE, r, c) for r in (64, 128, 192, 256) for c in (64, 128, 256)]
+    (_lib.LF_EXPERT_TILE, r, c) for r in (64, 128, 192, 256) for c in (64, 128, 192, 256)]
 
 
 def forced(x, w, plan, **options):
@@ -329,7 +329,7 @@ def test_every_plan(types, plan, k, device):
 
 
 @pytest.mark.parametrize("types", TYPES, ids="-".join)
-@pytest.mark.parametrize("plan", [p for p in PLANS if p[2] > 64 or p[0] != _lib.LF_EXPERT_TILE], ids=lambda p: "-".join(map(str, p)))
+@pytest.mark.parametrize("plan", PLANS, ids=lambda p: "-".join(map(str, p)))
 @pytest.mark.parametrize("n", [512, 776, 88])
 def test_every_plan_swiglu(types, plan, n, device):
     act, weight = types
@@ -345,7 +345,7 @@ def test_every_plan_swiglu(types, plan, n, device):
 
 
 @pytest.mark.parametrize("types", TYPES, ids="-".join)
-@pytest.mark.parametrize("columns", [64, 128, 256])
+@pytest.mark.parametrize("columns", [64, 128, 192, 256])
 def test_tiles_of_one_dense_product(types, columns, device):
     """Several row and column tiles of one segment, on every workgroup order; results do not depend on the tile."""
     act, weight = types
