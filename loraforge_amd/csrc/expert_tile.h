@@ -18,6 +18,14 @@
 // An expert's rows are cut into tiles of equal height (a multiple of 64, up to
 // 256), so an expert with few rows costs as much as they need: the body is chosen
 // by the tile's rows.
+//
+// What bounds it: at full tiles the board's power. Of a 256 x 256 tile's loop the
+// matrix instructions fill four fifths (2180 clocks of a stage's 2700 in MXFP4, 2110 of
+// 2440 in bf16), at 1.6 and 1.3 GHz of the card's 2.4; each step that
+// gave them more of it (scale handling, bank conflicts, the next tile's start under
+// this one's epilogue) lowered the clock by nearly as much. 4096 x 12288 x 4096: bf16 330-345
+// us (1.25 PFLOP/s; a library's product of 8192 cubed reaches 1.29), MXFP4 weights
+// 335-347, MXFP4 both 111-121 (3.6 PFLOP/s). Small tiles wait for LDS reads, few tiles leave CUs idle.
 #pragma once
 
 #include "expert_params.h"
@@ -413,9 +421,11 @@ struct Body {
     const int last = first + count - 1;
 
     // A copy covers eight rows of 128 bytes (of 32 bytes: 32 rows); row r's unit u
-    // sits at u ^ (r & 7), so that reads of one unit of consecutive rows meet no bank twice.
+    // sits at u ^ (r / 2 % 8): two rows fill the 64 banks, and the 16 lanes of a pass of a
+    // 16-byte read (which are not neighbours) then meet no bank twice. With r % 8 in its
+    // place 40 % of the LDS cycles were conflicts.
     const int r8 = lane >> 3;
-    const int xat = ((lane & 7) ^ r8) * 16;
+    const int xat = ((lane & 7) ^ ((wave & 1) * 4 + (r8 >> 1))) * 16;
     const int64_t w0 = int64_t(seg.expert) * p.n;
     const int wr = S::kWRow == 128 ? r8 : lane >> 1;
     const int wat = S::kWRow == 128 ? xat : (lane & 1) * 16;
@@ -442,7 +452,7 @@ struct Body {
     wleft = row_bytes_w - wat;
 
     xread = (32 * wm + c) * kXRow;  // fragment i: rows 64 i + 32 wm ..
-    xmask = (c & 7) * 16;
+    xmask = (c / 2 % 8) * 16;
     wread = (32 * kJ * wn + c) * S::kWRow;
     wmask = xmask;
     const int t = threadIdx.x;
