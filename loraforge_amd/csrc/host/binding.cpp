@@ -684,10 +684,42 @@ PyObject* mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return THPVariable_Wrap(std::move(out));
 }
 
-// product(x, weight, offsets or None, tokens or None, bias or None, swiglu) -> out or None:
-// mxfp4_linear (offsets None) and expert_linear with a fresh output.
+// A bf16 [rows, columns] output: the caller's (whose rows may be apart), or a new one.
+struct Output {
+  const at::Tensor* given = nullptr;
+  PyObject* object = nullptr;
+  at::Tensor made;
+  int64_t stride = 0;
+
+  Output(PyObject* arg, int64_t rows, int64_t columns, const at::Device& dev) {
+    if (arg == Py_None) {
+      made = at::empty({rows, columns}, at::TensorOptions().dtype(at::kBFloat16).device(dev));
+      stride = columns;
+      return;
+    }
+    const at::Tensor* t = matrix(arg, dev);
+    if (!t || t->size(0) != rows || t->size(1) != columns || t->stride(1) != 1) return;
+    stride = rows > 1 ? t->stride(0) : columns;
+    if (stride < columns) return;
+    given = t;
+    object = arg;
+  }
+  // Whether it can be written beside these inputs.
+  bool ok(std::initializer_list<const at::Tensor*> inputs) const {
+    return given ? !shares(*given, inputs) : made.defined() && on_gpu(made);
+  }
+  uint16_t* data() { return ptr<uint16_t>(given ? given : &made); }
+  PyObject* take() {
+    if (!object) return THPVariable_Wrap(std::move(made));
+    Py_INCREF(object);
+    return object;
+  }
+};
+
+// product(x, weight, offsets or None, tokens or None, bias or None, swiglu, out or None) -> out or None:
+// mxfp4_linear (offsets None) and expert_linear.
 PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 6 || (args[5] != Py_True && args[5] != Py_False)) return decline();
+  if (nargs != 7 || (args[5] != Py_True && args[5] != Py_False)) return decline();
   const bool grouped = args[2] != Py_None, swiglu = args[5] == Py_True;
   lf_expert_product a{};
   MxArg wm, xm;
@@ -743,12 +775,13 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* stream;
   if (!current(dev, &stream)) return decline();
   const int64_t width = swiglu ? n / 2 : n;
-  at::Tensor out = at::empty({a.rows, width}, w->options().dtype(at::kBFloat16));
-  if (!on_gpu(out)) return decline();
+  Output out(args[6], a.rows, width, dev);
+  auto optional = [&](int i) { return args[i] == Py_None ? nullptr : plain(args[i]); };
+  if (!out.ok({x, xm.scales, w, wm.scales, optional(2), optional(3), optional(4)})) return decline();
   a.x = x->data_ptr();
   a.w = w->data_ptr();
-  a.y = ptr<uint16_t>(&out);
-  a.y_stride = width;
+  a.y = out.data();
+  a.y_stride = out.stride;
   a.n = n;
   a.k = k;
   a.experts = experts;
@@ -756,7 +789,7 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int rc = unlocked([&] { return g_product(&a, stream); });
   if (rc == LF_EINVAL) return decline();
   if (rc != LF_OK) return failed();
-  return THPVariable_Wrap(std::move(out));
+  return out.take();
 }
 
 // route(logits, top_k, renormalize) -> (weights, experts, offsets, tokens, positions) or None
@@ -801,9 +834,9 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return a && b && c && d && e ? PyTuple_Pack(5, a.p, b.p, c.p, d.p, e.p) : nullptr;
 }
 
-// combine(rows, positions, weights, base or None) -> out or None
+// combine(rows, positions, weights, base or None, out or None) -> out or None
 PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 4) return decline();
+  if (nargs != 5) return decline();
   const at::Tensor* rows = plain(args[0]);
   if (!rows) return decline();
   const at::Device dev = rows->device();
@@ -829,15 +862,16 @@ PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   void* stream;
   if (!current(dev, &stream)) return decline();
-  at::Tensor out = at::empty({count, n}, rows->options());
-  if (!on_gpu(out)) return decline();
+  Output out(args[4], count, n, dev);
+  const bool onto = base && out.data() == ptr<uint16_t>(base) && out.stride == base_stride;  // (in place)
+  if (!out.ok({rows, positions, weights, onto ? nullptr : base})) return decline();
   const int rc = unlocked([&] {
     return g_combine(ptr<uint16_t>(rows), rows->size(0), rows_stride, ptr<int32_t>(positions), ptr<float>(weights), count,
-                     int32_t(top), n, ptr<uint16_t>(base), base_stride, ptr<uint16_t>(&out), n, stream);
+                     int32_t(top), n, ptr<uint16_t>(base), base_stride, out.data(), out.stride, stream);
   });
   if (rc == LF_EINVAL) return decline();
   if (rc != LF_OK) return failed();
-  return THPVariable_Wrap(std::move(out));
+  return out.take();
 }
 
 // init(addresses, raw_stream, get_device, arch_ok, workspaces, compute_units, lora_batch, mx_tensor)

@@ -129,8 +129,8 @@ def combine_experts(rows, positions, weights, *, base=None, out=None):
     """
     import torch
 
-    if out is None and getattr(rows, "is_cuda", False):
-        done = _lib.binding().combine(rows, positions, weights, base)
+    if getattr(rows, "is_cuda", False):
+        done = _lib.binding().combine(rows, positions, weights, base, out)
         if done is not None:
             return done
     tensor(rows, "rows", 2, torch.bfloat16)

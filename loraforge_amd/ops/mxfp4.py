@@ -145,8 +145,8 @@ def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out, plan=None
 
     grouped = experts is not None
     quantised = isinstance(weight, MXFP4Tensor)
-    if out is None and plan is None and (offsets is not None) == grouped and getattr(weight.codes if quantised else weight, "is_cuda", False):
-        done = _lib.binding().product(x, weight, offsets, tokens, bias, swiglu)
+    if plan is None and (offsets is not None) == grouped and getattr(weight.codes if quantised else weight, "is_cuda", False):
+        done = _lib.binding().product(x, weight, offsets, tokens, bias, swiglu, out)
         if done is not None:
             return done
     if quantised:

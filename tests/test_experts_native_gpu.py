@@ -50,8 +50,11 @@ def test_products(monkeypatch, rows, device):
             agree(monkeypatch, lambda: expert_linear(xi, w, offsets, bias=randn_like(w), swiglu=swiglu))
         agree(monkeypatch, lambda: expert_linear(xi, w, whole, tokens=tokens))
     agree(monkeypatch, lambda: expert_linear(x, dequantize_mxfp4(w), offsets))
-    out = torch.empty(rows, 192, dtype=torch.bfloat16, device=device)
-    assert torch.equal(mxfp4_linear(x, dense, out=out), mxfp4_linear(x, dense))
+    apart = torch.zeros(rows, 210, dtype=torch.bfloat16, device=device)
+    for out in (torch.empty(rows, 192, dtype=torch.bfloat16, device=device), apart[:, 5:197]):
+        for a in both(monkeypatch, lambda: mxfp4_linear(x, dense, out=out)):
+            assert a is out and torch.equal(out, mxfp4_linear(x, dense))
+    assert not apart[:, :5].any() and not apart[:, 197:].any()
 
 
 def randn_like(w):
@@ -70,6 +73,21 @@ def test_routing_and_combine(monkeypatch, tokens, device):
     agree(monkeypatch, lambda: combine_experts(rows, r.positions, r.weights))
     agree(monkeypatch, lambda: combine_experts(rows, r.positions, r.weights, base=base))
     agree(monkeypatch, lambda: route_experts(logits[:0], 4), native=False)
+    expected = combine_experts(rows, r.positions, r.weights, base=base)
+    out = torch.empty(tokens, 264, dtype=torch.bfloat16, device=device)[:, 8:]
+    for a in both(monkeypatch, lambda: combine_experts(rows, r.positions, r.weights, base=base, out=out)):
+        assert a is out and torch.equal(out, expected)
+    bases = iter([base.clone() for _ in range(3)])  # in place, each call on a base of its own
+
+    def onto():
+        b = next(bases)
+        return combine_experts(rows, r.positions, r.weights, base=b, out=b)
+
+    for a in both(monkeypatch, onto):
+        assert torch.equal(a, expected)
+    for other in (dict(), dict(base=rows[:tokens])):
+        with pytest.raises(ValueError, match="share storage"):
+            combine_experts(rows, r.positions, r.weights, out=rows[1 : tokens + 1], **other)
 
 
 def test_refusals_stay_the_operators_own(device):
