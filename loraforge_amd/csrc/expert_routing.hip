@@ -10,6 +10,12 @@
 // Order: choices sorted by expert, then by token and choice. Integer counts
 // only, each place computed from counts of what precedes it, so no result
 // depends on the order in which workgroups run.
+//
+// Bound by latency: loads, k dependent maxima, barriers, and for more than 64 tokens a
+// second launch, which needs all counts. 128 experts, top 8: 16 tokens 4.8 us in one
+// workgroup; 8191 tokens 5.5 us to choose and 5.8 to order (with a wave for each token
+// in turn, and places by counting choices wave by wave, 11.2 and 13.0). The sum is
+// HBM-bound: 8191 tokens of 8 rows of 4096 take 119 us (5.1 TB/s, a copy's rate).
 #include "common.h"
 #include "../../include/loraforge_amd.h"
 
