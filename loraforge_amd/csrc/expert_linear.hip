@@ -36,31 +36,31 @@ struct Costs {
 constexpr Costs kCosts[3] = {
     // bf16 x and weights
     {{
-         {{4.63f, 0.241f, 0.077f}, {5.00f, 0.323f, 0.171f}, {6.31f, 0.415f, 0.214f}, {5.61f, 0.433f, 0.265f}},
-         {{5.61f, 0.321f, 0.076f}, {6.02f, 0.367f, 0.181f}, {8.71f, 0.437f, 0.249f}, {8.34f, 0.541f, 0.324f}},
-         {{6.27f, 0.423f, 0.074f}, {7.25f, 0.418f, 0.212f}, {12.50f, 0.546f, 0.267f}, {7.93f, 0.773f, 0.428f}},
-         {{6.92f, 0.401f, 0.152f}, {9.45f, 0.494f, 0.321f}, {12.35f, 0.729f, 0.438f}, {10.18f, 0.934f, 0.588f}}},
-     {1.74f, 0.49f, 3.02f, 18.08f},
-     {{1.55f, 1.81f, 0.20f, 0.80f, 0.84f, 1.04f},
-      {2.39f, 0.00f, 0.81f, 1.00f, 5.77f, 0.45f}}},
+         {{4.57f, 0.230f, 0.081f}, {5.02f, 0.307f, 0.177f}, {6.20f, 0.395f, 0.230f}, {5.69f, 0.424f, 0.284f}},
+         {{5.61f, 0.298f, 0.078f}, {6.10f, 0.363f, 0.194f}, {8.72f, 0.436f, 0.268f}, {8.67f, 0.536f, 0.361f}},
+         {{6.14f, 0.399f, 0.087f}, {7.65f, 0.407f, 0.230f}, {12.39f, 0.557f, 0.290f}, {8.45f, 0.769f, 0.468f}},
+         {{6.99f, 0.407f, 0.155f}, {9.75f, 0.495f, 0.343f}, {12.54f, 0.725f, 0.466f}, {10.66f, 0.936f, 0.634f}}},
+     {1.86f, 0.45f, 3.02f, 18.04f},
+     {{1.54f, 1.83f, 0.19f, 0.81f, 0.86f, 1.02f},
+      {2.38f, 0.00f, 0.80f, 1.01f, 5.81f, 0.42f}}},
     // bf16 x, MXFP4 weights
     {{
-         {{4.62f, 0.311f, 0.051f}, {4.83f, 0.363f, 0.076f}, {6.19f, 0.456f, 0.085f}, {5.67f, 0.474f, 0.134f}},
-         {{5.27f, 0.431f, 0.047f}, {5.73f, 0.445f, 0.079f}, {8.63f, 0.570f, 0.082f}, {7.56f, 0.686f, 0.152f}},
-         {{6.12f, 0.527f, 0.058f}, {7.12f, 0.562f, 0.097f}, {11.34f, 0.721f, 0.116f}, {9.36f, 0.904f, 0.145f}},
-         {{6.75f, 0.512f, 0.106f}, {8.74f, 0.661f, 0.172f}, {15.07f, 0.922f, 0.138f}, {13.36f, 1.136f, 0.275f}}},
-     {1.57f, 1.91f, 1.90f, 4.11f},
-     {{1.70f, 1.40f, 0.00f, 0.73f, 0.00f, 1.11f},
-      {1.48f, 2.02f, 0.20f, 0.84f, 0.24f, 1.30f}}},
+         {{4.65f, 0.310f, 0.046f}, {4.90f, 0.360f, 0.075f}, {6.15f, 0.442f, 0.089f}, {5.67f, 0.472f, 0.132f}},
+         {{5.25f, 0.416f, 0.050f}, {5.83f, 0.440f, 0.081f}, {8.72f, 0.572f, 0.084f}, {7.54f, 0.683f, 0.164f}},
+         {{6.09f, 0.510f, 0.056f}, {7.26f, 0.556f, 0.098f}, {11.39f, 0.718f, 0.127f}, {9.62f, 0.901f, 0.160f}},
+         {{6.87f, 0.504f, 0.103f}, {8.78f, 0.655f, 0.195f}, {15.11f, 0.920f, 0.187f}, {13.46f, 1.123f, 0.358f}}},
+     {1.57f, 1.91f, 1.91f, 4.08f},
+     {{1.70f, 1.40f, 0.00f, 0.74f, 0.00f, 1.10f},
+      {1.52f, 2.01f, 0.20f, 0.84f, 0.24f, 1.30f}}},
     // MXFP4 x and weights
     {{
-         {{5.03f, 0.339f, 0.198f}, {5.43f, 0.431f, 0.301f}, {6.33f, 0.542f, 0.361f}, {5.39f, 0.630f, 0.524f}},
-         {{5.73f, 0.432f, 0.220f}, {6.25f, 0.501f, 0.296f}, {8.10f, 0.637f, 0.370f}, {7.04f, 0.731f, 0.541f}},
-         {{5.87f, 0.555f, 0.242f}, {6.32f, 0.685f, 0.375f}, {10.43f, 0.744f, 0.354f}, {8.60f, 0.937f, 0.430f}},
-         {{5.46f, 0.695f, 0.306f}, {7.15f, 0.788f, 0.441f}, {12.95f, 0.882f, 0.373f}, {10.37f, 1.087f, 0.625f}}},
-     {2.30f, 1.56f, 1.06f, 4.08f},
-     {{1.62f, 1.70f, 0.08f, 0.38f, 0.40f, 0.48f},
-      {1.44f, 2.08f, 0.35f, 0.45f, 0.86f, 0.49f}}},
+         {{5.05f, 0.339f, 0.192f}, {5.48f, 0.420f, 0.301f}, {6.37f, 0.526f, 0.351f}, {5.35f, 0.623f, 0.517f}},
+         {{5.71f, 0.418f, 0.224f}, {6.30f, 0.494f, 0.293f}, {8.21f, 0.631f, 0.376f}, {6.94f, 0.735f, 0.540f}},
+         {{5.87f, 0.543f, 0.232f}, {6.32f, 0.695f, 0.356f}, {10.66f, 0.744f, 0.357f}, {8.62f, 0.935f, 0.444f}},
+         {{5.59f, 0.680f, 0.308f}, {7.13f, 0.788f, 0.443f}, {12.74f, 0.884f, 0.394f}, {10.35f, 1.083f, 0.664f}}},
+     {2.31f, 1.56f, 1.06f, 4.12f},
+     {{1.66f, 1.68f, 0.08f, 0.38f, 0.42f, 0.48f},
+      {1.47f, 2.04f, 0.35f, 0.45f, 0.91f, 0.48f}}},
 };
 
 constexpr double kCus = 256;
@@ -73,7 +73,7 @@ double passes(double each, double cap, bool grouped) {
 
 double tile_us(const Costs& c, int rows, int columns, double each, double used, bool grouped, double width, double stages) {
   const double per = passes(each, rows, grouped);
-  const double height = std::min(rows / 64.0, std::max(1.0, grouped ? each / per / 64.0 + 0.5 : std::ceil(std::ceil(each / per) / 64.0)));
+  const double height = std::min(rows / 64.0, std::max(1.0, grouped ? (each / 64.0 + 0.5) / per : std::ceil(std::ceil(each / 64.0) / per)));
   const int low = std::min(3, int(height)), high = std::min(4, low + 1), j = columns / 64 - 1;
   const double part = height - low;
   auto mix = [&](float Costs::Tile::*m) { return (1.0 - part) * (c.tile[low - 1][j].*m) + part * (c.tile[high - 1][j].*m); };
@@ -87,8 +87,8 @@ double tile_us(const Costs& c, int rows, int columns, double each, double used, 
   return kLaunch + full * round + (rest > 0 ? fixed - kLaunch + stages * (stage + busy * rest) : 0.0);
 }
 
-// The plan of least time. (Against the fastest plan of each of those products: 1.8 to
-// 4.7 % slower on average by type, 61 % at most: 3 rows, n and k 1024, 7.1 and 4.4 us.)
+// The plan of least time. (Against the fastest plan of each of those products: 1.6 to
+// 4.8 % slower on average by type, 63 % at most: 256 tokens over 64 experts, n and k 1024, 21 and 13 us.)
 lf_expert_plan plan_of(const lf_expert_product& a) {
   const Costs& c = kCosts[a.x_scales ? 2 : a.w_scales ? 1 : 0];
   const bool grouped = a.offsets != nullptr && a.experts > 1;
