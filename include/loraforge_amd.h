@@ -343,7 +343,7 @@ int lf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t blo
  * offsets[e] .. offsets[e + 1] (tokens NULL: x[p]); fp32 sums, rounded once.
  * x bf16 [x_rows, k] with row stride x_stride, or packed MXFP4 with x_scales
  * (contiguous; then w is MXFP4 too); w [experts, n, k] bf16, or packed with
- * w_scales. k % 32 == 0 with an MXFP4 weight, else k % 8 == 0; x rows and w
+ * w_scales. k % 32 == 0 with an MXFP4 weight, else k % 8 == 0, k below 2^30 - 2^16; x rows and w
  * 16-byte aligned. offsets NULL: one expert with all `rows` (the dense
  * product). swiglu: w rows [0, n/2) gate, [n/2, n) up, y = silu(gate) * up in
  * fp32, n/2 columns. Rows of y that belong to no expert are not written. Bounds

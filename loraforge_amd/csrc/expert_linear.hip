@@ -137,8 +137,8 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   LF_REQUIRE(a != nullptr, "null pointer argument");
   LF_REQUIRE(a->rows >= 0 && a->x_rows >= 0 && a->n >= 1 && a->experts >= 1, "sizes must be positive");
   LF_REQUIRE(a->rows < (int64_t(1) << 31) - 65536 && a->x_rows < (int64_t(1) << 31) && a->n < (int64_t(1) << 31) - 65536 &&
-                 a->k < (int64_t(1) << 31) - 65536 && a->experts < 65536,
-             "sizes must fit signed int32 indexing, experts 65535");
+                 a->k < (int64_t(1) << 30) - 65536 && a->experts < 65536,
+             "sizes must fit signed int32 indexing (of a row's bytes: k below 2^30 - 2^16), experts 65535");
   const bool x_mx = a->x_scales != nullptr, w_mx = a->w_scales != nullptr;
   LF_REQUIRE(w_mx || !x_mx, "MXFP4 x needs an MXFP4 weight");
   LF_REQUIRE(a->k >= 1 && a->k % (w_mx ? 32 : 8) == 0, "k must be a multiple of 32 (MXFP4 weight) or 8 (bf16)");

@@ -99,6 +99,8 @@ def test_c_entry_points_refuse_without_device_work():
         (dict(x_rows=1), "each row"),
         (dict(y=None), "null"),
         (dict(rows=2**31), "int32"),
+        (dict(k=2**30, x_stride=2**30), "a row's bytes"),
+        (dict(w_scales=None, k=2**30, x_stride=2**30), "a row's bytes"),
         (dict(n=0), "positive"),
     ],
 )
