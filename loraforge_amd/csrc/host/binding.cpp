@@ -805,23 +805,24 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (stride < experts) return decline();
   void* stream;
   if (!current(x->device(), &stream)) return decline();
-  // One allocation for the five results (each at a multiple of 16 bytes) and the
-  // workspace behind them: five more calls of the allocator took 3 us of a call of 16 tokens.
+  // One allocation for the four integer results (each at a multiple of 16 bytes) and the
+  // workspace behind them: four more calls of the allocator took 3 us of a call of 16 tokens.
+  // (The weights have their own: torch.save refuses a storage that is seen as two types.)
   const int64_t need = g_route_ws(count, int32_t(experts));
   const auto padded = [](int64_t n) { return (n + 3) / 4 * 4; };
   const int64_t each = padded(count * top);
-  const at::Tensor all = at::empty({4 * each + padded(experts + 1) + (need + 3) / 4}, x->options().dtype(at::kInt));
-  if (!on_gpu(all)) return decline();
-  const auto part = [&](int64_t at, c10::IntArrayRef sizes, at::ScalarType type) {
-    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+  at::Tensor weights = at::empty({count, top}, x->options().dtype(at::kFloat));
+  const at::Tensor all = at::empty({3 * each + padded(experts + 1) + (need + 3) / 4}, x->options().dtype(at::kInt));
+  if (!on_gpu(weights) || !on_gpu(all)) return decline();
+  const auto part = [&](int64_t at, c10::IntArrayRef sizes) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
     t.unsafeGetTensorImpl()->set_storage_offset(at);
     t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
     return t;
   };
-  at::Tensor weights = part(0, {count, top}, at::kFloat), chosen = part(each, {count, top}, at::kInt);
-  at::Tensor tokens = part(2 * each, {count * top}, at::kInt), positions = part(3 * each, {count, top}, at::kInt);
-  at::Tensor offsets = part(4 * each, {experts + 1}, at::kInt);
-  int32_t* scratch = ptr<int32_t>(&all) + 4 * each + padded(experts + 1);
+  at::Tensor chosen = part(0, {count, top}), tokens = part(each, {count * top}), positions = part(2 * each, {count, top});
+  at::Tensor offsets = part(3 * each, {experts + 1});
+  int32_t* scratch = ptr<int32_t>(&all) + 3 * each + padded(experts + 1);
   const int rc = unlocked([&] {
     return g_route(x->data_ptr(), x->scalar_type() == at::kFloat, count, int32_t(experts), stride, int32_t(top),
                    args[2] == Py_True, ptr<float>(&weights), ptr<int32_t>(&chosen), ptr<int32_t>(&offsets),

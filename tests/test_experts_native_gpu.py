@@ -1,5 +1,7 @@
 """The MXFP4 and expert operators' native call path against their Python path: the same bits, and what it declines is served."""
 
+import io
+
 import pytest
 import torch
 
@@ -126,3 +128,15 @@ def test_refusals_stay_the_operators_own(device):
     shared = torch.zeros(8, 64, dtype=torch.bfloat16, device=device)
     with pytest.raises(ValueError, match="share storage"):
         mxfp4_linear(shared[:4], dense, out=shared[4:, :32])
+
+
+@pytest.mark.parametrize("tokens", [5, 100])
+def test_routing_can_be_saved(tokens, device):
+    """No two results of different types lie in one storage: torch.save refuses such tensors."""
+    r = route_experts(randn(device, tokens, 40), 3)
+    results = (r.weights, r.experts, r.offsets, r.tokens, r.positions)
+    file = io.BytesIO()
+    torch.save(results, file)
+    file.seek(0)
+    for a, b in zip(results, torch.load(file, weights_only=True)):
+        assert torch.equal(a, b)
