@@ -359,7 +359,7 @@ int lf_route_experts(const void* logits, int32_t fp32, int64_t tokens, int32_t e
                      int32_t* positions, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Kernel of a product: the weight stream with k split over the waves of a workgroup
- * (few rows and weights; `columns` weight rows a workgroup: 16 or 32), the one
+ * (few rows and weights; `columns` weight rows a workgroup: 16 or 32; `rows` rows of an expert: 16, 32 or 64), the one
  * with a wave for 16 weight rows (few rows per expert, many weights), or MFMA tiles
  * of at most `rows` x `columns` weight rows (each 64, 128, 192 or 256). */
 #define LF_EXPERT_STREAM 0

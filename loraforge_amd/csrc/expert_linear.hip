@@ -96,7 +96,7 @@ lf_expert_plan plan_of(const lf_expert_product& a) {
   const double used = grouped ? experts * (1.0 - std::pow(1.0 - 1.0 / experts, rows)) : 1.0;
   const double each = rows / used;  // rows of an expert that has any, on average
   const double n = double(a.n), k = double(a.k) / 1024.0;
-  lf_expert_plan best{LF_EXPERT_STREAM, 0, 16};
+  lf_expert_plan best{LF_EXPERT_STREAM, 64, 16};
   double least = std::numeric_limits<double>::infinity();
   // (No plan is faster than the used weights through HBM; of those that are at it, the one with less work.
   // bf16 weights of few rows come at 4.3 TB/s in tiles, 4.9 a wave for 16 of them, 5.5 streamed.)
@@ -106,14 +106,18 @@ lf_expert_plan plan_of(const lf_expert_product& a) {
     us = std::max(us, hbm / rate) + 0.1 * us;
     if (us < least) least = us, best = plan;
   };
-  for (int i = 0; i < 2; ++i) {
-    const Costs::Stream& s = c.stream[i];
-    const double groups = std::ceil(n / (16 << i)) * used / 512.0, busy = std::min(1.0, groups);
-    const double tiles = std::min(4.0, grouped ? std::max(1.0, each / 16.0 + 0.5) : each <= 16 ? 1.0 : each <= 32 ? 2.0 : 4.0);
-    offer(s.fixed + passes(each, 64, grouped) * (s.pass + k * (s.k + s.k_tile * tiles + (s.k_busy + s.k_tile_busy * tiles) * busy)) *
-                        std::max(1.0, groups),
-          {LF_EXPERT_STREAM, 0, 16 << i});
-  }
+  // A dense product may have its rows apart in passes of 16 or 32, so that few weight
+  // rows fill the CUs (87 x 528 x 7424: 12 us, in tiles 39; 64 x 2560 x 6144 20 and 28).
+  for (int i = 0; i < 2; ++i)
+    for (int part = grouped ? 64 : 16; part <= 64; part *= 2) {
+      const Costs::Stream& s = c.stream[i];
+      const double groups = std::ceil(n / (16 << i)) * used * passes(each, part, grouped) / 512.0, busy = std::min(1.0, groups);
+      const double again = grouped ? 0.0 : std::ceil(each / part) - 1.0;  // times that passes read weights that others read
+      const double most = std::min(each, double(part));
+      const double tiles = grouped ? std::min(4.0, std::max(1.0, each / 16.0 + 0.5)) : most <= 16 ? 1.0 : most <= 32 ? 2.0 : 4.0;
+      offer(s.fixed + (s.pass + k * (s.k + s.k_tile * tiles + (s.k_busy + s.k_tile_busy * tiles) * busy)) * std::max(1.0, groups) + again * hbm / 5.5,
+            {LF_EXPERT_STREAM, part, 16 << i});
+    }
   if (rows_fit(a)) {
     const double groups = std::ceil(n / 128.0) * used / 512.0;
     offer(c.rows.fixed + passes(each, 16, grouped) * (c.rows.pass + k * (c.rows.k + c.rows.k_busy * std::min(1.0, groups))) *
@@ -174,7 +178,8 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   auto s = static_cast<hipStream_t>(stream);
   if (plan.kernel == LF_EXPERT_STREAM) {
     LF_REQUIRE(plan.columns == 16 || plan.columns == 32, "stream plan: 16 or 32 columns");
-    return lf::expert::launch_stream(p, plan.columns / 16, s);
+    LF_REQUIRE(plan.rows == 0 || plan.rows == 16 || plan.rows == 32 || plan.rows == 64, "stream plan: 16, 32 or 64 rows (0: 64)");
+    return lf::expert::launch_stream(p, plan.rows ? plan.rows : 64, plan.columns / 16, s);
   }
   if (plan.kernel == LF_EXPERT_ROWS) {
     LF_REQUIRE(lf::expert::rows_fit(*a), "this product cannot run with a wave for 16 weight rows");

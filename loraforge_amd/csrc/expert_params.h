@@ -87,8 +87,8 @@ __device__ __forceinline__ float silu_mul_f32(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
-// `groups`: 16-row groups of weight rows per workgroup (1 or 2).
-int launch_stream(const Params& p, int groups, hipStream_t stream);
+// `part`: rows per workgroup (16, 32 or 64); `groups`: 16-row groups of weight rows (1 or 2).
+int launch_stream(const Params& p, int part, int groups, hipStream_t stream);
 int launch_rows(const Params& p, hipStream_t stream);
 // Tiles of at most `cap` rows x `columns` weight rows (one translation unit per pair of types).
 int launch_tiles_bf16(const Params& p, int cap, int columns, hipStream_t stream);

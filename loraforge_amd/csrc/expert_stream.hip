@@ -2,7 +2,8 @@
 // once and multiplied by the handful of rows of its expert, so the kernel is
 // bound by HBM, at the smallest sizes by latency.
 //
-// A workgroup owns 16 kF weight rows of one expert over the whole of k; its
+// A workgroup owns 16 kF weight rows of one expert over the whole of k, and up to 64 of
+// the expert's rows (16 or 32 where that leaves CUs idle: the weights then come from L2 again); its
 // eight waves take every eighth step of 128 k, so that together they read 512
 // (MXFP4) or 2048 (bf16) consecutive bytes of a row. Weights go from memory
 // straight into the operand layout of the matrix instructions (nobody else
@@ -163,44 +164,51 @@ __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg,
     const float v = p.swiglu ? silu_mul_f32(total(r, row), total(r + 8 * kF, row)) : total(r, row);
     p.y[int64_t(first + row) * p.y_stride + n] = uint16_t(f32_to_bf16(v));
   }
-  __syncthreads();
 }
 
-// Grid: column blocks x experts that have rows.
+// Grid: column blocks x passes of `part` rows (16, 32 or 64) of the experts (y, then z).
+// (A loop over passes in the kernel takes its registers past 128, into scratch.)
 template <bool kXMx, bool kWMx, int kF>
-__global__ __launch_bounds__(kThreads, 4) void stream_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, 4) void stream_kernel(Params p, int part) {
   __shared__ float red[kWaves * kF * kRowTiles * 256];
-  int index = blockIdx.y;
-  const Segment seg = find_segment(p, index, [](const Segment& s) { return s.end > s.begin ? 1 : 0; });
+  int index = int(blockIdx.z * gridDim.y + blockIdx.y);
+  Segment seg = find_segment(p, index, [&](const Segment& s) { return (s.end - s.begin + part - 1) / part; });
+  if (seg.end <= seg.begin) return;
+  seg.begin += index * part;
+  seg.end = min(seg.end, seg.begin + part);
   const int rows = seg.end - seg.begin;
-  if (rows <= 0) return;
   if (rows <= 16) {
     stream_rows<kXMx, kWMx, kF, 1>(p, seg, seg.begin, blockIdx.x, red);
   } else if (rows <= 32) {
     stream_rows<kXMx, kWMx, kF, 2>(p, seg, seg.begin, blockIdx.x, red);
   } else {
-    for (int first = seg.begin; first < seg.end; first += 64) stream_rows<kXMx, kWMx, kF, 4>(p, seg, first, blockIdx.x, red);
+    stream_rows<kXMx, kWMx, kF, 4>(p, seg, seg.begin, blockIdx.x, red);
   }
 }
 
 template <bool kXMx, bool kWMx>
-int launch_types(const Params& p, int groups, hipStream_t stream) {
-  const int segments = p.offsets ? (p.experts < p.rows ? p.experts : p.rows) : 1;
+int launch_types(const Params& p, int part, int groups, hipStream_t stream) {
+  // At most: a pass more than whole ones for every expert that has a row.
+  const int64_t used = p.offsets ? (p.experts < p.rows ? p.experts : p.rows) : 1;
+  const int64_t passes = (p.rows + used * (part - 1)) / part;
+  constexpr int64_t kMostY = 65535;
   const int64_t columns = (p.swiglu ? 8 : 16) * groups;
-  const dim3 grid(unsigned((p.width + columns - 1) / columns), unsigned(segments)), threads(kThreads);
+  const dim3 grid(unsigned((p.width + columns - 1) / columns), unsigned(passes < kMostY ? passes : kMostY),
+                  unsigned((passes + kMostY - 1) / kMostY)),
+      threads(kThreads);
   if (groups == 2)
-    hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 2>), grid, threads, 0, stream, p);
+    hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 2>), grid, threads, 0, stream, p, part);
   else
-    hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 1>), grid, threads, 0, stream, p);
+    hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 1>), grid, threads, 0, stream, p, part);
   LF_HIP(hipGetLastError());
   return kOk;
 }
 
 }  // namespace
 
-int launch_stream(const Params& p, int groups, hipStream_t stream) {
-  if (p.xs) return launch_types<true, true>(p, groups, stream);
-  return p.ws ? launch_types<false, true>(p, groups, stream) : launch_types<false, false>(p, groups, stream);
+int launch_stream(const Params& p, int part, int groups, hipStream_t stream) {
+  if (p.xs) return launch_types<true, true>(p, part, groups, stream);
+  return p.ws ? launch_types<false, true>(p, part, groups, stream) : launch_types<false, false>(p, part, groups, stream);
 }
 
 }  // namespace expert

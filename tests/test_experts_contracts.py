@@ -118,6 +118,16 @@ def plan(**sizes):
     return p
 
 
+def test_stream_plans_of_few_weight_rows():
+    """Rows in passes of their own where a product's weight rows would leave CUs idle; refusal of other heights."""
+    p = plan(rows=96, x_rows=96, n=528, k=7424, w_scales=16)
+    assert (p.kernel, p.rows) == (_lib.LF_EXPERT_STREAM, 16)
+    assert plan(rows=1024, x_rows=1024, n=528, k=7424, w_scales=16).kernel == _lib.LF_EXPERT_TILE
+    a = _lib.ExpertProduct(x=16, w=16, w_scales=16, y=16, x_stride=64, x_rows=2, rows=2, n=32, k=64, experts=1, y_stride=32)
+    a.plan = ctypes.pointer(_lib.ExpertPlan(_lib.LF_EXPERT_STREAM, 48, 16))
+    refused("16, 32 or 64 rows", _lib.library().lf_expert_linear(ctypes.byref(a), None))
+
+
 def test_plans():
     """Few rows stream the weights, many run in tiles, and what a kernel cannot take does not."""
     for rows in (1, 8, 16):

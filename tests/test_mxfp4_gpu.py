@@ -394,3 +394,39 @@ def test_scales_and_rows_at_odd_addresses(types, device):
     for plan in PLANS[1], PLANS[2], PLANS[3], PLANS[-1]:
         y = forced(x, w, plan, experts=1, offsets=segments([m]).to(device), tokens=tokens)
         close(y, *ox.product(xv[::-1], wv[0]))
+
+
+@pytest.mark.parametrize("types", TYPES, ids="-".join)
+@pytest.mark.parametrize("columns", [16, 32])
+@pytest.mark.parametrize("part", [16, 32, 64])
+def test_streamed_rows_in_passes(part, columns, types, device):
+    """A workgroup for each pass of 16, 32 or 64 rows: whole and broken passes, of ragged experts and of a dense product."""
+    act, weight = types
+    plan = (_lib.LF_EXPERT_STREAM, part, columns)
+    n, k = 104, 544
+    counts = [16, 0, 33, 64, 1, 131, 0]
+    x, xv = operand(randn(1, sum(counts), k), act, device)
+    w, wv = operand(randn(2, len(counts), n, k, std=0.05), weight, device)
+    y = forced(x, w, plan, experts=len(counts), offsets=segments(counts).to(device))
+    start = 0
+    for e, count in enumerate(counts):
+        if count:
+            close(y[start : start + count], *ox.product(xv[start : start + count], wv[e], None))
+        start += count
+    if weight == "mxfp4":
+        for m in (15, 64, 97):
+            x, xv = operand(randn(m, m, k), act, device)
+            dense, dv = operand(randn(3, n, k, std=0.05), weight, device)
+            close(forced(x, dense, plan), *ox.product(xv, dv, None))
+
+
+def test_passes_past_the_second_grid_dimension(device):
+    """65536 passes of 16 rows: more than a grid's second dimension holds."""
+    m = 65536 * 16 - 3
+    w, wv = operand(randn(4, 2, 32, std=0.5), "mxfp4", device)
+    x, xv = operand(randn(5, 64, 32), "bf16", device)
+    rows = torch.arange(m, device=device) % 64
+    y = forced(x[rows], w, (_lib.LF_EXPERT_STREAM, 16, 16))
+    first = forced(x, w, (_lib.LF_EXPERT_STREAM, 64, 16))
+    close(first, *ox.product(xv, wv, None))
+    assert torch.equal(y, first[rows])
