@@ -88,7 +88,8 @@ double tile_us(const Costs& c, int rows, int columns, double each, double used, 
 }
 
 // The plan of least time. (Against the fastest plan of each of those products: 1.6 to
-// 4.8 % slower on average by type, 63 % at most: 256 tokens over 64 experts, n and k 1024, 21 and 13 us.)
+// 4.8 % slower on average by type, 63 % at most: 256 tokens over 64 experts, n and k 1024, 21 and 13 us.
+// Over 80 dense products of 8..384 rows, n 528..8192: 10 % with bf16 x, 6 % with MXFP4 x, 43 % at most.)
 lf_expert_plan plan_of(const lf_expert_product& a) {
   const Costs& c = kCosts[a.x_scales ? 2 : a.w_scales ? 1 : 0];
   const bool grouped = a.offsets != nullptr && a.experts > 1;
@@ -115,7 +116,8 @@ lf_expert_plan plan_of(const lf_expert_product& a) {
       const double again = grouped ? 0.0 : std::ceil(each / part) - 1.0;  // times that passes read weights that others read
       const double most = std::min(each, double(part));
       const double tiles = grouped ? std::min(4.0, std::max(1.0, each / 16.0 + 0.5)) : most <= 16 ? 1.0 : most <= 32 ? 2.0 : 4.0;
-      offer(s.fixed + (s.pass + k * (s.k + s.k_tile * tiles + (s.k_busy + s.k_tile_busy * tiles) * busy)) * std::max(1.0, groups) + again * hbm / 5.5,
+      offer(s.fixed + (s.pass + k * (s.k + s.k_tile * tiles + (s.k_busy + s.k_tile_busy * tiles) * busy)) * std::max(1.0, groups) +
+                again * hbm / 5.5,
             {LF_EXPERT_STREAM, part, 16 << i});
     }
   if (rows_fit(a)) {
