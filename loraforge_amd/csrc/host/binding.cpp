@@ -864,7 +864,8 @@ PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* stream;
   if (!current(dev, &stream)) return decline();
   Output out(args[4], count, n, dev);
-  const bool onto = base && out.data() == ptr<uint16_t>(base) && out.stride == base_stride;  // (in place)
+  // In place. (An output that was not taken has no memory to ask for: ok() below declines it.)
+  const bool onto = base && out.given && ptr<uint16_t>(out.given) == ptr<uint16_t>(base) && out.stride == base_stride;
   if (!out.ok({rows, positions, weights, onto ? nullptr : base})) return decline();
   const int rc = unlocked([&] {
     return g_combine(ptr<uint16_t>(rows), rows->size(0), rows_stride, ptr<int32_t>(positions), ptr<float>(weights), count,
