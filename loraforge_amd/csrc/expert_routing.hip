@@ -380,7 +380,9 @@ extern "C" int lf_route_experts(const void* logits, int32_t fp32, int64_t tokens
   LF_REQUIRE(tokens >= 0 && experts >= 1 && experts <= lf::kMaxExperts, "experts must be in 1..%d", lf::kMaxExperts);
   LF_REQUIRE(top >= 1 && top <= lf::kMaxTop && top <= experts, "top_k must be in 1..min(experts, %d)", lf::kMaxTop);
   LF_REQUIRE(stride >= experts, "the row stride must cover the experts");
-  LF_REQUIRE(tokens * top < (int64_t(1) << 31) - (int64_t(1) << 16), "tokens * top_k must fit signed int32 indexing");
+  // (The count itself first: its product with top wraps round in 64 bits from 2^57 on.)
+  LF_REQUIRE(tokens < (int64_t(1) << 31) && tokens * top < (int64_t(1) << 31) - (int64_t(1) << 16),
+             "tokens * top_k must fit signed int32 indexing");
   LF_REQUIRE(offsets != nullptr, "null pointer argument");
   LF_REQUIRE(tokens == 0 || (logits && weights && chosen && token_of && positions), "null pointer argument");
   const int64_t need = lf_route_experts_workspace_size(tokens, experts);
