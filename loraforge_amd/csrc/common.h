@@ -80,9 +80,10 @@ __device__ __forceinline__ float round_bf16(float a) { return bf16_to_f32(f32_to
 //    to d near 2^128), skipped where 1 + e^-g overflowed (g below about
 //    -88.7: silu -0, as g / inf) or the quotient is infinite; silu has the
 //    sign of g, which also keeps -0 for g = -0.
-// Every SwiGLU path (lf_swiglu and the fused decode and prefill epilogues)
-// uses this one function, so a fused activation and the linear followed by
-// lf_swiglu give identical bits.
+// Every SwiGLU path of the NF4 linears (lf_swiglu and the fused decode and prefill
+// epilogues) uses this one function, so a fused activation and the linear followed by
+// lf_swiglu give identical bits. (The products with MXFP4 weights and of experts
+// round once, at the end: expert_params.h.)
 __device__ __forceinline__ float silu_times(float g, float u) {
   constexpr float kNegLog2eHi = -1.44269502162933349609375f;    // -log2(e) rounded to fp32
   constexpr float kNegLog2eLo = -1.925963033500011079e-08f;      // -log2(e) - kNegLog2eHi

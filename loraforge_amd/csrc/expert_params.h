@@ -78,10 +78,11 @@ __device__ __forceinline__ int64_t x_row_of(const Params& p, int pos) {
 }
 
 // SwiGLU in fp32: g / (1 + e^-g) * u from the hardware exp2 and reciprocal (1 ulp
-// each). The rounding of the exponent is worth |g| 2^-24 of the result, and past
-// g = -87.3 the reciprocal gives 0 for less than 1e-36: nothing beside the
-// rounding to bf16 that follows, at a third of the instructions of a correctly
-// rounded quotient (a 256 x 256 tile's epilogue 21.9k -> 12.5k cycles).
+// each). The rounding of the exponent is worth |g| 2^-24 of the result, little beside the
+// rounding to bf16 that follows; past g = -87.3 the reciprocal gives 0 where |silu(g)| is below
+// 1e-36, as the quotient in 32 bits does past -88.7. A third of the instructions of a correctly
+// rounded quotient (a 256 x 256 tile's epilogue 21.9k -> 12.5k cycles). Silu itself is not
+// rounded to bf16 here, as silu_times does for the paths that follow a reference which does.
 __device__ __forceinline__ float silu_mul_f32(float g, float u) {
   const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896341f);
   return g * __builtin_amdgcn_rcpf(1.0f + e) * u;

@@ -4,8 +4,8 @@
 // Choice: p = softmax(logits) over the experts of a token; the k largest
 // logits, of equal ones the lowest expert first; weight p_e, or p_e over the
 // sum of the chosen p. -inf: not allowed (fewer than k allowed experts leave
-// choices of expert -1 and weight 0). A token whose logits hold NaN or +inf has
-// NaN weights (NaN ranks below every number), as the formula gives.
+// choices of expert -1 and weight 0). A token whose logits hold NaN or +inf has NaN
+// weights for its choices, as the formula gives (NaN ranks with -inf: it is not chosen).
 //
 // Order: choices sorted by expert, then by token and choice. Integer counts
 // only, each place computed from counts of what precedes it, so no result

@@ -6,7 +6,8 @@
 // whole 128-byte row pieces: fragments loaded straight into the operand layout
 // (16 rows, one per lane) take the address unit 64 cycles a load, four times a copy's, and
 // bounded the kernel that splits k over its waves (expert_stream.hip) at 3.9 TB/s (24
-// tokens over 64 experts, top 4, 4096 x 4096 with SwiGLU: 114 us); this one takes 72.
+// tokens over 64 experts, top 4, 4096 x 4096 with SwiGLU: 114 us); this one takes 72, with
+// MXFP4 x as well (72-73 with its quantisation).
 //
 // Each wave streams its weights through a ring of three stages (16 rows x 128 bytes:
 // 256 k in MXFP4, 64 in bf16) without meeting the others; x comes in chunks of 8 KiB

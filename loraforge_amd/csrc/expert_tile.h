@@ -19,13 +19,20 @@
 // as can be, as even as can be, so that an expert costs what its rows need: the body
 // is chosen by the tile's rows. (With tiles of one height, 300 rows ran as 384.)
 //
-// What bounds it: at full tiles the board's power. Of a 256 x 256 tile's loop the
-// matrix instructions fill four fifths (2180 clocks of a stage's 2700 in MXFP4, 2110 of
-// 2440 in bf16), at 1.6 and 1.3 GHz of the card's 2.4; each step that
-// gave them more of it (scale handling, bank conflicts, the next tile's start under
-// this one's epilogue) lowered the clock by nearly as much. 4096 x 12288 x 4096: bf16 330-345
-// us (1.25 PFLOP/s; a library's product of 8192 cubed reaches 1.29), MXFP4 weights
-// 335-347, MXFP4 both 111-121 (3.6 PFLOP/s). Small tiles wait for LDS reads, few tiles leave CUs idle.
+// What bounds it, by clock stamps in a copy that records them. 4096 x 12288 x 4096, 768 tiles
+// of 256 x 256, three a CU; a stage's 64 matrix instructions of 32 clocks are 2048 of its clocks:
+//
+//                clocks of a tile: start   loop              end     all      matrix  clock     product
+//   bf16                           9.1k    150.9k (64 x 2358)  10.7k   170.7k   77 %    1.62 GHz  326-346 us
+//   MXFP4 weights                  7.5k    185.2k (64 x 2894)  10.7k   203.4k   64 %    1.88 GHz  331-340 us
+//   MXFP4 both                     7.1k    44.9k (16 x 2804)   10.9k   62.8k    52 %    1.65 GHz  111-112 us
+//
+// (Start: segment, addresses, first copies; end: the epilogue.) In bf16 the loop, which the matrix
+// instructions fill to 87 %, at a clock that falls under load (2.4 GHz without): MXFP4 weights cost
+// a fifth more clocks and the same time. 1.26 PFLOP/s (a library's product of 8192 cubed reaches 1.23).
+// With MXFP4 on both sides the loop is a quarter as long and start and end are 29 % of
+// a tile: 3.7 PFLOP/s. A workgroup takes all of a CU's LDS whatever its tile, so small
+// tiles have nothing beside them to cover their LDS reads; few tiles leave CUs idle.
 #pragma once
 
 #include "expert_params.h"

@@ -4,8 +4,9 @@
 // (clamped at -127), code = e2m1 nearest to x 2^-E, ties to even, saturated at 6. The
 // division by a power of two is exact, so codes do not depend on how they are computed.
 // HBM-bound: 2 or 4 bytes read and 17/32 written an element, and 17/32 read and 2
-// written on the way back: 24576 x 4096 in bf16 43-57 us and 37.7 back (4.5-5.9 and 6.7
-// TB/s; a copy reaches 5.1), 4096 x 4096 8.2 us. Seven rows take 2.2 us each way: one load's latency.
+// written on the way back: 24576 x 4096 in bf16 37-57 us (4.5-6.9 TB/s: the input, used again, may be in the
+// memory-side cache), in fp32 86 us (5.3 TB/s), and 37.7 back (6.7 TB/s; a copy reaches 5.1), 4096 x 4096
+// 8.2 us. Seven rows take 2.2 us each way: one load's latency.
 #include "mxfp4.h"
 #include "../../include/loraforge_amd.h"
 

@@ -52,7 +52,8 @@ def route_experts(logits, top_k: int, *, renormalize: bool = True) -> ExpertRout
     lowest expert first; -inf marks an expert that the token may not choose. A
     weight is the softmax probability over all experts, with ``renormalize``
     divided by the sum of the token's chosen ones. A token whose logits hold NaN or
-    +inf gets NaN weights (NaN ranks below every number).
+    +inf gets NaN weights for its choices (NaN ranks below every number and is not
+    chosen: of NaN and -inf alone, none is).
     """
     import torch
 
