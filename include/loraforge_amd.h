@@ -27,8 +27,10 @@ extern "C" {
  * lf_row_expand gained segments (arguments inserted mid-list).
  * 3: lf_lora gained num_slots (appended).
  * 4: lf_row_expand_tiled added.
- * 5: the MXFP4 and expert entry points added. */
-#define LF_ABI_VERSION 5
+ * 5: the MXFP4 and expert entry points added.
+ * 6: lf_fp8_quantize and lf_fp8_dequantize added, lf_expert_product gained
+ * x_fp8_scales and w_fp8_scales (appended). */
+#define LF_ABI_VERSION 6
 #define LF_OK 0
 #define LF_EINVAL 1
 #define LF_EHIP 2
@@ -326,6 +328,24 @@ int lf_mxfp4_quantize(const void* x, int32_t fp32, int64_t rows, int64_t k, int6
 int lf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t blocks, uint16_t* out, void* stream);
 
 /* --------------------------------------------------------------------------
+ * FP8: e4m3 codes (OCP: up to 448, 0x7f and 0xff NaN) with an fp32 scale for
+ * each 128 values of a row (scale_rows 1) or each 128 x 128 block of a matrix
+ * (scale_rows 128); the last block of a dimension may be shorter. A code stands
+ * for its value times the scale.
+ * lf_fp8_quantize: bf16 x [matrices, rows, k] with row stride x_stride (matrices
+ * rows * x_stride apart), k % 16 == 0, rows 16-byte aligned; codes [matrices,
+ * rows, k], scales [matrices, rows / scale_rows, k / 128] (rounded up), both
+ * contiguous. With A the block's largest magnitude, but at least 2^-100:
+ * scale = A / 448, codes are 448 x / A rounded to nearest, ties to even. A block
+ * that holds infinity or NaN gets scale NaN and zero codes.
+ * lf_fp8_dequantize: the values, rounded to bf16.
+ * ------------------------------------------------------------------------ */
+int lf_fp8_quantize(const uint16_t* x, int64_t matrices, int64_t rows, int64_t k, int64_t x_stride, int32_t scale_rows,
+                    uint8_t* codes, float* scales, void* stream);
+int lf_fp8_dequantize(const uint8_t* codes, const float* scales, int64_t matrices, int64_t rows, int64_t k,
+                      int32_t scale_rows, uint16_t* out, void* stream);
+
+/* --------------------------------------------------------------------------
  * Mixture of experts.
  * lf_route_experts: logits [tokens, experts] bf16 (fp32 != 0: fp32) with row
  * stride `stride`. Each token chooses the `top` experts of largest logit (of
@@ -343,10 +363,11 @@ int lf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t blo
  * offsets[e] .. offsets[e + 1] (tokens NULL: x[p]); fp32 sums, rounded once.
  * x bf16 [x_rows, k] with row stride x_stride, or packed MXFP4 with x_scales
  * (contiguous; then w is MXFP4 too); w [experts, n, k] bf16, or packed with
- * w_scales. k % 32 == 0 with an MXFP4 weight, else k % 8 == 0, k below 2^30 - 2^16; x rows and w
- * 16-byte aligned. offsets NULL: one expert with all `rows` (the dense
+ * w_scales, or e4m3 codes with w_fp8_scales [experts, n / 128, k / 128] (rounded up; x bf16, or
+ * contiguous e4m3 codes with x_fp8_scales [x_rows, k / 128]). k % 32 == 0 with an MXFP4 weight, k % 16
+ * == 0 with an FP8 one, else k % 8 == 0, k below 2^30 - 2^16; x rows and w 16-byte aligned. offsets NULL: one expert with all `rows` (the dense
  * product). swiglu: w rows [0, n/2) gate, [n/2, n) up, y = silu(gate) * up in
- * fp32, n/2 columns. Rows of y that belong to no expert are not written. Bounds
+ * fp32, n/2 columns (of an FP8 weight: n/2 a multiple of 128). Rows of y that belong to no expert are not written. Bounds
  * and tokens outside the buffers are clamped to them.
  *
  * lf_combine_experts: y[t] = base[t] + sum_j weights[t, j] rows[positions[t, j]]
@@ -389,10 +410,12 @@ typedef struct lf_expert_product {
   int64_t experts;
   int32_t swiglu;
   const lf_expert_plan* plan; /* NULL: the library chooses */
+  const float* x_fp8_scales;  /* not NULL: x is FP8 (and w) */
+  const float* w_fp8_scales;  /* not NULL: w is FP8 */
 } lf_expert_product;
 int lf_expert_linear(const lf_expert_product* product, void* stream);
 /* The plan that the library chooses for a product of these sizes, types (whether
- * x_scales, w_scales and offsets are given) and swiglu: host arithmetic. */
+ * its scales and offsets are given) and swiglu: host arithmetic. */
 int lf_expert_linear_plan(const lf_expert_product* product, lf_expert_plan* plan);
 
 int lf_combine_experts(const uint16_t* rows, int64_t num_rows, int64_t rows_stride, const int32_t* positions,

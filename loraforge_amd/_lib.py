@@ -26,7 +26,7 @@ LF_PLAN_PREFILL = 8
 LF_TEST_WITHHOLD_PARTIALS = 0x100
 LF_KERNEL_DECODE, LF_KERNEL_DECODE_WIDE, LF_KERNEL_DECODE_CHUNKS, LF_KERNEL_PREFILL = range(4)
 NOALLOC_SCRATCH_BYTES = 8 * 1024 * 1024
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 # Per device index, filled by the operators' Python paths: fit for the kernels
 # (gfx950), and compute units.
@@ -107,6 +107,8 @@ class ExpertProduct(ctypes.Structure):
         ("experts", c_int64),
         ("swiglu", c_int32),
         ("plan", ctypes.POINTER(ExpertPlan)),
+        ("x_fp8_scales", c_void_p),
+        ("w_fp8_scales", c_void_p),
     ]
 
 
@@ -194,6 +196,8 @@ _PROTOTYPES = {
     "lf_swiglu": (ctypes.c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
     "lf_mxfp4_quantize": (ctypes.c_int, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "lf_mxfp4_dequantize": (ctypes.c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "lf_fp8_quantize": (ctypes.c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p]),
+    "lf_fp8_dequantize": (ctypes.c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p]),
     "lf_route_experts_workspace_size": (c_int64, [c_int64, c_int32]),
     "lf_route_experts": (
         ctypes.c_int,
@@ -255,6 +259,8 @@ _BOUND = (
     "lf_route_experts",
     "lf_expert_linear",
     "lf_combine_experts",
+    "lf_fp8_quantize",
+    "lf_fp8_dequantize",
 )
 
 
@@ -263,13 +269,14 @@ def bind(module, **replaced) -> None:
     import torch
 
     from .ops.fused import LoraBatch
+    from .ops.fp8 import FP8Tensor
     from .ops.mxfp4 import MXFP4Tensor
 
     stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
     device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
     lib = library()
     addresses = tuple(replaced.get(name) or ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _BOUND)
-    module.init(addresses, stream, device, ARCH_OK, WORKSPACES, COMPUTE_UNITS, LoraBatch, MXFP4Tensor)
+    module.init(addresses, stream, device, ARCH_OK, WORKSPACES, COMPUTE_UNITS, LoraBatch, MXFP4Tensor, FP8Tensor)
 
 
 def binding():

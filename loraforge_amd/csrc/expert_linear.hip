@@ -1,4 +1,4 @@
-// C entry point of the products with bf16 or MXFP4 weights: checks and choice of kernel.
+// C entry point of the products with bf16, MXFP4 or FP8 weights: checks and choice of kernel.
 #include <algorithm>
 #include <cmath>
 #include <limits>
@@ -15,12 +15,13 @@ namespace {
 // take is streamed, whatever the rows: MXFP4 both, 4096 x 4096 x 480 58 us where k = 512 takes 15.5
 // in tiles; 2048 rows gathered from 2^20 + 5 of k = 8192 341 us, from 2^20 - 1 45.)
 bool tiles_fit(const lf_expert_product& a) {
+  if (a.w_fp8_scales) return false;
   if (a.x_scales) return a.k >= 512 && std::max(a.x_rows, a.n) * (a.k / 2) < (int64_t(1) << 32);
   return !a.w_scales || a.k >= 128;
 }
 
 // Scales are loaded 16 at a time.
-bool rows_fit(const lf_expert_product& a) { return !a.w_scales || a.k >= 512; }
+bool rows_fit(const lf_expert_product& a) { return !a.w_fp8_scales && (!a.w_scales || a.k >= 512); }
 
 // Times of the kernels in us, fitted to 2586 products (dense ones of 1..4096 rows,
 // n 1024..24576, k 1024..8192; 8..128 experts, 1..8192 tokens), every plan of each.
@@ -93,7 +94,7 @@ double tile_us(const Costs& c, int rows, int columns, double each, double used, 
 // 4.8 % slower on average by type, 63 % at most: 256 tokens over 64 experts, n and k 1024, 21 and 13 us.
 // Over 80 dense products of 8..384 rows, n 528..8192: 10 % with bf16 x, 6 % with MXFP4 x, 43 % at most.)
 lf_expert_plan plan_of(const lf_expert_product& a) {
-  const Costs& c = kCosts[a.x_scales ? 2 : a.w_scales ? 1 : 0];
+  const Costs& c = kCosts[a.x_scales || a.x_fp8_scales ? 2 : a.w_scales || a.w_fp8_scales ? 1 : 0];
   const bool grouped = a.offsets != nullptr && a.experts > 1;
   const double rows = double(a.rows), experts = double(a.experts);
   const double used = grouped ? experts * (1.0 - std::pow(1.0 - 1.0 / experts, rows)) : 1.0;
@@ -148,8 +149,12 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
                  a->k < (int64_t(1) << 30) - 65536 && a->experts < 65536,
              "sizes must fit signed int32 indexing (of a row's bytes: k below 2^30 - 2^16), experts 65535");
   const bool x_mx = a->x_scales != nullptr, w_mx = a->w_scales != nullptr;
+  const bool x_f8 = a->x_fp8_scales != nullptr, w_f8 = a->w_fp8_scales != nullptr;
+  LF_REQUIRE(!(x_mx && x_f8) && !(w_mx && w_f8), "an operand has scales of one type");
   LF_REQUIRE(w_mx || !x_mx, "MXFP4 x needs an MXFP4 weight");
-  LF_REQUIRE(a->k >= 1 && a->k % (w_mx ? 32 : 8) == 0, "k must be a multiple of 32 (MXFP4 weight) or 8 (bf16)");
+  LF_REQUIRE(w_f8 || !x_f8, "FP8 x needs an FP8 weight");
+  LF_REQUIRE(a->k >= 1 && a->k % (w_mx ? 32 : w_f8 ? 16 : 8) == 0, "k must be a multiple of 32 (MXFP4 weight), 16 (FP8) or 8 (bf16)");
+  LF_REQUIRE(!a->swiglu || !w_f8 || a->n % (2 * lf::fp8::kBlock) == 0, "SwiGLU needs whole blocks of 128 FP8 gate and up rows");
   LF_REQUIRE(!a->swiglu || a->n % 2 == 0, "SwiGLU needs gate and up rows of equal number");
   LF_REQUIRE(a->offsets || (a->experts == 1 && !a->tokens), "offsets required for more than one expert or with tokens");
   if (a->rows == 0) return lf::kOk;
@@ -158,13 +163,15 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   const int64_t width = a->swiglu ? a->n / 2 : a->n;
   LF_REQUIRE(a->y_stride >= width, "y_stride must cover the output columns");
   LF_REQUIRE(lf::aligned16(a->x) && lf::aligned16(a->w), "x and w must be 16-byte aligned");
-  LF_REQUIRE(x_mx || (a->x_stride >= a->k && a->x_stride % 8 == 0), "x rows must be 16-byte aligned");
+  LF_REQUIRE(x_mx || x_f8 || (a->x_stride >= a->k && a->x_stride % 8 == 0), "x rows must be 16-byte aligned");
   lf::expert::Params p{};
   p.x = static_cast<const char*>(a->x);
-  p.x_row = x_mx ? a->k / 2 : a->x_stride * 2;
+  p.x_row = x_mx ? a->k / 2 : x_f8 ? a->k : a->x_stride * 2;
   p.xs = a->x_scales;
   p.w = static_cast<const char*>(a->w);
   p.ws = a->w_scales;
+  p.xs8 = a->x_fp8_scales;
+  p.ws8 = a->w_fp8_scales;
   p.bias = a->bias;
   p.offsets = a->offsets;
   p.tokens = a->tokens;

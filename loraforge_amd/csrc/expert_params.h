@@ -1,5 +1,5 @@
-// Parameters of the products with bf16 or MXFP4 weights, dense and grouped by
-// expert (expert_stream.hip, expert_tile.h), and what both kernels share.
+// Parameters of the products with bf16, MXFP4 or FP8 weights, dense and grouped by
+// expert (expert_stream.hip, expert_rows.hip, expert_tile.h), and what the kernels share.
 //
 // Rows offsets[e] .. offsets[e + 1] of the product belong to expert e: row p is
 // x[tokens[p]] (x[p] without tokens) times the transpose of w[e]. The dense
@@ -7,17 +7,23 @@
 // indexes come from device memory; both are clamped to the buffers.
 #pragma once
 
+#include "fp8.h"
 #include "mxfp4.h"
 
 namespace lf {
 namespace expert {
 
+// Types of an operand.
+enum Type : int { kBf16, kMxfp4, kFp8 };
+
 struct Params {
-  const char* x;       // bf16 [x_rows, k], or packed codes
+  const char* x;       // bf16 [x_rows, k], or codes
   int64_t x_row;       // bytes from row to row
-  const uint8_t* xs;   // scale bytes [x_rows, k / 32] of packed x
-  const char* w;       // bf16 or packed [experts, n, k]
-  const uint8_t* ws;   // scale bytes [experts, n, k / 32] of packed w
+  const uint8_t* xs;   // scale bytes [x_rows, k / 32] of MXFP4 x
+  const char* w;       // bf16 or codes [experts, n, k]
+  const uint8_t* ws;   // scale bytes [experts, n, k / 32] of MXFP4 w
+  const float* xs8;    // scales [x_rows, k / 128 rounded up] of FP8 x
+  const float* ws8;    // scales [experts, n / 128, k / 128, both rounded up] of FP8 w
   const uint16_t* bias;    // [experts, n] or null
   const int32_t* offsets;  // [experts + 1], null: one expert with all rows
   const int32_t* tokens;   // [rows] or null
@@ -70,6 +76,11 @@ __device__ __forceinline__ Segment find_segment(const Params& p, int& index, Cou
     index -= __builtin_amdgcn_readlane(sum, 63);
   }
   return {0, 0, 0};
+}
+
+// Scales of the 128-row block that holds row `row` of expert e's FP8 weight, one for each 128 k.
+__device__ __forceinline__ const float* fp8_scales(const Params& p, int e, int row) {
+  return p.ws8 + (int64_t(e) * fp8::blocks_of(p.n) + row / fp8::kBlock) * fp8::blocks_of(p.k);
 }
 
 // Row of x behind row `pos` of the product.

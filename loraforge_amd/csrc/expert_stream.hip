@@ -7,11 +7,13 @@
 // eight waves take every eighth step of 128 k, so that together they read 512
 // (MXFP4) or 2048 (bf16) consecutive bytes of a row. Weights go from memory
 // straight into the operand layout of the matrix instructions (nobody else
-// needs them): v_mfma_f32_16x16x32_bf16 on MXFP4 weights decoded in registers
-// or on bf16 ones, v_mfma_scale_f32_16x16x128_f8f6f4 where x is MXFP4 too.
-// The weight is the A operand, 16 rows of x the B operand. The order of k
-// within a step is free as long as both operands agree on it: with MXFP4 weights
-// lane quarter q holds block q of the step (32 k, one scale), else 8 k of each.
+// needs them): v_mfma_f32_16x16x32_bf16 on MXFP4 or FP8 weights decoded in registers
+// or on bf16 ones, v_mfma_scale_f32_16x16x128_f8f6f4 where x is MXFP4 too, its form without
+// scales where both are FP8. The weight is the A operand, 16 rows of x the B operand. The order of k
+// within a step is free as long as both operands agree on it: with MXFP4 and FP8 weights
+// lane quarter q holds block q of the step (32 k, one MXFP4 scale), else 8 k of each. An FP8
+// scale is that of a whole step: a step's products are summed from zero and added
+// to the sums times x's and the weight's scale, in fp32.
 // The waves' partial sums meet in LDS, in a fixed order.
 #include "expert_params.h"
 
@@ -37,25 +39,33 @@ __device__ __forceinline__ int weight_row(const Params& p, int block, int r) {
 }
 
 // What one step needs of kN operand rows of a lane.
-template <bool kMx, int kN>
+template <int kType, int kN>
 struct Rows {
-  u32x4 v[kN][kMx ? 1 : 4];
-  uint32_t scale[kMx ? kN : 1];
+  u32x4 v[kN][kType == kMxfp4 ? 1 : kType == kFp8 ? 2 : 4];
+  uint32_t scale[kType == kBf16 ? 1 : kN];  // a byte, or a float's bits
 };
 
 struct RowPtr {
   const char* v;
-  const uint8_t* s;
+  const uint8_t* s;   // MXFP4
+  const float* s8;    // FP8: of the rows that the lane's sums belong to
 };
 
 // kBlocked: a lane's k of a step is block q (else 8 k of each block).
-template <bool kMx, bool kBlocked, int kN>
-__device__ __forceinline__ void load_rows(const Params& p, const RowPtr (&row)[kN], int step, int q, Rows<kMx, kN>& r) {
+template <int kType, bool kBlocked, int kN>
+__device__ __forceinline__ void load_rows(const Params& p, const RowPtr (&row)[kN], int step, int q, Rows<kType, kN>& r) {
   const int k0 = step * kStep;
   const bool whole = k0 + kStep <= p.k;
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    if constexpr (kMx) {
+    if constexpr (kType == kFp8) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int at = k0 + 32 * q + 16 * j;
+        r.v[i][j] = load16(whole || at < p.k ? row[i].v + at : reinterpret_cast<const char*>(&kZeros));
+      }
+      r.scale[i] = __float_as_uint(row[i].s8[step]);
+    } else if constexpr (kType == kMxfp4) {
       const int block = k0 / mx::kBlock + q;
       const bool in = whole || block < p.k / mx::kBlock;
       r.v[i][0] = load16(in ? row[i].v + block * 16 : reinterpret_cast<const char*>(&kZeros));
@@ -70,11 +80,33 @@ __device__ __forceinline__ void load_rows(const Params& p, const RowPtr (&row)[k
   }
 }
 
-template <bool kXMx, bool kWMx, int kF, int kT>
-__device__ __forceinline__ void contract(const Rows<kWMx, kF>& w, const Rows<kXMx, kT>& x, f32x4 (&acc)[kF][kT]) {
+template <int kX, int kW, int kF, int kT>
+__device__ __forceinline__ void contract(const Rows<kW, kF>& w, const Rows<kX, kT>& x, f32x4 (&acc)[kF][kT]) {
 #pragma unroll
   for (int f = 0; f < kF; ++f) {
-    if constexpr (kXMx) {
+    if constexpr (kW == kFp8) {
+      f32x4 sum[kT];
+      if constexpr (kX == kFp8) {
+#pragma unroll
+        for (int t = 0; t < kT; ++t) sum[t] = fp8::mfma16(fp8::operand(w.v[f][0], w.v[f][1]), fp8::operand(x.v[t][0], x.v[t][1]));
+      } else {
+#pragma unroll
+        for (int t = 0; t < kT; ++t) sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 codes = w.v[f][j >> 1];
+          const bf16x8 a = __builtin_bit_cast(bf16x8, fp8::decode8(codes[j % 2 * 2], codes[j % 2 * 2 + 1]));
+#pragma unroll
+          for (int t = 0; t < kT; ++t) sum[t] = lf::mfma16(a, __builtin_bit_cast(bf16x8, x.v[t][j]), sum[t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const float s = __uint_as_float(w.scale[f]) * (kX == kFp8 ? __uint_as_float(x.scale[kX == kFp8 ? t : 0]) : 1.0f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[f][t][e] = fmaf(s, sum[t][e], acc[f][t][e]);
+      }
+    } else if constexpr (kX == kMxfp4) {
 #pragma unroll
       for (int t = 0; t < kT; ++t)
         acc[f][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx::operand(w.v[f][0]), mx::operand(x.v[t][0]), acc[f][t],
@@ -83,7 +115,7 @@ __device__ __forceinline__ void contract(const Rows<kWMx, kF>& w, const Rows<kXM
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         u32x4 a;
-        if constexpr (kWMx)
+        if constexpr (kW == kMxfp4)
           a = mx::decode8(w.v[f][0][j], mx::scale_f32(w.scale[f]));
         else
           a = w.v[f][j];
@@ -96,22 +128,24 @@ __device__ __forceinline__ void contract(const Rows<kWMx, kF>& w, const Rows<kXM
 }
 
 // Rows first .. first + 16 kT - 1 (below the segment's end) of the workgroup's columns.
-template <bool kXMx, bool kWMx, int kF, int kT>
+template <int kX, int kW, int kF, int kT>
 __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg, int first, int block, float* red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = lane & 15, q = lane >> 4;
-  const int64_t w_row = kWMx ? p.k / 2 : int64_t(p.k) * 2;
+  const int64_t w_row = kW == kMxfp4 ? p.k / 2 : kW == kFp8 ? p.k : int64_t(p.k) * 2;
   const int blocks = p.k / mx::kBlock;
   RowPtr w[kF], x[kT];
 #pragma unroll
   for (int f = 0; f < kF; ++f) {
     const int64_t row = int64_t(seg.expert) * p.n + weight_row<kF>(p, block, 16 * f + c);
-    w[f] = {p.w + row * w_row, kWMx ? p.ws + row * blocks : nullptr};
+    w[f] = {p.w + row * w_row, kW == kMxfp4 ? p.ws + row * blocks : nullptr,
+            kW == kFp8 ? fp8_scales(p, seg.expert, weight_row<kF>(p, block, 16 * f + 4 * q)) : nullptr};
   }
 #pragma unroll
   for (int t = 0; t < kT; ++t) {
     const int64_t row = x_row_of(p, min(first + 16 * t + c, seg.end - 1));
-    x[t] = {p.x + row * p.x_row, kXMx ? p.xs + row * blocks : nullptr};
+    x[t] = {p.x + row * p.x_row, kX == kMxfp4 ? p.xs + row * blocks : nullptr,
+            kX == kFp8 ? p.xs8 + row * fp8::blocks_of(p.k) : nullptr};
   }
   f32x4 acc[kF][kT];
 #pragma unroll
@@ -120,23 +154,24 @@ __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg,
     for (int t = 0; t < kT; ++t) acc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // Steps requested together: as many as fit 128 registers, two workgroups a CU (an
-  // MXFP4 row takes nine with its scale and addresses).
-  constexpr int kRegs = (kWMx ? 9 : 16) * kF + (kXMx ? 9 : 16) * kT;
+  // MXFP4 row takes nine with its scale and addresses, an FP8 one thirteen).
+  constexpr int kRegsOf[3] = {16, 9, 13};
+  constexpr int kRegs = kRegsOf[kW] * kF + kRegsOf[kX] * kT;
   constexpr int kDepth = kRegs <= 18 ? 4 : kRegs <= 36 ? 2 : 1;
   const int steps = (p.k + kStep - 1) / kStep;
   for (int s = wave; s < steps; s += kDepth * kWaves) {
-    Rows<kWMx, kF> wr[kDepth];
-    Rows<kXMx, kT> xr[kDepth];
+    Rows<kW, kF> wr[kDepth];
+    Rows<kX, kT> xr[kDepth];
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       if (d && s + d * kWaves >= steps) break;
-      load_rows<kWMx, kWMx, kF>(p, w, s + d * kWaves, q, wr[d]);
-      load_rows<kXMx, kWMx, kT>(p, x, s + d * kWaves, q, xr[d]);
+      load_rows<kW, kW != kBf16, kF>(p, w, s + d * kWaves, q, wr[d]);
+      load_rows<kX, kW != kBf16, kT>(p, x, s + d * kWaves, q, xr[d]);
     }
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       if (d && s + d * kWaves >= steps) break;
-      contract<kXMx, kWMx, kF, kT>(wr[d], xr[d], acc);
+      contract<kX, kW, kF, kT>(wr[d], xr[d], acc);
     }
   }
 
@@ -168,7 +203,7 @@ __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg,
 
 // Grid: column blocks x passes of `part` rows (16, 32 or 64) of the experts (y, then z).
 // (A loop over passes in the kernel takes its registers past 128, into scratch.)
-template <bool kXMx, bool kWMx, int kF>
+template <int kX, int kW, int kF>
 __global__ __launch_bounds__(kThreads, 4) void stream_kernel(Params p, int part) {
   __shared__ float red[kWaves * kF * kRowTiles * 256];
   int index = int(blockIdx.z * gridDim.y + blockIdx.y);
@@ -178,15 +213,15 @@ __global__ __launch_bounds__(kThreads, 4) void stream_kernel(Params p, int part)
   seg.end = min(seg.end, seg.begin + part);
   const int rows = seg.end - seg.begin;
   if (rows <= 16) {
-    stream_rows<kXMx, kWMx, kF, 1>(p, seg, seg.begin, blockIdx.x, red);
+    stream_rows<kX, kW, kF, 1>(p, seg, seg.begin, blockIdx.x, red);
   } else if (rows <= 32) {
-    stream_rows<kXMx, kWMx, kF, 2>(p, seg, seg.begin, blockIdx.x, red);
+    stream_rows<kX, kW, kF, 2>(p, seg, seg.begin, blockIdx.x, red);
   } else {
-    stream_rows<kXMx, kWMx, kF, 4>(p, seg, seg.begin, blockIdx.x, red);
+    stream_rows<kX, kW, kF, 4>(p, seg, seg.begin, blockIdx.x, red);
   }
 }
 
-template <bool kXMx, bool kWMx>
+template <int kX, int kW>
 int launch_types(const Params& p, int part, int groups, hipStream_t stream) {
   // At most: a pass more than whole ones for every expert that has a row.
   const int64_t used = p.offsets ? (p.experts < p.rows ? p.experts : p.rows) : 1;
@@ -197,9 +232,9 @@ int launch_types(const Params& p, int part, int groups, hipStream_t stream) {
                   unsigned((passes + kMostY - 1) / kMostY)),
       threads(kThreads);
   if (groups == 2)
-    hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 2>), grid, threads, 0, stream, p, part);
+    hipLaunchKernelGGL((stream_kernel<kX, kW, 2>), grid, threads, 0, stream, p, part);
   else
-    hipLaunchKernelGGL((stream_kernel<kXMx, kWMx, 1>), grid, threads, 0, stream, p, part);
+    hipLaunchKernelGGL((stream_kernel<kX, kW, 1>), grid, threads, 0, stream, p, part);
   LF_HIP(hipGetLastError());
   return kOk;
 }
@@ -207,8 +242,10 @@ int launch_types(const Params& p, int part, int groups, hipStream_t stream) {
 }  // namespace
 
 int launch_stream(const Params& p, int part, int groups, hipStream_t stream) {
-  if (p.xs) return launch_types<true, true>(p, part, groups, stream);
-  return p.ws ? launch_types<false, true>(p, part, groups, stream) : launch_types<false, false>(p, part, groups, stream);
+  if (p.ws8)
+    return p.xs8 ? launch_types<kFp8, kFp8>(p, part, groups, stream) : launch_types<kBf16, kFp8>(p, part, groups, stream);
+  if (p.xs) return launch_types<kMxfp4, kMxfp4>(p, part, groups, stream);
+  return p.ws ? launch_types<kBf16, kMxfp4>(p, part, groups, stream) : launch_types<kBf16, kBf16>(p, part, groups, stream);
 }
 
 }  // namespace expert

@@ -42,6 +42,8 @@ decltype(&lf_route_experts_workspace_size) g_route_ws;
 decltype(&lf_route_experts) g_route;
 decltype(&lf_expert_linear) g_product;
 decltype(&lf_combine_experts) g_combine;
+decltype(&lf_fp8_quantize) g_fp8_quantize;
+decltype(&lf_fp8_dequantize) g_fp8_dequantize;
 
 PyObject* g_raw_stream;   // torch._C._cuda_getCurrentRawStream
 PyObject* g_get_device;   // torch._C._cuda_getDevice
@@ -50,6 +52,7 @@ PyObject* g_workspaces;   // the operators' workspace cache
 PyObject* g_multi_cus;    // device index -> compute units
 PyObject* g_lora_batch;   // ops.fused.LoraBatch
 PyObject* g_mx_tensor;    // ops.mxfp4.MXFP4Tensor
+PyObject* g_fp8_tensor;   // ops.fp8.FP8Tensor
 
 #define NAMES(X)                                                                                                     \
   X(absmax) X(shape) X(code) X(blocksize) X(quant_type) X(offset) X(state2) X(nested) X(_lf_prepared_scales)         \
@@ -605,7 +608,7 @@ PyObject* dequant_nested(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return THPVariable_Wrap(out);
 }
 
-// ---- MXFP4 and experts ------------------------------------------------------
+// ---- MXFP4, FP8 and experts -------------------------------------------------
 
 constexpr int64_t kMxBlock = 32;
 
@@ -631,6 +634,46 @@ struct MxArg {
     if (k == 0 || k % kMxBlock || scales->size(-1) != k / kMxBlock) return false;
     for (int64_t d = 0; d < codes->dim(); ++d)
       if (codes->size(d) >= (int64_t(1) << 31) || (d + 1 < codes->dim() && codes->size(d) != scales->size(d))) return false;
+    return true;
+  }
+};
+
+constexpr int64_t kFp8Block = 128;
+
+int64_t fp8_blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+// The tensors of an FP8Tensor (ops.fp8.scaled's checks): rows and k are its last dimensions,
+// scale_rows (1 or 128) the rows of a scale.
+struct Fp8Arg {
+  PyObject* held[2] = {};
+  const at::Tensor* codes = nullptr;
+  const at::Tensor* scales = nullptr;
+  int64_t rows = 0, k = 0;
+  int32_t scale_rows = 0;
+  ~Fp8Arg() {
+    for (PyObject* o : held) Py_XDECREF(o);
+  }
+  static bool is(PyObject* o) { return reinterpret_cast<PyObject*>(Py_TYPE(o)) == g_fp8_tensor; }
+  bool take(PyObject* o, int64_t dims = -1, int32_t want = 0) {
+    if (!is(o)) return false;
+    if (!(held[0] = PyObject_GetAttr(o, s_codes)) || !(held[1] = PyObject_GetAttr(o, s_scales))) return false;
+    codes = plain(held[0]);
+    scales = plain(held[1]);
+    if (!codes || !scales || codes->scalar_type() != at::kFloat8_e4m3fn || scales->scalar_type() != at::kFloat ||
+        codes->device() != scales->device() || codes->dim() < 2 || codes->dim() != scales->dim() ||
+        (dims >= 0 && codes->dim() != dims) || !codes->is_contiguous() || !scales->is_contiguous() || !aligned16(*codes))
+      return false;
+    rows = codes->size(-2);
+    k = codes->size(-1);
+    if (k == 0 || k % 16 || scales->size(-1) != fp8_blocks(k)) return false;
+    for (int64_t d = 0; d < codes->dim(); ++d)
+      if (codes->size(d) >= (int64_t(1) << 31) || (d + 2 < codes->dim() && codes->size(d) != scales->size(d))) return false;
+    if (scales->size(-2) == rows && want != kFp8Block)
+      scale_rows = 1;
+    else if (scales->size(-2) == fp8_blocks(rows) && want != 1)
+      scale_rows = kFp8Block;
+    else
+      return false;
     return true;
   }
 };
@@ -684,6 +727,52 @@ PyObject* mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// fp8_quantize(x, block_rows) -> (codes, scales) or None
+PyObject* fp8_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  long block_rows;
+  if (nargs != 2 || !small_int(args[1], 1, kFp8Block, &block_rows) || (block_rows != 1 && block_rows != kFp8Block)) return decline();
+  const at::Tensor* x = plain(args[0]);
+  if (!x || x->dim() < 2 || x->scalar_type() != at::kBFloat16 || x->numel() == 0) return decline();
+  const int64_t rows = x->size(-2), k = x->size(-1), matrices = x->numel() / (rows * k);
+  if (k % 16 || (x->dim() != 2 && !x->is_contiguous()) || matrices >= (int64_t(1) << 31)) return decline();
+  for (int64_t size : x->sizes())
+    if (size >= (int64_t(1) << 31)) return decline();
+  const int64_t stride = x->dim() == 2 && rows > 1 ? x->stride(0) : k;
+  if (x->stride(-1) != 1 || stride < k || stride % 8 || !aligned16(*x)) return decline();
+  void* stream;
+  if (!current(x->device(), &stream)) return decline();
+  std::vector<int64_t> sizes(x->sizes().begin(), x->sizes().end());
+  at::Tensor codes = at::empty(sizes, x->options().dtype(at::kFloat8_e4m3fn));
+  sizes.back() = fp8_blocks(k);
+  sizes[sizes.size() - 2] = block_rows == 1 ? rows : fp8_blocks(rows);
+  at::Tensor scales = at::empty(sizes, x->options().dtype(at::kFloat));
+  if (!on_gpu(codes) || !on_gpu(scales)) return decline();
+  const int rc = unlocked([&] {
+    return g_fp8_quantize(ptr<uint16_t>(x), matrices, rows, k, stride, int32_t(block_rows), ptr<uint8_t>(&codes),
+                          ptr<float>(&scales), stream);
+  });
+  if (rc == LF_EINVAL) return decline();
+  if (rc != LF_OK) return failed();
+  return pair_of(std::move(codes), std::move(scales));
+}
+
+// fp8_dequantize(t) -> values or None
+PyObject* fp8_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  Fp8Arg t;
+  if (nargs != 1 || !t.take(args[0]) || t.codes->numel() == 0) return decline();
+  void* stream;
+  if (!current(t.codes->device(), &stream)) return decline();
+  at::Tensor out = at::empty(t.codes->sizes(), t.codes->options().dtype(at::kBFloat16));
+  if (!on_gpu(out)) return decline();
+  const int rc = unlocked([&] {
+    return g_fp8_dequantize(ptr<uint8_t>(t.codes), ptr<float>(t.scales), out.numel() / (t.rows * t.k), t.rows, t.k, t.scale_rows,
+                            ptr<uint16_t>(&out), stream);
+  });
+  if (rc == LF_EINVAL) return decline();
+  if (rc != LF_OK) return failed();
+  return THPVariable_Wrap(std::move(out));
+}
+
 // A bf16 [rows, columns] output: the caller's (whose rows may be apart), or a new one.
 struct Output {
   const at::Tensor* given = nullptr;
@@ -717,15 +806,21 @@ struct Output {
 };
 
 // product(x, weight, offsets or None, tokens or None, bias or None, swiglu, out or None) -> out or None:
-// mxfp4_linear (offsets None) and expert_linear.
+// mxfp4_linear, fp8_linear (offsets None) and expert_linear.
 PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 7 || (args[5] != Py_True && args[5] != Py_False)) return decline();
   const bool grouped = args[2] != Py_None, swiglu = args[5] == Py_True;
   lf_expert_product a{};
   MxArg wm, xm;
+  Fp8Arg w8, x8;
   const at::Tensor* w = nullptr;
   int64_t k;
-  if (reinterpret_cast<PyObject*>(Py_TYPE(args[1])) == g_mx_tensor) {
+  if (Fp8Arg::is(args[1])) {
+    if (!w8.take(args[1], grouped ? 3 : 2, kFp8Block)) return decline();
+    w = w8.codes;
+    k = w8.k;
+    a.w_fp8_scales = ptr<float>(w8.scales);
+  } else if (reinterpret_cast<PyObject*>(Py_TYPE(args[1])) == g_mx_tensor) {
     if (!wm.take(args[1], grouped ? 3 : 2)) return decline();
     w = wm.codes;
     k = wm.k;
@@ -738,9 +833,13 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   const at::Device dev = w->device();
   const int64_t experts = grouped ? w->size(0) : 1, n = w->size(-2);
-  if (n == 0 || k == 0 || experts == 0 || (swiglu && n % 2)) return decline();
+  if (n == 0 || k == 0 || experts == 0 || (swiglu && n % (w8.codes ? 2 * kFp8Block : 2))) return decline();
   const at::Tensor* x;
-  if (reinterpret_cast<PyObject*>(Py_TYPE(args[0])) == g_mx_tensor) {
+  if (Fp8Arg::is(args[0])) {
+    if (!w8.codes || !x8.take(args[0], 2, 1) || x8.codes->device() != dev || x8.k != k) return decline();
+    x = x8.codes;
+    a.x_fp8_scales = ptr<float>(x8.scales);
+  } else if (reinterpret_cast<PyObject*>(Py_TYPE(args[0])) == g_mx_tensor) {
     if (!a.w_scales || !xm.take(args[0], 2) || xm.codes->device() != dev || xm.k != k) return decline();
     x = xm.codes;
     a.x_scales = ptr<uint8_t>(xm.scales);
@@ -777,7 +876,7 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t width = swiglu ? n / 2 : n;
   Output out(args[6], a.rows, width, dev);
   auto optional = [&](int i) { return args[i] == Py_None ? nullptr : plain(args[i]); };
-  if (!out.ok({x, xm.scales, w, wm.scales, optional(2), optional(3), optional(4)})) return decline();
+  if (!out.ok({x, xm.scales, x8.scales, w, wm.scales, w8.scales, optional(2), optional(3), optional(4)})) return decline();
   a.x = x->data_ptr();
   a.w = w->data_ptr();
   a.y = out.data();
@@ -876,16 +975,16 @@ PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return out.take();
 }
 
-// init(addresses, raw_stream, get_device, arch_ok, workspaces, compute_units, lora_batch, mx_tensor)
+// init(addresses, raw_stream, get_device, arch_ok, workspaces, compute_units, lora_batch, mx_tensor, fp8_tensor)
 PyObject* init(PyObject*, PyObject* args) {
-  PyObject *addresses, *raw, *dev, *arch, *ws, *cus, *batch, *packed;
-  if (!PyArg_ParseTuple(args, "O!OOO!O!O!O!O!", &PyTuple_Type, &addresses, &raw, &dev, &PyDict_Type, &arch, &PyDict_Type, &ws,
-                        &PyDict_Type, &cus, &PyType_Type, &batch, &PyType_Type, &packed))
+  PyObject *addresses, *raw, *dev, *arch, *ws, *cus, *batch, *packed, *eight;
+  if (!PyArg_ParseTuple(args, "O!OOO!O!O!O!O!O!", &PyTuple_Type, &addresses, &raw, &dev, &PyDict_Type, &arch, &PyDict_Type, &ws,
+                        &PyDict_Type, &cus, &PyType_Type, &batch, &PyType_Type, &packed, &PyType_Type, &eight))
     return nullptr;
-  constexpr int kEntries = 15;
+  constexpr int kEntries = 17;
   void* a[kEntries];
   if (PyTuple_GET_SIZE(addresses) != kEntries) {
-    PyErr_SetString(PyExc_ValueError, "fifteen entry points expected");
+    PyErr_SetString(PyExc_ValueError, "seventeen entry points expected");
     return nullptr;
   }
   for (int i = 0; i < kEntries; ++i)
@@ -908,13 +1007,16 @@ PyObject* init(PyObject*, PyObject* args) {
   g_route = reinterpret_cast<decltype(g_route)>(a[12]);
   g_product = reinterpret_cast<decltype(g_product)>(a[13]);
   g_combine = reinterpret_cast<decltype(g_combine)>(a[14]);
+  g_fp8_quantize = reinterpret_cast<decltype(g_fp8_quantize)>(a[15]);
+  g_fp8_dequantize = reinterpret_cast<decltype(g_fp8_dequantize)>(a[16]);
 #define INTERN(n) \
   if (!s_##n && !(s_##n = PyUnicode_InternFromString(#n))) return nullptr;
   NAMES(INTERN)
 #undef INTERN
-  PyObject** slot[7] = {&g_raw_stream, &g_get_device, &g_arch_ok, &g_workspaces, &g_multi_cus, &g_lora_batch, &g_mx_tensor};
-  PyObject* value[7] = {raw, dev, arch, ws, cus, batch, packed};
-  for (int i = 0; i < 7; ++i) {
+  PyObject** slot[8] = {&g_raw_stream, &g_get_device, &g_arch_ok, &g_workspaces, &g_multi_cus, &g_lora_batch, &g_mx_tensor,
+                        &g_fp8_tensor};
+  PyObject* value[8] = {raw, dev, arch, ws, cus, batch, packed, eight};
+  for (int i = 0; i < 8; ++i) {
     Py_INCREF(value[i]);
     Py_XDECREF(*slot[i]);
     *slot[i] = value[i];
@@ -940,6 +1042,8 @@ PyMethodDef methods[] = {
     {"dequant", reinterpret_cast<PyCFunction>(guarded<dequant>), METH_FASTCALL, nullptr},
     {"mx_quantize", reinterpret_cast<PyCFunction>(guarded<mx_quantize>), METH_FASTCALL, nullptr},
     {"mx_dequantize", reinterpret_cast<PyCFunction>(guarded<mx_dequantize>), METH_FASTCALL, nullptr},
+    {"fp8_quantize", reinterpret_cast<PyCFunction>(guarded<fp8_quantize>), METH_FASTCALL, nullptr},
+    {"fp8_dequantize", reinterpret_cast<PyCFunction>(guarded<fp8_dequantize>), METH_FASTCALL, nullptr},
     {"product", reinterpret_cast<PyCFunction>(guarded<product>), METH_FASTCALL, nullptr},
     {"route", reinterpret_cast<PyCFunction>(guarded<route>), METH_FASTCALL, nullptr},
     {"combine", reinterpret_cast<PyCFunction>(guarded<combine>), METH_FASTCALL, nullptr},

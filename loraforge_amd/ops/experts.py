@@ -8,8 +8,8 @@ A block of experts runs as
 
 with no host synchronisation: segment bounds stay on the device, buffers are
 sized for every choice (``tokens * top_k`` rows), and the calls can be captured
-in a HIP graph. Expert weights are bf16 or MXFP4 ``[E, N, K]``. The operators are
-for inference: tensors that require gradients are refused.
+in a HIP graph. ``expert_mlp`` is the whole block in one call. Expert weights are bf16, MXFP4 or
+FP8 ``[E, N, K]``. The operators are for inference: tensors that require gradients are refused.
 """
 
 from __future__ import annotations
@@ -19,7 +19,8 @@ from dataclasses import dataclass
 from .. import _lib
 from ..annotations import ExperimentalAPI
 from ._checks import distinct_output, require_arch, tensor
-from .mxfp4 import MXFP4Tensor, product
+from .fp8 import BLOCK, FP8Tensor, scaled
+from .mxfp4 import MXFP4Tensor, packed, product
 
 MAX_EXPERTS = 1024
 MAX_TOP = 64
@@ -103,18 +104,19 @@ def route_experts(logits, top_k: int, *, renormalize: bool = True) -> ExpertRout
 def expert_linear(x, weight, offsets, *, tokens=None, bias=None, swiglu: bool = False, out=None):
     """Rows ``offsets[e]`` to ``offsets[e + 1]`` times the transpose of ``weight[e]``, for every expert.
 
-    ``weight`` is bf16 ``[E, N, K]`` (K a multiple of 8) or an ``MXFP4Tensor``
-    of that shape; ``x`` bf16 ``[rows, K]`` with 16-byte aligned rows, or an
-    ``MXFP4Tensor`` beside an MXFP4 weight. With ``tokens`` (int32, one entry per
+    ``weight`` is bf16 ``[E, N, K]`` (K a multiple of 8), or an ``MXFP4Tensor`` or
+    ``FP8Tensor`` (a scale for each 128 x 128 block) of that shape; ``x`` bf16 ``[rows, K]``
+    with 16-byte aligned rows, or an ``MXFP4Tensor`` beside an MXFP4 weight, an ``FP8Tensor``
+    (a scale for each 128 values of a row) beside an FP8 one. With ``tokens`` (int32, one entry per
     row of the result) row ``p`` is ``x[tokens[p]]``, so the rows are gathered by the
     product itself; without, ``x`` is in expert order already. ``bias`` is bf16
-    ``[E, N]``, ``swiglu`` as in ``mxfp4_linear``. fp32 sums, rounded once to bf16.
+    ``[E, N]``, ``swiglu`` as in ``mxfp4_linear`` and ``fp8_linear``. fp32 sums, rounded once to bf16.
     Rows past ``offsets[E]`` belong to no expert and are left as they are.
     """
     import torch
 
-    if not isinstance(weight, (torch.Tensor, MXFP4Tensor)):
-        raise TypeError("weight must be a torch.Tensor or an MXFP4Tensor")
+    if not isinstance(weight, (torch.Tensor, MXFP4Tensor, FP8Tensor)):
+        raise TypeError("weight must be a torch.Tensor, an MXFP4Tensor or an FP8Tensor")
     if weight.ndim != 3:
         raise ValueError("weight must be 3D, [experts, n, k]")
     return product(x, weight, experts=weight.shape[0], offsets=offsets, tokens=tokens, bias=bias, swiglu=swiglu, out=out)
@@ -170,3 +172,82 @@ def combine_experts(rows, positions, weights, *, base=None, out=None):
                 positions.shape[1], n, _lib.ptr(base), 0 if base is None else stride(base, "base"), out.data_ptr(),
                 stride(out, "out"), _lib.stream_of(rows.device)))
     return out
+
+
+@ExperimentalAPI(reason="Whole mixture-of-experts MLP; gfx950 HIP kernels.")
+def expert_mlp(x, logits, gate_up, down, top_k: int, *, renormalize: bool = True, base=None, out=None):
+    """``out[t] = base[t] + sum_j weight_tj down_e (silu(gate_e x[t]) * (up_e x[t]))`` over the ``top_k`` experts of each token.
+
+    ``x`` bf16 ``[T, H]`` with 16-byte aligned rows; ``logits`` bf16 or fp32 ``[T, E]``, choices and
+    weights as ``route_experts`` makes them; ``gate_up`` ``[E, 2 I, H]`` (gate rows, then up rows) and
+    ``down`` ``[E, H, I]``, each bf16, an ``MXFP4Tensor`` or an ``FP8Tensor`` (a scale for
+    each 128 x 128 block); ``base`` bf16 ``[T, H]`` (a shared expert's output or the residual).
+    ``out`` may be ``base``. A token that may choose no expert is left with ``base`` (or zeros).
+    """
+    import torch
+
+    for name, w in (("gate_up", gate_up), ("down", down)):
+        if not isinstance(w, (torch.Tensor, MXFP4Tensor, FP8Tensor)):
+            raise TypeError(f"{name} must be a torch.Tensor, an MXFP4Tensor or an FP8Tensor")
+        if w.ndim != 3:
+            raise ValueError(f"{name} must be 3D, [experts, n, k]")
+    tensor(x, "x", 2, torch.bfloat16)
+    for name, w in (("gate_up", gate_up), ("down", down)):
+        _expert_weight(w, name, x.device)
+    experts, hidden, inter = down.shape
+    if tuple(gate_up.shape) != (experts, 2 * inter, hidden):
+        raise ValueError("gate_up must be [experts, 2 * inter, hidden] beside down [experts, hidden, inter]")
+    if isinstance(gate_up, FP8Tensor) and inter % BLOCK:
+        raise ValueError("gate_up must hold whole blocks of 128 FP8 gate and up rows")
+    count = x.shape[0]
+    if x.shape[1] != hidden:
+        raise ValueError("x must be [tokens, hidden]")
+    if x.numel() and (x.stride(1) != 1 or x.data_ptr() % 16 or (count > 1 and (x.stride(0) < hidden or x.stride(0) % 8))):
+        raise ValueError("x rows must be 16-byte aligned with unit stride")
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits must be a torch.Tensor")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("logits must have dtype torch.bfloat16 or torch.float32")
+    tensor(logits, "logits", 2, logits.dtype, x.device)
+    if tuple(logits.shape) != (count, experts):
+        raise ValueError("logits must be [tokens, experts]")
+    if type(renormalize) is not bool:
+        raise TypeError("renormalize must be a bool")
+    if base is not None:
+        tensor(base, "base", 2, torch.bfloat16, x.device)
+        if tuple(base.shape) != (count, hidden):
+            raise ValueError("base must be [tokens, columns]")
+    if out is None:
+        out = torch.empty(count, hidden, dtype=torch.bfloat16, device=x.device)
+    tensor(out, "out", 2, torch.bfloat16, x.device)
+    if tuple(out.shape) != (count, hidden):
+        raise ValueError("out must be [tokens, columns]")
+    same = base is not None and out.data_ptr() == base.data_ptr() and out.stride() == base.stride()
+    distinct_output(out, (x, logits, *_parts(gate_up), *_parts(down), None if same else base))
+    r = route_experts(logits, top_k, renormalize=renormalize)
+    if count == 0:
+        return out
+    h = expert_linear(x, gate_up, r.offsets, tokens=r.tokens, swiglu=True)
+    rows = expert_linear(h, down, r.offsets)
+    return combine_experts(rows, r.positions, r.weights, base=base, out=out)
+
+
+def _parts(w):
+    return (w.codes, w.scales) if isinstance(w, (MXFP4Tensor, FP8Tensor)) else (w,)
+
+
+def _expert_weight(w, name, device):
+    import torch
+
+    if isinstance(w, FP8Tensor):
+        scaled(w, name, 3, device, block_rows=BLOCK)
+    elif isinstance(w, MXFP4Tensor):
+        packed(w, name, 3, device)
+    else:
+        tensor(w, name, 3, torch.bfloat16, device)
+        if not w.is_contiguous() or w.data_ptr() % 16:
+            raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+        if w.shape[2] % 8:
+            raise ValueError(f"{name}'s last dimension must be a multiple of 8")
+    if 0 in tuple(w.shape):
+        raise ValueError(f"{name} must not be empty")

@@ -20,6 +20,7 @@ from dataclasses import dataclass
 
 from .. import _lib
 from ..annotations import ExperimentalAPI
+from . import fp8
 from ._checks import distinct_output, require_arch, tensor, vector
 
 BLOCK = 32
@@ -137,19 +138,23 @@ def dequantize_mxfp4(t: MXFP4Tensor, *, out=None):
 
 
 def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out, plan=None):
-    """The product that ``mxfp4_linear`` and ``expert_linear`` share; ``experts`` is None for the dense one.
+    """The product that ``mxfp4_linear``, ``fp8_linear`` and ``expert_linear`` share; ``experts`` is None for the dense ones.
 
     ``plan`` (``_lib.ExpertPlan``) forces a kernel; by default the library chooses.
     """
     import torch
 
     grouped = experts is not None
-    quantised = isinstance(weight, MXFP4Tensor)
+    quantised = isinstance(weight, (MXFP4Tensor, fp8.FP8Tensor))
+    eight = isinstance(weight, fp8.FP8Tensor)
     if plan is None and (offsets is not None) == grouped and getattr(weight.codes if quantised else weight, "is_cuda", False):
         done = _lib.binding().product(x, weight, offsets, tokens, bias, swiglu, out)
         if done is not None:
             return done
-    if quantised:
+    if eight:
+        fp8.scaled(weight, "weight", 3 if grouped else 2, block_rows=fp8.BLOCK)
+        shape, device = weight.shape, weight.device
+    elif quantised:
         shape = packed(weight, "weight", 3 if grouped else 2)
         device = weight.device
     else:
@@ -161,8 +166,17 @@ def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out, plan=None
     if n == 0 or k == 0 or (grouped and shape[0] == 0):
         raise ValueError("weight must not be empty")
     a = _lib.ExpertProduct()
-    if isinstance(x, MXFP4Tensor):
-        if not quantised:
+    if isinstance(x, fp8.FP8Tensor):
+        if not eight:
+            raise ValueError("an FP8 x needs an FP8 weight")
+        fp8.scaled(x, "x", 2, device, block_rows=1)
+        x_rows = x.shape[0]
+        if x.shape[1] != k:
+            raise ValueError("x must have the weight's inner dimension")
+        read = (x.codes, x.scales)
+        a.x, a.x_fp8_scales = x.codes.data_ptr(), x.scales.data_ptr()
+    elif isinstance(x, MXFP4Tensor):
+        if not quantised or eight:
             raise ValueError("an MXFP4 x needs an MXFP4 weight")
         x_rows = packed(x, "x", 2, device)[0]
         if x.shape[1] != k:
@@ -183,6 +197,8 @@ def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out, plan=None
         raise TypeError("swiglu must be a bool")
     if swiglu and n % 2:
         raise ValueError("swiglu needs as many gate as up rows")
+    if swiglu and eight and n % (2 * fp8.BLOCK):
+        raise ValueError("swiglu needs whole blocks of 128 FP8 gate and up rows")
     width = n // 2 if swiglu else n
     rows = x_rows
     if grouped:
@@ -211,7 +227,10 @@ def product(x, weight, *, experts, offsets, tokens, bias, swiglu, out, plan=None
         return out
     a.x_rows, a.rows, a.n, a.k, a.experts = x_rows, rows, n, k, experts if grouped else 1
     a.w = weights[0].data_ptr()
-    a.w_scales = weights[1].data_ptr() if quantised else None
+    if eight:
+        a.w_fp8_scales = weights[1].data_ptr()
+    elif quantised:
+        a.w_scales = weights[1].data_ptr()
     a.y, a.y_stride, a.swiglu = out.data_ptr(), out.stride(0) if rows > 1 else width, swiglu
     if plan is not None:
         a.plan = ctypes.pointer(plan)

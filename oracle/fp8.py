@@ -1,0 +1,60 @@
+"""Block-scaled FP8 in numpy, 64 bits. TEST INFRASTRUCTURE ONLY.
+
+The reference has none: the definition is that of e4m3 (OCP 8-bit floating
+point) with a scale for each 128 values of a row or each 128 x 128 block, restated here
+without the product's code. ``tests/test_oracle_fp8.py`` checks it against closed forms
+and brute force.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+
+BLOCK = 128
+# Values of the codes 0 .. 126: subnormals in steps of 2^-9, then eight to a power of two.
+LEVELS = np.array([i * 2.0**-9 for i in range(8)] + [(8 + i) * 2.0 ** (e - 3) for e in range(-6, 9) for i in range(8)][:119])
+LEAST = 2.0**-100
+
+
+def _grid(x, block_rows):
+    """``x`` ``[..., R, K]`` padded with zeros to whole blocks, as ``[..., R / rows, rows, K / 128, 128]``."""
+    r, k = x.shape[-2:]
+    pad = [(0, 0)] * (x.ndim - 2) + [(0, -r % block_rows), (0, -k % BLOCK)]
+    x = np.pad(x, pad)
+    return x.reshape(*x.shape[:-2], x.shape[-2] // block_rows, block_rows, x.shape[-1] // BLOCK, BLOCK)
+
+
+def nearest(a):
+    """The code of the level nearest to non-negative ``a`` (at most 448 and a rounding), of two equally near the even one."""
+    above = np.clip(np.searchsorted(LEVELS, a), 1, len(LEVELS) - 1)
+    low, high = a - LEVELS[above - 1], LEVELS[above] - a
+    return (above - ((low < high) | ((low == high) & (above % 2 == 1)))).astype(np.uint8)
+
+
+def quantize(x, block_rows=1):
+    """Codes (uint8) and fp32 scales of bf16-representable ``x`` ``[..., R, K]``."""
+    x = np.asarray(x, dtype=np.float64)
+    r, k = x.shape[-2:]
+    b = _grid(x, block_rows)
+    top = np.abs(b).max((-3, -1), keepdims=True)
+    finite = np.isfinite(top)
+    top = np.where(finite, np.maximum(top, LEAST), 1.0)
+    b = np.where(finite, b, 0.0)
+    codes = nearest(np.abs(b) * 448.0 / top) | (np.signbit(b) << 7).astype(np.uint8)
+    codes = np.where(finite, codes, 0).astype(np.uint8)
+    codes = codes.reshape(*codes.shape[:-4], codes.shape[-4] * block_rows, -1)[..., :r, :k]
+    with np.errstate(invalid="ignore"):
+        scales = np.where(finite, top / 448.0, np.nan).astype(np.float32)[..., :, 0, :, 0]
+    return np.ascontiguousarray(codes), np.ascontiguousarray(scales)
+
+
+def values(codes, scales):
+    """fp64 values of codes (NaN for 0x7f and 0xff) times their scales."""
+    codes = np.asarray(codes)
+    r, k = codes.shape[-2:]
+    magnitude = codes & 127
+    v = np.where(magnitude == 127, np.nan, LEVELS[np.minimum(magnitude, 126)]) * np.where(codes >> 7, -1.0, 1.0)
+    s = np.repeat(np.asarray(scales, np.float64), BLOCK, -1)[..., :k]
+    if s.shape[-2] != r:
+        s = np.repeat(s, BLOCK, -2)[..., :r, :]
+    return v * s
