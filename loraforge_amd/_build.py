@@ -47,7 +47,13 @@ HIP_FLAGS = [
 # register spill of such a result would store it before the load returned. (In the
 # expert tiles a spill in the loop would wait for every copy in flight.)
 NO_SCRATCH = {"nf4_gemv.hip", "nf4_decode_wide.hip", "row_ops.hip"} | {
-    f"nf4_prefill_rows_{part}.hip" for part in "abcd"} | {f"expert_tile_{types}.hip" for types in ("bf16", "mxw", "mx")}
+    f"nf4_prefill_rows_{part}.hip" for part in "abcd"} | {f"expert_tile_{types}.hip" for types in ("bf16", "mxw", "mx")} | {
+    f"fp8_tile_{types}.hip" for types in ("fp8", "w8")}
+
+# The FP8 tiles scale a block's products by vector instructions, so their matrix instructions have to
+# leave results in registers that those reach (by default the compiler gives them the others of the
+# 512 and copies each value over: 16 more instructions a pair of fragments).
+EXTRA_FLAGS = {f"fp8_tile_{types}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for types in ("fp8", "w8")}
 
 
 def hipcc() -> str:
@@ -78,7 +84,7 @@ def _scratch_users(remarks: list[str]) -> list[str]:
 def _compile(src: Path, obj: Path, verbose: bool) -> None:
     check = src.name in NO_SCRATCH
     extra = ["-Rpass-analysis=kernel-resource-usage"] if check else []
-    cmd = [hipcc(), *HIP_FLAGS, *extra, "-c", str(src), "-o", str(obj)]
+    cmd = [hipcc(), *HIP_FLAGS, *EXTRA_FLAGS.get(src.name, []), *extra, "-c", str(src), "-o", str(obj)]
     if verbose:
         print(" ".join(cmd), flush=True)
     result = subprocess.run(cmd, capture_output=True, text=True)

@@ -15,7 +15,10 @@ namespace {
 // take is streamed, whatever the rows: MXFP4 both, 4096 x 4096 x 480 58 us where k = 512 takes 15.5
 // in tiles; 2048 rows gathered from 2^20 + 5 of k = 8192 341 us, from 2^20 - 1 45.)
 bool tiles_fit(const lf_expert_product& a) {
-  if (a.w_fp8_scales) return false;
+  if (a.w_fp8_scales) {  // offsets below 2^31
+    const int64_t x_row = a.x_fp8_scales ? a.k : a.x_stride * 2;
+    return a.x_rows * std::max(x_row, a.k) < (int64_t(1) << 31) && (a.n + 512) * a.k < (int64_t(1) << 31);
+  }
   if (a.x_scales) return a.k >= 512 && std::max(a.x_rows, a.n) * (a.k / 2) < (int64_t(1) << 32);
   return !a.w_scales || a.k >= 128;
 }
@@ -94,7 +97,7 @@ double tile_us(const Costs& c, int rows, int columns, double each, double used, 
 // 4.8 % slower on average by type, 63 % at most: 256 tokens over 64 experts, n and k 1024, 21 and 13 us.
 // Over 80 dense products of 8..384 rows, n 528..8192: 10 % with bf16 x, 6 % with MXFP4 x, 43 % at most.)
 lf_expert_plan plan_of(const lf_expert_product& a) {
-  const Costs& c = kCosts[a.x_scales || a.x_fp8_scales ? 2 : a.w_scales || a.w_fp8_scales ? 1 : 0];
+  const Costs& c = kCosts[a.x_scales ? 2 : a.x_fp8_scales ? 2 : a.w_scales || a.w_fp8_scales ? 1 : 0];
   const bool grouped = a.offsets != nullptr && a.experts > 1;
   const double rows = double(a.rows), experts = double(a.experts);
   const double used = grouped ? experts * (1.0 - std::pow(1.0 - 1.0 / experts, rows)) : 1.0;
@@ -130,10 +133,10 @@ lf_expert_plan plan_of(const lf_expert_product& a) {
           {LF_EXPERT_ROWS, 0, 128});
   }
   if (tiles_fit(a)) {
-    const double stage_k = a.x_scales ? 256.0 : 64.0;
+    const double stage_k = a.x_scales ? 256.0 : a.w_fp8_scales ? 128.0 : 64.0;
     for (int height = 64; height <= 256; height += 64)
       for (int columns = 64; columns <= 256; columns += 64)
-        offer(tile_us(c, height, columns, each, used, grouped, n, std::ceil(double(a.k) / stage_k)), {LF_EXPERT_TILE, height, columns});
+        if (!a.w_fp8_scales || height <= (a.x_fp8_scales ? (columns == 256 ? 192 : 256) : columns == 256 ? 128 : 192)) offer(tile_us(c, height, columns, each, used, grouped, n, std::ceil(double(a.k) / stage_k)), {LF_EXPERT_TILE, height, columns});
   }
   return best;
 }
@@ -199,6 +202,12 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   LF_REQUIRE(plan.kernel == LF_EXPERT_TILE && lf::expert::tiles_fit(*a), "this product cannot run in tiles");
   LF_REQUIRE(plan.rows >= 64 && plan.rows <= 256 && plan.rows % 64 == 0, "tile plan: 64, 128, 192 or 256 rows");
   LF_REQUIRE(plan.columns >= 64 && plan.columns <= 256 && plan.columns % 64 == 0, "tile plan: 64, 128, 192 or 256 columns");
+  if (w_f8) {
+    // (Sums of 256 x 256 products leave no registers for a block's: tiles of 256 columns have fewer rows.)
+    const int most = x_f8 ? (plan.columns == 256 ? 192 : 256) : plan.columns == 256 ? 128 : 192;
+    LF_REQUIRE(plan.rows <= most, "tile plan: at most %d rows beside %d columns of FP8 weights", most, int(plan.columns));
+    return x_f8 ? lf::expert::launch_tiles_fp8(p, plan.rows, plan.columns, s) : lf::expert::launch_tiles_w8(p, plan.rows, plan.columns, s);
+  }
   if (x_mx) return lf::expert::launch_tiles_mx(p, plan.rows, plan.columns, s);
   return w_mx ? lf::expert::launch_tiles_mxw(p, plan.rows, plan.columns, s)
               : lf::expert::launch_tiles_bf16(p, plan.rows, plan.columns, s);

@@ -106,6 +106,8 @@ int launch_rows(const Params& p, hipStream_t stream);
 int launch_tiles_bf16(const Params& p, int cap, int columns, hipStream_t stream);
 int launch_tiles_mxw(const Params& p, int cap, int columns, hipStream_t stream);
 int launch_tiles_mx(const Params& p, int cap, int columns, hipStream_t stream);
+int launch_tiles_fp8(const Params& p, int cap, int columns, hipStream_t stream);  // (fp8_tile.h: both operands FP8)
+int launch_tiles_w8(const Params& p, int cap, int columns, hipStream_t stream);   // bf16 x, FP8 weights
 
 }  // namespace expert
 }  // namespace lf

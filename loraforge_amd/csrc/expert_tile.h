@@ -87,6 +87,101 @@ struct Frags {
 __device__ __forceinline__ void reads_done() { __builtin_amdgcn_s_waitcnt(0xC07F); }  // lgkmcnt(0), which the compiler sees
 __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 
+// Bias, activation, rounding and stores. Each wave passes its sums through LDS of
+// its own, two fragment rows (64 rows of the tile) at a time: acc[i][j][4 g + e] is
+// row c of fragment row i and weight row 8 g + 4 h + e of fragment j, and in LDS a
+// row's columns follow each other, so that eight lanes or more store whole cache
+// lines and the code is short (an unrolled epilogue straight from the
+// registers took longer to fetch than to run).
+template <int kI, int kJ, bool kSwiglu>
+__device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][kJ], char* lds, int expert, int first, int count,
+                                       int nt) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  constexpr int kRowBytes = 32 * kJ * 4 + 16;             // (padded: rows start at other banks)
+  constexpr int kColumns = kSwiglu ? 16 * kJ : 32 * kJ;   // output columns of the wave
+  constexpr int kParts = kColumns / 8;  // lanes that share a row (of kLanes, a power of two)
+  constexpr int kLanes = kParts <= 2 ? 2 : kParts <= 4 ? 4 : kParts <= 8 ? 8 : 16, kRows = 64 / kLanes;
+  char* mine = lds + wave * 64 * kRowBytes;
+  const int wm = wave & 1, wn = wave >> 1, c = lane & 31;
+  const bool idle = lane % kLanes >= kParts;
+  const int part = idle ? 0 : lane % kLanes, in_row = lane / kLanes;
+  // With SwiGLU eight columns are half of a fragment's gate values, their up values 16 on.
+  const int local = kSwiglu ? part / 2 * 32 + part % 2 * 8 : part * 8;
+  const int col = (nt * 2 + wn) * kColumns + part * 8;
+  float add[8], add_up[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) add[e] = add_up[e] = 0.f;
+  if (p.bias) {
+    const uint16_t* bias = p.bias + int64_t(expert) * p.n;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = min(col + e, p.width - 1);
+      add[e] = bf16_to_f32(bias[at]);
+      if (kSwiglu) add_up[e] = bf16_to_f32(bias[at + p.width]);
+    }
+  }
+  const bool vec = p.y_vec && col + 8 <= p.width;
+  const bool all_vec = __ballot(!vec) == 0;
+  // Eight output columns of staged row r.
+  auto output = [&](int r) {
+    const f32x4* v = reinterpret_cast<const f32x4*>(mine + r * kRowBytes + local * 4);
+    const f32x4 half[2] = {v[0], v[1]};
+    f32x4 up[2];
+    if (kSwiglu) up[0] = v[4], up[1] = v[5];
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float a = half[e >> 1][(e & 1) * 2] + add[2 * e], b = half[e >> 1][(e & 1) * 2 + 1] + add[2 * e + 1];
+      if (kSwiglu) {
+        a = silu_mul_f32(a, up[e >> 1][(e & 1) * 2] + add_up[2 * e]);
+        b = silu_mul_f32(b, up[e >> 1][(e & 1) * 2 + 1] + add_up[2 * e + 1]);
+      }
+      o[e] = pack_bf16x2(a, b);
+    }
+    return u32x4{o[0], o[1], o[2], o[3]};
+  };
+#pragma unroll
+  for (int pair = 0; pair < (kI + 1) / 2; ++pair) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (2 * pair + i < kI) {
+            const f32x16& a = acc[2 * pair + i][j];
+            *reinterpret_cast<f32x4*>(mine + (32 * i + c) * kRowBytes + (32 * j + 8 * g + 4 * h) * 4) =
+                f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+          }
+    const int staged = min(2, kI - 2 * pair) * 32;
+    auto place = [&](int r) { return (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31); };
+    if (all_vec) {
+      constexpr int kTogether = 32 / kRows < 4 ? 32 / kRows : 4;  // rows whose reads go out together
+#pragma unroll 1
+      for (int r0 = in_row; r0 < staged; r0 += kTogether * kRows) {
+        u32x4 o[kTogether];
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) o[k] = output(r0 + k * kRows);
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+          const int row = place(r0 + k * kRows);
+          if (row < count && !idle) *reinterpret_cast<u32x4*>(p.y + int64_t(first + row) * p.y_stride + col) = o[k];
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int r = in_row; r < staged; r += kRows) {
+        const u32x4 o = output(r);
+        uint16_t* y = p.y + int64_t(first + place(r)) * p.y_stride + col;
+        if (place(r) >= count || idle) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (col + e < p.width) y[e] = uint16_t(o[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+}
+
 template <bool kXMx, bool kWMx, int kI, int kJ>
 struct Body {
   using S = Shape<kXMx, kWMx, kI, kJ>;
@@ -486,102 +581,9 @@ struct Body {
     wait_vm<0>();
     lds_barrier();
     if (p.swiglu)
-      finish<true>(lds, seg.expert, first, count, nt);
+      finish<kI, kJ, true>(p, acc, lds, seg.expert, first, count, nt);
     else
-      finish<false>(lds, seg.expert, first, count, nt);
-  }
-
-  // Bias, activation, rounding and stores. Each wave passes its sums through LDS of
-  // its own, two fragment rows (64 rows of the tile) at a time: acc[i][j][4 g + e] is
-  // row c of fragment row i and weight row 8 g + 4 h + e of fragment j, and in LDS a
-  // row's columns follow each other, so that eight lanes or more store whole cache
-  // lines and the code is short (an unrolled epilogue straight from the
-  // registers took longer to fetch than to run).
-  template <bool kSwiglu>
-  __device__ __forceinline__ void finish(char* lds, int expert, int first, int count, int nt) {
-    constexpr int kRowBytes = 32 * kJ * 4 + 16;             // (padded: rows start at other banks)
-    constexpr int kColumns = kSwiglu ? 16 * kJ : 32 * kJ;   // output columns of the wave
-    constexpr int kParts = kColumns / 8;  // lanes that share a row (of kLanes, a power of two)
-    constexpr int kLanes = kParts <= 2 ? 2 : kParts <= 4 ? 4 : kParts <= 8 ? 8 : 16, kRows = 64 / kLanes;
-    char* mine = lds + wave * 64 * kRowBytes;
-    const int wm = wave & 1, wn = wave >> 1, c = lane & 31;
-    const bool idle = lane % kLanes >= kParts;
-    const int part = idle ? 0 : lane % kLanes, in_row = lane / kLanes;
-    // With SwiGLU eight columns are half of a fragment's gate values, their up values 16 on.
-    const int local = kSwiglu ? part / 2 * 32 + part % 2 * 8 : part * 8;
-    const int col = (nt * 2 + wn) * kColumns + part * 8;
-    float add[8], add_up[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) add[e] = add_up[e] = 0.f;
-    if (p.bias) {
-      const uint16_t* bias = p.bias + int64_t(expert) * p.n;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int at = min(col + e, p.width - 1);
-        add[e] = bf16_to_f32(bias[at]);
-        if (kSwiglu) add_up[e] = bf16_to_f32(bias[at + p.width]);
-      }
-    }
-    const bool vec = p.y_vec && col + 8 <= p.width;
-    const bool all_vec = __ballot(!vec) == 0;
-    // Eight output columns of staged row r.
-    auto output = [&](int r) {
-      const f32x4* v = reinterpret_cast<const f32x4*>(mine + r * kRowBytes + local * 4);
-      const f32x4 half[2] = {v[0], v[1]};
-      f32x4 up[2];
-      if (kSwiglu) up[0] = v[4], up[1] = v[5];
-      uint32_t o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float a = half[e >> 1][(e & 1) * 2] + add[2 * e], b = half[e >> 1][(e & 1) * 2 + 1] + add[2 * e + 1];
-        if (kSwiglu) {
-          a = silu_mul_f32(a, up[e >> 1][(e & 1) * 2] + add_up[2 * e]);
-          b = silu_mul_f32(b, up[e >> 1][(e & 1) * 2 + 1] + add_up[2 * e + 1]);
-        }
-        o[e] = pack_bf16x2(a, b);
-      }
-      return u32x4{o[0], o[1], o[2], o[3]};
-    };
-#pragma unroll
-    for (int pair = 0; pair < (kI + 1) / 2; ++pair) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < kJ; ++j)
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            if (2 * pair + i < kI) {
-              const f32x16& a = acc[2 * pair + i][j];
-              *reinterpret_cast<f32x4*>(mine + (32 * i + c) * kRowBytes + (32 * j + 8 * g + 4 * h) * 4) =
-                  f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
-            }
-      const int staged = min(2, kI - 2 * pair) * 32;
-      auto place = [&](int r) { return (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31); };
-      if (all_vec) {
-        constexpr int kTogether = 32 / kRows < 4 ? 32 / kRows : 4;  // rows whose reads go out together
-#pragma unroll 1
-        for (int r0 = in_row; r0 < staged; r0 += kTogether * kRows) {
-          u32x4 o[kTogether];
-#pragma unroll
-          for (int k = 0; k < kTogether; ++k) o[k] = output(r0 + k * kRows);
-#pragma unroll
-          for (int k = 0; k < kTogether; ++k) {
-            const int row = place(r0 + k * kRows);
-            if (row < count && !idle) *reinterpret_cast<u32x4*>(p.y + int64_t(first + row) * p.y_stride + col) = o[k];
-          }
-        }
-      } else {
-#pragma unroll 1
-        for (int r = in_row; r < staged; r += kRows) {
-          const u32x4 o = output(r);
-          uint16_t* y = p.y + int64_t(first + place(r)) * p.y_stride + col;
-          if (place(r) >= count || idle) continue;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (col + e < p.width) y[e] = uint16_t(o[e >> 1] >> (16 * (e & 1)));
-        }
-      }
-    }
+      finish<kI, kJ, false>(p, acc, lds, seg.expert, first, count, nt);
   }
 };
 
@@ -603,22 +605,32 @@ __device__ __forceinline__ int total_tiles(const Params& p, int cap) {
   return __builtin_amdgcn_readfirstlane(sum);
 }
 
-template <bool kXMx, bool kWMx, int kJ>
-__global__ __launch_bounds__(kThreads, 1) void tile_kernel(Params p, int cap, int column_tiles) {
-  extern __shared__ char lds[];
+struct Place {
+  Segment seg;
+  int first, count, nt;  // rows of the product, column tile; count 0: no tile
+};
+
+__device__ __forceinline__ Place locate(const Params& p, int cap, int column_tiles) {
   const int items = total_tiles(p, cap) * column_tiles;
   const int share = (items + kXcds - 1) / kXcds, local = blockIdx.x / kXcds;
   int index = int(blockIdx.x % kXcds) * share + local;
-  if (local >= share || index >= items) return;
+  if (local >= share || index >= items) return {{0, 0, 0}, 0, 0, 0};
   const Segment seg = find_segment(p, index, [&](const Segment& s) { return tiles_of(s, cap) * column_tiles; });
   const int rows = seg.end - seg.begin, tiles = tiles_of(seg, cap);
-  if (rows <= 0) return;
+  if (rows <= 0) return {{0, 0, 0}, 0, 0, 0};
   const int group = index / (kGroup * column_tiles), in_group = index - group * kGroup * column_tiles;
   const int group_tiles = min(kGroup, tiles - group * kGroup);
   const int mt = group * kGroup + in_group % group_tiles, nt = in_group / group_tiles;
   // 64-row steps of the expert, shared out evenly: the first tiles get one more.
   const int steps = (rows + 63) / 64, each = steps / tiles, more = steps - each * tiles;
-  const int first = seg.begin + 64 * (mt * each + min(mt, more)), count = min(64 * (each + (mt < more)), seg.end - first);
+  const int first = seg.begin + 64 * (mt * each + min(mt, more));
+  return {seg, first, min(64 * (each + (mt < more)), seg.end - first), nt};
+}
+
+template <bool kXMx, bool kWMx, int kJ>
+__global__ __launch_bounds__(kThreads, 1) void tile_kernel(Params p, int cap, int column_tiles) {
+  extern __shared__ char lds[];
+  const auto [seg, first, count, nt] = locate(p, cap, column_tiles);
   if (count <= 0) return;
   switch ((count + 63) / 64) {
     case 1: Body<kXMx, kWMx, 1, kJ>(p).run(lds, seg, first, count, nt); break;
@@ -629,8 +641,8 @@ __global__ __launch_bounds__(kThreads, 1) void tile_kernel(Params p, int cap, in
 }
 
 // Launches tiles of at most `cap` rows (64, 128, 192 or 256) x 64 kJ weight rows.
-template <bool kXMx, bool kWMx, int kJ>
-int launch(const Params& p, int cap, hipStream_t stream) {
+template <int kJ>
+int launch_kernel(void (*kernel)(Params, int, int), const Params& p, int cap, hipStream_t stream) {
   const int64_t columns = p.swiglu ? 32 * kJ : 64 * kJ;
   const int64_t column_tiles = (p.width + columns - 1) / columns;
   // At most: a tile more than whole ones for every expert that has a row.
@@ -638,9 +650,13 @@ int launch(const Params& p, int cap, hipStream_t stream) {
   const int64_t row_tiles = (p.rows + used * (cap - 1)) / cap;
   LF_REQUIRE(row_tiles * column_tiles < (int64_t(1) << 30), "too many tiles");
   const unsigned grid = unsigned((row_tiles * column_tiles + kXcds - 1) / kXcds * kXcds);
-  hipLaunchKernelGGL((tile_kernel<kXMx, kWMx, kJ>), dim3(grid), dim3(kThreads), kLds, stream, p, cap, int(column_tiles));
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), kLds, stream, p, cap, int(column_tiles));
   LF_HIP(hipGetLastError());
   return kOk;
+}
+template <bool kXMx, bool kWMx, int kJ>
+int launch(const Params& p, int cap, hipStream_t stream) {
+  return launch_kernel<kJ>(tile_kernel<kXMx, kWMx, kJ>, p, cap, stream);
 }
 
 }  // namespace tile

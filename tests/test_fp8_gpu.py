@@ -3,7 +3,8 @@
 Codes and scales have to be the oracle's, bit for bit (a scale is one division, rounded
 once). A product may be off by the oracle's bound on fp32 sums, whose count of roundings
 covers those of the scales (a product of two and one a block, each 2^-24 of a block's
-sum), and half a bf16 ulp of the result (2^-8 of it), plus the smallest bf16 subnormal.
+sum), beside FP8 x by what the 8-bit matrix instructions drop (``oracle.fp8.product``), and half a bf16
+ulp of the result (2^-8 of it), plus the smallest bf16 subnormal.
 """
 
 import numpy as np
@@ -13,7 +14,6 @@ import torch
 from loraforge_amd import _lib
 from loraforge_amd.ops import FP8Tensor, dequantize_fp8, expert_linear, fp8_linear, quantize_fp8, quantize_mxfp4
 from loraforge_amd.ops.mxfp4 import product
-from oracle import experts as ox
 from oracle import fp8 as of
 from tests.test_mxfp4_gpu import RAGGED, close, randn, segments
 
@@ -141,7 +141,7 @@ def check_linear(m, n, k, act, device, *, swiglu=False, bias=False, seed=1):
     w, wv = weight(seed + 1, n, k, device=device)
     b = randn(seed + 2, n) if bias else None
     y = fp8_linear(x, w, bias=None if b is None else b.to(device), swiglu=swiglu)
-    close(y, *ox.product(xv, wv, None if b is None else b.double().numpy(), swiglu))
+    close(y, *of.product(xv, wv, None if b is None else b.double().numpy(), swiglu, act == "fp8"))
 
 
 @pytest.mark.parametrize("act", ["bf16", "fp8"])
@@ -171,7 +171,7 @@ def test_linear_strided_x_and_out(m, device):
     out_store = torch.zeros(m, n + 5, dtype=torch.bfloat16, device=device)
     y = fp8_linear(x, w, out=out_store[:, 2 : 2 + n])
     assert y.data_ptr() == out_store[:, 2:].data_ptr()
-    close(y, *ox.product(store[:, 8 : 8 + k].double().numpy(), wv))
+    close(y, *of.product(store[:, 8 : 8 + k].double().numpy(), wv))
     assert not out_store[:, :2].any() and not out_store[:, 2 + n :].any()
 
 
@@ -190,7 +190,7 @@ def test_linear_nan_stays_in_its_row_and_block(m, act, device):
     columns = [33, *range(128, 256)]
     assert torch.isnan(y[7]).all() and torch.isnan(y[:, columns]).all()
     rest_rows, rest_cols = [i for i in range(m) if i != 7], [j for j in range(n) if j not in columns]
-    close(y[rest_rows][:, rest_cols], *ox.product(xv[rest_rows], wv[rest_cols]))
+    close(y[rest_rows][:, rest_cols], *of.product(xv[rest_rows], wv[rest_cols], both=act == "fp8"))
 
 
 def test_linear_no_rows_and_repeatable(device):
@@ -224,7 +224,8 @@ def test_expert_linear_ragged(counts, act, gather, device):
         own = np.arange(start, start + count)
         if count:
             close(y[start : start + count],
-                  *ox.product(xv[tokens[own] if gather else own], wv[e], None if b is None else b[e].double().numpy(), swiglu))
+                  *of.product(xv[tokens[own] if gather else own], wv[e], None if b is None else b[e].double().numpy(), swiglu,
+                              act == "fp8"))
         start += count
 
 
@@ -239,7 +240,7 @@ def test_expert_linear_rows_without_expert_stay(counts, act, device):
     out = torch.full((rows, n), 3.0, dtype=torch.bfloat16, device=device)
     expert_linear(x, w, segments(counts).to(device), tokens=tokens.to(device), out=out)
     assert (out[sum(counts) :] == 3.0).all()
-    close(out[: counts[0]], *ox.product(xv[tokens[: counts[0]].numpy()], wv[0]))
+    close(out[: counts[0]], *of.product(xv[tokens[: counts[0]].numpy()], wv[0], both=act == "fp8"))
 
 
 def test_products_on_a_side_stream_and_in_a_graph(device):
@@ -303,7 +304,21 @@ def test_refusals(device):
 # Every kernel, forced
 # --------------------------------------------------------------------------
 
-PLANS = [(_lib.LF_EXPERT_STREAM, part, c) for part in (16, 32, 64) for c in (16, 32)]
+STREAM = [(_lib.LF_EXPERT_STREAM, part, c) for part in (16, 32, 64) for c in (16, 32)]
+
+
+def tiles(act):
+    """Tile heights that there are beside a width: the sums leave no registers for more."""
+    most = {"fp8": (256, 192), "bf16": (192, 128)}[act]
+    return [(_lib.LF_EXPERT_TILE, r, c) for c in (64, 128, 192, 256) for r in (64, 128, 192, 256) if r <= most[c == 256]]
+
+
+PLANS = {act: STREAM + tiles(act) for act in ("bf16", "fp8")}
+BOTH = [(act, plan) for act in PLANS for plan in PLANS[act]]
+
+
+def name(v):
+    return "-".join(map(str, v)) if isinstance(v, tuple) else v
 
 
 def forced(x, w, plan, **options):
@@ -311,9 +326,8 @@ def forced(x, w, plan, **options):
     return product(x, w, **{**arguments, **options}, plan=_lib.ExpertPlan(*plan))
 
 
-@pytest.mark.parametrize("act", ["bf16", "fp8"])
-@pytest.mark.parametrize("plan", PLANS, ids=lambda p: "-".join(map(str, p)))
-@pytest.mark.parametrize("k", [128, 416, 2896])
+@pytest.mark.parametrize("act,plan", BOTH, ids=name)
+@pytest.mark.parametrize("k", [16, 128, 416, 2896])
 def test_every_plan(act, plan, k, device):
     counts = [130, 0, 1, 64, 257, 33, 190]
     n, rows = 328, sum(counts)
@@ -324,12 +338,11 @@ def test_every_plan(act, plan, k, device):
     start = 0
     for e, count in enumerate(counts):
         if count:
-            close(y[start : start + count], *ox.product(xv[start : start + count], wv[e], b[e].double().numpy()))
+            close(y[start : start + count], *of.product(xv[start : start + count], wv[e], b[e].double().numpy(), False, act == "fp8"))
         start += count
 
 
-@pytest.mark.parametrize("act", ["bf16", "fp8"])
-@pytest.mark.parametrize("plan", PLANS, ids=lambda p: "-".join(map(str, p)))
+@pytest.mark.parametrize("act,plan", BOTH, ids=name)
 @pytest.mark.parametrize("n", [256, 768])
 def test_every_plan_swiglu(act, plan, n, device):
     k, counts = 544, [70, 3, 200]
@@ -339,14 +352,15 @@ def test_every_plan_swiglu(act, plan, n, device):
     y = forced(x, w, plan, experts=len(counts), offsets=segments(counts).to(device), bias=b.to(device), swiglu=True)
     start = 0
     for e, count in enumerate(counts):
-        close(y[start : start + count], *ox.product(xv[start : start + count], wv[e], b[e].double().numpy(), True))
+        close(y[start : start + count], *of.product(xv[start : start + count], wv[e], b[e].double().numpy(), True, act == "fp8"))
         start += count
 
 
 @pytest.mark.parametrize("act", ["bf16", "fp8"])
 @pytest.mark.parametrize("k", [8208, 12304])
 def test_long_k_exact_on_every_kernel(act, k, device):
-    """Small integers with scales that are powers of two: fp32 sums in any order are exact, so results are equal."""
+    """Small integers with scales that are powers of two: fp32 sums in any order are exact (and products of
+    integers to 8 within 13 bits of one another), so results are equal."""
     rng = np.random.default_rng(k)
     counts, n = [70, 0, 1, 130], 136
     blocks = -(-k // 128)
@@ -368,7 +382,7 @@ def test_long_k_exact_on_every_kernel(act, k, device):
     exact = np.concatenate([xv[own == e] @ wv[e].T for e in range(len(counts))])
     assert max((np.abs(xv[own == e]) @ np.abs(wv[e]).T).max() for e in (0, 2, 3)) * 4 < 2**24
     expected = torch.from_numpy(exact).float().bfloat16()
-    for plan in PLANS:
+    for plan in PLANS[act]:
         y = forced(x, w, plan, experts=len(counts), offsets=segments(counts).to(device))
         assert torch.equal(y.cpu(), expected), plan
 
@@ -388,11 +402,67 @@ def test_extreme_scales_on_every_kernel(act, device):
         x.scales[::3] = 1e-41
         x.scales[1::3] *= 2.0**-70
         xv = of.values(x.codes.view(torch.uint8).cpu().numpy(), x.scales.cpu().numpy())
-    y, bound = ox.product(xv, wv)
+    y, bound = of.product(xv, wv, both=act == "fp8")
     # (A product of two scales below the normal range may be flushed: at most 2^-126 of a block's code sum of 448^2 128.)
     bound = bound + 2.0**-126 * 448**2 * 128 * 17
-    for plan in PLANS:
+    for plan in PLANS[act]:
         close(forced(x, FP8Tensor(w.codes[None], w.scales[None]), plan, experts=1, offsets=segments([m]).to(device)), y, bound)
+
+
+@pytest.mark.parametrize("act", ["bf16", "fp8"])
+def test_tiles_of_one_dense_product(act, device):
+    """Several row and column tiles of one segment; results do not depend on the tile."""
+    m, n, k = 1300, 712, 528
+    x, xv = operand(randn(40, m, k), act, device)
+    w, wv = weight(41, 1, n, k, device=device)
+    first = None
+    for plan in tiles(act):
+        y = forced(x, w, plan, experts=1, offsets=segments([m]).to(device))
+        if first is None:
+            first = y
+            close(y, *of.product(xv, wv[0], both=act == "fp8"))
+        assert torch.equal(y, first), plan
+
+
+@pytest.mark.parametrize("act", ["bf16", "fp8"])
+def test_gathered_rows_and_output_of_any_alignment(act, device):
+    m, n, k = 200, 264, 592
+    x, xv = operand(randn(42, m, k), act, device)
+    w, wv = weight(43, 1, n, k, device=device)
+    tokens = torch.arange(m - 1, -1, -1, dtype=torch.int32, device=device)
+    want = of.product(xv[::-1], wv[0], both=act == "fp8")
+    for plan in PLANS[act]:
+        for pad, at in ((0, 0), (8, 8), (3, 1)):
+            store = torch.zeros(m, n + pad, dtype=torch.bfloat16, device=device)
+            out = store[:, at : at + n]
+            forced(x, w, plan, experts=1, offsets=segments([m]).to(device), tokens=tokens, out=out)
+            close(out, *want)
+            assert not store[:, :at].any() and not store[:, at + n :].any()
+
+
+@pytest.mark.parametrize("act", ["bf16", "fp8"])
+@pytest.mark.parametrize("over", [False, True])
+def test_rows_around_2_gib(act, over, device):
+    """x whose rows end just below and above 2 GiB (the tiles' offsets): only its last rows are named."""
+    n, k, rows = 96, 4096, 130
+    total = 2**31 // (k if act == "fp8" else 2 * k) + (5 if over else -1)
+    last, lv = operand(randn(64, rows, k), act, device)
+    w, wv = weight(65, 1, n, k, device=device)
+    tokens = torch.arange(total - rows, total, dtype=torch.int32, device=device)
+    if act == "fp8":
+        x = FP8Tensor(torch.zeros(total, k, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                      torch.zeros(total, k // 128, device=device))
+        x.codes.view(torch.uint8)[-rows:], x.scales[-rows:] = last.codes.view(torch.uint8), last.scales
+    else:
+        x = torch.zeros(total, k, dtype=torch.bfloat16, device=device)
+        x[-rows:] = last
+    close(expert_linear(x, w, segments([rows]).to(device), tokens=tokens), *of.product(lv, wv[0], both=act == "fp8"))
+    for plan in PLANS[act]:
+        if over and plan[0] == _lib.LF_EXPERT_TILE:
+            with pytest.raises(ValueError, match="tiles"):
+                forced(x, w, plan, experts=1, offsets=segments([rows]).to(device), tokens=tokens)
+        else:
+            close(forced(x, w, plan, experts=1, offsets=segments([rows]).to(device), tokens=tokens), *of.product(lv, wv[0], both=act == "fp8"))
 
 
 def test_weights_past_4_gib(device):
@@ -407,5 +477,6 @@ def test_weights_past_4_gib(device):
     columns = np.arange(0, n, 97)
     for rows in (2, 130):
         offsets[-1] = rows
-        for xi, xv in ((x[:rows], x[:rows].double().cpu().numpy()), operand(x[:rows].cpu(), "fp8", device)):
-            close(expert_linear(xi, w, offsets.to(device))[:, columns], *ox.product(xv, wv[columns]))
+        for act in ("bf16", "fp8"):
+            xi, xv = operand(x[:rows].cpu(), act, device)
+            close(expert_linear(xi, w, offsets.to(device))[:, columns], *of.product(xv, wv[columns], both=act == "fp8"))

@@ -47,3 +47,16 @@ def test_quantize_zero_tiny_and_not_finite():
     codes, scales = of.quantize(x)
     assert (scales[:2] == np.float32(2.0**-100 / 448)).all() and not codes[0].any()
     assert np.isnan(of.values(codes, scales)[2:]).all() and not codes[2:].any()
+
+
+def test_product_bounds():
+    """Beside FP8 x the bound grows by what eight aligned products may lose, and covers a model of that loss."""
+    rng = np.random.default_rng(3)
+    x, w = (of.values(*of.quantize(rng.standard_normal((5, 48)) * np.exp2(rng.integers(-6, 7, (5, 48))))) for _ in range(2))
+    y, bound = of.product(x, w)
+    y8, bound8 = of.product(x, w, both=True)
+    assert np.array_equal(y, y8) and (bound8 > bound).all()
+    p = (x[:, None] * w[None]).reshape(5, 5, 6, 8)
+    unit = np.exp2(np.floor(np.log2(np.abs(p).max(-1, keepdims=True))) - 13)
+    kept = (np.trunc(p / unit) * unit).sum((-1, -2))
+    assert (np.abs(kept - y) <= bound8 - bound).all() and (np.abs(kept - y) > bound).any()
