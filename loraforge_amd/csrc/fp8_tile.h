@@ -71,20 +71,41 @@ struct Body {
   static constexpr int kPairs = kI * kJ;
   const Params& p;
   int lane, wave, h, stages, blocks;
+  int plain_stages;  // first ones that need no checks
   // Copies: buffers, the lane's offset of each x row that it copies (its 16-byte unit added), of
   // its first weight row (the others a uniform step apart) and of its rows' scales.
   __amdgpu_buffer_rsrc_t xbuf, wbuf, xsbuf, wsbuf;
   uint32_t xrow[S::kXCopies], wrow, wstep, xsrow, wsrow;
+  // (With 192 sums they are kept where vector instructions do not reach, and fetched for each copy: left to itself the
+  // compiler moves ten times as many values to and fro.)
+  static constexpr bool kFar = kI * kJ * 16 > (kX8 ? 160 : 112);
   int xunit, wunit;  // byte of the lane's unit in a stage's row
   // Operand reads: byte offsets in a slot of unit n of fragment 0, and of its scales.
   uint32_t xat[S::kXUnits], wat[4], xsat, wsat;
   f32x16 acc[kI][kJ];
   u32x4 x[kI][S::kXUnits], w[kX8 ? 2 : 1][4], wd[kX8 ? 1 : 8];
-  float sx[kX8 ? kI : 1], sw[2][2];  // x rows'; gate (or all) and up rows' of a weight fragment, two in turn
+  // Weight scales of the gate (or all) and the up rows, two in turn: of a wave's rows where those lie in one
+  // block of 128 each (all widths but 192), else of a fragment's. x rows' scales, in scale[i][0] until they are
+  // multiplied with the weights'.
+  static constexpr bool kOneBlock = kJ != 3;
+  float sw[2][2], scale[kI][2];
   f32x16 t[2];
   float due[2];  // scales of the pair whose products wait in T
 
   __device__ __forceinline__ Body(const Params& p_) : p(p_) {}
+
+  static __device__ __forceinline__ uint32_t far(uint32_t v) {
+    if constexpr (kFar) asm volatile("v_accvgpr_write_b32 %0, %1" : "=a"(v) : "v"(v));
+    return v;
+  }
+  static __device__ __forceinline__ uint32_t near(uint32_t v) {
+    if constexpr (kFar) {
+      uint32_t to;
+      asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(to) : "a"(v));
+      return to;
+    }
+    return v;
+  }
 
   __device__ __forceinline__ int weight_row(int nt, int r) const {
     if (!p.swiglu) return min(nt * 64 * kJ + r, p.n - 1);
@@ -92,36 +113,71 @@ struct Body {
     return min(column, p.width - 1) + (r / 16 % 2 ? p.width : 0);
   }
 
-  // Copies first .. last - 1 of stage st into a slot.
+  // A stage's copies in the order of their issue: x, its scales and the weight fragments that are read before the
+  // stage's first barrier (kEarly of them), then the others. (Copies j and kJ + j are fragment j's, for both halves of the
+  // tile. The weights' scales are read with each fragment where they are not one for all: with the late ones then.)
+  static constexpr int kEarlyFrags = kJ >= 3 ? 2 : kJ == 2 ? 1 : 0;
+  static constexpr int kEarly = kJ == 1 ? 0 : S::kXCopies + 2 * kEarlyFrags + (kX8 ? 1 : 0) + (kOneBlock ? 1 : 0);
+  static constexpr int kLate = S::kLoads - kEarly;
+  // Pair of the first of two weight fragments that begins with the first barrier and the read of the second fragment
+  // (not the first pair: the barrier would wait for the reads behind the last stage).
+  static constexpr int kRead = kI > 1 ? 1 : 0;
+
+  // Copies first .. last - 1 of stage st into a slot. kChecked: any stage of any tile; else st is a whole stage of
+  // k, and all of the tile's weight rows are there (their step is then part of the uniform offset).
+  template <bool kChecked>
   __device__ __forceinline__ void copy(const Slot& to, int st, int first, int last) {
     if (first >= last) return;
-    const uint32_t xpast = st * S::kXRow + xunit < (kX8 ? p.k : 2 * p.k) ? 0u : kPast;
-    const uint32_t wpast = st * kWRow + wunit < p.k ? 0u : kPast;
-    const uint32_t spast = st < blocks ? 0u : kPast;
-    const int base = min(st, blocks - 1);  // (below every buffer's end, where the range check may subtract it)
+    uint32_t xpast = 0, wpast = 0, spast = 0;
+    int base = st;
+    if constexpr (kChecked) {
+      xpast = st * S::kXRow + xunit < (kX8 ? p.k : 2 * p.k) ? 0u : kPast;
+      wpast = st * kWRow + wunit < p.k ? 0u : kPast;
+      spast = st < blocks ? 0u : kPast;
+      base = min(st, blocks - 1);  // (below every buffer's end, where the range check may subtract it)
+    }
+    int at = 0;
+    auto now = [&]() {
+      const bool in = at >= first && at < last;
+      ++at;
+      return in;
+    };
+    auto weights = [&](int d) {
+      if (!now()) return;
+      if constexpr (kChecked)
+        copy16(wbuf, to.w + (d * 4 + wave) * 1024, (wrow | wpast) + d * wstep, base * kWRow);
+      else
+        copy16(wbuf, to.w + (d * 4 + wave) * 1024, wrow, base * kWRow + d * wstep);
+    };
+    auto weight_scales = [&]() {
+      if (now()) copy4(wsbuf, to.s + wave * 256, wsrow | spast, base * 4);
+    };
 #pragma unroll
     for (int d = 0; d < S::kXCopies; ++d)
-      if (d >= first && d < last) copy16(xbuf, to.x + (d * 4 + wave) * 1024, xrow[d] | xpast, base * S::kXRow);
+      if (now()) copy16(xbuf, to.x + (d * 4 + wave) * 1024, near(xrow[d]) | xpast, base * S::kXRow);
 #pragma unroll
-    for (int d = 0; d < S::kWCopies; ++d)
-      if (d + S::kXCopies >= first && d + S::kXCopies < last)
-        copy16(wbuf, to.w + (d * 4 + wave) * 1024, (wrow | wpast) + d * wstep, base * kWRow);
-    constexpr int kScale = S::kXCopies + S::kWCopies;
-    if (kScale >= first && kScale < last) copy4(wsbuf, to.s + wave * 256, wsrow | spast, base * 4);
-    if (kX8 && kScale + 1 >= first && kScale + 1 < last) copy4(xsbuf, to.s + kThreads * 4 + wave * 256, xsrow | spast, base * 4);
+    for (int j = 0; j < kEarlyFrags; ++j) weights(j), weights(kJ + j);
+    if constexpr (kX8)
+      if (now()) copy4(xsbuf, to.s + kThreads * 4 + wave * 256, xsrow | spast, base * 4);
+    weight_scales();
+#pragma unroll
+    for (int j = kEarlyFrags; j < kJ; ++j) weights(j), weights(kJ + j);
   }
 
   __device__ __forceinline__ void read_x(const Slot& from, int i) {
 #pragma unroll
     for (int u = 0; u < S::kXUnits; ++u) x[i][u] = *reinterpret_cast<const u32x4*>(from.x + xat[u] + i * 64 * S::kXRow);
-    if constexpr (kX8) sx[i] = *reinterpret_cast<const float*>(from.s + kThreads * 4 + xsat + i * 64 * 4);
+    if constexpr (kX8) scale[i][0] = *reinterpret_cast<const float*>(from.s + kThreads * 4 + xsat + i * 64 * 4);
   }
-  // Weight fragment j and its scales, into buffer b.
+  __device__ __forceinline__ void read_ws(const Slot& from, int j, int b) {
+    sw[b][0] = *reinterpret_cast<const float*>(from.s + wsat + j * 32 * 4);
+    sw[b][1] = *reinterpret_cast<const float*>(from.s + wsat + j * 32 * 4 + 16 * 4);
+  }
+  // Weight fragment j into buffer b, and its scales.
   __device__ __forceinline__ void read_w(const Slot& from, int j, int b) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) w[kX8 ? b : 0][u] = *reinterpret_cast<const u32x4*>(from.w + wat[u] + j * 32 * kWRow);
-    sw[b][0] = *reinterpret_cast<const float*>(from.s + wsat + j * 32 * 4);
-    sw[b][1] = *reinterpret_cast<const float*>(from.s + wsat + j * 32 * 4 + 16 * 4);
+    if constexpr (!kOneBlock) read_ws(from, j, b);
   }
   // Unit m (8 k of a lane) of the weight fragment that was read last.
   __device__ __forceinline__ void decode(int m) {
@@ -135,16 +191,14 @@ struct Body {
       if (r >= first && r < last) sums[r] = fmaf(due[r / 8], from[r], sums[r]);
   }
 
-  // The first copies of a stage go out behind the last weight fragment of the stage that frees their slot, the
-  // others spread over this many pairs of the stage after (of one fragment: none, as that has to be waited for at once).
-  static constexpr int kFirst = kJ == 1 ? S::kLoads : S::kLoads / 2;
-  static constexpr int kRest = kJ == 1 ? 1 : (kPairs + 2) / 3;
-  static_assert(kJ == 1 || kRest <= (kJ - 1) * kI, "all copies of a stage go out before the barrier that awaits them");
-
   // Stage st, at place kPos of a round: its x fragments, its first weight fragment and their scales are
-  // read. `next` holds the stage after it; `prev` is the slot that the stage before has freed.
-  template <int kPos>
-  __device__ __forceinline__ void stage(const Slot& prev, const Slot& cur, const Slot& next, int st) {
+  // read. `next` holds the stage after it. Two barriers: behind the first, x and the early weight fragments of
+  // `cur` have been read by every wave, and their copies for the stage that comes into it go out; behind the second
+  // (at the last weight fragment) the late ones. So a copy has a stage and a third or more until it is
+  // waited for (with one barrier and all copies behind it they had two thirds on average: their latency,
+  // some 2000 clocks under load, then bounded every tile: 4096 x 12288 x 4096 in 192 x 256 2340 clocks a stage).
+  template <int kPos, bool kChecked>
+  __device__ __forceinline__ void stage(const Slot& cur, const Slot& next, int st) {
     constexpr int kWBase = kPos * kJ, kTBase = kPos * kPairs;
     constexpr int kSteps = kX8 ? 2 : 8;
 #pragma unroll
@@ -152,10 +206,17 @@ struct Body {
       const int j = n / kI, i = n % kI;
       const int b = (kWBase + j) & 1, tn = (kTBase + n) & 1;
       const bool last = j == kJ - 1;
-      if (n == (kJ - 1) * kI) {
-        // Every wave has read all of `cur`, and `next` has arrived: at most the stages after it are on their way.
+      constexpr int kFirst = kJ == 2 ? kRead : (kEarlyFrags - 1) * kI, kLast = (kJ - 1) * kI;  // pairs that begin with a barrier
+      if (kJ > 1 && n == kFirst) {
+        // The late copies of `cur` have arrived.
         reads_done();
-        wait_vm<(S::kSlots - 2) * S::kLoads>();
+        wait_vm<(S::kSlots - 1) * S::kLoads>();
+        barrier_only();
+      }
+      if (n == kLast) {
+        // The early copies of `next` have arrived (and the first of the late ones, where those are the scales).
+        reads_done();
+        wait_vm<kJ == 1 ? (S::kSlots - 2) * S::kLoads : (S::kSlots - 1) * S::kLoads - (kOneBlock ? 0 : 1)>();
         barrier_only();
       }
       const int pi = n ? (n - 1) % kI : kI - 1, pj = n ? (n - 1) / kI : kJ - 1;  // the pair whose products wait
@@ -172,29 +233,55 @@ struct Body {
           t[tn] = mfma32(vec_bf16x8(wd[m]), vec_bf16x8(x[i][m]), m == 0 ? f32x16{} : t[tn]);
         }
         pin();
+        // (Reads and copies first: the products that wait are not there yet.)
         if (m == 0) {
-          if (i == 0) {
+          if (i == (kJ == 2 && !last ? kRead : 0)) {
             if (last)
               read_w(next, 0, (kWBase + kJ) & 1);
             else
               read_w(cur, j + 1, b ^ 1);
+            if (kOneBlock && last) read_ws(next, 0, (kPos + 1) & 1);
           }
-          if (last) copy(cur, st + S::kSlots, i * kFirst / kI, (i + 1) * kFirst / kI);
+          constexpr int kOver = kLast - kFirst;  // pairs that the early copies are spread over
+          if (last)
+            copy<kChecked>(cur, st + S::kSlots, kEarly + i * kLate / kI, kEarly + (i + 1) * kLate / kI);
+          else if (n >= kFirst)
+            copy<kChecked>(cur, st + S::kSlots, (n - kFirst) * kEarly / kOver, (n - kFirst + 1) * kEarly / kOver);
+          pin();
         }
-        if (m == kSteps / 2 && n < kRest)
-          copy(prev, st + S::kSlots - 1, kFirst + n * (S::kLoads - kFirst) / kRest, kFirst + (n + 1) * (S::kLoads - kFirst) / kRest);
         // (The next fragment's weights take the place of those that this pair, the fragment's last, is done with.)
         if (!kX8 && i == kI - 1 && m > 0) decode(m - 1);
-        settle(acc[pi][pj], t[tn ^ 1], m * 16 / kSteps, (m + 1) * 16 / kSteps);
+        // A block's products are done some 12 clocks after its last instruction, so fewer of them are added at first.
+        if constexpr (kX8)
+          settle(acc[pi][pj], t[tn ^ 1], m ? 6 : 0, m ? 16 : 6);
+        else if (m)
+          settle(acc[pi][pj], t[tn ^ 1], (m - 1) * 16 / 7, m * 16 / 7);
       }
       if (!kX8 && i == kI - 1) decode(kSteps - 1);
-      due[0] = sw[b][0];
-      due[1] = sw[b][1];
+      const int sb = kOneBlock ? kPos & 1 : b;
       if constexpr (kX8) {
-        due[0] *= sx[i];
-        due[1] *= sx[i];
+        if (kOneBlock && j == 0) {
+          scale[i][1] = scale[i][0] * sw[sb][1];
+          scale[i][0] *= sw[sb][0];
+        }
+        due[0] = kOneBlock ? scale[i][0] : scale[i][0] * sw[sb][0];
+        due[1] = kOneBlock ? scale[i][1] : scale[i][0] * sw[sb][1];
+      } else {
+        due[0] = sw[sb][0];
+        due[1] = sw[sb][1];
       }
       if (last) read_x(next, i);
+    }
+  }
+
+  template <bool kChecked>
+  __device__ __forceinline__ void round(const Slot (&slot)[4], int st) {
+    constexpr int kN = S::kSlots;
+    stage<0, kChecked>(slot[0], slot[1], st);
+    stage<1, kChecked>(slot[1], slot[2 % kN], st + 1);
+    if constexpr (kN == 4) {
+      stage<2, kChecked>(slot[2], slot[3], st + 2);
+      stage<3, kChecked>(slot[3], slot[0], st + 3);
     }
   }
 
@@ -204,24 +291,20 @@ struct Body {
     constexpr int kN = S::kSlots;
     const Slot slot[4] = {{x0, w0, s0}, {x1, w1, s1}, {x2, w2, s2}, {x3, w3, s3}};
 #pragma unroll
-    for (int n = 0; n < kN - 1; ++n) copy(slot[n], n, 0, S::kLoads);
-    copy(slot[kN - 1], kN - 1, 0, kFirst);
-    wait_vm<(kN - 2) * S::kLoads + kFirst>();
+    for (int n = 0; n < kN; ++n) copy<true>(slot[n], n, 0, S::kLoads);
+    wait_vm<(kN - 1) * S::kLoads>();
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < kI; ++i) read_x(slot[0], i);
     read_w(slot[0], 0, 0);
+    if (kOneBlock) read_ws(slot[0], 0, 0);
 #pragma unroll
     for (int m = 0; m < 8; ++m)
       if (!kX8) decode(m);
-    for (int st = 0; st < stages; st += kN) {  // (whole rounds: stages past the end are zeros)
-      stage<0>(slot[kN - 1], slot[0], slot[1], st);
-      stage<1>(slot[0], slot[1], slot[2 % kN], st + 1);
-      if constexpr (kN == 4) {
-        stage<2>(slot[1], slot[2], slot[3], st + 2);
-        stage<3>(slot[2], slot[3], slot[0], st + 3);
-      }
-    }
+    // Rounds that copy whole stages of whole tiles, then those that may not (stages past the end are zeros).
+    int st = 0;
+    for (; st + 2 * kN <= plain_stages; st += kN) round<false>(slot, st);
+    for (; st < stages; st += kN) round<true>(slot, st);
     settle(acc[kI - 1][kJ - 1], t[(kN * kPairs - 1) & 1], 0, 16);
   }
 
@@ -233,6 +316,8 @@ struct Body {
     const int wm = wave & 1, wn = wave >> 1, c = lane & 31;
     blocks = int(fp8::blocks_of(p.k));
     stages = blocks;
+    plain_stages = p.swiglu ? ((nt + 1) * 32 * kJ <= p.width ? p.k / fp8::kBlock : 0)
+                            : ((nt + 1) * 64 * kJ <= p.n ? p.k / fp8::kBlock : 0);
     const int last = first + count - 1;
 
     // Rows of 128 bytes: row r's unit u sits at u ^ (r / 2 % 8), eight rows a copy; rows of 256 bytes: at u ^ (r % 16),
@@ -249,7 +334,7 @@ struct Body {
 #pragma unroll
     for (int d = 0; d < S::kXCopies; ++d) {
       const int64_t row = x_row_of(p, min(first + kXRows * (d * 4 + wave) + xr, last));
-      xrow[d] = uint32_t(row * p.x_row) + xunit;
+      xrow[d] = far(uint32_t(row * p.x_row) + xunit);
     }
     // (Weight rows past n lie past the buffer's end, or are up rows in the place of gate columns that nobody stores.)
     const int r0 = 8 * wave + wr;
