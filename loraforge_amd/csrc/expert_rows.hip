@@ -11,10 +11,12 @@
 //
 // Each wave streams its weights through a ring of three stages (16 rows x 128 bytes:
 // 256 k in MXFP4, 64 in bf16) without meeting the others; x comes in chunks of 8 KiB
-// for all waves, two buffers, one barrier a chunk. v_mfma_f32_16x16x32_bf16 (MXFP4
+// for all waves, two buffers, one barrier a chunk. v_mfma_f32_16x16x32_bf16 (MXFP4 and FP8
 // weights decoded in registers), v_mfma_scale_f32_16x16x128_f8f6f4 where x is MXFP4
-// too; the weight is the A operand, up to 16 rows of x the B operand. Lane quarter q
-// takes units (of 16 bytes) 2 q and 2 q + 1 of a stage, so its two scales are neighbours.
+// too, its form without scales where both are FP8; the weight is the A operand, up to 16 rows of x the
+// B operand. Lane quarter q takes units (of 16 bytes) 2 q and 2 q + 1 of a stage, so its two MXFP4 scales are
+// neighbours. A stage of FP8 weights is 128 k, one block of scales: its products are summed from zero and added
+// times x's scale (copied with x's chunks) and the weights' (uniform loads, a stage ahead).
 #include "expert_params.h"
 #include "lds_pipeline.h"
 
@@ -39,6 +41,11 @@ __device__ __forceinline__ void lds_write16(uint32_t at, const u32x4& v) {
 __device__ __forceinline__ uint32_t lds_scales(uint32_t at) {
   uint32_t v;
   asm volatile("ds_read_u16 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float lds_float(uint32_t at) {
+  float v;
+  asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(at) : "memory");
   return v;
 }
 __device__ __forceinline__ void lds_four(u32x4 (&v)[4], const uint32_t (&at)[4], uint32_t base) {
@@ -79,9 +86,11 @@ struct ScaleLoad {
   __device__ __forceinline__ void store(uint32_t area) const { lds_write16(area + (threadIdx.x & 63) * 16, mx::drop_bytes(v, skip)); }
 };
 
-template <bool kXMx, bool kWMx>
+template <int kX, int kW>
 struct Rows {
-  static constexpr int kXStage = kWMx && !kXMx ? 512 : 128;  // bytes of an x row per stage
+  static constexpr bool kXMx = kX == kMxfp4, kWMx = kW == kMxfp4, kX8 = kX == kFp8, kW8 = kW == kFp8;
+  static constexpr int kXStage = kWMx && !kXMx ? 512 : kW8 && !kX8 ? 256 : 128;  // bytes of an x row per stage
+  static constexpr int kScaleBytes = kXMx ? 2 * kScaleUnit : kWMx ? kScaleUnit : kX8 ? 2 * 256 : 0;  // of a wave
 
   // Rows first .. first + 15 of the segment, 128 weight rows of block `block`.
   static __device__ __forceinline__ void run(const Params& p, const Segment& seg, int first, int block, char* lds) {
@@ -91,12 +100,12 @@ struct Rows {
     const int shift = count <= 4 ? 2 : count <= 8 ? 3 : 4;  // rows of an x chunk, rounded up: 4, 8 or 16
     const int x_piece = kXBytes >> shift;                   // bytes of a row in a chunk
     const int chunk_stages = x_piece / kXStage;
-    const int row_bytes_x = kXMx ? p.k / 2 : p.k * 2, row_bytes_w = kWMx ? p.k / 2 : p.k * 2;
+    const int row_bytes_x = kXMx ? p.k / 2 : kX8 ? p.k : p.k * 2, row_bytes_w = kWMx ? p.k / 2 : kW8 ? p.k : p.k * 2;
     const int stages = (row_bytes_w + 127) / 128, blocks = p.k / mx::kBlock;
     const char* zeros = reinterpret_cast<const char*>(&kZeros);
     char* xbuf = lds;
     char* ring = lds + 2 * kXBytes + wave * kRing * kSlot;
-    char* scale_area = lds + 2 * kXBytes + kWaves * kRing * kSlot + wave * kScaleUnit * (kXMx ? 2 : 1);
+    char* scale_area = lds + 2 * kXBytes + kWaves * kRing * kSlot + wave * kScaleBytes;
 
     // Weight row r of the wave: a column each, or (SwiGLU) gate rows 0 .. 7 and up rows 8 .. 15 of eight columns.
     const int column0 = block * (p.swiglu ? 64 : 128) + wave * (p.swiglu ? 8 : 16);
@@ -119,10 +128,23 @@ struct Rows {
       copy16(in ? wsrc[0] + st * 128 : zeros, slot);
       copy16(in ? wsrc[1] + st * 128 : zeros, slot + 1024);
     };
+    const float* xs8 = kX8 ? p.xs8 + x_row(lane / chunk_stages) * stages : nullptr;
     auto copy_x = [&](int ch) {
       const bool in = ch * x_piece + xat < row_bytes_x;
       copy16(in ? xsrc + int64_t(ch) * x_piece : zeros, xbuf + (ch & 1) * kXBytes + wave * 1024);
+      if constexpr (kX8) {  // the chunk's 64 scales, a copy for each wave
+        const int st = ch * chunk_stages + (lane & (chunk_stages - 1));
+        copy4(st < stages ? xs8 + st : reinterpret_cast<const float*>(zeros), scale_area + (ch & 1) * 256);
+      }
     };
+    // FP8: the scales of the gate (or all) and the up rows' blocks.
+    const float *ws8 = nullptr, *us8 = nullptr;
+    float s8 = 0.f, u8 = 0.f;
+    if constexpr (kW8) {
+      ws8 = fp8_scales(p, seg.expert, min(column0, p.width - 1));
+      us8 = p.swiglu ? fp8_scales(p, seg.expert, min(column0, p.width - 1) + p.width) : ws8;
+      s8 = sload(ws8, 0), u8 = sload(us8, 0);
+    }
     ScaleLoad ws, xs;
     if constexpr (kWMx) {
       ws.row = p.ws + weight_row(lane >> 2) * blocks;
@@ -145,7 +167,7 @@ struct Rows {
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        xread[s][j] = uint32_t(xc * x_piece + (((kXStage == 512 ? 4 * (2 * q + s) + j : 2 * q + s) ^ (xc & 7)) * 16));
+        xread[s][j] = uint32_t(xc * x_piece + (((kXStage == 512 ? 4 * (2 * q + s) + j : kXStage == 256 ? 4 * q + j : 2 * q + s) ^ (xc & 7)) * 16));
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int st = 0; st < stages; ++st) {
       // Stage st has arrived, and the x chunk that starts with it (copied before it).
@@ -168,7 +190,29 @@ struct Rows {
       uint32_t wscale = 0, xscale = 0;
       if constexpr (kWMx) wscale = lds_scales(scale_at + c * 64 + st % kScaleStages * 8 + 2 * q);
       if constexpr (kXMx) xscale = lds_scales(scale_at + kScaleUnit + xc * 64 + st % kScaleStages * 8 + 2 * q);
-      if constexpr (kXStage == 512) {
+      if constexpr (kW8) {
+        const float w_scale = q >= 2 ? u8 : s8;
+        const int ahead = min(st + 1, stages - 1);
+        s8 = sload(ws8, ahead), u8 = sload(us8, ahead);
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        float scale = w_scale;
+        if constexpr (kX8) {
+          u32x4 v[4];
+          const uint32_t at[4] = {slot + wread[0], slot + wread[1], x_base + xread[0][0], x_base + xread[1][0]};
+          lds_four(v, at, 0);
+          scale *= lds_float(scale_at + (st / chunk_stages & 1) * 256 + (xc * chunk_stages + st % chunk_stages) * 4);
+          sum = fp8::mfma16(fp8::operand(v[0], v[1]), fp8::operand(v[2], v[3]));
+        } else {
+          u32x4 w[2], x[4];
+          lds_two(w, slot + wread[0], slot + wread[1]);
+          lds_four(x, xread[0], x_base);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sum = lf::mfma16(vec_bf16x8(fp8::decode8(w[j >> 1][j % 2 * 2], w[j >> 1][j % 2 * 2 + 1])), vec_bf16x8(x[j]), sum);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(scale, sum[e], acc[e]);
+      } else if constexpr (kXStage == 512) {
         u32x4 w[2];
         lds_two(w, slot + wread[0], slot + wread[1]);
 #pragma unroll
@@ -219,21 +263,21 @@ struct Rows {
 };
 
 // Grid: blocks of 128 weight rows x experts that have rows.
-template <bool kXMx, bool kWMx>
+template <int kX, int kW>
 __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
   extern __shared__ char lds[];
   int index = blockIdx.y;
   const Segment seg = find_segment(p, index, [](const Segment& s) { return s.end > s.begin ? 1 : 0; });
-  for (int first = seg.begin; first < seg.end; first += 16) Rows<kXMx, kWMx>::run(p, seg, first, blockIdx.x, lds);
+  for (int first = seg.begin; first < seg.end; first += 16) Rows<kX, kW>::run(p, seg, first, blockIdx.x, lds);
 }
 
-template <bool kXMx, bool kWMx>
+template <int kX, int kW>
 int launch_types(const Params& p, hipStream_t stream) {
   const int segments = p.offsets ? (p.experts < p.rows ? p.experts : p.rows) : 1;
   const int columns = p.swiglu ? 64 : 128;
   const dim3 grid(unsigned((p.width + columns - 1) / columns), unsigned(segments));
-  const unsigned lds = 2 * kXBytes + kWaves * (kRing * kSlot + kScaleUnit * (kXMx ? 2 : 1));
-  hipLaunchKernelGGL((rows_kernel<kXMx, kWMx>), grid, dim3(kThreads), lds, stream, p);
+  const unsigned lds = 2 * kXBytes + kWaves * (kRing * kSlot + Rows<kX, kW>::kScaleBytes);
+  hipLaunchKernelGGL((rows_kernel<kX, kW>), grid, dim3(kThreads), lds, stream, p);
   LF_HIP(hipGetLastError());
   return kOk;
 }
@@ -241,8 +285,9 @@ int launch_types(const Params& p, hipStream_t stream) {
 }  // namespace
 
 int launch_rows(const Params& p, hipStream_t stream) {
-  if (p.xs) return launch_types<true, true>(p, stream);
-  return p.ws ? launch_types<false, true>(p, stream) : launch_types<false, false>(p, stream);
+  if (p.ws8) return p.xs8 ? launch_types<kFp8, kFp8>(p, stream) : launch_types<kBf16, kFp8>(p, stream);
+  if (p.xs) return launch_types<kMxfp4, kMxfp4>(p, stream);
+  return p.ws ? launch_types<kBf16, kMxfp4>(p, stream) : launch_types<kBf16, kBf16>(p, stream);
 }
 
 }  // namespace expert

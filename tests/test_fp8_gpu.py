@@ -313,7 +313,7 @@ def tiles(act):
     return [(_lib.LF_EXPERT_TILE, r, c) for c in (64, 128, 192, 256) for r in (64, 128, 192, 256) if r <= most[c == 256]]
 
 
-PLANS = {act: STREAM + tiles(act) for act in ("bf16", "fp8")}
+PLANS = {act: STREAM + [(_lib.LF_EXPERT_ROWS, 0, 128)] + tiles(act) for act in ("bf16", "fp8")}
 BOTH = [(act, plan) for act in PLANS for plan in PLANS[act]]
 
 
