@@ -29,7 +29,7 @@ extern "C" {
  * 4: lf_row_expand_tiled added.
  * 5: the MXFP4 and expert entry points added.
  * 6: lf_fp8_quantize and lf_fp8_dequantize added, lf_expert_product gained
- * x_fp8_scales and w_fp8_scales (appended). */
+ * x_fp8_scales and w_fp8_scales (appended), lf_expert_mlp added. */
 #define LF_ABI_VERSION 6
 #define LF_OK 0
 #define LF_EINVAL 1
@@ -421,6 +421,44 @@ int lf_expert_linear_plan(const lf_expert_product* product, lf_expert_plan* plan
 int lf_combine_experts(const uint16_t* rows, int64_t num_rows, int64_t rows_stride, const int32_t* positions,
                        const float* weights, int64_t tokens, int32_t top, int64_t n, const uint16_t* base,
                        int64_t base_stride, uint16_t* y, int64_t y_stride, void* stream);
+
+/* The whole MLP of a few tokens over their experts in two launches:
+ * y[t] = base[t] + sum_j weight_tj down_e (silu(gate_e x[t]) * (up_e x[t])), choices and weights as lf_route_experts
+ * makes them. x bf16 [tokens, hidden], logits [tokens, experts] (fp32 != 0: fp32, else bf16), gate_up [experts,
+ * 2 inter, hidden] (gate rows, then up rows), down [experts, hidden, inter], both of `type`, with the scales of
+ * lf_expert_linear (MXFP4 bytes, 4-byte aligned; FP8 floats); base bf16 [tokens, hidden] or NULL (y may be base). Sums in
+ * fp32; weight_tj silu(gate) * up is rounded to bf16, y once.
+ * lf_expert_mlp_workspace_size: bytes (16-byte aligned, need not be cleared, not shared by calls that overlap), or -1 for
+ * sizes that the two kernels do not take: more than 32 tokens, 256 choices, 256 experts, top 16; hidden above 8192 (4096
+ * from 17 tokens on); widths that are no multiples of 8 (bf16), 16 (FP8; inter of 128), 128 (MXFP4). */
+#define LF_EXPERT_BF16 0
+#define LF_EXPERT_MXFP4 1
+#define LF_EXPERT_FP8 2
+typedef struct lf_expert_mlp_call {
+  const void* x;
+  int64_t x_stride; /* elements, as all strides */
+  const void* logits;
+  int64_t logits_stride;
+  int32_t fp32;
+  int32_t renormalize;
+  int64_t tokens;
+  int64_t hidden;
+  int64_t inter;
+  int32_t experts;
+  int32_t top;
+  int32_t type; /* of the weights */
+  const void* gate_up;
+  const void* gate_up_scales;
+  const void* down;
+  const void* down_scales;
+  const uint16_t* base;
+  int64_t base_stride;
+  uint16_t* y;
+  int64_t y_stride;
+} lf_expert_mlp_call;
+int64_t lf_expert_mlp_workspace_size(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter,
+                                     int32_t type);
+int lf_expert_mlp(const lf_expert_mlp_call* call, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

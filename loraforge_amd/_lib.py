@@ -112,6 +112,34 @@ class ExpertProduct(ctypes.Structure):
     ]
 
 
+LF_EXPERT_BF16, LF_EXPERT_MXFP4, LF_EXPERT_FP8 = range(3)
+
+
+class ExpertMlp(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("logits", c_void_p),
+        ("logits_stride", c_int64),
+        ("fp32", c_int32),
+        ("renormalize", c_int32),
+        ("tokens", c_int64),
+        ("hidden", c_int64),
+        ("inter", c_int64),
+        ("experts", c_int32),
+        ("top", c_int32),
+        ("type", c_int32),
+        ("gate_up", c_void_p),
+        ("gate_up_scales", c_void_p),
+        ("down", c_void_p),
+        ("down_scales", c_void_p),
+        ("base", c_void_p),
+        ("base_stride", c_int64),
+        ("y", c_void_p),
+        ("y_stride", c_int64),
+    ]
+
+
 _PROTOTYPES = {
     "lf_last_error": (ctypes.c_char_p, []),
     "lf_abi_version": (ctypes.c_int, []),
@@ -205,6 +233,8 @@ _PROTOTYPES = {
     ),
     "lf_expert_linear_plan": (ctypes.c_int, [ctypes.POINTER(ExpertProduct), ctypes.POINTER(ExpertPlan)]),
     "lf_expert_linear": (ctypes.c_int, [ctypes.POINTER(ExpertProduct), c_void_p]),
+    "lf_expert_mlp_workspace_size": (c_int64, [c_int64, c_int32, c_int32, c_int64, c_int64, c_int32]),
+    "lf_expert_mlp": (ctypes.c_int, [ctypes.POINTER(ExpertMlp), c_void_p, c_int64, c_void_p]),
     "lf_combine_experts": (
         ctypes.c_int,
         [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_int64,

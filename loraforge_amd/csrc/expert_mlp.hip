@@ -1,0 +1,603 @@
+// A whole mixture-of-experts MLP for a few tokens (a decode step), in two launches:
+// y[t] = base[t] + sum_j s_tj down_e (silu(gate_e x[t]) * (up_e x[t])), e the j-th choice of token t.
+//
+// Bound by HBM: every weight of a chosen expert is read once; beside it, launches, routing and
+// joins are latency. Four operators in a chain (route, product, product, combine) take
+// four launches for it.
+//
+// First launch. Every workgroup routes all tokens by itself (as expert_routing.hip does: the
+// logits come from L2, and nobody waits for another workgroup), x in registers meanwhile.
+// Then it takes items in turn: 8 columns of one chosen expert, 8 gate and 8 up rows over the whole of k.
+// Its eight waves share k (stage s of 128 bytes of a row to wave s % 8), each streaming its weights through a
+// ring of its own in LDS by direct copies; the ring runs on from one item to the next. The weight is
+// the A operand of 16 x 16 matrix instructions, *all* tokens are the B operand (of x, held
+// in registers: at most 128 of them, which is what bounds tokens and k): columns of tokens
+// that did not choose the expert are computed and dropped, which costs nothing beside the bytes.
+// The waves' sums meet in LDS, in a fixed order; the intermediate s silu(g) u is rounded to bf16
+// once, with the routing weight in it, so that the second product needs no weights.
+//
+// Second launch. With rows of the intermediate in expert order, y is one product whose k runs
+// over (chosen experts) x (intermediate): a workgroup owns 16 columns of y, its waves share that long
+// k, and their sums meet once at the end. Tokens are the columns of B again; a token that did not choose the
+// stage's expert reads zeros (past the end of a buffer).
+#include "expert_choose.h"
+#include "expert_params.h"
+#include "lds_pipeline.h"
+#include "../../include/loraforge_amd.h"
+
+namespace lf {
+namespace expert {
+namespace {
+
+constexpr int kWaves = 8;            // of the first launch
+constexpr int kThreads = 64 * kWaves;
+constexpr int kMostTokens = 32;      // a token is a bit of a mask, and a column of two tiles at most
+constexpr int kMostExperts = 256;
+constexpr int kMostTop = 16;
+constexpr int kMostChoices = 256;
+constexpr int kSlotWeights = 16 * 128;
+constexpr uint32_t kPast = 0x80000000u;  // past the end of every buffer here
+
+struct MlpParams {
+  const char* x;  // bf16 [tokens, hidden]
+  int64_t x_row;  // bytes
+  const void* logits;
+  int64_t logits_stride;
+  int32_t fp32, tokens, experts, top, renormalize;
+  int32_t hidden, inter;
+  const char *gate_up, *down;            // [experts, 2 inter, hidden], [experts, hidden, inter]
+  const uint8_t *gate_up_s, *down_s;     // MXFP4 scales
+  const float *gate_up_s8, *down_s8;     // FP8 scales
+  const uint16_t* base;                  // bf16 [tokens, hidden] or null
+  int64_t base_stride;
+  uint16_t* y;
+  int64_t y_stride;
+  uint16_t* h;   // [tokens * top, inter], rows in expert order
+  int4* table;   // x of entry 0: chosen experts; entry 1 + u: expert, first row, mask of its tokens
+};
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+template <int kType>
+struct Format {
+  static constexpr int kStage = kType == kBf16 ? 64 : kType == kFp8 ? 128 : 256;  // k of 128 bytes
+  static constexpr int kUnits = kStage / 32;        // 16-byte units of x that a lane holds of a stage
+  static constexpr int kCopies = kType == kMxfp4 ? 3 : 2;
+  static constexpr int kSlot = kSlotWeights + (kType == kMxfp4 ? 256 : 0);
+  static __host__ __device__ __forceinline__ int64_t row_bytes(int64_t k) { return kType == kBf16 ? 2 * k : kType == kFp8 ? k : k / 2; }
+};
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+
+// LDS accesses beside copies in flight, each block with its own wait (the compiler would wait for every copy).
+__device__ __forceinline__ void lds_two(u32x4 (&v)[2], uint32_t a, uint32_t b) {
+  asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v[0]), "=&v"(v[1]) : "v"(a), "v"(b) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_scales(uint32_t at) {
+  uint32_t v;
+  asm volatile("ds_read_u16 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void lds_write16(uint32_t at, const f32x4& v) {
+  // (Sums of a matrix instruction: the compiler does not wait for them before an asm block.)
+  asm volatile("s_nop 15\n\ts_nop 3\n\tds_write_b128 %0, %1" ::"v"(at), "v"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_word(uint32_t at) {
+  uint32_t v;
+  asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(at) : "memory");
+  return v;
+}
+// Words at `at`, at + 1024, ... (one for each of eight waves), summed in that order.
+__device__ __forceinline__ float lds_sum8(uint32_t at) {
+  float v[8];
+  asm volatile(
+      "ds_read_b32 %0, %8\n\t"
+      "ds_read_b32 %1, %8 offset:1024\n\t"
+      "ds_read_b32 %2, %8 offset:2048\n\t"
+      "ds_read_b32 %3, %8 offset:3072\n\t"
+      "ds_read_b32 %4, %8 offset:4096\n\t"
+      "ds_read_b32 %5, %8 offset:5120\n\t"
+      "ds_read_b32 %6, %8 offset:6144\n\t"
+      "ds_read_b32 %7, %8 offset:7168\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(at)
+      : "memory");
+  float sum = v[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) sum += v[i];
+  return sum;
+}
+
+// Copies of one stage of 16 weight rows: eight rows of 128 bytes each, unit u of row r at u ^ (r & 7), and of MXFP4
+// the eight scale bytes of each row (lanes 32 to 63 fetch nothing).
+template <int kType>
+struct Copier {
+  uint32_t at[2], unit, scale_at;  // the lane's offsets of the first and the second eight rows; its unit's byte in a stage
+  uint32_t row_bytes, blocks4;     // of a weight row: bytes, and words of scales
+
+  // Rows r and 8 + r of the 16 are `row0` + r and `row1` + r, in rows of `k`.
+  __device__ __forceinline__ Copier(int k, uint32_t row0, uint32_t row1) {
+    const int lane = threadIdx.x & 63, r8 = lane >> 3;
+    row_bytes = uint32_t(Format<kType>::row_bytes(k));
+    unit = uint32_t(((lane & 7) ^ r8) * 16);
+    at[0] = (row0 + r8) * row_bytes + unit;
+    at[1] = (row1 + r8) * row_bytes + unit;
+    blocks4 = uint32_t(k / mx::kBlock / 4);
+    const uint32_t r = lane >> 1;
+    scale_at = lane < 32 ? ((r < 8 ? row0 + r : row1 + r - 8) * blocks4 + (lane & 1)) * 4 : kPast;
+  }
+  // Stage `stage` (`live`: there is one) into `slot`. Past the end of a row the buffers give zeros.
+  __device__ __forceinline__ void copy(__amdgpu_buffer_rsrc_t w, __amdgpu_buffer_rsrc_t s, int stage, bool live, char* slot) const {
+    const uint32_t past = live && stage * 128 + unit < row_bytes ? 0u : kPast;
+    const uint32_t base = live ? stage * 128 : 0;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (LdsPtr)slot, 16, at[0] | past, base, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (LdsPtr)(slot + 1024), 16, at[1] | past, base, 0, 0);
+    if constexpr (kType == kMxfp4) {
+      const uint32_t gone = live && stage * 2 + (threadIdx.x & 1) < blocks4 ? 0u : kPast;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(s, (LdsPtr)(slot + kSlotWeights), 4, scale_at | gone, live ? stage * 8 : 0, 0, 0);
+    }
+  }
+};
+
+// One stage: 16 weight rows (in the slot) times kT tiles of 16 rows of x (units of a lane's quarter of the stage's k).
+// `scale`: FP8, of the lane's weight rows. kMasked: only the tokens of `mask` take part in the stage, so that what is not
+// finite in an expert's weights (NaN times zero is NaN) reaches no other token.
+template <int kType, int kT, bool kMasked>
+__device__ __forceinline__ void contract(uint32_t slot, const u32x4 (&x)[kT][Format<kType>::kUnits], float scale, uint32_t mask, f32x4 (&acc)[kT]) {
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  u32x4 w[2];
+  lds_two(w, slot + c * 128 + ((2 * q) ^ (c & 7)) * 16, slot + c * 128 + ((2 * q + 1) ^ (c & 7)) * 16);
+  constexpr bool kApart = kMasked || kType == kFp8;  // a stage's products from zero
+  f32x4 sum[kT];
+#pragma unroll
+  for (int t = 0; t < kT; ++t) sum[t] = kApart ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[t];
+  if constexpr (kType == kBf16) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int t = 0; t < kT; ++t) sum[t] = lf::mfma16(vec_bf16x8(w[j]), vec_bf16x8(x[t][j]), sum[t]);
+  } else if constexpr (kType == kFp8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bf16x8 a = vec_bf16x8(fp8::decode8(w[j >> 1][j % 2 * 2], w[j >> 1][j % 2 * 2 + 1]));
+#pragma unroll
+      for (int t = 0; t < kT; ++t) sum[t] = lf::mfma16(a, vec_bf16x8(x[t][j]), sum[t]);
+    }
+  } else {
+    const uint32_t scales = lds_scales(slot + kSlotWeights + c * 8 + 2 * q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float s = mx::scale_f32(j < 4 ? scales & 0xffu : scales >> 8);
+      const bf16x8 a = vec_bf16x8(mx::decode8(w[j >> 2][j & 3], s));
+#pragma unroll
+      for (int t = 0; t < kT; ++t) sum[t] = lf::mfma16(a, vec_bf16x8(x[t][j]), sum[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = kType == kFp8 ? fmaf(scale, sum[t][e], acc[t][e]) : kApart ? acc[t][e] + sum[t][e] : sum[t][e];
+      acc[t][e] = !kMasked || (mask >> (16 * t + c) & 1) ? v : acc[t][e];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Routing by one workgroup: chosen experts in order, with the masks of their tokens and their first rows
+// in expert order; weights by row.
+// ---------------------------------------------------------------------------
+struct Routing {
+  uint32_t mask[kMostExperts];   // by expert
+  int first[kMostExperts];
+  int wave_total[kMostExperts / 64];
+  int used;
+  int4 chosen[kMostChoices];     // expert, first row, mask
+  float weight[kMostChoices];
+};
+
+template <bool kFp32, int kPer>
+__device__ __forceinline__ Choice choose_token(const MlpParams& p, int t) {
+  return choose_experts<kFp32, 16, kPer>(p.logits, p.logits_stride, p.experts, p.top, p.renormalize, t, t < p.tokens);
+}
+
+__device__ __forceinline__ void route(const MlpParams& p, Routing& r) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int t = tid >> 4, j = tid & 15;
+  if (tid < kMostExperts) r.mask[tid] = 0;
+  Choice c{-1, 0.f};
+  if (wave * 4 < p.tokens) {  // (a wave as a whole: its lanes take maxima together)
+    if (p.fp32)
+      c = p.experts > 128 ? choose_token<true, 16>(p, t) : p.experts > 64 ? choose_token<true, 8>(p, t) : choose_token<true, 4>(p, t);
+    else
+      c = p.experts > 128 ? choose_token<false, 16>(p, t) : p.experts > 64 ? choose_token<false, 8>(p, t) : choose_token<false, 4>(p, t);
+  }
+  const bool live = t < p.tokens && j < p.top && c.expert >= 0;
+  __syncthreads();
+  if (live) atomicOr(&r.mask[c.expert], 1u << t);  // (a token chooses an expert once: no order shows)
+  __syncthreads();
+  // Places: counts of chosen experts and of choices before each, in one word.
+  uint32_t mask = 0;
+  int mine = 0, sum = 0;
+  if (tid < kMostExperts) {
+    mask = r.mask[tid];
+    mine = (mask != 0) << 16 | __popc(mask);
+    sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += up;
+    }
+    if (lane == 63) r.wave_total[wave] = sum;
+  }
+  __syncthreads();
+  if (tid < kMostExperts) {
+    int before = sum - mine;
+    for (int w = 0; w < wave; ++w) before += r.wave_total[w];
+    r.first[tid] = before & 0xffff;
+    if (mask) r.chosen[before >> 16] = make_int4(tid, before & 0xffff, int(mask), 0);
+    if (tid == kMostExperts - 1) r.used = (before + mine) >> 16;
+  }
+  __syncthreads();
+  if (live) r.weight[r.first[c.expert] + __popc(r.mask[c.expert] & ((1u << t) - 1))] = c.weight;
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------
+// First launch: routing, gate and up products, SwiGLU.
+// ---------------------------------------------------------------------------
+template <int kType, int kT, int kStages>
+struct GateUp {
+  using F = Format<kType>;
+  static constexpr bool kTwo = kT == 1 && kStages * F::kUnits <= 16;  // two workgroups on a CU: 64 registers of x
+  static constexpr int kRing = kTwo ? 3 : 5;                    // stages
+  static constexpr int kRed = 2 * kT * kWaves * 1024;
+  static constexpr int kLds = kWaves * kRing * F::kSlot + kRed;
+};
+
+template <int kType, int kT, int kStages>
+__global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2)) void gate_up_kernel(MlpParams p) {
+  using F = Format<kType>;
+  using G = GateUp<kType, kT, kStages>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ Routing routing;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, q = lane >> 4;
+  const int stages = int((F::row_bytes(p.hidden) + 127) / 128);
+  const int mine = stages > wave ? (stages - wave + kWaves - 1) / kWaves : 0;  // stages wave, wave + 8, ...
+
+  // x: unit n of a lane holds k 8 n .. of its quarter of the stage.
+  u32x4 x[kStages][kT][F::kUnits];
+#pragma unroll
+  for (int i = 0; i < kStages; ++i)
+#pragma unroll
+    for (int t = 0; t < kT; ++t)
+#pragma unroll
+      for (int n = 0; n < F::kUnits; ++n) {
+        const int token = 16 * t + c, k = (wave + kWaves * i) * F::kStage + q * (F::kStage / 4) + 8 * n;
+        x[i][t][n] = u32x4{0u, 0u, 0u, 0u};
+        if (token < p.tokens && k < p.hidden) x[i][t][n] = *reinterpret_cast<const u32x4*>(p.x + token * p.x_row + k * 2);
+      }
+
+  route(p, routing);
+  wait_vm<0>();  // (x; or the compiler would wait for it, and every copy, in the loop)
+  const int used = __builtin_amdgcn_readfirstlane(routing.used);
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) p.table[0] = make_int4(used, 0, 0, 0);
+    if (int(threadIdx.x) < used) p.table[1 + threadIdx.x] = routing.chosen[threadIdx.x];
+  }
+
+  // Items: eight columns of a chosen expert each.
+  const int groups = p.inter / 8, items = used * groups;
+  const int64_t row_bytes = F::row_bytes(p.hidden);
+  const uint32_t extent = uint32_t((p.inter + 8) * row_bytes);
+  const int blocks = int(fp8::blocks_of(p.hidden));
+  const Copier<kType> copier(p.hidden, 0, p.inter);
+  char* const ring = lds + wave * G::kRing * F::kSlot;
+  const uint32_t ring_at = lds_addr(ring), red_at = lds_addr(lds + kWaves * G::kRing * F::kSlot);
+  const uint32_t chosen_at = lds_addr(&routing.chosen[0]), weight_at = lds_addr(&routing.weight[0]);
+
+  // The stage that is copied next: of item `to`, the wave's stage number `step`.
+  int to = blockIdx.x, step = 0, in = 0;
+  __amdgpu_buffer_rsrc_t wbuf = buffer(p.gate_up, 0), sbuf = buffer(p.gate_up_s, 0);
+  auto aim = [&]() {  // buffers of item `to`
+    if (to >= items) return;
+    const int u = to / groups, column = (to - u * groups) * 8;
+    const int e = __builtin_amdgcn_readfirstlane(int(lds_word(chosen_at + u * 16)));
+    const int64_t row = int64_t(e) * 2 * p.inter + column;
+    wbuf = buffer(p.gate_up + row * row_bytes, extent);
+    if constexpr (kType == kMxfp4) sbuf = buffer(p.gate_up_s + row * (p.hidden / mx::kBlock), uint32_t(p.inter + 8) * (p.hidden / mx::kBlock));
+  };
+  auto copy_next = [&]() {
+    copier.copy(wbuf, sbuf, wave + kWaves * step, to < items, ring + in * F::kSlot);
+    in = in + 1 == G::kRing ? 0 : in + 1;
+    if (++step == mine) {
+      step = 0;
+      to += gridDim.x;
+      aim();
+    }
+  };
+  if (mine > 0) {
+    aim();
+    for (int n = 0; n < G::kRing - 1; ++n) copy_next();
+  }
+
+  int out = 0, turn = 0;
+  for (int item = blockIdx.x; item < items; item += gridDim.x, turn ^= 1) {
+    const int u = item / groups, column = (item - u * groups) * 8;
+    const float *gate_s = nullptr, *up_s = nullptr;
+    float gs = 0.f, us = 0.f;
+    if constexpr (kType == kFp8) {
+      const int e = __builtin_amdgcn_readfirstlane(int(lds_word(chosen_at + u * 16)));
+      const int64_t first = int64_t(e) * fp8::blocks_of(2 * p.inter);
+      gate_s = p.gate_up_s8 + (first + column / fp8::kBlock) * blocks;
+      up_s = p.gate_up_s8 + (first + (p.inter + column) / fp8::kBlock) * blocks;
+      gs = sload(gate_s, min(wave, blocks - 1)), us = sload(up_s, min(wave, blocks - 1));
+    }
+    f32x4 acc[kT];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      if (i < mine) {
+        wait_vm<(G::kRing - 2) * F::kCopies>();
+        copy_next();  // (into the slot whose reads are done)
+        float scale = 0.f;
+        if constexpr (kType == kFp8) {
+          scale = q >= 2 ? us : gs;
+          const int ahead = min(wave + kWaves * (i + 1), blocks - 1);
+          gs = sload(gate_s, ahead), us = sload(up_s, ahead);
+        }
+        contract<kType, kT, false>(ring_at + out * F::kSlot, x[i], scale, 0u, acc);
+        out = out + 1 == G::kRing ? 0 : out + 1;
+      }
+    }
+    // Sums as [turn][tile][wave][token][row]; two places in turn, so one barrier an item.
+    const uint32_t red = red_at + turn * (G::kRed / 2);
+#pragma unroll
+    for (int t = 0; t < kT; ++t) lds_write16(red + (t * kWaves + wave) * 1024 + c * 64 + q * 16, acc[t]);
+    lds_barrier();
+    if (threadIdx.x < 128 * kT) {
+      const int token = threadIdx.x >> 3, r = threadIdx.x & 7;
+      const uint32_t from = red + (token >> 4) * kWaves * 1024 + (token & 15) * 64 + r * 4;
+      const uint32_t mask = lds_word(chosen_at + u * 16 + 8);
+      if (mask >> token & 1) {
+        const int row = int(lds_word(chosen_at + u * 16 + 4)) + __popc(mask & ((1u << token) - 1));
+        const float g = lds_sum8(from), up = lds_sum8(from + 32);
+        p.h[int64_t(row) * p.inter + column + r] = uint16_t(f32_to_bf16(silu_mul_f32(g, up) * __uint_as_float(lds_word(weight_at + row * 4))));
+      }
+    }
+  }
+  wait_vm<0>();  // (copies past the last item are on their way into this workgroup's LDS)
+}
+
+// ---------------------------------------------------------------------------
+// Second launch: down products over all chosen experts at once.
+// ---------------------------------------------------------------------------
+constexpr int kDownRing = 4;
+
+template <int kType, int kT, int kW>
+constexpr int down_lds() {
+  return kW * kDownRing * Format<kType>::kSlot + kT * kW * 1024;
+}
+
+template <int kType, int kT, int kW>
+__global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
+  using F = Format<kType>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, q = lane >> 4;
+  const int column = blockIdx.x * 16;
+  const int64_t row_bytes = F::row_bytes(p.inter);
+  const int per = int((row_bytes + 127) / 128);  // stages of an expert
+  const int used = sload(reinterpret_cast<const int*>(p.table), 0), total = used * per;
+  const int blocks = int(fp8::blocks_of(p.inter));
+  const Copier<kType> copier(p.inter, 0, 8);
+  const uint32_t extent = uint32_t((p.hidden - column) * row_bytes);  // (rows past the last one: zeros)
+  char* const ring = lds + wave * kDownRing * F::kSlot;
+  const uint32_t ring_at = lds_addr(ring), red_at = lds_addr(lds + kW * kDownRing * F::kSlot);
+
+  // Stages wave, wave + kW, ... of the experts' one after another, each as (chosen expert, stage).
+  struct At {
+    int n, u, s;
+  };
+  const int jump_u = kW / per, jump_s = kW % per;
+  auto next = [&](At& a) {
+    a.n += kW;
+    a.u += jump_u;
+    a.s += jump_s;
+    if (a.s >= per) a.s -= per, ++a.u;
+  };
+  // (Past the last one the last one again: their copies and rows of x are zeros.)
+  auto entry = [&](int u) { return sload(reinterpret_cast<const i32x4*>(p.table), 1 + min(u, used - 1)); };
+  At to{wave, wave / per, wave % per}, x_at = to, at = to;
+  int in = 0, out = 0;
+  auto copy_next = [&]() {
+    const int64_t row = int64_t(entry(to.u)[0]) * p.hidden + column;
+    const auto wbuf = buffer(p.down + row * row_bytes, extent);
+    auto sbuf = wbuf;
+    if constexpr (kType == kMxfp4) sbuf = buffer(p.down_s + row * (p.inter / mx::kBlock), uint32_t(p.hidden - column) * (p.inter / mx::kBlock));
+    copier.copy(wbuf, sbuf, to.s, to.n < total, ring + in * F::kSlot);
+    in = in + 1 == kDownRing ? 0 : in + 1;
+    next(to);
+  };
+  const auto hbuf = buffer(p.h, uint32_t(p.tokens) * p.top * p.inter * 2);
+  auto load_x = [&](u32x4 (&x)[kT][F::kUnits]) {  // returns the mask of the stage's tokens
+    const i32x4 chosen = entry(x_at.u);
+    const uint32_t mask = x_at.n < total ? uint32_t(chosen[2]) : 0u;
+    const int k0 = x_at.s * F::kStage + q * (F::kStage / 4);
+    const bool whole = (x_at.s + 1) * F::kStage <= p.inter;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const int token = 16 * t + c;
+      const uint32_t row = uint32_t(chosen[1] + __popc(mask & ((1u << token) - 1))) * uint32_t(p.inter) + k0;
+      const uint32_t from = mask >> token & 1 ? row * 2 : kPast;
+#pragma unroll
+      for (int n = 0; n < F::kUnits; ++n)
+        x[t][n] = __builtin_amdgcn_raw_buffer_load_b128(hbuf, whole || k0 + 8 * n < p.inter ? from + 16 * n : kPast, 0, 0);
+    }
+    next(x_at);
+    return mask;
+  };
+  f32x4 acc[kT];
+#pragma unroll
+  for (int t = 0; t < kT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto step = [&](const u32x4 (&x)[kT][F::kUnits], uint32_t mask, u32x4 (&ahead)[kT][F::kUnits]) {
+    // Behind the copies of this stage went those of kDownRing - 2 more, and as many stages of x.
+    wait_vm<(kDownRing - 2) * (F::kCopies + kT * F::kUnits)>();
+    const uint32_t mask_ahead = load_x(ahead);
+    asm volatile("" ::: "memory");
+    copy_next();
+    float scale = 0.f;
+    if constexpr (kType == kFp8) {
+      const int64_t block = int64_t(entry(at.u)[0]) * fp8::blocks_of(p.hidden) + column / fp8::kBlock;
+      scale = sload(p.down_s8 + block * blocks, at.s);
+    }
+    contract<kType, kT, true>(ring_at + out * F::kSlot, x, scale, mask, acc);
+    out = out + 1 == kDownRing ? 0 : out + 1;
+    next(at);
+    return mask_ahead;
+  };
+  u32x4 x0[kT][F::kUnits], x1[kT][F::kUnits];
+  if (wave < total) {
+    // (x behind all copies but the last, as in every step: what the compiler waits for before x is the same then.)
+    for (int n = 0; n < kDownRing - 2; ++n) copy_next();
+    asm volatile("" ::: "memory");
+    uint32_t mask = load_x(x0);
+    asm volatile("" ::: "memory");
+    copy_next();
+    wait_vm<(kDownRing - 2) * F::kCopies + kT * F::kUnits>();  // (the first stage; the second has two of x behind it)
+    while (at.n < total) {
+      mask = step(x0, mask, x1);
+      if (at.n >= total) break;
+      mask = step(x1, mask, x0);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kT; ++t) lds_write16(red_at + (t * kW + wave) * 1024 + c * 64 + q * 16, acc[t]);
+  wait_vm<0>();
+  lds_barrier();
+  for (int i = threadIdx.x; i < 256 * kT; i += 64 * kW) {
+    const int token = i >> 4, n = column + (i & 15);
+    if (token >= p.tokens || n >= p.hidden) continue;
+    const uint32_t from = red_at + (token >> 4) * kW * 1024 + (token & 15) * 64 + (i & 15) * 4;
+    float sum = lds_sum8(from);
+    if constexpr (kW == 16) sum += lds_sum8(from + 8 * 1024);
+    if (p.base) sum += bf16_to_f32(p.base[token * p.base_stride + n]);
+    p.y[token * p.y_stride + n] = uint16_t(f32_to_bf16(sum));
+  }
+}
+
+// ---------------------------------------------------------------------------
+
+template <class K>
+int launch(K kernel, unsigned grid, unsigned threads, unsigned lds, const MlpParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, stream, p);
+  LF_HIP(hipGetLastError());
+  return kOk;
+}
+
+template <int kType, int kT, int kStages>
+int launch_gate_up(const MlpParams& p, hipStream_t stream) {
+  using G = GateUp<kType, kT, kStages>;
+  return launch(gate_up_kernel<kType, kT, kStages>, G::kTwo ? 512 : 256, kThreads, G::kLds, p, stream);
+}
+
+// Registers of x: 32, 64 or (one workgroup a CU) all of 128.
+template <int kType, int kT>
+int launch_gate_up(const MlpParams& p, hipStream_t stream) {
+  const int per_wave = int(((Format<kType>::row_bytes(p.hidden) + 127) / 128 + kWaves - 1) / kWaves);
+  constexpr int kAll = 32 / (kT * Format<kType>::kUnits);
+  if constexpr (kAll >= 8)
+    if (per_wave <= kAll / 4) return launch_gate_up<kType, kT, kAll / 4>(p, stream);
+  if (per_wave <= kAll / 2) return launch_gate_up<kType, kT, kAll / 2>(p, stream);
+  return launch_gate_up<kType, kT, kAll>(p, stream);
+}
+
+template <int kType, int kT>
+int launch_both(const MlpParams& p, hipStream_t stream) {
+  if (const int rc = launch_gate_up<kType, kT>(p, stream)) return rc;
+  const unsigned grid = unsigned((p.hidden + 15) / 16);
+  // Few workgroups get twice the waves (MXFP4 and two tiles of tokens: more registers than such waves have).
+  if constexpr (kType != kMxfp4 || kT == 1)
+    if (grid <= 160) return launch(down_kernel<kType, kT, 16>, grid, 1024, down_lds<kType, kT, 16>(), p, stream);
+  return launch(down_kernel<kType, kT, 8>, grid, 512, down_lds<kType, kT, 8>(), p, stream);
+}
+
+template <int kType>
+int launch_type(const MlpParams& p, hipStream_t stream) {
+  return p.tokens <= 16 ? launch_both<kType, 1>(p, stream) : launch_both<kType, 2>(p, stream);
+}
+
+int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace expert
+}  // namespace lf
+
+// Bytes of workspace, or -1 where the two kernels cannot take the sizes.
+extern "C" int64_t lf_expert_mlp_workspace_size(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
+  using namespace lf::expert;
+  if (tokens < 1 || tokens > kMostTokens || experts < 1 || experts > kMostExperts || top < 1 || top > kMostTop || top > experts ||
+      tokens * top > kMostChoices || type < LF_EXPERT_BF16 || type > LF_EXPERT_FP8)
+    return -1;
+  const int64_t unit = type == LF_EXPERT_BF16 ? 8 : type == LF_EXPERT_FP8 ? 16 : 128;
+  if (hidden < 1 || inter < 1 || hidden % unit || inter % unit || (type == LF_EXPERT_FP8 && inter % lf::fp8::kBlock)) return -1;
+  // x of a wave's stages in 128 registers; an expert's weights within 31 bits.
+  if (hidden > (tokens <= 16 ? 8192 : 4096) || inter > (int64_t(1) << 20) || (hidden + 16) * (inter + 16) * 2 >= (int64_t(1) << 31))
+    return -1;
+  return padded16(tokens * top * inter * 2) + 16 * (1 + kMostChoices);
+}
+
+extern "C" int lf_expert_mlp(const lf_expert_mlp_call* a, void* workspace, int64_t workspace_bytes, void* stream) {
+  LF_REQUIRE(a != nullptr, "null pointer argument");
+  const int64_t need = lf_expert_mlp_workspace_size(a->tokens, a->experts, a->top, a->hidden, a->inter, a->type);
+  LF_REQUIRE(need >= 0, "an expert MLP of these sizes has to run as routing, products and sum");
+  LF_REQUIRE(workspace != nullptr && workspace_bytes >= need, "workspace of %lld bytes required", static_cast<long long>(need));
+  LF_REQUIRE(lf::aligned16(workspace), "the workspace must be 16-byte aligned");
+  LF_REQUIRE(a->x && a->logits && a->gate_up && a->down && a->y, "null pointer argument");
+  LF_REQUIRE((a->type == LF_EXPERT_BF16) == (a->gate_up_scales == nullptr) && (a->gate_up_scales == nullptr) == (a->down_scales == nullptr),
+             "MXFP4 and FP8 weights need scales, bf16 weights have none");
+  LF_REQUIRE(lf::aligned16(a->x) && a->x_stride % 8 == 0 && a->x_stride >= a->hidden, "x rows must be 16-byte aligned");
+  LF_REQUIRE(lf::aligned16(a->gate_up) && lf::aligned16(a->down), "weights must be 16-byte aligned");
+  LF_REQUIRE(reinterpret_cast<uintptr_t>(a->gate_up_scales) % 4 == 0 && reinterpret_cast<uintptr_t>(a->down_scales) % 4 == 0,
+             "scales must be 4-byte aligned");
+  LF_REQUIRE(a->logits_stride >= a->experts, "the row stride must cover the experts");
+  LF_REQUIRE(a->y_stride >= a->hidden && (!a->base || a->base_stride >= a->hidden), "row strides must cover the columns");
+  lf::expert::MlpParams p{};
+  p.x = static_cast<const char*>(a->x);
+  p.x_row = a->x_stride * 2;
+  p.logits = a->logits;
+  p.logits_stride = a->logits_stride;
+  p.fp32 = a->fp32 ? 1 : 0;
+  p.tokens = int32_t(a->tokens);
+  p.experts = a->experts;
+  p.top = a->top;
+  p.renormalize = a->renormalize ? 1 : 0;
+  p.hidden = int32_t(a->hidden);
+  p.inter = int32_t(a->inter);
+  p.gate_up = static_cast<const char*>(a->gate_up);
+  p.down = static_cast<const char*>(a->down);
+  if (a->type == LF_EXPERT_FP8) {
+    p.gate_up_s8 = static_cast<const float*>(a->gate_up_scales);
+    p.down_s8 = static_cast<const float*>(a->down_scales);
+  } else {
+    p.gate_up_s = static_cast<const uint8_t*>(a->gate_up_scales);
+    p.down_s = static_cast<const uint8_t*>(a->down_scales);
+  }
+  p.base = a->base;
+  p.base_stride = a->base_stride;
+  p.y = a->y;
+  p.y_stride = a->y_stride;
+  p.h = static_cast<uint16_t*>(workspace);
+  p.table = reinterpret_cast<int4*>(static_cast<char*>(workspace) + lf::expert::padded16(a->tokens * a->top * a->inter * 2));
+  auto s = static_cast<hipStream_t>(stream);
+  switch (a->type) {
+    case LF_EXPERT_BF16: return lf::expert::launch_type<lf::expert::kBf16>(p, s);
+    case LF_EXPERT_MXFP4: return lf::expert::launch_type<lf::expert::kMxfp4>(p, s);
+    default: return lf::expert::launch_type<lf::expert::kFp8>(p, s);
+  }
+}

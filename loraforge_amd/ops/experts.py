@@ -14,6 +14,7 @@ FP8 ``[E, N, K]``. The operators are for inference: tensors that require gradien
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 from .. import _lib
@@ -224,12 +225,50 @@ def expert_mlp(x, logits, gate_up, down, top_k: int, *, renormalize: bool = True
         raise ValueError("out must be [tokens, columns]")
     same = base is not None and out.data_ptr() == base.data_ptr() and out.stride() == base.stride()
     distinct_output(out, (x, logits, *_parts(gate_up), *_parts(down), None if same else base))
-    r = route_experts(logits, top_k, renormalize=renormalize)
+    if type(top_k) is not int or not 1 <= top_k <= min(experts, MAX_TOP):
+        raise ValueError(f"top_k must be in 1..min(experts, {MAX_TOP})")
+    if logits.numel() and (logits.stride(1) != 1 or (count > 1 and logits.stride(0) < experts)):
+        raise ValueError("logits must have unit column stride and rows apart")
+    for t, name in ((base, "base"), (out, "out")):
+        if t is not None and t.numel() and (t.stride(1) != 1 or (count > 1 and t.stride(0) < hidden)):
+            raise ValueError(f"{name} must have unit column stride and rows apart")
+    require_arch(x.device)
     if count == 0:
         return out
+    if type(gate_up) is type(down) and _expert_mlp(x, logits, gate_up, down, top_k, renormalize, base, out):
+        return out
+    r = route_experts(logits, top_k, renormalize=renormalize)
     h = expert_linear(x, gate_up, r.offsets, tokens=r.tokens, swiglu=True)
     rows = expert_linear(h, down, r.offsets)
     return combine_experts(rows, r.positions, r.weights, base=base, out=out)
+
+
+def _expert_mlp(x, logits, gate_up, down, top_k, renormalize, base, out) -> bool:
+    """The MLP of a few tokens in two launches; False where those do not take it."""
+    import torch
+
+    (count, hidden), (experts, _, inter) = x.shape, down.shape
+    kind = (_lib.LF_EXPERT_MXFP4 if isinstance(down, MXFP4Tensor) else _lib.LF_EXPERT_FP8 if isinstance(down, FP8Tensor)
+            else _lib.LF_EXPERT_BF16)
+    lib = _lib.library()
+    size = lib.lf_expert_mlp_workspace_size(count, experts, top_k, hidden, inter, kind)
+    parts = _parts(gate_up), _parts(down)
+    if size < 0 or any(t.data_ptr() % 4 for part in parts for t in part[1:]):
+        return False
+    a = _lib.ExpertMlp()
+    a.x, a.logits, a.y = x.data_ptr(), logits.data_ptr(), out.data_ptr()
+    a.x_stride, a.logits_stride, a.y_stride = (t.stride(0) if count > 1 else t.shape[1] for t in (x, logits, out))
+    a.fp32, a.renormalize, a.type = logits.dtype == torch.float32, renormalize, kind
+    a.tokens, a.hidden, a.inter, a.experts, a.top = count, hidden, inter, experts, top_k
+    a.gate_up, a.down = parts[0][0].data_ptr(), parts[1][0].data_ptr()
+    if kind != _lib.LF_EXPERT_BF16:
+        a.gate_up_scales, a.down_scales = parts[0][1].data_ptr(), parts[1][1].data_ptr()
+    if base is not None:
+        a.base, a.base_stride = base.data_ptr(), base.stride(0) if count > 1 else hidden
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(lib.lf_expert_mlp(ctypes.byref(a), scratch.data_ptr(), size, _lib.stream_of(x.device)))
+    return True
 
 
 def _parts(w):
