@@ -49,25 +49,35 @@ struct Choice {
   float weight;
 };
 
-// The choices of the token of these kLanes lanes (row t of `logits`, rows `stride` apart; not `live`: no token,
-// but there is a first row); lane l
-// of them holds experts l, l + kLanes, ... and at the end choice l.
-// k rounds of a maximum over keys in the order of the logits. A bf16 key leaves 16 bits
-// for the expert (lowest first), so one maximum finds both; fp32 takes a second one.
-template <bool kFp32, int kLanes, int kPer>
-__device__ __forceinline__ Choice choose_experts(const void* logits, int64_t stride, int experts, int top, bool renormalize, int t, bool live) {
+// A token's logits (row t of `logits`, rows `stride` apart) in the kLanes lanes that share it: lane l holds
+// experts l, l + kLanes, ...; -inf past the last, and everywhere if not `live` (there is a first row all the same:
+// addresses are clamped instead of loads skipped, as the compiler waits for a load behind each condition).
+template <int kLanes, int kPer>
+__device__ __forceinline__ void load_logits(const void* logits, bool fp32, int64_t stride, int experts, int t, bool live, float (&value)[kPer]) {
   const int lane = threadIdx.x & (kLanes - 1);
-  uint32_t key[kPer];
-  float value[kPer];
-  // (Addresses clamped instead of loads skipped: the compiler waits for a load behind each condition.)
+  const int64_t row = int64_t(live ? t : 0) * stride;
+  if (fp32) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t at = int64_t(live ? t : 0) * stride + min(lane + i * kLanes, experts - 1);
-    value[i] = kFp32 ? static_cast<const float*>(logits)[at] : bf16_to_f32(static_cast<const uint16_t*>(logits)[at]);
+    for (int i = 0; i < kPer; ++i) value[i] = static_cast<const float*>(logits)[row + min(lane + i * kLanes, experts - 1)];
+  } else {
+    uint16_t bits[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) bits[i] = static_cast<const uint16_t*>(logits)[row + min(lane + i * kLanes, experts - 1)];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) value[i] = bf16_to_f32(bits[i]);
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
     if (!live || lane + i * kLanes >= experts) value[i] = -__builtin_huge_valf();
+}
+
+// The choices of the token whose logits these kLanes lanes hold; lane l gets choice l.
+// k rounds of a maximum over keys in the order of the logits. The key of a logit that is a bf16 (kFp32 false) leaves
+// 16 bits for the expert (lowest first), so one maximum finds both; fp32 takes a second one.
+template <bool kFp32, int kLanes, int kPer>
+__device__ __forceinline__ Choice choose_experts(const float (&value)[kPer], int top, bool renormalize) {
+  const int lane = threadIdx.x & (kLanes - 1);
+  uint32_t key[kPer];
   bool odd = false;  // NaN or +inf
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {

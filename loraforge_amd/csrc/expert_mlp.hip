@@ -20,6 +20,8 @@
 // over (chosen experts) x (intermediate): a workgroup owns 16 columns of y, its waves share that long
 // k, and their sums meet once at the end. Tokens are the columns of B again; a token that did not choose the
 // stage's expert reads zeros (past the end of a buffer).
+#include <type_traits>
+
 #include "expert_choose.h"
 #include "expert_params.h"
 #include "lds_pipeline.h"
@@ -32,6 +34,7 @@ namespace {
 constexpr int kWaves = 8;            // of the first launch
 constexpr int kThreads = 64 * kWaves;
 constexpr int kMostTokens = 32;      // a token is a bit of a mask, and a column of two tiles at most
+constexpr int kFewTokens = 2;        // routed by ranks
 constexpr int kMostExperts = 256;
 constexpr int kMostTop = 16;
 constexpr int kMostChoices = 256;
@@ -70,6 +73,30 @@ struct Format {
 typedef __attribute__((address_space(3))) void* LdsPtr;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+
+// Exchanges units between the quarters of a wave: of kUnits loads, load n of lane quarter q becomes unit 4 (n % (kUnits / 4)) + q of
+// quarter n / (kUnits / 4).
+template <int kUnits>
+__device__ __forceinline__ void transpose_quarters(u32x4 (&v)[kUnits]) {
+  constexpr int kPer = kUnits / 4;  // loads of a quarter
+  u32x4 to[kUnits];
+#pragma unroll
+  for (int h = 0; h < kPer; ++h)
+#pragma unroll
+    for (int word = 0; word < 4; ++word) {
+      // Rows n = kPer q + h, q = 0 .. 3: a 4 x 4 transpose, first within pairs of quarters, then between pairs.
+      const auto ab = __builtin_amdgcn_permlane16_swap(v[h][word], v[kPer + h][word], false, false);
+      const auto cd = __builtin_amdgcn_permlane16_swap(v[2 * kPer + h][word], v[3 * kPer + h][word], false, false);
+      const auto ac = __builtin_amdgcn_permlane32_swap(ab[0], cd[0], false, false);
+      const auto bd = __builtin_amdgcn_permlane32_swap(ab[1], cd[1], false, false);
+      to[4 * h][word] = ac[0];
+      to[4 * h + 1][word] = bd[0];
+      to[4 * h + 2][word] = ac[1];
+      to[4 * h + 3][word] = bd[1];
+    }
+#pragma unroll
+  for (int n = 0; n < kUnits; ++n) v[n] = to[n];
 }
 
 // LDS accesses beside copies in flight, each block with its own wait (the compiler would wait for every copy).
@@ -193,57 +220,158 @@ __device__ __forceinline__ void contract(uint32_t slot, const u32x4 (&x)[kT][For
 struct Routing {
   uint32_t mask[kMostExperts];   // by expert
   int first[kMostExperts];
-  int wave_total[kMostExperts / 64];
+  uint32_t rank[kFewTokens * 64];  // of a few tokens: a byte each for a lane's experts
   int used;
   int4 chosen[kMostChoices];     // expert, first row, mask
   float weight[kMostChoices];
 };
 
-template <bool kFp32, int kPer>
-__device__ __forceinline__ Choice choose_token(const MlpParams& p, int t) {
-  return choose_experts<kFp32, 16, kPer>(p.logits, p.logits_stride, p.experts, p.top, p.renormalize, t, t < p.tokens);
+// Inclusive sums over the lanes of a wave: within rows of 16 lanes, then the rows' totals.
+__device__ __forceinline__ int scan_lanes(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
+  return v;
+}
+
+// The tables, from masks that a barrier has passed. Each wave writes them for itself (all the same), so that it needs
+// no barrier to read what it wrote.
+__device__ __forceinline__ void tabulate(Routing& r) {
+  const int lane = threadIdx.x & 63;
+  // Places: counts of chosen experts and of choices before each of the lane's four experts, in one word.
+  constexpr int kPer = kMostExperts / 64;
+  uint32_t mask[kPer];
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    mask[i] = r.mask[kPer * lane + i];
+    mine += (mask[i] != 0) << 16 | __popc(mask[i]);
+  }
+  const int sum = scan_lanes(mine);
+  r.used = __builtin_amdgcn_readlane(sum, 63) >> 16;
+  int before = sum - mine;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    r.first[kPer * lane + i] = before & 0xffff;
+    if (mask[i]) r.chosen[before >> 16] = make_int4(kPer * lane + i, before & 0xffff, int(mask[i]), 0);
+    before += (mask[i] != 0) << 16 | __popc(mask[i]);
+  }
+}
+
+// (Weights are read behind the barrier of an item's sums.)
+__device__ __forceinline__ void keep_weight(Routing& r, int t, int e, float weight) {
+  r.weight[r.first[e] + __popc(r.mask[e] & ((1u << t) - 1))] = weight;
+}
+
+// One or two tokens: the rank of every expert of a token by counting those before it, as many waves a token
+// as there are, each against a part of the experts. (Rounds of maxima, as for more tokens, are a chain of a few
+// hundred clocks each, but as long for 16 tokens as for one: routing takes 6200 clocks here, of 4 tokens it took
+// 13500, in rounds 8200.)
+template <int kPer>
+__device__ __forceinline__ void route_few(const MlpParams& p, Routing& r) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int share = p.tokens == 1 ? kWaves : kWaves / kFewTokens;  // waves of a token
+  const int t = wave / share, part = wave & (share - 1);
+  const bool live = t < p.tokens;  // (always: each of one or two tokens has its waves)
+  float value[kPer];
+  load_logits<64>(p.logits, p.fp32, p.logits_stride, p.experts, t, live, value);
+  if (threadIdx.x < kMostExperts) r.mask[threadIdx.x] = 0;
+  if (threadIdx.x < kFewTokens * 64) r.rank[threadIdx.x] = 0;
+  uint32_t key[kPer];
+  int rank[kPer];
+  bool odd = false;  // NaN or +inf
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    key[i] = order_key(value[i]);
+    rank[i] = 0;
+    odd |= !(value[i] < __builtin_huge_valf());
+  }
+  const bool bad = __ballot(odd) != 0;
+  const int lanes = 64 / share;
+  for (int l0 = part * lanes; l0 < (part + 1) * lanes; l0 += 2) {
+#pragma unroll
+    for (int l1 = 0; l1 < 2; ++l1)
+#pragma unroll
+      for (int n = 0; n < kPer; ++n) {  // expert l + 64 n against the lane's
+        const int l = l0 + l1;
+        const uint32_t other = uint32_t(__builtin_amdgcn_readlane(int(key[n]), l));
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          rank[i] += n < i ? other >= key[i] : n > i ? other > key[i] : other > key[i] || (other == key[i] && l < lane);
+      }
+  }
+  wait_vm<0>();  // (x has come too)
+  __syncthreads();
+  // (Whole numbers below 256: no order shows, and no byte reaches the next.)
+  uint32_t packed = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) packed |= uint32_t(rank[i]) << (8 * i);
+  atomicAdd(&r.rank[t * 64 + lane], packed);
+  __syncthreads();
+  packed = r.rank[t * 64 + lane];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) rank[i] = int(packed >> (8 * i) & 0xffu);
+  bool mine[kPer];
+  float weight[kPer];
+  if (live && part == 0) {
+    float peak = 0.f, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      mine[i] = rank[i] < p.top && key[i] != 0;
+      const uint64_t first = __ballot(rank[i] == 0);
+      if (first) peak = __uint_as_float(uint32_t(__builtin_amdgcn_readlane(int(__float_as_uint(key_value(key[i]))), __builtin_ctzll(first))));
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      weight[i] = key[i] != 0 ? expf(key_value(key[i]) - peak) : 0.0f;
+      total += mine[i] || !p.renormalize ? weight[i] : 0.0f;
+    }
+    total = sum_across<64>(total);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      weight[i] = bad ? __builtin_nanf("") : weight[i] / total;
+      if (mine[i]) atomicOr(&r.mask[lane + 64 * i], 1u << t);  // (a token chooses an expert once: no order shows)
+    }
+  }
+  __syncthreads();
+  tabulate(r);
+  if (live && part == 0) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (mine[i]) keep_weight(r, t, lane + 64 * i, weight[i]);
+  }
+}
+
+// More tokens: 16 lanes each.
+template <int kPer>
+__device__ __forceinline__ void route_many(const MlpParams& p, Routing& r) {
+  const int t = threadIdx.x >> 4, j = threadIdx.x & 15;
+  if (threadIdx.x < kMostExperts) r.mask[threadIdx.x] = 0;
+  float value[kPer];
+  load_logits<16>(p.logits, p.fp32, p.logits_stride, p.experts, t, t < p.tokens, value);
+  Choice c{-1, 0.f};
+  // (A wave as a whole: its lanes take maxima together.)
+  if (int(threadIdx.x & ~63u) / 16 < p.tokens) c = choose_experts<true, 16>(value, p.top, p.renormalize);
+  const bool live = t < p.tokens && j < p.top && c.expert >= 0;
+  wait_vm<0>();  // (x has come too, if it was asked for)
+  __syncthreads();
+  if (live) atomicOr(&r.mask[c.expert], 1u << t);
+  __syncthreads();
+  tabulate(r);
+  if (live) keep_weight(r, t, c.expert, c.weight);
 }
 
 __device__ __forceinline__ void route(const MlpParams& p, Routing& r) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int t = tid >> 4, j = tid & 15;
-  if (tid < kMostExperts) r.mask[tid] = 0;
-  Choice c{-1, 0.f};
-  if (wave * 4 < p.tokens) {  // (a wave as a whole: its lanes take maxima together)
-    if (p.fp32)
-      c = p.experts > 128 ? choose_token<true, 16>(p, t) : p.experts > 64 ? choose_token<true, 8>(p, t) : choose_token<true, 4>(p, t);
-    else
-      c = p.experts > 128 ? choose_token<false, 16>(p, t) : p.experts > 64 ? choose_token<false, 8>(p, t) : choose_token<false, 4>(p, t);
+  if (p.tokens <= kFewTokens) {
+    if (p.experts <= 128) route_few<2>(p, r);
+    else route_few<4>(p, r);
+  } else {
+    if (p.experts <= 128) route_many<8>(p, r);
+    else route_many<16>(p, r);
   }
-  const bool live = t < p.tokens && j < p.top && c.expert >= 0;
-  __syncthreads();
-  if (live) atomicOr(&r.mask[c.expert], 1u << t);  // (a token chooses an expert once: no order shows)
-  __syncthreads();
-  // Places: counts of chosen experts and of choices before each, in one word.
-  uint32_t mask = 0;
-  int mine = 0, sum = 0;
-  if (tid < kMostExperts) {
-    mask = r.mask[tid];
-    mine = (mask != 0) << 16 | __popc(mask);
-    sum = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += up;
-    }
-    if (lane == 63) r.wave_total[wave] = sum;
-  }
-  __syncthreads();
-  if (tid < kMostExperts) {
-    int before = sum - mine;
-    for (int w = 0; w < wave; ++w) before += r.wave_total[w];
-    r.first[tid] = before & 0xffff;
-    if (mask) r.chosen[before >> 16] = make_int4(tid, before & 0xffff, int(mask), 0);
-    if (tid == kMostExperts - 1) r.used = (before + mine) >> 16;
-  }
-  __syncthreads();
-  if (live) r.weight[r.first[c.expert] + __popc(r.mask[c.expert] & ((1u << t) - 1))] = c.weight;
-  __syncthreads();
 }
 
 // ---------------------------------------------------------------------------
@@ -271,19 +399,32 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
 
   // x: unit n of a lane holds k 8 n .. of its quarter of the stage.
   u32x4 x[kStages][kT][F::kUnits];
-#pragma unroll
-  for (int i = 0; i < kStages; ++i)
-#pragma unroll
-    for (int t = 0; t < kT; ++t)
-#pragma unroll
-      for (int n = 0; n < F::kUnits; ++n) {
-        const int token = 16 * t + c, k = (wave + kWaves * i) * F::kStage + q * (F::kStage / 4) + 8 * n;
-        x[i][t][n] = u32x4{0u, 0u, 0u, 0u};
-        if (token < p.tokens && k < p.hidden) x[i][t][n] = *reinterpret_cast<const u32x4*>(p.x + token * p.x_row + k * 2);
+  const auto xbuf = buffer(p.x, uint32_t((p.tokens - 1) * p.x_row + p.hidden * 2));
+  // A few rows go through LDS (where the weights come later) while the tokens are routed: KiB by KiB, unit u of row t at
+  // u ^ t. (A load of 16 rows takes the address unit as long for one row as for 16.)
+  const int pieces = (p.hidden * 2 + 1023) / 1024, pitch = pieces * 1024;
+  const bool through_lds = kT == 1 && p.tokens <= kWaves && p.tokens * pitch <= G::kLds;
+  if (through_lds)
+    for (int t = 0; t < p.tokens; ++t)
+      for (int piece = wave; piece < pieces; piece += kWaves) {
+        const int at = piece * 1024 + (lane ^ t) * 16;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (LdsPtr)(lds + t * pitch + piece * 1024), 16,
+                                                 at < p.hidden * 2 ? uint32_t(t * p.x_row) + at : kPast, 0, 0, 0);
       }
-
   route(p, routing);
-  wait_vm<0>();  // (x; or the compiler would wait for it, and every copy, in the loop)
+  if (through_lds) {  // (tokens past the last one: its row again, in columns that nobody stores)
+    const int t = min(c, p.tokens - 1);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i)
+      if (i < mine)
+#pragma unroll
+        for (int n = 0; n < F::kUnits; ++n) {
+          const int unit = ((wave + kWaves * i) * F::kStage + q * (F::kStage / 4)) / 8 + n;
+          x[i][0][n] = *reinterpret_cast<const u32x4*>(lds + t * pitch + (unit ^ t) * 16);
+        }
+    lds_barrier();
+  }
+
   const int used = __builtin_amdgcn_readfirstlane(routing.used);
   if (blockIdx.x == 0) {
     if (threadIdx.x == 0) p.table[0] = make_int4(used, 0, 0, 0);
@@ -300,23 +441,36 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
   const uint32_t ring_at = lds_addr(ring), red_at = lds_addr(lds + kWaves * G::kRing * F::kSlot);
   const uint32_t chosen_at = lds_addr(&routing.chosen[0]), weight_at = lds_addr(&routing.weight[0]);
 
+  // Items blockIdx.x, + gridDim.x, ... as (chosen expert, group of columns).
+  struct At {
+    int item, u, group;
+  };
+  const int jump_u = gridDim.x / groups, jump_group = gridDim.x - jump_u * groups;
+  auto next = [&](At& a) __attribute__((always_inline)) {
+    a.item += gridDim.x;
+    a.u += jump_u;
+    a.group += jump_group;
+    if (a.group >= groups) a.group -= groups, ++a.u;
+  };
+  At to{int(blockIdx.x), int(blockIdx.x) / groups, 0};
+  to.group = to.item - to.u * groups;
+  At at = to;
   // The stage that is copied next: of item `to`, the wave's stage number `step`.
-  int to = blockIdx.x, step = 0, in = 0;
+  int step = 0, in = 0;
   __amdgpu_buffer_rsrc_t wbuf = buffer(p.gate_up, 0), sbuf = buffer(p.gate_up_s, 0);
-  auto aim = [&]() {  // buffers of item `to`
-    if (to >= items) return;
-    const int u = to / groups, column = (to - u * groups) * 8;
-    const int e = __builtin_amdgcn_readfirstlane(int(lds_word(chosen_at + u * 16)));
-    const int64_t row = int64_t(e) * 2 * p.inter + column;
+  auto aim = [&]() __attribute__((always_inline)) {  // buffers of item `to`
+    if (to.item >= items) return;
+    const int e = __builtin_amdgcn_readfirstlane(int(lds_word(chosen_at + to.u * 16)));
+    const int64_t row = int64_t(e) * 2 * p.inter + to.group * 8;
     wbuf = buffer(p.gate_up + row * row_bytes, extent);
     if constexpr (kType == kMxfp4) sbuf = buffer(p.gate_up_s + row * (p.hidden / mx::kBlock), uint32_t(p.inter + 8) * (p.hidden / mx::kBlock));
   };
-  auto copy_next = [&]() {
-    copier.copy(wbuf, sbuf, wave + kWaves * step, to < items, ring + in * F::kSlot);
+  auto copy_next = [&]() __attribute__((always_inline)) {
+    copier.copy(wbuf, sbuf, wave + kWaves * step, to.item < items, ring + in * F::kSlot);
     in = in + 1 == G::kRing ? 0 : in + 1;
     if (++step == mine) {
       step = 0;
-      to += gridDim.x;
+      next(to);
       aim();
     }
   };
@@ -324,10 +478,33 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
     aim();
     for (int n = 0; n < G::kRing - 1; ++n) copy_next();
   }
+  if (!through_lds) {
+    // Loaded with quarter after quarter of a load's 64 bytes of a row, if the lane's own lie further apart (16 rows of
+    // 4 x 16 bytes at 128 bytes from one another come four times over from L2: 10 us of 16 tokens)...
+#pragma unroll
+    for (int i = 0; i < kStages; ++i)
+#pragma unroll
+      for (int t = 0; t < kT; ++t)
+#pragma unroll
+        for (int n = 0; n < F::kUnits; ++n) {
+          const int token = 16 * t + c;
+          const int k = (wave + kWaves * i) * F::kStage + (kType == kBf16 ? q * 16 + 8 * n : 32 * n + 8 * q);
+          const uint32_t from = token < p.tokens && k < p.hidden ? uint32_t(token * p.x_row) + k * 2 : kPast;
+          x[i][t][n] = __builtin_amdgcn_raw_buffer_load_b128(xbuf, from, 0, 0);
+        }
+    wait_vm<0>();  // (or the compiler would wait for x, and every copy, in the loop)
+    if constexpr (kType != kBf16) {
+      // ... and exchanged between the quarters: unit j of quarter q is load kUnits / 4 q + j / 4 of quarter j % 4.
+#pragma unroll
+      for (int i = 0; i < kStages; ++i)
+#pragma unroll
+        for (int t = 0; t < kT; ++t) transpose_quarters<F::kUnits>(x[i][t]);
+    }
+  }
 
   int out = 0, turn = 0;
-  for (int item = blockIdx.x; item < items; item += gridDim.x, turn ^= 1) {
-    const int u = item / groups, column = (item - u * groups) * 8;
+  for (; at.item < items; next(at), turn ^= 1) {
+    const int u = at.u, column = at.group * 8;
     const float *gate_s = nullptr, *up_s = nullptr;
     float gs = 0.f, us = 0.f;
     if constexpr (kType == kFp8) {
@@ -405,17 +582,17 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
     int n, u, s;
   };
   const int jump_u = kW / per, jump_s = kW % per;
-  auto next = [&](At& a) {
+  auto next = [&](At& a) __attribute__((always_inline)) {
     a.n += kW;
     a.u += jump_u;
     a.s += jump_s;
     if (a.s >= per) a.s -= per, ++a.u;
   };
-  // (Past the last one the last one again: their copies and rows of x are zeros.)
-  auto entry = [&](int u) { return sload(reinterpret_cast<const i32x4*>(p.table), 1 + min(u, used - 1)); };
+  // (Past the last one whatever is there: copies and rows of x are zeros then. So no entry waits for their number.)
+  auto entry = [&](int u) { return sload(reinterpret_cast<const i32x4*>(p.table), 1 + min(u, kMostChoices - 1)); };
   At to{wave, wave / per, wave % per}, x_at = to, at = to;
   int in = 0, out = 0;
-  auto copy_next = [&]() {
+  auto copy_next = [&]() __attribute__((always_inline)) {
     const int64_t row = int64_t(entry(to.u)[0]) * p.hidden + column;
     const auto wbuf = buffer(p.down + row * row_bytes, extent);
     auto sbuf = wbuf;
@@ -425,7 +602,7 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
     next(to);
   };
   const auto hbuf = buffer(p.h, uint32_t(p.tokens) * p.top * p.inter * 2);
-  auto load_x = [&](u32x4 (&x)[kT][F::kUnits]) {  // returns the mask of the stage's tokens
+  auto load_x = [&](u32x4 (&x)[kT][F::kUnits]) __attribute__((always_inline)) {  // returns the mask of the stage's tokens
     const i32x4 chosen = entry(x_at.u);
     const uint32_t mask = x_at.n < total ? uint32_t(chosen[2]) : 0u;
     const int k0 = x_at.s * F::kStage + q * (F::kStage / 4);
@@ -445,7 +622,7 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
   f32x4 acc[kT];
 #pragma unroll
   for (int t = 0; t < kT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto step = [&](const u32x4 (&x)[kT][F::kUnits], uint32_t mask, u32x4 (&ahead)[kT][F::kUnits]) {
+  auto step = [&](const u32x4 (&x)[kT][F::kUnits], uint32_t mask, u32x4 (&ahead)[kT][F::kUnits]) __attribute__((always_inline)) {
     // Behind the copies of this stage went those of kDownRing - 2 more, and as many stages of x.
     wait_vm<(kDownRing - 2) * (F::kCopies + kT * F::kUnits)>();
     const uint32_t mask_ahead = load_x(ahead);

@@ -47,7 +47,9 @@ struct RouteParams {
 // The choices of token t, as `choose_experts` makes them, stored; returns the lane's.
 template <bool kFp32, int kLanes, int kPer>
 __device__ __forceinline__ int choose(const RouteParams& p, int t, bool live) {
-  const Choice c = choose_experts<kFp32, kLanes, kPer>(p.logits, p.stride, p.experts, p.top, p.renormalize, t, live);
+  float value[kPer];
+  load_logits<kLanes>(p.logits, kFp32, p.stride, p.experts, t, live, value);
+  const Choice c = choose_experts<kFp32, kLanes>(value, p.top, p.renormalize);
   const int lane = threadIdx.x & (kLanes - 1);
   if (live && lane < p.top) {
     p.weights[int64_t(t) * p.top + lane] = c.weight;
