@@ -429,7 +429,7 @@ int lf_combine_experts(const uint16_t* rows, int64_t num_rows, int64_t rows_stri
  * lf_expert_linear (MXFP4 bytes, 4-byte aligned; FP8 floats); base bf16 [tokens, hidden] or NULL (y may be base). Sums in
  * fp32; weight_tj silu(gate) * up is rounded to bf16, y once.
  * lf_expert_mlp_workspace_size: bytes (16-byte aligned, need not be cleared, not shared by calls that overlap), or -1 for
- * sizes that the two kernels do not take: more than 32 tokens, 256 choices, 256 experts, top 16; hidden above 8192 (4096
+ * sizes that the two kernels do not take: more than 32 tokens (MXFP4 16), 256 choices, 256 experts, top 16; hidden above 8192 (4096
  * from 17 tokens on); widths that are no multiples of 8 (bf16), 16 (FP8; inter of 128), 128 (MXFP4). */
 #define LF_EXPERT_BF16 0
 #define LF_EXPERT_MXFP4 1

@@ -291,6 +291,8 @@ _BOUND = (
     "lf_combine_experts",
     "lf_fp8_quantize",
     "lf_fp8_dequantize",
+    "lf_expert_mlp_workspace_size",
+    "lf_expert_mlp",
 )
 
 

@@ -23,14 +23,21 @@ bool tiles_fit(const lf_expert_product& a) {
   return !a.w_scales || a.k >= 128;
 }
 
+// The highest tile of so many columns. (Sums of 256 x 256 products leave no registers for a block's of FP8 weights.)
+int most_rows(const lf_expert_product& a, int columns) {
+  if (!a.w_fp8_scales) return 256;
+  return a.x_fp8_scales ? (columns == 256 ? 192 : 256) : columns == 256 ? 128 : 192;
+}
+
 // Scales are loaded 16 at a time.
 bool rows_fit(const lf_expert_product& a) { return !a.w_scales || a.k >= 512; }
 
 // Times of the kernels in us, fitted to 2586 products (dense ones of 1..4096 rows,
-// n 1024..24576, k 1024..8192; 8..128 experts, 1..8192 tokens), every plan of each.
+// n 1024..24576, k 1024..8192; 8..128 experts, 1..8192 tokens), every plan of each; with FP8 weights to 1080
+// (dense ones of 1..4096 rows, n 528..24576, k 1024..12288; 8..128 experts, 2..32768 choices).
 struct Costs {
   struct Tile {
-    float fixed, stage, busy;  // of a tile, of a stage (64 k; 256 k of MXFP4 x), and what all CUs at work add to a stage
+    float fixed, stage, busy;  // of a tile, of a stage (64 k; 256 k of MXFP4 x; 128 k of FP8 weights), and what all CUs at work add to a stage
   } tile[4][4];                // [rows / 64 - 1][columns / 64 - 1]
   struct Rows {
     float fixed, pass, k, k_busy;  // of the launch, of a pass of 16 rows, of 1024 k of it, and what two workgroups on every CU add
@@ -39,7 +46,7 @@ struct Costs {
     float fixed, pass, k, k_tile, k_busy, k_tile_busy;  // the same, with a part for each 16-row tile of a pass (at most 64 rows)
   } stream[2];                                           // [16, 32 columns]
 };
-constexpr Costs kCosts[3] = {
+constexpr Costs kCosts[5] = {
     // bf16 x and weights
     {{
          {{4.57f, 0.230f, 0.081f}, {5.02f, 0.307f, 0.177f}, {6.20f, 0.395f, 0.230f}, {5.69f, 0.424f, 0.284f}},
@@ -67,6 +74,24 @@ constexpr Costs kCosts[3] = {
      {2.31f, 1.56f, 1.06f, 4.12f},
      {{1.66f, 1.68f, 0.08f, 0.38f, 0.42f, 0.48f},
       {1.47f, 2.04f, 0.35f, 0.45f, 0.91f, 0.48f}}},
+    // bf16 x, FP8 weights (stages of 128 k; no tiles of those heights beside those columns where there is none)
+    {{
+         {{5.44f, 0.343f, 0.104f}, {6.17f, 0.511f, 0.192f}, {7.00f, 0.630f, 0.257f}, {6.96f, 0.772f, 0.352f}},
+         {{4.89f, 0.594f, 0.330f}, {7.88f, 0.712f, 0.339f}, {11.23f, 0.879f, 0.438f}, {10.93f, 1.105f, 0.668f}},
+         {{6.25f, 0.780f, 0.275f}, {9.50f, 0.973f, 0.402f}, {13.09f, 1.388f, 0.504f}, {}},
+         {{}, {}, {}, {}}},
+     {1.99f, 1.56f, 2.52f, 7.29f},
+     {{1.30f, 1.81f, 0.00f, 0.79f, 0.00f, 1.19f},
+      {1.11f, 2.47f, 0.18f, 0.91f, 0.31f, 1.46f}}},
+    // FP8 x and weights
+    {{
+         {{4.73f, 0.207f, 0.179f}, {5.18f, 0.324f, 0.296f}, {6.33f, 0.424f, 0.399f}, {5.63f, 0.544f, 0.394f}},
+         {{4.92f, 0.306f, 0.285f}, {6.37f, 0.438f, 0.385f}, {8.83f, 0.551f, 0.382f}, {8.12f, 0.615f, 0.551f}},
+         {{5.79f, 0.414f, 0.286f}, {6.93f, 0.516f, 0.412f}, {11.29f, 0.713f, 0.377f}, {10.54f, 0.854f, 0.453f}},
+         {{3.08f, 0.792f, 0.365f}, {6.74f, 0.679f, 0.480f}, {12.08f, 0.979f, 0.332f}, {}}},
+     {2.65f, 0.79f, 2.10f, 7.86f},
+     {{1.43f, 1.98f, 0.06f, 0.49f, 0.33f, 0.67f},
+      {0.95f, 2.65f, 0.30f, 0.62f, 0.77f, 0.65f}}},
 };
 
 constexpr double kCus = 256;
@@ -95,9 +120,10 @@ double tile_us(const Costs& c, int rows, int columns, double each, double used, 
 
 // The plan of least time. (Against the fastest plan of each of those products: 1.6 to
 // 4.8 % slower on average by type, 63 % at most: 256 tokens over 64 experts, n and k 1024, 21 and 13 us.
-// Over 80 dense products of 8..384 rows, n 528..8192: 10 % with bf16 x, 6 % with MXFP4 x, 43 % at most.)
+// Over 80 dense products of 8..384 rows, n 528..8192: 10 % with bf16 x, 6 % with MXFP4 x, 43 % at most.
+// FP8 weights: 5 % beside bf16 x, 4 beside FP8 x; 90 % at most: 384 tokens' 768 choices among 32 experts, n 1024, k 2048, 40 and 21 us.)
 lf_expert_plan plan_of(const lf_expert_product& a) {
-  const Costs& c = kCosts[a.x_scales ? 2 : a.x_fp8_scales ? 2 : a.w_scales || a.w_fp8_scales ? 1 : 0];
+  const Costs& c = kCosts[a.w_fp8_scales ? (a.x_fp8_scales ? 4 : 3) : a.x_scales ? 2 : a.w_scales ? 1 : 0];
   const bool grouped = a.offsets != nullptr && a.experts > 1;
   const double rows = double(a.rows), experts = double(a.experts);
   const double used = grouped ? experts * (1.0 - std::pow(1.0 - 1.0 / experts, rows)) : 1.0;
@@ -106,10 +132,11 @@ lf_expert_plan plan_of(const lf_expert_product& a) {
   lf_expert_plan best{LF_EXPERT_STREAM, 64, 16};
   double least = std::numeric_limits<double>::infinity();
   // (No plan is faster than the used weights through HBM; of those that are at it, the one with less work.
-  // bf16 weights of few rows come at 4.3 TB/s in tiles, 4.9 a wave for 16 of them, 5.5 streamed.)
-  const double hbm = used * n * double(a.k) * (a.w_scales ? 17.0 / 32.0 : 2.0) * 1e-6;
+  // bf16 weights of few rows come at 4.3 TB/s in tiles, 4.9 a wave for 16 of them, 5.5 streamed; FP8 ones at 4.4, 4.6 and 4.9.)
+  const double hbm = used * n * double(a.k) * (a.w_scales ? 17.0 / 32.0 : a.w_fp8_scales ? 1.0 : 2.0) * 1e-6;
   auto offer = [&](double us, lf_expert_plan plan) {
-    const double rate = a.w_scales || plan.kernel == LF_EXPERT_STREAM ? 5.5 : plan.kernel == LF_EXPERT_ROWS ? 4.9 : 4.3;
+    const bool stream = plan.kernel == LF_EXPERT_STREAM, wave = plan.kernel == LF_EXPERT_ROWS;
+    const double rate = a.w_fp8_scales ? (stream ? 4.9 : wave ? 4.6 : 4.4) : a.w_scales || stream ? 5.5 : wave ? 4.9 : 4.3;
     us = std::max(us, hbm / rate) + 0.1 * us;
     if (us < least) least = us, best = plan;
   };
@@ -136,7 +163,8 @@ lf_expert_plan plan_of(const lf_expert_product& a) {
     const double stage_k = a.x_scales ? 256.0 : a.w_fp8_scales ? 128.0 : 64.0;
     for (int height = 64; height <= 256; height += 64)
       for (int columns = 64; columns <= 256; columns += 64)
-        if (!a.w_fp8_scales || height <= (a.x_fp8_scales ? (columns == 256 ? 192 : 256) : columns == 256 ? 128 : 192)) offer(tile_us(c, height, columns, each, used, grouped, n, std::ceil(double(a.k) / stage_k)), {LF_EXPERT_TILE, height, columns});
+        if (height <= most_rows(a, columns))
+          offer(tile_us(c, height, columns, each, used, grouped, n, std::ceil(double(a.k) / stage_k)), {LF_EXPERT_TILE, height, columns});
   }
   return best;
 }
@@ -203,8 +231,7 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   LF_REQUIRE(plan.rows >= 64 && plan.rows <= 256 && plan.rows % 64 == 0, "tile plan: 64, 128, 192 or 256 rows");
   LF_REQUIRE(plan.columns >= 64 && plan.columns <= 256 && plan.columns % 64 == 0, "tile plan: 64, 128, 192 or 256 columns");
   if (w_f8) {
-    // (Sums of 256 x 256 products leave no registers for a block's: tiles of 256 columns have fewer rows.)
-    const int most = x_f8 ? (plan.columns == 256 ? 192 : 256) : plan.columns == 256 ? 128 : 192;
+    const int most = lf::expert::most_rows(*a, plan.columns);
     LF_REQUIRE(plan.rows <= most, "tile plan: at most %d rows beside %d columns of FP8 weights", most, int(plan.columns));
     return x_f8 ? lf::expert::launch_tiles_fp8(p, plan.rows, plan.columns, s) : lf::expert::launch_tiles_w8(p, plan.rows, plan.columns, s);
   }

@@ -33,7 +33,10 @@ namespace {
 
 constexpr int kWaves = 8;            // of the first launch
 constexpr int kThreads = 64 * kWaves;
-constexpr int kMostTokens = 32;      // a token is a bit of a mask, and a column of two tiles at most
+// A token is a bit of a mask, and a column of two tiles at most. MXFP4 weights take one tile: levels made for two
+// cost more than the launches (128 experts, top 8, 4096 x 1024, 24 tokens: 156 us, in a chain 137; FP8 weights
+// 221 and 281, bf16 395 and 414; 16 tokens MXFP4 113 and 120).
+constexpr int kMostTokens = 32;
 constexpr int kFewTokens = 2;        // routed by ranks
 constexpr int kMostExperts = 256;
 constexpr int kMostTop = 16;
@@ -698,15 +701,16 @@ template <int kType, int kT>
 int launch_both(const MlpParams& p, hipStream_t stream) {
   if (const int rc = launch_gate_up<kType, kT>(p, stream)) return rc;
   const unsigned grid = unsigned((p.hidden + 15) / 16);
-  // Few workgroups get twice the waves (MXFP4 and two tiles of tokens: more registers than such waves have).
-  if constexpr (kType != kMxfp4 || kT == 1)
-    if (grid <= 160) return launch(down_kernel<kType, kT, 16>, grid, 1024, down_lds<kType, kT, 16>(), p, stream);
+  // Few workgroups get twice the waves.
+  if (grid <= 160) return launch(down_kernel<kType, kT, 16>, grid, 1024, down_lds<kType, kT, 16>(), p, stream);
   return launch(down_kernel<kType, kT, 8>, grid, 512, down_lds<kType, kT, 8>(), p, stream);
 }
 
 template <int kType>
 int launch_type(const MlpParams& p, hipStream_t stream) {
-  return p.tokens <= 16 ? launch_both<kType, 1>(p, stream) : launch_both<kType, 2>(p, stream);
+  if constexpr (kType != kMxfp4)
+    if (p.tokens > 16) return launch_both<kType, 2>(p, stream);
+  return launch_both<kType, 1>(p, stream);
 }
 
 int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -718,7 +722,7 @@ int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
 // Bytes of workspace, or -1 where the two kernels cannot take the sizes.
 extern "C" int64_t lf_expert_mlp_workspace_size(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
   using namespace lf::expert;
-  if (tokens < 1 || tokens > kMostTokens || experts < 1 || experts > kMostExperts || top < 1 || top > kMostTop || top > experts ||
+  if (tokens < 1 || tokens > (type == LF_EXPERT_MXFP4 ? 16 : kMostTokens) || experts < 1 || experts > kMostExperts || top < 1 || top > kMostTop || top > experts ||
       tokens * top > kMostChoices || type < LF_EXPERT_BF16 || type > LF_EXPERT_FP8)
     return -1;
   const int64_t unit = type == LF_EXPERT_BF16 ? 8 : type == LF_EXPERT_FP8 ? 16 : 128;

@@ -44,6 +44,8 @@ decltype(&lf_expert_linear) g_product;
 decltype(&lf_combine_experts) g_combine;
 decltype(&lf_fp8_quantize) g_fp8_quantize;
 decltype(&lf_fp8_dequantize) g_fp8_dequantize;
+decltype(&lf_expert_mlp_workspace_size) g_mlp_ws;
+decltype(&lf_expert_mlp) g_mlp;
 
 PyObject* g_raw_stream;   // torch._C._cuda_getCurrentRawStream
 PyObject* g_get_device;   // torch._C._cuda_getDevice
@@ -975,16 +977,106 @@ PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return out.take();
 }
 
+// The weights [experts, n, k] of expert_mlp (ops.experts._expert_weight's checks).
+struct ExpertsArg {
+  MxArg mx;
+  Fp8Arg f8;
+  const at::Tensor* w = nullptr;
+  const at::Tensor* scales = nullptr;
+  int32_t type = 0;
+  int64_t k = 0;
+  bool take(PyObject* o) {
+    if (Fp8Arg::is(o)) {
+      if (!f8.take(o, 3, kFp8Block)) return false;
+      type = LF_EXPERT_FP8, w = f8.codes, scales = f8.scales, k = f8.k;
+    } else if (reinterpret_cast<PyObject*>(Py_TYPE(o)) == g_mx_tensor) {
+      if (!mx.take(o, 3)) return false;
+      type = LF_EXPERT_MXFP4, w = mx.codes, scales = mx.scales, k = mx.k;
+    } else {
+      w = plain(o);
+      if (!w || w->dim() != 3 || w->scalar_type() != at::kBFloat16 || !w->is_contiguous() || !aligned16(*w)) return false;
+      type = LF_EXPERT_BF16, k = w->size(2);
+    }
+    return w->numel() > 0 && (!scales || reinterpret_cast<uintptr_t>(scales->data_ptr()) % 4 == 0);
+  }
+};
+
+// mlp(x, logits, gate_up, down, top_k, renormalize, base or None, out or None) -> out or None: the sizes of
+// expert_mlp that two launches take. (The checks and the call through ctypes take 34 us on the host, this 8.5.)
+PyObject* mlp(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 8 || (args[5] != Py_True && args[5] != Py_False)) return decline();
+  ExpertsArg gate_up, down;
+  if (!gate_up.take(args[2]) || !down.take(args[3]) || gate_up.type != down.type) return decline();
+  const at::Device dev = down.w->device();
+  const int64_t experts = down.w->size(0), hidden = down.w->size(1), inter = down.k;
+  if (gate_up.w->device() != dev || gate_up.w->size(0) != experts || gate_up.w->size(1) != 2 * inter || gate_up.k != hidden)
+    return decline();
+  const at::Tensor* x = matrix(args[0], dev);
+  if (!x || x->size(1) != hidden || x->stride(1) != 1 || !aligned16(*x)) return decline();
+  const int64_t count = x->size(0);
+  // The strides of `t`, whose rows are apart; less than `width` if they are not.
+  const auto stride = [&](const at::Tensor& t, int64_t width) { return count > 1 ? t.stride(0) : width; };
+  lf_expert_mlp_call a{};
+  a.x_stride = stride(*x, hidden);
+  if (count == 0 || a.x_stride < hidden || a.x_stride % 8) return decline();
+  const at::Tensor* logits = plain(args[1]);
+  if (!logits || logits->dim() != 2 || logits->device() != dev ||
+      (logits->scalar_type() != at::kBFloat16 && logits->scalar_type() != at::kFloat) || logits->size(0) != count ||
+      logits->size(1) != experts || logits->stride(1) != 1 || stride(*logits, experts) < experts)
+    return decline();
+  long top;
+  if (!small_int(args[4], 1, 64, &top) || top > experts) return decline();
+  const at::Tensor* base = nullptr;
+  if (args[6] != Py_None) {
+    base = matrix(args[6], dev);
+    if (!base || base->size(0) != count || base->size(1) != hidden || base->stride(1) != 1) return decline();
+    a.base = ptr<uint16_t>(base);
+    a.base_stride = stride(*base, hidden);
+    if (a.base_stride < hidden) return decline();
+  }
+  if (experts >= (int64_t(1) << 31)) return decline();
+  const int64_t need = g_mlp_ws(count, int32_t(experts), int32_t(top), hidden, inter, down.type);
+  if (need < 0) return decline();
+  void* stream;
+  if (!current(dev, &stream)) return decline();
+  Output out(args[7], count, hidden, dev);
+  const bool onto = base && out.given && ptr<uint16_t>(out.given) == ptr<uint16_t>(base) && out.stride == a.base_stride;
+  if (!out.ok({x, logits, gate_up.w, gate_up.scales, down.w, down.scales, onto ? nullptr : base})) return decline();
+  const at::Tensor scratch = at::empty({need}, x->options().dtype(at::kByte));
+  if (!on_gpu(scratch)) return decline();
+  a.x = x->data_ptr();
+  a.logits = logits->data_ptr();
+  a.logits_stride = stride(*logits, experts);
+  a.fp32 = logits->scalar_type() == at::kFloat;
+  a.renormalize = args[5] == Py_True;
+  a.tokens = count;
+  a.hidden = hidden;
+  a.inter = inter;
+  a.experts = int32_t(experts);
+  a.top = int32_t(top);
+  a.type = down.type;
+  a.gate_up = gate_up.w->data_ptr();
+  a.gate_up_scales = ptr<void>(gate_up.scales);
+  a.down = down.w->data_ptr();
+  a.down_scales = ptr<void>(down.scales);
+  a.y = out.data();
+  a.y_stride = out.stride;
+  const int rc = unlocked([&] { return g_mlp(&a, scratch.data_ptr(), need, stream); });
+  if (rc == LF_EINVAL) return decline();
+  if (rc != LF_OK) return failed();
+  return out.take();
+}
+
 // init(addresses, raw_stream, get_device, arch_ok, workspaces, compute_units, lora_batch, mx_tensor, fp8_tensor)
 PyObject* init(PyObject*, PyObject* args) {
   PyObject *addresses, *raw, *dev, *arch, *ws, *cus, *batch, *packed, *eight;
   if (!PyArg_ParseTuple(args, "O!OOO!O!O!O!O!O!", &PyTuple_Type, &addresses, &raw, &dev, &PyDict_Type, &arch, &PyDict_Type, &ws,
                         &PyDict_Type, &cus, &PyType_Type, &batch, &PyType_Type, &packed, &PyType_Type, &eight))
     return nullptr;
-  constexpr int kEntries = 17;
+  constexpr int kEntries = 19;
   void* a[kEntries];
   if (PyTuple_GET_SIZE(addresses) != kEntries) {
-    PyErr_SetString(PyExc_ValueError, "seventeen entry points expected");
+    PyErr_SetString(PyExc_ValueError, "nineteen entry points expected");
     return nullptr;
   }
   for (int i = 0; i < kEntries; ++i)
@@ -1009,6 +1101,8 @@ PyObject* init(PyObject*, PyObject* args) {
   g_combine = reinterpret_cast<decltype(g_combine)>(a[14]);
   g_fp8_quantize = reinterpret_cast<decltype(g_fp8_quantize)>(a[15]);
   g_fp8_dequantize = reinterpret_cast<decltype(g_fp8_dequantize)>(a[16]);
+  g_mlp_ws = reinterpret_cast<decltype(g_mlp_ws)>(a[17]);
+  g_mlp = reinterpret_cast<decltype(g_mlp)>(a[18]);
 #define INTERN(n) \
   if (!s_##n && !(s_##n = PyUnicode_InternFromString(#n))) return nullptr;
   NAMES(INTERN)
@@ -1047,6 +1141,7 @@ PyMethodDef methods[] = {
     {"product", reinterpret_cast<PyCFunction>(guarded<product>), METH_FASTCALL, nullptr},
     {"route", reinterpret_cast<PyCFunction>(guarded<route>), METH_FASTCALL, nullptr},
     {"combine", reinterpret_cast<PyCFunction>(guarded<combine>), METH_FASTCALL, nullptr},
+    {"mlp", reinterpret_cast<PyCFunction>(guarded<mlp>), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

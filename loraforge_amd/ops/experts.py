@@ -187,6 +187,10 @@ def expert_mlp(x, logits, gate_up, down, top_k: int, *, renormalize: bool = True
     """
     import torch
 
+    if getattr(x, "is_cuda", False):
+        done = _lib.binding().mlp(x, logits, gate_up, down, top_k, renormalize, base, out)
+        if done is not None:
+            return done
     for name, w in (("gate_up", gate_up), ("down", down)):
         if not isinstance(w, (torch.Tensor, MXFP4Tensor, FP8Tensor)):
             raise TypeError(f"{name} must be a torch.Tensor, an MXFP4Tensor or an FP8Tensor")
