@@ -422,15 +422,17 @@ int lf_combine_experts(const uint16_t* rows, int64_t num_rows, int64_t rows_stri
                        const float* weights, int64_t tokens, int32_t top, int64_t n, const uint16_t* base,
                        int64_t base_stride, uint16_t* y, int64_t y_stride, void* stream);
 
-/* The whole MLP of a few tokens over their experts in two launches:
+/* The whole MLP of a few tokens over their experts:
  * y[t] = base[t] + sum_j weight_tj down_e (silu(gate_e x[t]) * (up_e x[t])), choices and weights as lf_route_experts
  * makes them. x bf16 [tokens, hidden], logits [tokens, experts] (fp32 != 0: fp32, else bf16), gate_up [experts,
  * 2 inter, hidden] (gate rows, then up rows), down [experts, hidden, inter], both of `type`, with the scales of
  * lf_expert_linear (MXFP4 bytes, 4-byte aligned; FP8 floats); base bf16 [tokens, hidden] or NULL (y may be base). Sums in
- * fp32; weight_tj silu(gate) * up is rounded to bf16, y once.
+ * fp32; silu(gate) * up is held in 16 bits of mantissa (a pair of bf16), y rounded once.
+ * Up to 8 tokens, 256 experts, top 16 and hidden 8192 (widths multiples of 128 for MXFP4) run in two launches, else four.
  * lf_expert_mlp_workspace_size: bytes (16-byte aligned, need not be cleared, not shared by calls that overlap), or -1 for
- * sizes that the two kernels do not take: more than 32 tokens (MXFP4 16), 256 choices, 256 experts, top 16; hidden above 8192 (4096
- * from 17 tokens on); widths that are no multiples of 8 (bf16), 16 (FP8; inter of 128), 128 (MXFP4). */
+ * sizes that it does not take: more than 32 choices for each expert on average (tokens * top against experts; there the
+ * products are bound by their matrix instructions, and lf_route_experts, lf_expert_linear and lf_combine_experts hold what lies between them in
+ * bf16), 1024 experts, top 64; widths that are no multiples of 8 (bf16), 16 (FP8; inter of 128), 32 (MXFP4). */
 #define LF_EXPERT_BF16 0
 #define LF_EXPERT_MXFP4 1
 #define LF_EXPERT_FP8 2

@@ -169,12 +169,7 @@ lf_expert_plan plan_of(const lf_expert_product& a) {
   return best;
 }
 
-}  // namespace
-}  // namespace expert
-}  // namespace lf
-
-extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
-  LF_REQUIRE(a != nullptr, "null pointer argument");
+int launch(const lf_expert_product* a, Pair pair, void* stream) {
   LF_REQUIRE(a->rows >= 0 && a->x_rows >= 0 && a->n >= 1 && a->experts >= 1, "sizes must be positive");
   LF_REQUIRE(a->rows < (int64_t(1) << 31) - 65536 && a->x_rows < (int64_t(1) << 31) && a->n < (int64_t(1) << 31) - 65536 &&
                  a->k < (int64_t(1) << 30) - 65536 && a->experts < 65536,
@@ -216,6 +211,7 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   p.width = int(width);
   p.swiglu = a->swiglu ? 1 : 0;
   p.y_vec = lf::aligned16(a->y) && a->y_stride % 8 == 0;
+  p.pair = pair;
   const lf_expert_plan plan = a->plan ? *a->plan : lf::expert::plan_of(*a);
   auto s = static_cast<hipStream_t>(stream);
   if (plan.kernel == LF_EXPERT_STREAM) {
@@ -238,6 +234,18 @@ extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
   if (x_mx) return lf::expert::launch_tiles_mx(p, plan.rows, plan.columns, s);
   return w_mx ? lf::expert::launch_tiles_mxw(p, plan.rows, plan.columns, s)
               : lf::expert::launch_tiles_bf16(p, plan.rows, plan.columns, s);
+}
+
+}  // namespace
+
+int launch_pairs(const lf_expert_product& a, Pair pair, hipStream_t stream) { return launch(&a, pair, stream); }
+
+}  // namespace expert
+}  // namespace lf
+
+extern "C" int lf_expert_linear(const lf_expert_product* a, void* stream) {
+  LF_REQUIRE(a != nullptr, "null pointer argument");
+  return lf::expert::launch(a, lf::expert::kSingle, stream);
 }
 
 extern "C" int lf_expert_linear_plan(const lf_expert_product* a, lf_expert_plan* plan) {

@@ -11,15 +11,20 @@
 // Its eight waves share k (stage s of 128 bytes of a row to wave s % 8), each streaming its weights through a
 // ring of its own in LDS by direct copies; the ring runs on from one item to the next. The weight is
 // the A operand of 16 x 16 matrix instructions, *all* tokens are the B operand (of x, held
-// in registers: at most 128 of them, which is what bounds tokens and k): columns of tokens
+// in registers: at most 128 of them, which bounds k): columns of tokens
 // that did not choose the expert are computed and dropped, which costs nothing beside the bytes.
-// The waves' sums meet in LDS, in a fixed order; the intermediate s silu(g) u is rounded to bf16
-// once, with the routing weight in it, so that the second product needs no weights.
+// The waves' sums meet in LDS, in a fixed order; the intermediate s silu(g) u, with the routing weight
+// in it so that the second product needs no weights, is kept as a pair of bf16 (rounded to one, it is as far
+// from the formula as y's own rounding: 1.0 times as much again, and 1.5 of both).
 //
 // Second launch. With rows of the intermediate in expert order, y is one product whose k runs
 // over (chosen experts) x (intermediate): a workgroup owns 16 columns of y, its waves share that long
-// k, and their sums meet once at the end. Tokens are the columns of B again; a token that did not choose the
+// k, and their sums meet once at the end. Tokens are the columns of B again, twice: for the high and for the low halves of
+// their pairs, which of up to eight tokens fit one tile. A token that did not choose the
 // stage's expert reads zeros (past the end of a buffer).
+//
+// More tokens, and widths that these do not take: routing, gate and up product, down product and sum one after
+// another, in the kernels of the operators, with pairs between the products and rows of fp32 before the sum.
 #include <type_traits>
 
 #include "expert_choose.h"
@@ -33,14 +38,18 @@ namespace {
 
 constexpr int kWaves = 8;            // of the first launch
 constexpr int kThreads = 64 * kWaves;
-// A token is a bit of a mask, and a column of two tiles at most. MXFP4 weights take one tile: levels made for two
-// cost more than the launches (128 experts, top 8, 4096 x 1024, 24 tokens: 156 us, in a chain 137; FP8 weights
-// 221 and 281, bf16 395 and 414; 16 tokens MXFP4 113 and 120).
-constexpr int kMostTokens = 32;
+// Eight tokens: with the halves of their pairs 16 columns of the second launch. (A second tile for up to 16 takes the address
+// unit twice as long for x as for the weights: 128 experts, top 8, 4096 x 1024, MXFP4, 12 tokens 111 us, in a chain 107.)
+constexpr int kMostTokens = 8;
+// Choices of an expert, on average, up to which a chain keeps pairs: they double the rows of the down product, which costs
+// little while its weights' bytes bound it (16 experts, top 4, 4096 x 2048, 64 tokens, 16 choices each: MXFP4 76 us and 68 with
+// the intermediate in bf16, FP8 105 and 104, bf16 205 and 202; 128 tokens 97 and 85, 123 and 108, 215 and 207; 512 tokens 237
+// and 170, 259 and 209, 278 and 228).
+constexpr int kMostEach = 32;
 constexpr int kFewTokens = 2;        // routed by ranks
 constexpr int kMostExperts = 256;
 constexpr int kMostTop = 16;
-constexpr int kMostChoices = 256;
+constexpr int kMostChoices = kMostTokens * kMostTop;
 constexpr int kSlotWeights = 16 * 128;
 constexpr uint32_t kPast = 0x80000000u;  // past the end of every buffer here
 
@@ -58,7 +67,7 @@ struct MlpParams {
   int64_t base_stride;
   uint16_t* y;
   int64_t y_stride;
-  uint16_t* h;   // [tokens * top, inter], rows in expert order
+  uint16_t* h;   // [tokens * top, 2, inter], rows in expert order, halves of pairs
   int4* table;   // x of entry 0: chosen experts; entry 1 + u: expert, first row, mask of its tokens
 };
 
@@ -173,47 +182,37 @@ struct Copier {
   }
 };
 
-// One stage: 16 weight rows (in the slot) times kT tiles of 16 rows of x (units of a lane's quarter of the stage's k).
-// `scale`: FP8, of the lane's weight rows. kMasked: only the tokens of `mask` take part in the stage, so that what is not
-// finite in an expert's weights (NaN times zero is NaN) reaches no other token.
-template <int kType, int kT, bool kMasked>
-__device__ __forceinline__ void contract(uint32_t slot, const u32x4 (&x)[kT][Format<kType>::kUnits], float scale, uint32_t mask, f32x4 (&acc)[kT]) {
+// One stage: 16 weight rows (in the slot) times 16 columns of x (units of a lane's quarter of the stage's k).
+// `scale`: FP8, of the lane's weight rows. kMasked: only columns whose token (c % 8) is in `mask` take part in the stage, so that
+// what is not finite in an expert's weights (NaN times zero is NaN) reaches no other token.
+template <int kType, bool kMasked>
+__device__ __forceinline__ void contract(uint32_t slot, const u32x4 (&x)[Format<kType>::kUnits], float scale, uint32_t mask, f32x4& acc) {
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   u32x4 w[2];
   lds_two(w, slot + c * 128 + ((2 * q) ^ (c & 7)) * 16, slot + c * 128 + ((2 * q + 1) ^ (c & 7)) * 16);
   constexpr bool kApart = kMasked || kType == kFp8;  // a stage's products from zero
-  f32x4 sum[kT];
-#pragma unroll
-  for (int t = 0; t < kT; ++t) sum[t] = kApart ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[t];
+  f32x4 sum = kApart ? f32x4{0.f, 0.f, 0.f, 0.f} : acc;
   if constexpr (kType == kBf16) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int t = 0; t < kT; ++t) sum[t] = lf::mfma16(vec_bf16x8(w[j]), vec_bf16x8(x[t][j]), sum[t]);
+    for (int j = 0; j < 2; ++j) sum = lf::mfma16(vec_bf16x8(w[j]), vec_bf16x8(x[j]), sum);
   } else if constexpr (kType == kFp8) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bf16x8 a = vec_bf16x8(fp8::decode8(w[j >> 1][j % 2 * 2], w[j >> 1][j % 2 * 2 + 1]));
-#pragma unroll
-      for (int t = 0; t < kT; ++t) sum[t] = lf::mfma16(a, vec_bf16x8(x[t][j]), sum[t]);
-    }
+    for (int j = 0; j < 4; ++j)
+      sum = lf::mfma16(vec_bf16x8(fp8::decode8(w[j >> 1][j % 2 * 2], w[j >> 1][j % 2 * 2 + 1])), vec_bf16x8(x[j]), sum);
   } else {
     const uint32_t scales = lds_scales(slot + kSlotWeights + c * 8 + 2 * q);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float s = mx::scale_f32(j < 4 ? scales & 0xffu : scales >> 8);
-      const bf16x8 a = vec_bf16x8(mx::decode8(w[j >> 2][j & 3], s));
-#pragma unroll
-      for (int t = 0; t < kT; ++t) sum[t] = lf::mfma16(a, vec_bf16x8(x[t][j]), sum[t]);
+      sum = lf::mfma16(vec_bf16x8(mx::decode8(w[j >> 2][j & 3], s)), vec_bf16x8(x[j]), sum);
     }
   }
+  const bool in = !kMasked || (mask >> (c & 7) & 1);
 #pragma unroll
-  for (int t = 0; t < kT; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float v = kType == kFp8 ? fmaf(scale, sum[t][e], acc[t][e]) : kApart ? acc[t][e] + sum[t][e] : sum[t][e];
-      acc[t][e] = !kMasked || (mask >> (16 * t + c) & 1) ? v : acc[t][e];
-    }
+  for (int e = 0; e < 4; ++e) {
+    const float v = kType == kFp8 ? fmaf(scale, sum[e], acc[e]) : kApart ? acc[e] + sum[e] : sum[e];
+    acc[e] = in ? v : acc[e];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -380,19 +379,19 @@ __device__ __forceinline__ void route(const MlpParams& p, Routing& r) {
 // ---------------------------------------------------------------------------
 // First launch: routing, gate and up products, SwiGLU.
 // ---------------------------------------------------------------------------
-template <int kType, int kT, int kStages>
+template <int kType, int kStages>
 struct GateUp {
   using F = Format<kType>;
-  static constexpr bool kTwo = kT == 1 && kStages * F::kUnits <= 16;  // two workgroups on a CU: 64 registers of x
+  static constexpr bool kTwo = kStages * F::kUnits <= 16;  // two workgroups on a CU: 64 registers of x
   static constexpr int kRing = kTwo ? 3 : 5;                    // stages
-  static constexpr int kRed = 2 * kT * kWaves * 1024;
+  static constexpr int kRed = 2 * kWaves * 1024;
   static constexpr int kLds = kWaves * kRing * F::kSlot + kRed;
 };
 
-template <int kType, int kT, int kStages>
-__global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2)) void gate_up_kernel(MlpParams p) {
+template <int kType, int kStages>
+__global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) void gate_up_kernel(MlpParams p) {
   using F = Format<kType>;
-  using G = GateUp<kType, kT, kStages>;
+  using G = GateUp<kType, kStages>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Routing routing;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -401,12 +400,12 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
   const int mine = stages > wave ? (stages - wave + kWaves - 1) / kWaves : 0;  // stages wave, wave + 8, ...
 
   // x: unit n of a lane holds k 8 n .. of its quarter of the stage.
-  u32x4 x[kStages][kT][F::kUnits];
+  u32x4 x[kStages][F::kUnits];
   const auto xbuf = buffer(p.x, uint32_t((p.tokens - 1) * p.x_row + p.hidden * 2));
   // A few rows go through LDS (where the weights come later) while the tokens are routed: KiB by KiB, unit u of row t at
   // u ^ t. (A load of 16 rows takes the address unit as long for one row as for 16.)
   const int pieces = (p.hidden * 2 + 1023) / 1024, pitch = pieces * 1024;
-  const bool through_lds = kT == 1 && p.tokens <= kWaves && p.tokens * pitch <= G::kLds;
+  const bool through_lds = p.tokens * pitch <= G::kLds;
   if (through_lds)
     for (int t = 0; t < p.tokens; ++t)
       for (int piece = wave; piece < pieces; piece += kWaves) {
@@ -423,7 +422,7 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
 #pragma unroll
         for (int n = 0; n < F::kUnits; ++n) {
           const int unit = ((wave + kWaves * i) * F::kStage + q * (F::kStage / 4)) / 8 + n;
-          x[i][0][n] = *reinterpret_cast<const u32x4*>(lds + t * pitch + (unit ^ t) * 16);
+          x[i][n] = *reinterpret_cast<const u32x4*>(lds + t * pitch + (unit ^ t) * 16);
         }
     lds_barrier();
   }
@@ -487,21 +486,16 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
 #pragma unroll
     for (int i = 0; i < kStages; ++i)
 #pragma unroll
-      for (int t = 0; t < kT; ++t)
-#pragma unroll
-        for (int n = 0; n < F::kUnits; ++n) {
-          const int token = 16 * t + c;
-          const int k = (wave + kWaves * i) * F::kStage + (kType == kBf16 ? q * 16 + 8 * n : 32 * n + 8 * q);
-          const uint32_t from = token < p.tokens && k < p.hidden ? uint32_t(token * p.x_row) + k * 2 : kPast;
-          x[i][t][n] = __builtin_amdgcn_raw_buffer_load_b128(xbuf, from, 0, 0);
-        }
+      for (int n = 0; n < F::kUnits; ++n) {
+        const int k = (wave + kWaves * i) * F::kStage + (kType == kBf16 ? q * 16 + 8 * n : 32 * n + 8 * q);
+        const uint32_t from = c < p.tokens && k < p.hidden ? uint32_t(c * p.x_row) + k * 2 : kPast;
+        x[i][n] = __builtin_amdgcn_raw_buffer_load_b128(xbuf, from, 0, 0);
+      }
     wait_vm<0>();  // (or the compiler would wait for x, and every copy, in the loop)
     if constexpr (kType != kBf16) {
       // ... and exchanged between the quarters: unit j of quarter q is load kUnits / 4 q + j / 4 of quarter j % 4.
 #pragma unroll
-      for (int i = 0; i < kStages; ++i)
-#pragma unroll
-        for (int t = 0; t < kT; ++t) transpose_quarters<F::kUnits>(x[i][t]);
+      for (int i = 0; i < kStages; ++i) transpose_quarters<F::kUnits>(x[i]);
     }
   }
 
@@ -517,9 +511,7 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
       up_s = p.gate_up_s8 + (first + (p.inter + column) / fp8::kBlock) * blocks;
       gs = sload(gate_s, min(wave, blocks - 1)), us = sload(up_s, min(wave, blocks - 1));
     }
-    f32x4 acc[kT];
-#pragma unroll
-    for (int t = 0; t < kT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
       if (i < mine) {
@@ -531,23 +523,23 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
           const int ahead = min(wave + kWaves * (i + 1), blocks - 1);
           gs = sload(gate_s, ahead), us = sload(up_s, ahead);
         }
-        contract<kType, kT, false>(ring_at + out * F::kSlot, x[i], scale, 0u, acc);
+        contract<kType, false>(ring_at + out * F::kSlot, x[i], scale, 0u, acc);
         out = out + 1 == G::kRing ? 0 : out + 1;
       }
     }
-    // Sums as [turn][tile][wave][token][row]; two places in turn, so one barrier an item.
+    // Sums as [turn][wave][token][row]; two places in turn, so one barrier an item.
     const uint32_t red = red_at + turn * (G::kRed / 2);
-#pragma unroll
-    for (int t = 0; t < kT; ++t) lds_write16(red + (t * kWaves + wave) * 1024 + c * 64 + q * 16, acc[t]);
+    lds_write16(red + wave * 1024 + c * 64 + q * 16, acc);
     lds_barrier();
-    if (threadIdx.x < 128 * kT) {
+    if (threadIdx.x < 8 * kMostTokens) {
       const int token = threadIdx.x >> 3, r = threadIdx.x & 7;
-      const uint32_t from = red + (token >> 4) * kWaves * 1024 + (token & 15) * 64 + r * 4;
+      const uint32_t from = red + token * 64 + r * 4;
       const uint32_t mask = lds_word(chosen_at + u * 16 + 8);
       if (mask >> token & 1) {
         const int row = int(lds_word(chosen_at + u * 16 + 4)) + __popc(mask & ((1u << token) - 1));
         const float g = lds_sum8(from), up = lds_sum8(from + 32);
-        p.h[int64_t(row) * p.inter + column + r] = uint16_t(f32_to_bf16(silu_mul_f32(g, up) * __uint_as_float(lds_word(weight_at + row * 4))));
+        uint16_t* h = p.h + int64_t(row) * 2 * p.inter + column + r;
+        split_pair(silu_mul_f32(g, up) * __uint_as_float(lds_word(weight_at + row * 4)), h[0], h[p.inter]);
       }
     }
   }
@@ -559,12 +551,12 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2
 // ---------------------------------------------------------------------------
 constexpr int kDownRing = 4;
 
-template <int kType, int kT, int kW>
+template <int kType, int kW>
 constexpr int down_lds() {
-  return kW * kDownRing * Format<kType>::kSlot + kT * kW * 1024;
+  return kW * kDownRing * Format<kType>::kSlot + kW * 1024;
 }
 
-template <int kType, int kT, int kW>
+template <int kType, int kW>
 __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
   using F = Format<kType>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -604,30 +596,26 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
     in = in + 1 == kDownRing ? 0 : in + 1;
     next(to);
   };
-  const auto hbuf = buffer(p.h, uint32_t(p.tokens) * p.top * p.inter * 2);
-  auto load_x = [&](u32x4 (&x)[kT][F::kUnits]) __attribute__((always_inline)) {  // returns the mask of the stage's tokens
+  const auto hbuf = buffer(p.h, uint32_t(p.tokens) * p.top * p.inter * 4);
+  auto load_x = [&](u32x4 (&x)[F::kUnits]) __attribute__((always_inline)) {  // returns the mask of the stage's tokens
     const i32x4 chosen = entry(x_at.u);
     const uint32_t mask = x_at.n < total ? uint32_t(chosen[2]) : 0u;
     const int k0 = x_at.s * F::kStage + q * (F::kStage / 4);
     const bool whole = (x_at.s + 1) * F::kStage <= p.inter;
+    // Column c: token c % 8, of the pairs the high half before column 8, then the low one.
+    const int token = c & 7;
+    const uint32_t row = uint32_t((chosen[1] + __popc(mask & ((1u << token) - 1))) * 2 + (c >> 3)) * uint32_t(p.inter) + k0;
+    const uint32_t from = mask >> token & 1 ? row * 2 : kPast;
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      const int token = 16 * t + c;
-      const uint32_t row = uint32_t(chosen[1] + __popc(mask & ((1u << token) - 1))) * uint32_t(p.inter) + k0;
-      const uint32_t from = mask >> token & 1 ? row * 2 : kPast;
-#pragma unroll
-      for (int n = 0; n < F::kUnits; ++n)
-        x[t][n] = __builtin_amdgcn_raw_buffer_load_b128(hbuf, whole || k0 + 8 * n < p.inter ? from + 16 * n : kPast, 0, 0);
-    }
+    for (int n = 0; n < F::kUnits; ++n)
+      x[n] = __builtin_amdgcn_raw_buffer_load_b128(hbuf, whole || k0 + 8 * n < p.inter ? from + 16 * n : kPast, 0, 0);
     next(x_at);
     return mask;
   };
-  f32x4 acc[kT];
-#pragma unroll
-  for (int t = 0; t < kT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto step = [&](const u32x4 (&x)[kT][F::kUnits], uint32_t mask, u32x4 (&ahead)[kT][F::kUnits]) __attribute__((always_inline)) {
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto step = [&](const u32x4 (&x)[F::kUnits], uint32_t mask, u32x4 (&ahead)[F::kUnits]) __attribute__((always_inline)) {
     // Behind the copies of this stage went those of kDownRing - 2 more, and as many stages of x.
-    wait_vm<(kDownRing - 2) * (F::kCopies + kT * F::kUnits)>();
+    wait_vm<(kDownRing - 2) * (F::kCopies + F::kUnits)>();
     const uint32_t mask_ahead = load_x(ahead);
     asm volatile("" ::: "memory");
     copy_next();
@@ -636,12 +624,12 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
       const int64_t block = int64_t(entry(at.u)[0]) * fp8::blocks_of(p.hidden) + column / fp8::kBlock;
       scale = sload(p.down_s8 + block * blocks, at.s);
     }
-    contract<kType, kT, true>(ring_at + out * F::kSlot, x, scale, mask, acc);
+    contract<kType, true>(ring_at + out * F::kSlot, x, scale, mask, acc);
     out = out + 1 == kDownRing ? 0 : out + 1;
     next(at);
     return mask_ahead;
   };
-  u32x4 x0[kT][F::kUnits], x1[kT][F::kUnits];
+  u32x4 x0[F::kUnits], x1[F::kUnits];
   if (wave < total) {
     // (x behind all copies but the last, as in every step: what the compiler waits for before x is the same then.)
     for (int n = 0; n < kDownRing - 2; ++n) copy_next();
@@ -649,23 +637,23 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
     uint32_t mask = load_x(x0);
     asm volatile("" ::: "memory");
     copy_next();
-    wait_vm<(kDownRing - 2) * F::kCopies + kT * F::kUnits>();  // (the first stage; the second has two of x behind it)
+    wait_vm<(kDownRing - 2) * F::kCopies + F::kUnits>();  // (the first stage; the second has two of x behind it)
     while (at.n < total) {
       mask = step(x0, mask, x1);
       if (at.n >= total) break;
       mask = step(x1, mask, x0);
     }
   }
-#pragma unroll
-  for (int t = 0; t < kT; ++t) lds_write16(red_at + (t * kW + wave) * 1024 + c * 64 + q * 16, acc[t]);
+  lds_write16(red_at + wave * 1024 + c * 64 + q * 16, acc);
   wait_vm<0>();
   lds_barrier();
-  for (int i = threadIdx.x; i < 256 * kT; i += 64 * kW) {
-    const int token = i >> 4, n = column + (i & 15);
-    if (token >= p.tokens || n >= p.hidden) continue;
-    const uint32_t from = red_at + (token >> 4) * kW * 1024 + (token & 15) * 64 + (i & 15) * 4;
-    float sum = lds_sum8(from);
-    if constexpr (kW == 16) sum += lds_sum8(from + 8 * 1024);
+  if (threadIdx.x < 16 * kMostTokens) {
+    const int token = threadIdx.x >> 4, n = column + (threadIdx.x & 15);
+    if (token >= p.tokens || n >= p.hidden) return;
+    const uint32_t high = red_at + threadIdx.x * 4, low = high + 16 * kMostTokens * 4;
+    float sum = lds_sum8(high), rest = lds_sum8(low);
+    if constexpr (kW == 16) sum += lds_sum8(high + 8 * 1024), rest += lds_sum8(low + 8 * 1024);
+    sum += rest;
     if (p.base) sum += bf16_to_f32(p.base[token * p.base_stride + n]);
     p.y[token * p.y_stride + n] = uint16_t(f32_to_bf16(sum));
   }
@@ -680,57 +668,124 @@ int launch(K kernel, unsigned grid, unsigned threads, unsigned lds, const MlpPar
   return kOk;
 }
 
-template <int kType, int kT, int kStages>
+template <int kType, int kStages>
 int launch_gate_up(const MlpParams& p, hipStream_t stream) {
-  using G = GateUp<kType, kT, kStages>;
-  return launch(gate_up_kernel<kType, kT, kStages>, G::kTwo ? 512 : 256, kThreads, G::kLds, p, stream);
+  using G = GateUp<kType, kStages>;
+  return launch(gate_up_kernel<kType, kStages>, G::kTwo ? 512 : 256, kThreads, G::kLds, p, stream);
 }
 
 // Registers of x: 32, 64 or (one workgroup a CU) all of 128.
-template <int kType, int kT>
+template <int kType>
 int launch_gate_up(const MlpParams& p, hipStream_t stream) {
   const int per_wave = int(((Format<kType>::row_bytes(p.hidden) + 127) / 128 + kWaves - 1) / kWaves);
-  constexpr int kAll = 32 / (kT * Format<kType>::kUnits);
+  constexpr int kAll = 32 / Format<kType>::kUnits;
   if constexpr (kAll >= 8)
-    if (per_wave <= kAll / 4) return launch_gate_up<kType, kT, kAll / 4>(p, stream);
-  if (per_wave <= kAll / 2) return launch_gate_up<kType, kT, kAll / 2>(p, stream);
-  return launch_gate_up<kType, kT, kAll>(p, stream);
-}
-
-template <int kType, int kT>
-int launch_both(const MlpParams& p, hipStream_t stream) {
-  if (const int rc = launch_gate_up<kType, kT>(p, stream)) return rc;
-  const unsigned grid = unsigned((p.hidden + 15) / 16);
-  // Few workgroups get twice the waves.
-  if (grid <= 160) return launch(down_kernel<kType, kT, 16>, grid, 1024, down_lds<kType, kT, 16>(), p, stream);
-  return launch(down_kernel<kType, kT, 8>, grid, 512, down_lds<kType, kT, 8>(), p, stream);
+    if (per_wave <= kAll / 4) return launch_gate_up<kType, kAll / 4>(p, stream);
+  if (per_wave <= kAll / 2) return launch_gate_up<kType, kAll / 2>(p, stream);
+  return launch_gate_up<kType, kAll>(p, stream);
 }
 
 template <int kType>
 int launch_type(const MlpParams& p, hipStream_t stream) {
-  if constexpr (kType != kMxfp4)
-    if (p.tokens > 16) return launch_both<kType, 2>(p, stream);
-  return launch_both<kType, 1>(p, stream);
+  if (const int rc = launch_gate_up<kType>(p, stream)) return rc;
+  const unsigned grid = unsigned((p.hidden + 15) / 16);
+  // Few workgroups get twice the waves.
+  if (grid <= 160) return launch(down_kernel<kType, 16>, grid, 1024, down_lds<kType, 16>(), p, stream);
+  return launch(down_kernel<kType, 8>, grid, 512, down_lds<kType, 8>(), p, stream);
 }
 
 int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// What the two kernels take.
+bool fused_fits(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
+  if (tokens > kMostTokens || experts > kMostExperts || top > kMostTop) return false;
+  if (type == LF_EXPERT_MXFP4 && (hidden % 128 || inter % 128)) return false;
+  // x of a wave's stages in 128 registers; an expert's weights within 31 bits.
+  return hidden <= 8192 && inter <= (int64_t(1) << 20) && (hidden + 16) * (inter + 16) * 2 < (int64_t(1) << 31);
+}
+
+// Parts of the workspace of a chain, each 16-byte aligned.
+struct ChainSpace {
+  int64_t weights, chosen, offsets, tokens, positions, scratch, h, rows, bytes;
+  ChainSpace(int64_t count, int32_t experts, int32_t top, int64_t hidden, int64_t inter) {
+    int64_t at = 0;
+    auto part = [&](int64_t size) { return at += padded16(size), at - padded16(size); };
+    const int64_t choices = count * top;
+    weights = part(choices * 4);
+    chosen = part(choices * 4);
+    offsets = part((experts + 1) * 4);
+    tokens = part(choices * 4);
+    positions = part(choices * 4);
+    scratch = part(lf_route_experts_workspace_size(count, experts));
+    h = part(choices * inter * 4);
+    rows = part(choices * hidden * 4);
+    bytes = at;
+  }
+};
+
+int launch_chain(const lf_expert_mlp_call& a, char* space, hipStream_t stream) {
+  const ChainSpace part(a.tokens, a.experts, a.top, a.hidden, a.inter);
+  const int64_t choices = a.tokens * a.top;
+  auto* weights = reinterpret_cast<float*>(space + part.weights);
+  auto* offsets = reinterpret_cast<int32_t*>(space + part.offsets);
+  auto* tokens = reinterpret_cast<int32_t*>(space + part.tokens);
+  auto* positions = reinterpret_cast<int32_t*>(space + part.positions);
+  if (const int rc = lf_route_experts(a.logits, a.fp32, a.tokens, a.experts, a.logits_stride, a.top, a.renormalize, weights,
+                                      reinterpret_cast<int32_t*>(space + part.chosen), offsets, tokens, positions,
+                                      space + part.scratch, part.h - part.scratch, stream))
+    return rc;
+  lf_expert_product g{};
+  g.x = a.x;
+  g.x_stride = a.x_stride;
+  g.x_rows = a.tokens;
+  g.w = a.gate_up;
+  g.offsets = offsets;
+  g.tokens = tokens;
+  g.y = reinterpret_cast<uint16_t*>(space + part.h);
+  g.k = a.hidden;
+  g.y_stride = a.inter;
+  g.rows = choices;
+  g.n = 2 * a.inter;
+  g.experts = a.experts;
+  g.swiglu = 1;
+  lf_expert_product d{};
+  d.x = g.y;
+  d.x_stride = a.inter;
+  d.x_rows = d.rows = 2 * choices;
+  d.w = a.down;
+  d.offsets = offsets;
+  d.y = reinterpret_cast<uint16_t*>(space + part.rows);
+  d.y_stride = d.n = a.hidden;
+  d.k = a.inter;
+  d.experts = a.experts;
+  if (a.type == LF_EXPERT_FP8) {
+    g.w_fp8_scales = static_cast<const float*>(a.gate_up_scales);
+    d.w_fp8_scales = static_cast<const float*>(a.down_scales);
+  } else {
+    g.w_scales = static_cast<const uint8_t*>(a.gate_up_scales);
+    d.w_scales = static_cast<const uint8_t*>(a.down_scales);
+  }
+  if (const int rc = launch_pairs(g, kSplit, stream)) return rc;
+  if (const int rc = launch_pairs(d, kJoin, stream)) return rc;
+  return combine_f32(reinterpret_cast<const float*>(space + part.rows), choices, positions, weights, a.tokens, a.top, a.hidden,
+                     a.base, a.base_stride, a.y, a.y_stride, stream);
+}
 
 }  // namespace
 }  // namespace expert
 }  // namespace lf
 
-// Bytes of workspace, or -1 where the two kernels cannot take the sizes.
+// Bytes of workspace, or -1 for what this entry point does not take.
 extern "C" int64_t lf_expert_mlp_workspace_size(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
   using namespace lf::expert;
-  if (tokens < 1 || tokens > (type == LF_EXPERT_MXFP4 ? 16 : kMostTokens) || experts < 1 || experts > kMostExperts || top < 1 || top > kMostTop || top > experts ||
-      tokens * top > kMostChoices || type < LF_EXPERT_BF16 || type > LF_EXPERT_FP8)
+  if (type < LF_EXPERT_BF16 || type > LF_EXPERT_FP8 || tokens < 1 || experts < 1 || experts > 1024 || top < 1 || top > 64 || top > experts)
     return -1;
-  const int64_t unit = type == LF_EXPERT_BF16 ? 8 : type == LF_EXPERT_FP8 ? 16 : 128;
+  const int64_t unit = type == LF_EXPERT_BF16 ? 8 : type == LF_EXPERT_FP8 ? 16 : 32;
   if (hidden < 1 || inter < 1 || hidden % unit || inter % unit || (type == LF_EXPERT_FP8 && inter % lf::fp8::kBlock)) return -1;
-  // x of a wave's stages in 128 registers; an expert's weights within 31 bits.
-  if (hidden > (tokens <= 16 ? 8192 : 4096) || inter > (int64_t(1) << 20) || (hidden + 16) * (inter + 16) * 2 >= (int64_t(1) << 31))
-    return -1;
-  return padded16(tokens * top * inter * 2) + 16 * (1 + kMostChoices);
+  if (hidden >= (int64_t(1) << 24) || inter >= (int64_t(1) << 24)) return -1;
+  if (fused_fits(tokens, experts, top, hidden, inter, type)) return padded16(tokens * top * inter * 4) + 16 * (1 + kMostChoices);
+  if (tokens > kMostEach * int64_t(experts) / top) return -1;
+  return ChainSpace(tokens, experts, top, hidden, inter).bytes;
 }
 
 extern "C" int lf_expert_mlp(const lf_expert_mlp_call* a, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -748,6 +803,9 @@ extern "C" int lf_expert_mlp(const lf_expert_mlp_call* a, void* workspace, int64
              "scales must be 4-byte aligned");
   LF_REQUIRE(a->logits_stride >= a->experts, "the row stride must cover the experts");
   LF_REQUIRE(a->y_stride >= a->hidden && (!a->base || a->base_stride >= a->hidden), "row strides must cover the columns");
+  auto s = static_cast<hipStream_t>(stream);
+  if (!lf::expert::fused_fits(a->tokens, a->experts, a->top, a->hidden, a->inter, a->type))
+    return lf::expert::launch_chain(*a, static_cast<char*>(workspace), s);
   lf::expert::MlpParams p{};
   p.x = static_cast<const char*>(a->x);
   p.x_row = a->x_stride * 2;
@@ -774,8 +832,7 @@ extern "C" int lf_expert_mlp(const lf_expert_mlp_call* a, void* workspace, int64
   p.y = a->y;
   p.y_stride = a->y_stride;
   p.h = static_cast<uint16_t*>(workspace);
-  p.table = reinterpret_cast<int4*>(static_cast<char*>(workspace) + lf::expert::padded16(a->tokens * a->top * a->inter * 2));
-  auto s = static_cast<hipStream_t>(stream);
+  p.table = reinterpret_cast<int4*>(static_cast<char*>(workspace) + lf::expert::padded16(a->tokens * a->top * a->inter * 4));
   switch (a->type) {
     case LF_EXPERT_BF16: return lf::expert::launch_type<lf::expert::kBf16>(p, s);
     case LF_EXPERT_MXFP4: return lf::expert::launch_type<lf::expert::kMxfp4>(p, s);

@@ -9,9 +9,18 @@
 
 #include "fp8.h"
 #include "mxfp4.h"
+#include "../../include/loraforge_amd.h"
 
 namespace lf {
 namespace expert {
+
+// Rows held as pairs: a value of 32 bits as the sum of two of bf16 (17 bits or more of it), so that a product's
+// result keeps them into the next one. Row r of such an x is rows 2 r and 2 r + 1, two rows of the product.
+enum Pair : int {
+  kSingle,  // y bf16
+  kSplit,   // y: bf16 pairs, rows 2 r and 2 r + 1 of y
+  kJoin,    // x: pairs (`rows` and `x_rows` count both), y: fp32, one row for each pair
+};
 
 // Types of an operand.
 enum Type : int { kBf16, kMxfp4, kFp8 };
@@ -33,6 +42,7 @@ struct Params {
   int width;   // output columns: n, or n / 2 with SwiGLU
   int y_vec;   // rows of y are 16-byte aligned
   int swiglu;  // w rows [gate | up]: y = silu(gate) * up
+  int pair;    // Pair
 };
 
 // Zeros that lanes past the end of k load instead of what follows the row.
@@ -45,8 +55,9 @@ struct Segment {
 // Bounds of expert e's rows.
 __device__ __forceinline__ Segment segment_of(const Params& p, int e) {
   if (!p.offsets) return {0, 0, p.rows};
-  const int begin = min(max(p.offsets[e], 0), p.rows);
-  return {e, begin, min(max(p.offsets[e + 1], begin), p.rows)};
+  const int twice = p.pair == kJoin ? 1 : 0;
+  const int begin = min(max(p.offsets[e] << twice, 0), p.rows);
+  return {e, begin, min(max(p.offsets[e + 1] << twice, begin), p.rows)};
 }
 
 // Searches the experts in order, 64 at a time, for the one that holds item
@@ -99,6 +110,13 @@ __device__ __forceinline__ float silu_mul_f32(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
+// A value as a pair: the nearest bf16, and the nearest to what that leaves (nothing where it is not finite).
+__device__ __forceinline__ void split_pair(float v, uint16_t& high, uint16_t& low) {
+  high = uint16_t(f32_to_bf16(v));
+  const float rest = v - bf16_to_f32(high);
+  low = (high & 0x7f80u) == 0x7f80u ? uint16_t(0) : uint16_t(f32_to_bf16(rest));
+}
+
 // `part`: rows per workgroup (16, 32 or 64); `groups`: 16-row groups of weight rows (1 or 2).
 int launch_stream(const Params& p, int part, int groups, hipStream_t stream);
 int launch_rows(const Params& p, hipStream_t stream);
@@ -108,6 +126,11 @@ int launch_tiles_mxw(const Params& p, int cap, int columns, hipStream_t stream);
 int launch_tiles_mx(const Params& p, int cap, int columns, hipStream_t stream);
 int launch_tiles_fp8(const Params& p, int cap, int columns, hipStream_t stream);  // (fp8_tile.h: both operands FP8)
 int launch_tiles_w8(const Params& p, int cap, int columns, hipStream_t stream);   // bf16 x, FP8 weights
+// A product that leaves or takes pairs (expert_linear.hip).
+int launch_pairs(const lf_expert_product& a, Pair pair, hipStream_t stream);
+// lf_combine_experts of contiguous fp32 rows (expert_routing.hip).
+int combine_f32(const float* rows, int64_t num_rows, const int32_t* positions, const float* weights, int64_t tokens, int32_t top,
+                int64_t n, const uint16_t* base, int64_t base_stride, uint16_t* y, int64_t y_stride, hipStream_t stream);
 
 }  // namespace expert
 }  // namespace lf

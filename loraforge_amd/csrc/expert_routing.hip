@@ -16,7 +16,10 @@
 // workgroup; 8191 tokens 5.5 us to choose and 5.8 to order (with a wave for each token
 // in turn, and places by counting choices wave by wave, 11.2 and 13.0). The sum is
 // HBM-bound: 8191 tokens of 8 rows of 4096 take 119 us (5.1 TB/s, a copy's rate).
+#include <type_traits>
+
 #include "expert_choose.h"
+#include "expert_params.h"
 #include "../../include/loraforge_amd.h"
 
 namespace lf {
@@ -226,7 +229,7 @@ void launch_route(const RouteParams& p, hipStream_t s) {
 constexpr int kCombineThreads = 256;
 
 struct CombineParams {
-  const uint16_t* rows;
+  const void* rows;  // bf16, or fp32
   int64_t rows_stride, num_rows;
   const int32_t* positions;
   const float* weights;
@@ -240,7 +243,7 @@ struct CombineParams {
 };
 
 // Eight columns per thread (16-byte accesses), or one.
-template <int kVec>
+template <class Row, int kVec>
 __global__ __launch_bounds__(kCombineThreads) void combine_kernel(CombineParams p) {
   const int64_t chunks = p.n / kVec, total = p.tokens * chunks;
   for (int64_t i = int64_t(blockIdx.x) * kCombineThreads + threadIdx.x; i < total; i += int64_t(gridDim.x) * kCombineThreads) {
@@ -248,8 +251,11 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(CombineParams 
     float sum[kVec];
 #pragma unroll
     for (int k = 0; k < kVec; ++k) sum[k] = 0.0f;
-    auto add = [&](const uint16_t* src, float w) {
-      if constexpr (kVec == 8) {
+    auto add = [&](const auto* src, float w) {
+      if constexpr (std::is_same_v<decltype(src), const float*>) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) sum[k] = fmaf(w, src[k], sum[k]);
+      } else if constexpr (kVec == 8) {
         const uint4 v = *reinterpret_cast<const uint4*>(src);
         const uint32_t word[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -264,7 +270,7 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(CombineParams 
     if (p.base) add(p.base + t * p.base_stride + c, 1.0f);
     for (int j = 0; j < p.top; ++j) {
       const int64_t row = p.positions[t * p.top + j];
-      if (row >= 0 && row < p.num_rows) add(p.rows + row * p.rows_stride + c, p.weights[t * p.top + j]);
+      if (row >= 0 && row < p.num_rows) add(static_cast<const Row*>(p.rows) + row * p.rows_stride + c, p.weights[t * p.top + j]);
     }
     uint16_t* dst = p.y + t * p.y_stride + c;
     if constexpr (kVec == 8)
@@ -275,7 +281,33 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(CombineParams 
   }
 }
 
+template <class Row>
+int launch_combine(const Row* rows, int64_t num_rows, int64_t rows_stride, const int32_t* positions, const float* weights,
+                   int64_t tokens, int32_t top, int64_t n, const uint16_t* base, int64_t base_stride, uint16_t* y,
+                   int64_t y_stride, hipStream_t s) {
+  const bool vec = n % 8 == 0 && rows_stride % 8 == 0 && y_stride % 8 == 0 && aligned16(rows) && aligned16(y) &&
+                   (!base || (base_stride % 8 == 0 && aligned16(base)));
+  const CombineParams p{rows, rows_stride, num_rows, positions, weights, base, base_stride, y, y_stride, tokens, top, n};
+  const int64_t want = (tokens * (vec ? n / 8 : n) + kCombineThreads - 1) / kCombineThreads;
+  const dim3 grid(unsigned(want < 65536 ? want : 65536)), threads(kCombineThreads);
+  if (vec)
+    hipLaunchKernelGGL((combine_kernel<Row, 8>), grid, threads, 0, s, p);
+  else
+    hipLaunchKernelGGL((combine_kernel<Row, 1>), grid, threads, 0, s, p);
+  LF_HIP(hipGetLastError());
+  return kOk;
+}
+
 }  // namespace
+
+namespace expert {
+
+int combine_f32(const float* rows, int64_t num_rows, const int32_t* positions, const float* weights, int64_t tokens, int32_t top,
+                int64_t n, const uint16_t* base, int64_t base_stride, uint16_t* y, int64_t y_stride, hipStream_t stream) {
+  return launch_combine(rows, num_rows, n, positions, weights, tokens, top, n, base, base_stride, y, y_stride, stream);
+}
+
+}  // namespace expert
 }  // namespace lf
 
 extern "C" int64_t lf_route_experts_workspace_size(int64_t tokens, int32_t experts) {
@@ -321,16 +353,6 @@ extern "C" int lf_combine_experts(const uint16_t* rows, int64_t num_rows, int64_
   if (tokens == 0) return lf::kOk;
   LF_REQUIRE(positions && weights && y && (rows || num_rows == 0), "null pointer argument");
   LF_REQUIRE(rows_stride >= n && y_stride >= n && (!base || base_stride >= n), "row strides must cover n columns");
-  const bool vec = n % 8 == 0 && rows_stride % 8 == 0 && y_stride % 8 == 0 && lf::aligned16(rows) && lf::aligned16(y) &&
-                   (!base || (base_stride % 8 == 0 && lf::aligned16(base)));
-  lf::CombineParams p{rows, rows_stride, num_rows, positions, weights, base, base_stride, y, y_stride, tokens, top, n};
-  const int64_t want = (tokens * (vec ? n / 8 : n) + lf::kCombineThreads - 1) / lf::kCombineThreads;
-  const dim3 grid(unsigned(want < 65536 ? want : 65536)), threads(lf::kCombineThreads);
-  auto s = static_cast<hipStream_t>(stream);
-  if (vec)
-    hipLaunchKernelGGL(lf::combine_kernel<8>, grid, threads, 0, s, p);
-  else
-    hipLaunchKernelGGL(lf::combine_kernel<1>, grid, threads, 0, s, p);
-  LF_HIP(hipGetLastError());
-  return lf::kOk;
+  return lf::launch_combine(rows, num_rows, rows_stride, positions, weights, tokens, top, n, base, base_stride, y, y_stride,
+                            static_cast<hipStream_t>(stream));
 }

@@ -250,6 +250,23 @@ struct Rows {
     // Copies for stages past the end are on their way, and other waves still read x.
     wait_vm<0>();
     barrier_only();
+    if (p.pair != kSingle) {
+      if (p.pair == kJoin)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] += __shfl_xor(out[e], 1, 64);
+      if (c >= count || (p.swiglu && q >= 2) || (p.pair == kJoin && (c & 1))) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (column + e >= p.width) continue;
+        if (p.pair == kJoin) {
+          reinterpret_cast<float*>(p.y)[int64_t((first + c) >> 1) * p.y_stride + column + e] = out[e];
+        } else {
+          uint16_t* y = p.y + int64_t(first + c) * 2 * p.y_stride + column + e;
+          split_pair(out[e], y[0], y[p.y_stride]);
+        }
+      }
+      return;
+    }
     if (c >= count || (p.swiglu && q >= 2)) return;
     uint16_t* y = p.y + int64_t(first + c) * p.y_stride + column;
     if (p.y_vec && column + 4 <= p.width) {

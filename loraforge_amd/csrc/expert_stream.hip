@@ -196,8 +196,17 @@ __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg,
     const int r = (i & (columns - 1)), row = (i >> shift) / kF;
     const int n = block * columns + r;
     if (first + row >= seg.end || n >= p.width) continue;
+    if (p.pair == kJoin) {  // (a pair's rows are in one pass)
+      if (!(row & 1)) reinterpret_cast<float*>(p.y)[int64_t((first + row) >> 1) * p.y_stride + n] = total(r, row) + total(r, row + 1);
+      continue;
+    }
     const float v = p.swiglu ? silu_mul_f32(total(r, row), total(r + 8 * kF, row)) : total(r, row);
-    p.y[int64_t(first + row) * p.y_stride + n] = uint16_t(f32_to_bf16(v));
+    if (p.pair == kSplit) {
+      uint16_t* y = p.y + int64_t(first + row) * 2 * p.y_stride + n;
+      split_pair(v, y[0], y[p.y_stride]);
+    } else {
+      p.y[int64_t(first + row) * p.y_stride + n] = uint16_t(f32_to_bf16(v));
+    }
   }
 }
 

@@ -121,14 +121,13 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
     }
   }
   const bool vec = p.y_vec && col + 8 <= p.width;
-  const bool all_vec = __ballot(!vec) == 0;
+  const bool all_vec = p.pair == kSingle && __ballot(!vec) == 0;
   // Eight output columns of staged row r.
-  auto output = [&](int r) {
+  auto values = [&](int r, float (&out)[8]) {
     const f32x4* v = reinterpret_cast<const f32x4*>(mine + r * kRowBytes + local * 4);
     const f32x4 half[2] = {v[0], v[1]};
     f32x4 up[2];
     if (kSwiglu) up[0] = v[4], up[1] = v[5];
-    uint32_t o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float a = half[e >> 1][(e & 1) * 2] + add[2 * e], b = half[e >> 1][(e & 1) * 2 + 1] + add[2 * e + 1];
@@ -136,9 +135,14 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
         a = silu_mul_f32(a, up[e >> 1][(e & 1) * 2] + add_up[2 * e]);
         b = silu_mul_f32(b, up[e >> 1][(e & 1) * 2 + 1] + add_up[2 * e + 1]);
       }
-      o[e] = pack_bf16x2(a, b);
+      out[2 * e] = a;
+      out[2 * e + 1] = b;
     }
-    return u32x4{o[0], o[1], o[2], o[3]};
+  };
+  auto output = [&](int r) {
+    float v[8];
+    values(r, v);
+    return u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
   };
 #pragma unroll
   for (int pair = 0; pair < (kI + 1) / 2; ++pair) {
@@ -171,12 +175,39 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
     } else {
 #pragma unroll 1
       for (int r = in_row; r < staged; r += kRows) {
-        const u32x4 o = output(r);
-        uint16_t* y = p.y + int64_t(first + place(r)) * p.y_stride + col;
-        if (place(r) >= count || idle) continue;
+        const int64_t row = first + place(r);
+        if (place(r) >= count || idle || (p.pair == kJoin && (r & 1))) continue;
+        float v[8];
+        values(r, v);
+        if (p.pair == kJoin) {  // (a pair's rows are in one tile, one behind the other)
+          float low[8];
+          values(r + 1, low);
+          float* y = reinterpret_cast<float*>(p.y) + (row >> 1) * p.y_stride + col;
+          if (vec) {
+            reinterpret_cast<f32x4*>(y)[0] = f32x4{v[0] + low[0], v[1] + low[1], v[2] + low[2], v[3] + low[3]};
+            reinterpret_cast<f32x4*>(y)[1] = f32x4{v[4] + low[4], v[5] + low[5], v[6] + low[6], v[7] + low[7]};
+          } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (col + e < p.width) y[e] = uint16_t(o[e >> 1] >> (16 * (e & 1)));
+            for (int e = 0; e < 8; ++e)
+              if (col + e < p.width) y[e] = v[e] + low[e];
+          }
+          continue;
+        }
+        uint16_t high[8], low[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split_pair(v[e], high[e], low[e]);
+        uint16_t* y = p.y + (p.pair == kSplit ? 2 * row : row) * p.y_stride + col;
+        if (vec && p.pair == kSplit) {
+          *reinterpret_cast<u32x4*>(y) = __builtin_bit_cast(u32x4, high);
+          *reinterpret_cast<u32x4*>(y + p.y_stride) = __builtin_bit_cast(u32x4, low);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e < p.width) {
+              y[e] = high[e];
+              if (p.pair == kSplit) y[p.y_stride + e] = low[e];
+            }
+        }
       }
     }
   }

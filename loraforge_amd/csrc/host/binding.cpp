@@ -1002,7 +1002,7 @@ struct ExpertsArg {
 };
 
 // mlp(x, logits, gate_up, down, top_k, renormalize, base or None, out or None) -> out or None: the sizes of
-// expert_mlp that two launches take. (The checks and the call through ctypes take 34 us on the host, this 8.5.)
+// expert_mlp that the library takes in one call. (The checks and the call through ctypes take 34 us on the host, this 8.5.)
 PyObject* mlp(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 8 || (args[5] != Py_True && args[5] != Py_False)) return decline();
   ExpertsArg gate_up, down;

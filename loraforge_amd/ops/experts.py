@@ -184,6 +184,8 @@ def expert_mlp(x, logits, gate_up, down, top_k: int, *, renormalize: bool = True
     ``down`` ``[E, H, I]``, each bf16, an ``MXFP4Tensor`` or an ``FP8Tensor`` (a scale for
     each 128 x 128 block); ``base`` bf16 ``[T, H]`` (a shared expert's output or the residual).
     ``out`` may be ``base``. A token that may choose no expert is left with ``base`` (or zeros).
+    fp32 sums, rounded once to bf16; what lies between the products is held in 16 bits of mantissa where an expert
+    has 32 choices or fewer on average, in bf16 above.
     """
     import torch
 
@@ -248,7 +250,7 @@ def expert_mlp(x, logits, gate_up, down, top_k: int, *, renormalize: bool = True
 
 
 def _expert_mlp(x, logits, gate_up, down, top_k, renormalize, base, out) -> bool:
-    """The MLP of a few tokens in two launches; False where those do not take it."""
+    """The MLP of a few tokens in one call of the library; False where it does not take it."""
     import torch
 
     (count, hidden), (experts, _, inter) = x.shape, down.shape
