@@ -109,3 +109,107 @@ def test_c_product_refusals(change, match):
     for name, value in change.items():
         setattr(a, name, value)
     refused(match, _lib.library().lf_expert_linear(ctypes.byref(a), None))
+
+
+# --------------------------------------------------------------------------
+# The whole expert MLP
+# --------------------------------------------------------------------------
+
+
+def mlp(**change):
+    """A call that holds together but for ``change``; refused before any pointer is followed."""
+    call = dict(x=16, x_stride=256, logits=16, logits_stride=8, tokens=4, hidden=256, inter=128, experts=8, top=2, type=_lib.LF_EXPERT_BF16,
+                gate_up=16, down=16, y=16, y_stride=256)
+    workspace, size = change.pop("workspace", 16), change.pop("size", None)
+    a = _lib.ExpertMlp(**{**call, **change})
+    if size is None:
+        size = 1 << 30
+    return _lib.library().lf_expert_mlp(ctypes.byref(a), ctypes.c_void_p(workspace), size, None)
+
+
+@pytest.mark.parametrize(
+    "change,match",
+    [
+        (dict(tokens=0), "as routing, products and sum"),
+        (dict(tokens=129), "as routing, products and sum"),  # 258 choices of 8 experts
+        (dict(tokens=2**62), "as routing, products and sum"),
+        (dict(experts=1025, logits_stride=1025), "as routing, products and sum"),
+        (dict(top=9), "as routing, products and sum"),
+        (dict(top=0), "as routing, products and sum"),
+        (dict(experts=200, top=65, logits_stride=200), "as routing, products and sum"),
+        (dict(hidden=260, x_stride=264, y_stride=260), "as routing, products and sum"),
+        (dict(inter=100), "as routing, products and sum"),
+        (dict(inter=192, type=_lib.LF_EXPERT_FP8), "as routing, products and sum"),
+        (dict(hidden=272, type=_lib.LF_EXPERT_MXFP4), "as routing, products and sum"),
+        (dict(type=3), "as routing, products and sum"),
+        (dict(type=-1), "as routing, products and sum"),
+        (dict(workspace=None), "workspace of"),
+        (dict(size=64), "workspace of"),
+        (dict(workspace=24), "16-byte"),
+        (dict(x=None), "null"),
+        (dict(logits=None), "null"),
+        (dict(gate_up=None), "null"),
+        (dict(down=None), "null"),
+        (dict(y=None), "null"),
+        (dict(type=_lib.LF_EXPERT_FP8), "need scales"),
+        (dict(type=_lib.LF_EXPERT_MXFP4, gate_up_scales=16), "need scales"),
+        (dict(gate_up_scales=16, down_scales=16), "need scales"),
+        (dict(type=_lib.LF_EXPERT_MXFP4, gate_up_scales=17, down_scales=16), "4-byte"),
+        (dict(x=8), "16-byte"),
+        (dict(x_stride=260), "16-byte"),
+        (dict(x_stride=248), "16-byte"),
+        (dict(gate_up=24), "16-byte"),
+        (dict(down=8), "16-byte"),
+        (dict(logits_stride=7), "row stride"),
+        (dict(y_stride=255), "row strides"),
+        (dict(base=16, base_stride=255), "row strides"),
+    ],
+)
+def test_c_expert_mlp_refusals(change, match):
+    refused(match, mlp(**change))
+
+
+def test_c_expert_mlp_null_call():
+    refused("null", _lib.library().lf_expert_mlp(None, ctypes.c_void_p(16), 64, None))
+
+
+def test_expert_mlp_workspace():
+    size = _lib.library().lf_expert_mlp_workspace_size
+    bf16, mx, f8 = _lib.LF_EXPERT_BF16, _lib.LF_EXPERT_MXFP4, _lib.LF_EXPERT_FP8
+    # Two launches: pairs of the intermediate and a table. Four: also the routing and rows of fp32.
+    for kind in (bf16, mx, f8):
+        assert 8 * 4 * 256 * 4 <= size(8, 64, 4, 512, 256, kind) < 8 * 4 * 256 * 4 + 4096
+        assert size(9, 64, 4, 512, 256, kind) >= 9 * 4 * (256 + 512) * 4
+        assert size(512, 64, 4, 512, 256, kind) > 0 > size(513, 64, 4, 512, 256, kind)
+        assert size(1, 1024, 64, 512, 256, kind) > 0
+        assert size(1, 64, 4, 2**24, 256, kind) == size(1, 64, 4, 512, 2**24, kind) == -1
+    assert size(1, 64, 4, 520, 264, bf16) > 0 > size(1, 64, 4, 516, 264, bf16)
+    assert size(1, 64, 4, 528, 256, f8) > 0 > size(1, 64, 4, 520, 256, f8)
+    assert size(1, 64, 4, 544, 288, mx) > 0 > size(1, 64, 4, 528, 256, mx)
+
+
+def test_fp8_plans():
+    """Few rows stream the weights, many run in tiles of a height that leaves registers for a block's products."""
+    def plan(**sizes):
+        a = _lib.ExpertProduct(**{**dict(x=16, w=16, y=16, w_fp8_scales=16, x_stride=4096, x_rows=64, rows=64, n=4096, k=4096, experts=1), **sizes})
+        p = _lib.ExpertPlan()
+        _lib.check(_lib.library().lf_expert_linear_plan(ctypes.byref(a), ctypes.byref(p)))
+        return p
+
+    for types in ({}, dict(x_fp8_scales=16)):
+        for rows in (1, 8, 16):
+            assert plan(rows=rows, x_rows=rows, **types).kernel != _lib.LF_EXPERT_TILE
+        for rows in (300, 1024, 4096, 8192):
+            for n, k in ((4096, 4096), (11008, 4096), (12288, 4096), (1024, 8192)):
+                p = plan(rows=rows, x_rows=rows, n=n, k=k, **types)
+                assert p.kernel == _lib.LF_EXPERT_TILE
+                assert p.rows <= ((192 if p.columns == 256 else 256) if types else (128 if p.columns == 256 else 192))
+        assert plan(rows=32, x_rows=32, experts=128, offsets=16, **types).kernel != _lib.LF_EXPERT_TILE
+        # Offsets of 31 bits in tiles: above, the weights are streamed.
+        assert plan(rows=4096, x_rows=2**20, **types).kernel == _lib.LF_EXPERT_STREAM or not types
+    assert plan(rows=4096, x_rows=2**19, x_fp8_scales=16).kernel != _lib.LF_EXPERT_TILE
+    a = _lib.ExpertProduct(x=16, w=16, w_fp8_scales=16, y=16, x_stride=64, x_rows=2, rows=2, n=32, k=64, experts=1, y_stride=32)
+    for rows, columns, x_scales in ((256, 64, None), (192, 256, None), (256, 256, 16)):
+        a.x_fp8_scales = x_scales
+        a.plan = ctypes.pointer(_lib.ExpertPlan(_lib.LF_EXPERT_TILE, rows, columns))
+        refused("at most", _lib.library().lf_expert_linear(ctypes.byref(a), None))
