@@ -242,6 +242,30 @@ struct CombineParams {
   int64_t n;
 };
 
+// What is read in place of a row that is none.
+__device__ const u32x4 kNothing[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+
+template <int kVec>
+__device__ __forceinline__ void load_row(const uint16_t* src, float (&v)[kVec]) {
+  if constexpr (kVec == 8) {
+    const u32x4 word = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[2 * k] = bf16_lo(word[k]), v[2 * k + 1] = bf16_hi(word[k]);
+  } else {
+    v[0] = bf16_to_f32(*src);
+  }
+}
+template <int kVec>
+__device__ __forceinline__ void load_row(const float* src, float (&v)[kVec]) {
+  if constexpr (kVec == 8) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(src)[0], b = reinterpret_cast<const f32x4*>(src)[1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = a[k], v[4 + k] = b[k];
+  } else {
+    v[0] = *src;
+  }
+}
+
 // Eight columns per thread (16-byte accesses), or one.
 template <class Row, int kVec>
 __global__ __launch_bounds__(kCombineThreads) void combine_kernel(CombineParams p) {
@@ -251,26 +275,32 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(CombineParams 
     float sum[kVec];
 #pragma unroll
     for (int k = 0; k < kVec; ++k) sum[k] = 0.0f;
-    auto add = [&](const auto* src, float w) {
-      if constexpr (std::is_same_v<decltype(src), const float*>) {
+    // (Rows are asked for four at a time: one behind the other, their latency was most of a few tokens' time.)
+    constexpr int kTogether = 4;
+    if (p.base) {
+      float v[kVec];
+      load_row<kVec>(p.base + t * p.base_stride + c, v);
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) sum[k] = fmaf(w, src[k], sum[k]);
-      } else if constexpr (kVec == 8) {
-        const uint4 v = *reinterpret_cast<const uint4*>(src);
-        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+      for (int k = 0; k < kVec; ++k) sum[k] += v[k];
+    }
+    for (int j0 = 0; j0 < p.top; j0 += kTogether) {
+      float v[kTogether][kVec], w[kTogether];
+      bool in[kTogether];
+      int64_t row[kTogether];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          sum[2 * k] = fmaf(w, bf16_lo(word[k]), sum[2 * k]);
-          sum[2 * k + 1] = fmaf(w, bf16_hi(word[k]), sum[2 * k + 1]);
-        }
-      } else {
-        sum[0] = fmaf(w, bf16_to_f32(*src), sum[0]);
+      for (int i = 0; i < kTogether; ++i) {
+        const int64_t at = t * p.top + min(j0 + i, p.top - 1);
+        row[i] = p.positions[at];
+        w[i] = p.weights[at];
+        in[i] = j0 + i < p.top && row[i] >= 0 && row[i] < p.num_rows;
       }
-    };
-    if (p.base) add(p.base + t * p.base_stride + c, 1.0f);
-    for (int j = 0; j < p.top; ++j) {
-      const int64_t row = p.positions[t * p.top + j];
-      if (row >= 0 && row < p.num_rows) add(static_cast<const Row*>(p.rows) + row * p.rows_stride + c, p.weights[t * p.top + j]);
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i)
+        load_row<kVec>(in[i] ? static_cast<const Row*>(p.rows) + row[i] * p.rows_stride + c : reinterpret_cast<const Row*>(&kNothing), v[i]);
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i)
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) sum[k] = in[i] ? fmaf(w[i], v[i][k], sum[k]) : sum[k];
     }
     uint16_t* dst = p.y + t * p.y_stride + c;
     if constexpr (kVec == 8)
