@@ -250,31 +250,35 @@ struct Rows {
     // Copies for stages past the end are on their way, and other waves still read x.
     wait_vm<0>();
     barrier_only();
-    if (p.pair != kSingle) {
-      if (p.pair == kJoin)
+    if (p.pair == kJoin) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] += __shfl_xor(out[e], 1, 64);
-      if (c >= count || (p.swiglu && q >= 2) || (p.pair == kJoin && (c & 1))) return;
+      for (int e = 0; e < 4; ++e) out[e] += __shfl_xor(out[e], 1, 64);
+      if (c >= count || (c & 1)) return;
+      float* y = reinterpret_cast<float*>(p.y) + int64_t((first + c) >> 1) * p.y_stride + column;
+      if (p.y_vec && column + 4 <= p.width) {
+        *reinterpret_cast<f32x4*>(y) = f32x4{out[0], out[1], out[2], out[3]};
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (column + e >= p.width) continue;
-        if (p.pair == kJoin) {
-          reinterpret_cast<float*>(p.y)[int64_t((first + c) >> 1) * p.y_stride + column + e] = out[e];
-        } else {
-          uint16_t* y = p.y + int64_t(first + c) * 2 * p.y_stride + column + e;
-          split_pair(out[e], y[0], y[p.y_stride]);
-        }
+        for (int e = 0; e < 4; ++e)
+          if (column + e < p.width) y[e] = out[e];
       }
       return;
     }
     if (c >= count || (p.swiglu && q >= 2)) return;
-    uint16_t* y = p.y + int64_t(first + c) * p.y_stride + column;
+    uint16_t high[4], low[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split_pair(out[e], high[e], low[e]);
+    uint16_t* y = p.y + int64_t(first + c) * (p.pair == kSplit ? 2 : 1) * p.y_stride + column;
     if (p.y_vec && column + 4 <= p.width) {
-      *reinterpret_cast<u32x2*>(y) = u32x2{pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3])};
+      *reinterpret_cast<u32x2*>(y) = __builtin_bit_cast(u32x2, high);
+      if (p.pair == kSplit) *reinterpret_cast<u32x2*>(y + p.y_stride) = __builtin_bit_cast(u32x2, low);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (column + e < p.width) y[e] = uint16_t(f32_to_bf16(out[e]));
+        if (column + e < p.width) {
+          y[e] = high[e];
+          if (p.pair == kSplit) y[p.y_stride + e] = low[e];
+        }
     }
   }
 };
