@@ -228,17 +228,6 @@ struct Routing {
   float weight[kMostChoices];
 };
 
-// Inclusive sums over the lanes of a wave: within rows of 16 lanes, then the rows' totals.
-__device__ __forceinline__ int scan_lanes(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
-  return v;
-}
-
 // The tables, from masks that a barrier has passed. Each wave writes them for itself (all the same), so that it needs
 // no barrier to read what it wrote.
 __device__ __forceinline__ void tabulate(Routing& r) {

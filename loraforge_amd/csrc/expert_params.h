@@ -60,6 +60,17 @@ __device__ __forceinline__ Segment segment_of(const Params& p, int e) {
   return {e, begin, min(max(p.offsets[e + 1] << twice, begin), p.rows)};
 }
 
+// Inclusive sums over the lanes of a wave: within rows of 16 lanes, then the rows' totals.
+__device__ __forceinline__ int scan_lanes(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
+  return v;
+}
+
 // Searches the experts in order, 64 at a time, for the one that holds item
 // `index`, where expert e has count(segment) items; `index` becomes the item's
 // number within it. Uniform; an index past the last item finds an empty segment.
@@ -71,12 +82,7 @@ __device__ __forceinline__ Segment find_segment(const Params& p, int& index, Cou
     Segment s{0, 0, 0};
     if (base + lane < p.experts) s = segment_of(p, base + lane);
     const int mine = count(s);
-    int sum = mine;  // inclusive sums over the lanes
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += up;
-    }
+    const int sum = scan_lanes(mine);
     const uint64_t past = __ballot(sum > index);
     if (past) {
       const int at = __builtin_ctzll(past);
