@@ -46,7 +46,7 @@ HIP_FLAGS = [
 # issue loads the compiler does not track (waited for explicitly), and a
 # register spill of such a result would store it before the load returned. (In the
 # expert tiles a spill in the loop would wait for every copy in flight.)
-NO_SCRATCH = {"expert_mlp.hip", "nf4_gemv.hip", "nf4_decode_wide.hip", "row_ops.hip"} | {
+NO_SCRATCH = {"expert_mlp.hip", "expert_stream.hip", "expert_rows.hip", "nf4_gemv.hip", "nf4_decode_wide.hip", "row_ops.hip"} | {
     f"nf4_prefill_rows_{part}.hip" for part in "abcd"} | {f"expert_tile_{types}.hip" for types in ("bf16", "mxw", "mx")} | {
     f"fp8_tile_{types}.hip" for types in ("fp8", "w8")}
 

@@ -210,6 +210,11 @@ __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg,
   }
 }
 
+// Rows of a pass. (32 weight rows in FP8 beside 64 rows, whose products of a step are summed apart from the sums so far, take
+// more than the 128 registers of a wave: passes of 32 then.)
+template <int kW, int kF>
+constexpr int kMostRows = kW == kFp8 && kF == 2 ? 32 : 64;
+
 // Grid: column blocks x passes of `part` rows (16, 32 or 64) of the experts (y, then z).
 // (A loop over passes in the kernel takes its registers past 128, into scratch.)
 template <int kX, int kW, int kF>
@@ -225,13 +230,14 @@ __global__ __launch_bounds__(kThreads, 4) void stream_kernel(Params p, int part)
     stream_rows<kX, kW, kF, 1>(p, seg, seg.begin, blockIdx.x, red);
   } else if (rows <= 32) {
     stream_rows<kX, kW, kF, 2>(p, seg, seg.begin, blockIdx.x, red);
-  } else {
+  } else if constexpr (kMostRows<kW, kF> > 32) {
     stream_rows<kX, kW, kF, 4>(p, seg, seg.begin, blockIdx.x, red);
   }
 }
 
 template <int kX, int kW>
 int launch_types(const Params& p, int part, int groups, hipStream_t stream) {
+  if (groups == 2 && part > kMostRows<kW, 2>) part = kMostRows<kW, 2>;
   // At most: a pass more than whole ones for every expert that has a row.
   const int64_t used = p.offsets ? (p.experts < p.rows ? p.experts : p.rows) : 1;
   const int64_t passes = (p.rows + used * (part - 1)) / part;
