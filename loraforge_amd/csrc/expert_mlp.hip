@@ -3,7 +3,11 @@
 //
 // Bound by HBM: every weight of a chosen expert is read once; beside it, launches, routing and
 // joins are latency. Four operators in a chain (route, product, product, combine) take
-// four launches for it.
+// four launches for it. In a graph, us beside the chain's (128 experts, top 8, 4096 x 1024): one token MXFP4 19.5 (29; the
+// bytes 10.4 at a copy's rate), FP8 24.8 (32; 19.6), bf16 37 (46; 39); 8 tokens 74 (82; 67), 127 (129; 125), 223 (250; 250).
+// The first launch reads at 5.6 TB/s once it is under way (FP8, 7 tokens: 193 MB in 35 us), the second at 4.2 (98 MB in
+// 23). Of one token's 19.5 us the first launch is 10.3 (routing 4, until weights that it asked for come 7),
+// the second 7.5 (2 until weights come, 1.5 for the join).
 //
 // First launch. Every workgroup routes all tokens by itself (as expert_routing.hip does: the
 // logits come from L2, and nobody waits for another workgroup), x in registers meanwhile.
@@ -39,7 +43,7 @@ namespace {
 constexpr int kWaves = 8;            // of the first launch
 constexpr int kThreads = 64 * kWaves;
 // Eight tokens: with the halves of their pairs 16 columns of the second launch. (A second tile for up to 16 takes the address
-// unit twice as long for x as for the weights: 128 experts, top 8, 4096 x 1024, MXFP4, 12 tokens 111 us, in a chain 107.)
+// unit twice as long for x as for the weights: 128 experts, top 8, 4096 x 1024, MXFP4, 12 tokens 111 us, in a chain 100.)
 constexpr int kMostTokens = 8;
 // Choices of an expert, on average, up to which a chain keeps pairs: they double the rows of the down product, which costs
 // little while its weights' bytes bound it (16 experts, top 4, 4096 x 2048, 64 tokens, 16 choices each: MXFP4 76 us and 68 with
@@ -678,8 +682,11 @@ template <int kType>
 int launch_type(const MlpParams& p, hipStream_t stream) {
   if (const int rc = launch_gate_up<kType>(p, stream)) return rc;
   const unsigned grid = unsigned((p.hidden + 15) / 16);
-  // Few workgroups get twice the waves.
-  if (grid <= 160) return launch(down_kernel<kType, 16>, grid, 1024, down_lds<kType, 16>(), p, stream);
+  // Few workgroups get twice the waves: 64 experts, top 4, 2048 x 1024, 8 tokens FP8 39.6 us with them and 43.7 without, bf16
+  // 69.2 and 71.0; 32 experts, 1024 x 2048, FP8 48.6 and 54.0, bf16 70.3 and 77.9. (Not of MXFP4 weights, whose bytes are few: a
+  // token 13.8 and 13.1, eight tokens 30.9 and 31.4.)
+  if constexpr (kType != kMxfp4)
+    if (grid <= 160) return launch(down_kernel<kType, 16>, grid, 1024, down_lds<kType, 16>(), p, stream);
   return launch(down_kernel<kType, 8>, grid, 512, down_lds<kType, 8>(), p, stream);
 }
 

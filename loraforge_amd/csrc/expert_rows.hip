@@ -16,7 +16,10 @@
 // too, its form without scales where both are FP8; the weight is the A operand, up to 16 rows of x the
 // B operand. Lane quarter q takes units (of 16 bytes) 2 q and 2 q + 1 of a stage, so its two MXFP4 scales are
 // neighbours. A stage of FP8 weights is 128 k, one block of scales: its products are summed from zero and added
-// times x's scale (copied with x's chunks) and the weights' (uniform loads, a stage ahead).
+// times x's scale (copied with x's chunks) and the weights' (uniform loads, a stage ahead). The down products of 64 tokens over
+// 128 experts, top 8, 4096 x 1024, with x in pairs: MXFP4 68 us (267 MB, 3.9 TB/s: four stages to a workgroup). (Workgroups
+// that run two to eight blocks of 128 rows, ring and x running on from one to the next: 4 to 8 % less for 12 tokens, as much
+// more for 16 experts, none for 64 tokens.)
 #include "expert_params.h"
 #include "lds_pipeline.h"
 

