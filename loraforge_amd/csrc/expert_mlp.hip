@@ -138,13 +138,13 @@ __device__ __forceinline__ float lds_sum8(uint32_t at) {
   float v[8];
   asm volatile(
       "ds_read_b32 %0, %8\n\t"
-      "ds_read_b32 %1, %8 offset:1024\n\t"
-      "ds_read_b32 %2, %8 offset:2048\n\t"
-      "ds_read_b32 %3, %8 offset:3072\n\t"
-      "ds_read_b32 %4, %8 offset:4096\n\t"
-      "ds_read_b32 %5, %8 offset:5120\n\t"
-      "ds_read_b32 %6, %8 offset:6144\n\t"
-      "ds_read_b32 %7, %8 offset:7168\n\t"
+      "ds_read_b32 %1, %8 offset:0x400\n\t"
+      "ds_read_b32 %2, %8 offset:0x800\n\t"
+      "ds_read_b32 %3, %8 offset:0xc00\n\t"
+      "ds_read_b32 %4, %8 offset:0x1000\n\t"
+      "ds_read_b32 %5, %8 offset:0x1400\n\t"
+      "ds_read_b32 %6, %8 offset:0x1800\n\t"
+      "ds_read_b32 %7, %8 offset:0x1c00\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
       : "v"(at)
