@@ -17,7 +17,7 @@ namespace {
 bool tiles_fit(const lf_expert_product& a) {
   if (a.w_fp8_scales) {  // offsets below 2^31
     const int64_t x_row = a.x_fp8_scales ? a.k : a.x_stride * 2;
-    return a.x_rows * std::max(x_row, a.k) < (int64_t(1) << 31) && (a.n + 512) * a.k < (int64_t(1) << 31);
+    return a.x_rows < (int64_t(1) << 31) / std::max(x_row, a.k) && (a.n + 512) * a.k < (int64_t(1) << 31);
   }
   if (a.x_scales) return a.k >= 512 && std::max(a.x_rows, a.n) * (a.k / 2) < (int64_t(1) << 32);
   return !a.w_scales || a.k >= 128;

@@ -802,6 +802,8 @@ extern "C" int lf_expert_mlp(const lf_expert_mlp_call* a, void* workspace, int64
   auto s = static_cast<hipStream_t>(stream);
   if (!lf::expert::fused_fits(a->tokens, a->experts, a->top, a->hidden, a->inter, a->type))
     return lf::expert::launch_chain(*a, static_cast<char*>(workspace), s);
+  LF_REQUIRE(a->tokens == 1 || a->x_stride < ((int64_t(1) << 30) - a->hidden) / (a->tokens - 1),
+             "x rows of up to 8 tokens must lie within 2 GiB");
   lf::expert::MlpParams p{};
   p.x = static_cast<const char*>(a->x);
   p.x_row = a->x_stride * 2;

@@ -261,6 +261,8 @@ def _expert_mlp(x, logits, gate_up, down, top_k, renormalize, base, out) -> bool
     parts = _parts(gate_up), _parts(down)
     if size < 0 or any(t.data_ptr() % 4 for part in parts for t in part[1:]):
         return False
+    if 1 < count <= 8 and x.stride(0) >= (2**30 - hidden) // (count - 1):  # (32-bit offsets)
+        return False
     a = _lib.ExpertMlp()
     a.x, a.logits, a.y = x.data_ptr(), logits.data_ptr(), out.data_ptr()
     a.x_stride, a.logits_stride, a.y_stride = (t.stride(0) if count > 1 else t.shape[1] for t in (x, logits, out))

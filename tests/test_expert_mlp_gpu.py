@@ -204,6 +204,64 @@ def test_keeps_16_bits_between_the_products(kind, tokens, experts, device):
     assert off <= 2.0**-9
 
 
+@pytest.mark.parametrize("tokens", [8, 9])
+def test_rows_of_x_far_apart(tokens, device):
+    """The last rows of long sequences: 2 GiB and more between the first and the last."""
+    x, logits, gate_up, down = case("bf16", tokens, 8, 256, 128, device)
+    apart = torch.empty(tokens, 2**27 + 2**25, dtype=torch.bfloat16, device=device)
+    far = apart[:, 64:320]
+    far.copy_(x)
+    assert torch.equal(expert_mlp(far[:2], logits[:2], gate_up, down, 2), expert_mlp(x[:2], logits[:2], gate_up, down, 2))
+    close(expert_mlp(far, logits, gate_up, down, 2), expected(x, logits, gate_up, down, 2))
+
+
+@pytest.mark.parametrize("tokens", [3, 20])
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_weights_past_32_bits(kind, tokens, device):
+    """Experts whose weights lie past 4 GiB: as in a tensor of those experts alone."""
+    experts, hidden, inter = 80, 4096, 8192
+    x, _, gate_up, down = case(kind, tokens, 2, hidden, inter, device)
+
+    def spread(w):
+        t = w if kind == "bf16" else w.codes
+        big = torch.zeros(experts, *t.shape[1:], dtype=t.dtype, device=device)
+        raw, part = (big, t) if kind == "bf16" else (big.view(torch.uint8), t.view(torch.uint8))
+        raw[0], raw[experts - 1] = part[0], part[1]
+        if kind == "bf16":
+            return big
+        scales = torch.zeros(experts, *w.scales.shape[1:], device=device)
+        scales[0], scales[experts - 1] = w.scales[0], w.scales[1]
+        return FP8Tensor(big, scales)
+
+    few = torch.randn(tokens, 2, device=device)
+    logits = torch.full((tokens, experts), -np.inf, device=device)
+    logits[:, 0], logits[:, experts - 1] = few[:, 0], few[:, 1]
+    y, alone = expert_mlp(x, logits, spread(gate_up), spread(down), 2), expert_mlp(x, few, gate_up, down, 2)
+    if tokens <= 8:
+        assert torch.equal(y, alone)
+        return
+    # (Of 80 experts the products may run in another kernel, whose sums have another order: the formula and the
+    # bound of ``expected``, on the GPU in 64 bits.)
+    def sums(a, w):
+        return a @ w.T, (2.0 * a.shape[1] + 16.0) * 2.0**-24 * (a.abs() @ w.abs().T)
+
+    share = few.double().softmax(1)
+    want = torch.zeros(tokens, hidden, dtype=torch.float64, device=device)
+    bound = torch.zeros_like(want)
+    for e in range(2):
+        gu, dn = (torch.from_numpy(values(w[e : e + 1] if kind == "bf16" else FP8Tensor(w.codes[e : e + 1], w.scales[e : e + 1]))[0]).to(device)
+                  for w in (gate_up, down))
+        (g, u), (dg, du) = (t.chunk(2, 1) for t in sums(x.double(), gu))
+        act = g / (1.0 + (-g).exp())
+        h = act * u
+        h_bound = 1.1 * dg * (u.abs() + du) + (act.abs() + 1.1 * dg) * du + 2.0**-21 * h.abs()
+        term, term_bound = sums(h, dn)
+        want += share[:, e : e + 1] * term
+        bound += share[:, e : e + 1] * (term_bound + ((2.0**-16 + 2.0**-20) * h.abs() + h_bound) @ dn.abs().T + 2.0**-21 * term.abs())
+    for got in (y, alone):
+        close(got, (want.cpu().numpy(), bound.cpu().numpy()))
+
+
 def test_no_tokens(device):
     x, logits, gate_up, down = case("bf16", 2, 4, 128, 128, device)
     assert expert_mlp(x[:0], logits[:0], gate_up, down, 2).shape == (0, 128)

@@ -162,6 +162,8 @@ def mlp(**change):
         (dict(down=8), "16-byte"),
         (dict(logits_stride=7), "row stride"),
         (dict(y_stride=255), "row strides"),
+        (dict(x_stride=2**29), "within 2 GiB"),
+        (dict(x_stride=2**62), "within 2 GiB"),
         (dict(base=16, base_stride=255), "row strides"),
     ],
 )
