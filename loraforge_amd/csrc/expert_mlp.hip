@@ -28,7 +28,8 @@
 // stage's expert reads zeros (past the end of a buffer).
 //
 // More tokens, and widths that these do not take: routing, gate and up product, down product and sum one after
-// another, in the kernels of the operators, with pairs between the products and rows of fp32 before the sum.
+// another, in the kernels of the operators, with pairs between the products and rows of fp32 before the sum; up to 16 tokens with
+// the first launch in place of the first two.
 #include <type_traits>
 
 #include "expert_choose.h"
@@ -45,6 +46,10 @@ constexpr int kThreads = 64 * kWaves;
 // Eight tokens: with the halves of their pairs 16 columns of the second launch. (A second tile for up to 16 takes the address
 // unit twice as long for x as for the weights: 128 experts, top 8, 4096 x 1024, MXFP4, 12 tokens 111 us, in a chain 100.)
 constexpr int kMostTokens = 8;
+// What the first launch takes, one tile of x, also ahead of the operators' down product and sum, in place of the routing and the
+// gate and up product: 16 tokens over 32 experts, top 4, 2048 x 1408, bf16 95 us and 118; 128 experts, top 8, 4096 x 1024, 12 tokens MXFP4
+// 98.6 and 99.5, FP8 155 and 161, bf16 287 and 312; 8 experts, top 2, 8192 x 1024, 16 tokens MXFP4 35.8 and 40.4 (bf16 82.8 and 80.2).
+constexpr int kMostFirst = 16;
 // Choices of an expert, on average, up to which a chain keeps pairs: they double the rows of the down product, which costs
 // little while its weights' bytes bound it (16 experts, top 4, 4096 x 2048, 64 tokens, 16 choices each: MXFP4 76 us and 68 with
 // the intermediate in bf16, FP8 105 and 104, bf16 205 and 202; 128 tokens 97 and 85, 123 and 108, 215 and 207; 512 tokens 237
@@ -53,7 +58,7 @@ constexpr int kMostEach = 32;
 constexpr int kFewTokens = 2;        // routed by ranks
 constexpr int kMostExperts = 256;
 constexpr int kMostTop = 16;
-constexpr int kMostChoices = kMostTokens * kMostTop;
+constexpr int kMostChoices = kMostFirst * kMostTop;
 constexpr int kSlotWeights = 16 * 128;
 constexpr uint32_t kPast = 0x80000000u;  // past the end of every buffer here
 
@@ -73,6 +78,9 @@ struct MlpParams {
   int64_t y_stride;
   uint16_t* h;   // [tokens * top, 2, inter], rows in expert order, halves of pairs
   int4* table;   // x of entry 0: chosen experts; entry 1 + u: expert, first row, mask of its tokens
+  // Ahead of the operators (else null): what lf_route_experts gives, and h without weights.
+  int32_t *offsets, *positions;
+  float* weights;
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -356,7 +364,18 @@ __device__ __forceinline__ void route_many(const MlpParams& p, Routing& r) {
   if (live) atomicOr(&r.mask[c.expert], 1u << t);
   __syncthreads();
   tabulate(r);
-  if (live) keep_weight(r, t, c.expert, c.weight);
+  if (live) keep_weight(r, t, c.expert, p.positions ? 1.0f : c.weight);
+  if (p.positions && blockIdx.x == 0) {
+    if (t < p.tokens && j < p.top) {
+      p.positions[t * p.top + j] = live ? r.first[c.expert] + __popc(r.mask[c.expert] & ((1u << t) - 1)) : -1;
+      p.weights[t * p.top + j] = live ? c.weight : 0.0f;
+    }
+    if (threadIdx.x < kMostExperts) {
+      const int e = threadIdx.x, first = r.first[e], end = first + __popc(r.mask[e]);
+      if (e < p.experts) p.offsets[e] = first;
+      if (e == p.experts - 1) p.offsets[e + 1] = end;
+    }
+  }
 }
 
 __device__ __forceinline__ void route(const MlpParams& p, Routing& r) {
@@ -421,7 +440,7 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) v
   }
 
   const int used = __builtin_amdgcn_readfirstlane(routing.used);
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == 0 && p.table) {
     if (threadIdx.x == 0) p.table[0] = make_int4(used, 0, 0, 0);
     if (int(threadIdx.x) < used) p.table[1 + threadIdx.x] = routing.chosen[threadIdx.x];
   }
@@ -524,7 +543,7 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) v
     const uint32_t red = red_at + turn * (G::kRed / 2);
     lds_write16(red + wave * 1024 + c * 64 + q * 16, acc);
     lds_barrier();
-    if (threadIdx.x < 8 * kMostTokens) {
+    if (threadIdx.x < 8 * kMostFirst) {
       const int token = threadIdx.x >> 3, r = threadIdx.x & 7;
       const uint32_t from = red + token * 64 + r * 4;
       const uint32_t mask = lds_word(chosen_at + u * 16 + 8);
@@ -679,8 +698,7 @@ int launch_gate_up(const MlpParams& p, hipStream_t stream) {
 }
 
 template <int kType>
-int launch_type(const MlpParams& p, hipStream_t stream) {
-  if (const int rc = launch_gate_up<kType>(p, stream)) return rc;
+int launch_down(const MlpParams& p, hipStream_t stream) {
   const unsigned grid = unsigned((p.hidden + 15) / 16);
   // Few workgroups get twice the waves: 64 experts, top 4, 2048 x 1024, 8 tokens FP8 39.6 us with them and 43.7 without, bf16
   // 69.2 and 71.0; 32 experts, 1024 x 2048, FP8 48.6 and 54.0, bf16 70.3 and 77.9. (Not of MXFP4 weights, whose bytes are few: a
@@ -692,12 +710,56 @@ int launch_type(const MlpParams& p, hipStream_t stream) {
 
 int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
 
-// What the two kernels take.
-bool fused_fits(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
-  if (tokens > kMostTokens || experts > kMostExperts || top > kMostTop) return false;
+// What the first kernel takes, and (up to kMostTokens) the second.
+bool first_fits(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
+  if (tokens > kMostFirst || experts > kMostExperts || top > kMostTop) return false;
   if (type == LF_EXPERT_MXFP4 && (hidden % 128 || inter % 128)) return false;
   // x of a wave's stages in 128 registers; an expert's weights within 31 bits.
   return hidden <= 8192 && inter <= (int64_t(1) << 20) && (hidden + 16) * (inter + 16) * 2 < (int64_t(1) << 31);
+}
+
+bool fused_fits(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
+  return tokens <= kMostTokens && first_fits(tokens, experts, top, hidden, inter, type);
+}
+
+// (32-bit offsets of x in the first kernel.)
+bool x_within(const lf_expert_mlp_call& a) {
+  return a.tokens == 1 || a.x_stride < ((int64_t(1) << 30) - a.hidden) / (a.tokens - 1);
+}
+
+MlpParams params_of(const lf_expert_mlp_call& a) {
+  MlpParams p{};
+  p.x = static_cast<const char*>(a.x);
+  p.x_row = a.x_stride * 2;
+  p.logits = a.logits;
+  p.logits_stride = a.logits_stride;
+  p.fp32 = a.fp32 ? 1 : 0;
+  p.tokens = int32_t(a.tokens);
+  p.experts = a.experts;
+  p.top = a.top;
+  p.renormalize = a.renormalize ? 1 : 0;
+  p.hidden = int32_t(a.hidden);
+  p.inter = int32_t(a.inter);
+  p.gate_up = static_cast<const char*>(a.gate_up);
+  p.down = static_cast<const char*>(a.down);
+  if (a.type == LF_EXPERT_FP8) {
+    p.gate_up_s8 = static_cast<const float*>(a.gate_up_scales);
+    p.down_s8 = static_cast<const float*>(a.down_scales);
+  } else {
+    p.gate_up_s = static_cast<const uint8_t*>(a.gate_up_scales);
+    p.down_s = static_cast<const uint8_t*>(a.down_scales);
+  }
+  p.base = a.base;
+  p.base_stride = a.base_stride;
+  p.y = a.y;
+  p.y_stride = a.y_stride;
+  return p;
+}
+
+int launch_first(const MlpParams& p, int32_t type, hipStream_t stream) {
+  return type == LF_EXPERT_BF16    ? launch_gate_up<kBf16>(p, stream)
+         : type == LF_EXPERT_MXFP4 ? launch_gate_up<kMxfp4>(p, stream)
+                                   : launch_gate_up<kFp8>(p, stream);
 }
 
 // Parts of the workspace of a chain, each 16-byte aligned.
@@ -726,26 +788,40 @@ int launch_chain(const lf_expert_mlp_call& a, char* space, hipStream_t stream) {
   auto* offsets = reinterpret_cast<int32_t*>(space + part.offsets);
   auto* tokens = reinterpret_cast<int32_t*>(space + part.tokens);
   auto* positions = reinterpret_cast<int32_t*>(space + part.positions);
-  if (const int rc = lf_route_experts(a.logits, a.fp32, a.tokens, a.experts, a.logits_stride, a.top, a.renormalize, weights,
-                                      reinterpret_cast<int32_t*>(space + part.chosen), offsets, tokens, positions,
-                                      space + part.scratch, part.h - part.scratch, stream))
-    return rc;
-  lf_expert_product g{};
-  g.x = a.x;
-  g.x_stride = a.x_stride;
-  g.x_rows = a.tokens;
-  g.w = a.gate_up;
-  g.offsets = offsets;
-  g.tokens = tokens;
-  g.y = reinterpret_cast<uint16_t*>(space + part.h);
-  g.k = a.hidden;
-  g.y_stride = a.inter;
-  g.rows = choices;
-  g.n = 2 * a.inter;
-  g.experts = a.experts;
-  g.swiglu = 1;
+  auto* h = reinterpret_cast<uint16_t*>(space + part.h);
+  // The first kernel, or routing and product: see kMostFirst.
+  if (first_fits(a.tokens, a.experts, a.top, a.hidden, a.inter, a.type) && x_within(a)) {
+    MlpParams p = params_of(a);
+    p.h = h;
+    p.offsets = offsets;
+    p.positions = positions;
+    p.weights = weights;
+    if (const int rc = launch_first(p, a.type, stream)) return rc;
+  } else {
+    if (const int rc = lf_route_experts(a.logits, a.fp32, a.tokens, a.experts, a.logits_stride, a.top, a.renormalize, weights,
+                                        reinterpret_cast<int32_t*>(space + part.chosen), offsets, tokens, positions,
+                                        space + part.scratch, part.h - part.scratch, stream))
+      return rc;
+    lf_expert_product g{};
+    g.x = a.x;
+    g.x_stride = a.x_stride;
+    g.x_rows = a.tokens;
+    g.w = a.gate_up;
+    g.offsets = offsets;
+    g.tokens = tokens;
+    g.y = h;
+    g.k = a.hidden;
+    g.y_stride = a.inter;
+    g.rows = choices;
+    g.n = 2 * a.inter;
+    g.experts = a.experts;
+    g.swiglu = 1;
+    if (a.type == LF_EXPERT_FP8) g.w_fp8_scales = static_cast<const float*>(a.gate_up_scales);
+    else g.w_scales = static_cast<const uint8_t*>(a.gate_up_scales);
+    if (const int rc = launch_pairs(g, kSplit, stream)) return rc;
+  }
   lf_expert_product d{};
-  d.x = g.y;
+  d.x = h;
   d.x_stride = a.inter;
   d.x_rows = d.rows = 2 * choices;
   d.w = a.down;
@@ -754,14 +830,8 @@ int launch_chain(const lf_expert_mlp_call& a, char* space, hipStream_t stream) {
   d.y_stride = d.n = a.hidden;
   d.k = a.inter;
   d.experts = a.experts;
-  if (a.type == LF_EXPERT_FP8) {
-    g.w_fp8_scales = static_cast<const float*>(a.gate_up_scales);
-    d.w_fp8_scales = static_cast<const float*>(a.down_scales);
-  } else {
-    g.w_scales = static_cast<const uint8_t*>(a.gate_up_scales);
-    d.w_scales = static_cast<const uint8_t*>(a.down_scales);
-  }
-  if (const int rc = launch_pairs(g, kSplit, stream)) return rc;
+  if (a.type == LF_EXPERT_FP8) d.w_fp8_scales = static_cast<const float*>(a.down_scales);
+  else d.w_scales = static_cast<const uint8_t*>(a.down_scales);
   if (const int rc = launch_pairs(d, kJoin, stream)) return rc;
   return combine_f32(reinterpret_cast<const float*>(space + part.rows), choices, positions, weights, a.tokens, a.top, a.hidden,
                      a.base, a.base_stride, a.y, a.y_stride, stream);
@@ -802,38 +872,14 @@ extern "C" int lf_expert_mlp(const lf_expert_mlp_call* a, void* workspace, int64
   auto s = static_cast<hipStream_t>(stream);
   if (!lf::expert::fused_fits(a->tokens, a->experts, a->top, a->hidden, a->inter, a->type))
     return lf::expert::launch_chain(*a, static_cast<char*>(workspace), s);
-  LF_REQUIRE(a->tokens == 1 || a->x_stride < ((int64_t(1) << 30) - a->hidden) / (a->tokens - 1),
-             "x rows of up to 8 tokens must lie within 2 GiB");
-  lf::expert::MlpParams p{};
-  p.x = static_cast<const char*>(a->x);
-  p.x_row = a->x_stride * 2;
-  p.logits = a->logits;
-  p.logits_stride = a->logits_stride;
-  p.fp32 = a->fp32 ? 1 : 0;
-  p.tokens = int32_t(a->tokens);
-  p.experts = a->experts;
-  p.top = a->top;
-  p.renormalize = a->renormalize ? 1 : 0;
-  p.hidden = int32_t(a->hidden);
-  p.inter = int32_t(a->inter);
-  p.gate_up = static_cast<const char*>(a->gate_up);
-  p.down = static_cast<const char*>(a->down);
-  if (a->type == LF_EXPERT_FP8) {
-    p.gate_up_s8 = static_cast<const float*>(a->gate_up_scales);
-    p.down_s8 = static_cast<const float*>(a->down_scales);
-  } else {
-    p.gate_up_s = static_cast<const uint8_t*>(a->gate_up_scales);
-    p.down_s = static_cast<const uint8_t*>(a->down_scales);
-  }
-  p.base = a->base;
-  p.base_stride = a->base_stride;
-  p.y = a->y;
-  p.y_stride = a->y_stride;
+  LF_REQUIRE(lf::expert::x_within(*a), "x rows of up to 8 tokens must lie within 2 GiB");
+  lf::expert::MlpParams p = lf::expert::params_of(*a);
   p.h = static_cast<uint16_t*>(workspace);
   p.table = reinterpret_cast<int4*>(static_cast<char*>(workspace) + lf::expert::padded16(a->tokens * a->top * a->inter * 4));
+  if (const int rc = lf::expert::launch_first(p, a->type, s)) return rc;
   switch (a->type) {
-    case LF_EXPERT_BF16: return lf::expert::launch_type<lf::expert::kBf16>(p, s);
-    case LF_EXPERT_MXFP4: return lf::expert::launch_type<lf::expert::kMxfp4>(p, s);
-    default: return lf::expert::launch_type<lf::expert::kFp8>(p, s);
+    case LF_EXPERT_BF16: return lf::expert::launch_down<lf::expert::kBf16>(p, s);
+    case LF_EXPERT_MXFP4: return lf::expert::launch_down<lf::expert::kMxfp4>(p, s);
+    default: return lf::expert::launch_down<lf::expert::kFp8>(p, s);
   }
 }
