@@ -15,7 +15,7 @@
 // Its eight waves share k (stage s of 128 bytes of a row to wave s % 8), each streaming its weights through a
 // ring of its own in LDS by direct copies; the ring runs on from one item to the next. The weight is
 // the A operand of 16 x 16 matrix instructions, *all* tokens are the B operand (of x, held
-// in registers: at most 128 of them, which bounds k): columns of tokens
+// in registers: at most 128 of them, which bounds tokens and k): columns of tokens
 // that did not choose the expert are computed and dropped, which costs nothing beside the bytes.
 // The waves' sums meet in LDS, in a fixed order; the intermediate s silu(g) u, with the routing weight
 // in it so that the second product needs no weights, is kept as a pair of bf16 (rounded to one, it is as far
@@ -28,7 +28,7 @@
 // stage's expert reads zeros (past the end of a buffer).
 //
 // More tokens, and widths that these do not take: routing, gate and up product, down product and sum one after
-// another, in the kernels of the operators, with pairs between the products and rows of fp32 before the sum; up to 16 tokens with
+// another, in the kernels of the operators, with pairs between the products and rows of fp32 before the sum; up to 32 tokens with
 // the first launch in place of the first two.
 #include <type_traits>
 
@@ -46,10 +46,13 @@ constexpr int kThreads = 64 * kWaves;
 // Eight tokens: with the halves of their pairs 16 columns of the second launch. (A second tile for up to 16 takes the address
 // unit twice as long for x as for the weights: 128 experts, top 8, 4096 x 1024, MXFP4, 12 tokens 111 us, in a chain 100.)
 constexpr int kMostTokens = 8;
-// What the first launch takes, one tile of x, also ahead of the operators' down product and sum, in place of the routing and the
-// gate and up product: 16 tokens over 32 experts, top 4, 2048 x 1408, bf16 95 us and 118; 128 experts, top 8, 4096 x 1024, 12 tokens MXFP4
-// 98.6 and 99.5, FP8 155 and 161, bf16 287 and 312; 8 experts, top 2, 8192 x 1024, 16 tokens MXFP4 35.8 and 40.4 (bf16 82.8 and 80.2).
-constexpr int kMostFirst = 16;
+// What the first launch takes, two tiles of x, also ahead of the operators' down product and sum, in place of the routing and the
+// gate and up product: 16 tokens over 32 experts, top 4, 2048 x 1408, bf16 96 us and 117, 24 tokens 104 and 122; 128 experts, top 8,
+// 4096 x 1024, 12 tokens MXFP4 98.6 and 99.5, FP8 155 and 161, bf16 287 and 312, 24 tokens FP8 209 and 221, bf16 395 and 399; 8 experts,
+// top 2, 8192 x 1024, 16 tokens MXFP4 35.8 and 40.4 (bf16 82.8 and 80.2). Of MXFP4 weights one tile (levels made for two
+// cost more than the launch), of FP8 weights two only for a hidden width above 2048: below, an item is two stages or
+// fewer to a wave and its join weighs more (24 tokens over 60 experts, top 6, 1024 x 512, 34.8 us and 29.6; 2048 x 1408 59.4 and 56.9).
+constexpr int kMostFirst = 32;
 // Choices of an expert, on average, up to which a chain keeps pairs: they double the rows of the down product, which costs
 // little while its weights' bytes bound it (16 experts, top 4, 4096 x 2048, 64 tokens, 16 choices each: MXFP4 76 us and 68 with
 // the intermediate in bf16, FP8 105 and 104, bf16 205 and 202; 128 tokens 97 and 85, 123 and 108, 215 and 207; 512 tokens 237
@@ -58,7 +61,7 @@ constexpr int kMostEach = 32;
 constexpr int kFewTokens = 2;        // routed by ranks
 constexpr int kMostExperts = 256;
 constexpr int kMostTop = 16;
-constexpr int kMostChoices = kMostFirst * kMostTop;
+constexpr int kMostChoices = 256;
 constexpr int kSlotWeights = 16 * 128;
 constexpr uint32_t kPast = 0x80000000u;  // past the end of every buffer here
 
@@ -194,37 +197,41 @@ struct Copier {
   }
 };
 
-// One stage: 16 weight rows (in the slot) times 16 columns of x (units of a lane's quarter of the stage's k).
+// One stage: 16 weight rows (in the slot) times kT tiles of 16 columns of x (units of a lane's quarter of the stage's k).
 // `scale`: FP8, of the lane's weight rows. kMasked: only columns whose token (c % 8) is in `mask` take part in the stage, so that
 // what is not finite in an expert's weights (NaN times zero is NaN) reaches no other token.
-template <int kType, bool kMasked>
-__device__ __forceinline__ void contract(uint32_t slot, const u32x4 (&x)[Format<kType>::kUnits], float scale, uint32_t mask, f32x4& acc) {
+template <int kType, int kT, bool kMasked>
+__device__ __forceinline__ void contract(uint32_t slot, const u32x4 (&x)[kT][Format<kType>::kUnits], float scale, uint32_t mask, f32x4 (&acc)[kT]) {
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   u32x4 w[2];
   lds_two(w, slot + c * 128 + ((2 * q) ^ (c & 7)) * 16, slot + c * 128 + ((2 * q + 1) ^ (c & 7)) * 16);
   constexpr bool kApart = kMasked || kType == kFp8;  // a stage's products from zero
-  f32x4 sum = kApart ? f32x4{0.f, 0.f, 0.f, 0.f} : acc;
+  f32x4 sum[kT];
+#pragma unroll
+  for (int t = 0; t < kT; ++t) sum[t] = kApart ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[t];
+  auto multiply = [&](const u32x4& a, int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) sum[t] = lf::mfma16(vec_bf16x8(a), vec_bf16x8(x[t][j]), sum[t]);
+  };
   if constexpr (kType == kBf16) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) sum = lf::mfma16(vec_bf16x8(w[j]), vec_bf16x8(x[j]), sum);
+    for (int j = 0; j < 2; ++j) multiply(w[j], j);
   } else if constexpr (kType == kFp8) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      sum = lf::mfma16(vec_bf16x8(fp8::decode8(w[j >> 1][j % 2 * 2], w[j >> 1][j % 2 * 2 + 1])), vec_bf16x8(x[j]), sum);
+    for (int j = 0; j < 4; ++j) multiply(fp8::decode8(w[j >> 1][j % 2 * 2], w[j >> 1][j % 2 * 2 + 1]), j);
   } else {
     const uint32_t scales = lds_scales(slot + kSlotWeights + c * 8 + 2 * q);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float s = mx::scale_f32(j < 4 ? scales & 0xffu : scales >> 8);
-      sum = lf::mfma16(vec_bf16x8(mx::decode8(w[j >> 2][j & 3], s)), vec_bf16x8(x[j]), sum);
-    }
+    for (int j = 0; j < 8; ++j) multiply(mx::decode8(w[j >> 2][j & 3], mx::scale_f32(j < 4 ? scales & 0xffu : scales >> 8)), j);
   }
   const bool in = !kMasked || (mask >> (c & 7) & 1);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float v = kType == kFp8 ? fmaf(scale, sum[e], acc[e]) : kApart ? acc[e] + sum[e] : sum[e];
-    acc[e] = in ? v : acc[e];
-  }
+  for (int t = 0; t < kT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = kType == kFp8 ? fmaf(scale, sum[t][e], acc[t][e]) : kApart ? acc[t][e] + sum[t][e] : sum[t][e];
+      acc[t][e] = in ? v : acc[t][e];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -391,19 +398,19 @@ __device__ __forceinline__ void route(const MlpParams& p, Routing& r) {
 // ---------------------------------------------------------------------------
 // First launch: routing, gate and up products, SwiGLU.
 // ---------------------------------------------------------------------------
-template <int kType, int kStages>
+template <int kType, int kT, int kStages>
 struct GateUp {
   using F = Format<kType>;
-  static constexpr bool kTwo = kStages * F::kUnits <= 16;  // two workgroups on a CU: 64 registers of x
+  static constexpr bool kTwo = kT == 1 && kStages * F::kUnits <= 16;  // two workgroups on a CU: 64 registers of x
   static constexpr int kRing = kTwo ? 3 : 5;                    // stages
-  static constexpr int kRed = 2 * kWaves * 1024;
+  static constexpr int kRed = 2 * kT * kWaves * 1024;
   static constexpr int kLds = kWaves * kRing * F::kSlot + kRed;
 };
 
-template <int kType, int kStages>
-__global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) void gate_up_kernel(MlpParams p) {
+template <int kType, int kT, int kStages>
+__global__ __launch_bounds__(kThreads, (GateUp<kType, kT, kStages>::kTwo ? 4 : 2)) void gate_up_kernel(MlpParams p) {
   using F = Format<kType>;
-  using G = GateUp<kType, kStages>;
+  using G = GateUp<kType, kT, kStages>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Routing routing;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -412,12 +419,12 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) v
   const int mine = stages > wave ? (stages - wave + kWaves - 1) / kWaves : 0;  // stages wave, wave + 8, ...
 
   // x: unit n of a lane holds k 8 n .. of its quarter of the stage.
-  u32x4 x[kStages][F::kUnits];
+  u32x4 x[kStages][kT][F::kUnits];
   const auto xbuf = buffer(p.x, uint32_t((p.tokens - 1) * p.x_row + p.hidden * 2));
   // A few rows go through LDS (where the weights come later) while the tokens are routed: KiB by KiB, unit u of row t at
   // u ^ t. (A load of 16 rows takes the address unit as long for one row as for 16.)
   const int pieces = (p.hidden * 2 + 1023) / 1024, pitch = pieces * 1024;
-  const bool through_lds = p.tokens * pitch <= G::kLds;
+  const bool through_lds = kT == 1 && p.tokens * pitch <= G::kLds;
   if (through_lds)
     for (int t = 0; t < p.tokens; ++t)
       for (int piece = wave; piece < pieces; piece += kWaves) {
@@ -434,7 +441,7 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) v
 #pragma unroll
         for (int n = 0; n < F::kUnits; ++n) {
           const int unit = ((wave + kWaves * i) * F::kStage + q * (F::kStage / 4)) / 8 + n;
-          x[i][n] = *reinterpret_cast<const u32x4*>(lds + t * pitch + (unit ^ t) * 16);
+          x[i][0][n] = *reinterpret_cast<const u32x4*>(lds + t * pitch + (unit ^ t) * 16);
         }
     lds_barrier();
   }
@@ -498,16 +505,20 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) v
 #pragma unroll
     for (int i = 0; i < kStages; ++i)
 #pragma unroll
-      for (int n = 0; n < F::kUnits; ++n) {
-        const int k = (wave + kWaves * i) * F::kStage + (kType == kBf16 ? q * 16 + 8 * n : 32 * n + 8 * q);
-        const uint32_t from = c < p.tokens && k < p.hidden ? uint32_t(c * p.x_row) + k * 2 : kPast;
-        x[i][n] = __builtin_amdgcn_raw_buffer_load_b128(xbuf, from, 0, 0);
-      }
+      for (int t = 0; t < kT; ++t)
+#pragma unroll
+        for (int n = 0; n < F::kUnits; ++n) {
+          const int token = 16 * t + c, k = (wave + kWaves * i) * F::kStage + (kType == kBf16 ? q * 16 + 8 * n : 32 * n + 8 * q);
+          const uint32_t from = token < p.tokens && k < p.hidden ? uint32_t(token * p.x_row) + k * 2 : kPast;
+          x[i][t][n] = __builtin_amdgcn_raw_buffer_load_b128(xbuf, from, 0, 0);
+        }
     wait_vm<0>();  // (or the compiler would wait for x, and every copy, in the loop)
     if constexpr (kType != kBf16) {
       // ... and exchanged between the quarters: unit j of quarter q is load kUnits / 4 q + j / 4 of quarter j % 4.
 #pragma unroll
-      for (int i = 0; i < kStages; ++i) transpose_quarters<F::kUnits>(x[i]);
+      for (int i = 0; i < kStages; ++i)
+#pragma unroll
+        for (int t = 0; t < kT; ++t) transpose_quarters<F::kUnits>(x[i][t]);
     }
   }
 
@@ -523,7 +534,9 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) v
       up_s = p.gate_up_s8 + (first + (p.inter + column) / fp8::kBlock) * blocks;
       gs = sload(gate_s, min(wave, blocks - 1)), us = sload(up_s, min(wave, blocks - 1));
     }
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[kT];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
       if (i < mine) {
@@ -535,17 +548,18 @@ __global__ __launch_bounds__(kThreads, (GateUp<kType, kStages>::kTwo ? 4 : 2)) v
           const int ahead = min(wave + kWaves * (i + 1), blocks - 1);
           gs = sload(gate_s, ahead), us = sload(up_s, ahead);
         }
-        contract<kType, false>(ring_at + out * F::kSlot, x[i], scale, 0u, acc);
+        contract<kType, kT, false>(ring_at + out * F::kSlot, x[i], scale, 0u, acc);
         out = out + 1 == G::kRing ? 0 : out + 1;
       }
     }
-    // Sums as [turn][wave][token][row]; two places in turn, so one barrier an item.
+    // Sums as [turn][tile][wave][token][row]; two places in turn, so one barrier an item.
     const uint32_t red = red_at + turn * (G::kRed / 2);
-    lds_write16(red + wave * 1024 + c * 64 + q * 16, acc);
+#pragma unroll
+    for (int t = 0; t < kT; ++t) lds_write16(red + (t * kWaves + wave) * 1024 + c * 64 + q * 16, acc[t]);
     lds_barrier();
-    if (threadIdx.x < 8 * kMostFirst) {
+    if (threadIdx.x < 128 * kT) {
       const int token = threadIdx.x >> 3, r = threadIdx.x & 7;
-      const uint32_t from = red + token * 64 + r * 4;
+      const uint32_t from = red + (token >> 4) * kWaves * 1024 + (token & 15) * 64 + r * 4;
       const uint32_t mask = lds_word(chosen_at + u * 16 + 8);
       if (mask >> token & 1) {
         const int row = int(lds_word(chosen_at + u * 16 + 4)) + __popc(mask & ((1u << token) - 1));
@@ -609,7 +623,7 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
     next(to);
   };
   const auto hbuf = buffer(p.h, uint32_t(p.tokens) * p.top * p.inter * 4);
-  auto load_x = [&](u32x4 (&x)[F::kUnits]) __attribute__((always_inline)) {  // returns the mask of the stage's tokens
+  auto load_x = [&](u32x4 (&x)[1][F::kUnits]) __attribute__((always_inline)) {  // returns the mask of the stage's tokens
     const i32x4 chosen = entry(x_at.u);
     const uint32_t mask = x_at.n < total ? uint32_t(chosen[2]) : 0u;
     const int k0 = x_at.s * F::kStage + q * (F::kStage / 4);
@@ -620,12 +634,12 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
     const uint32_t from = mask >> token & 1 ? row * 2 : kPast;
 #pragma unroll
     for (int n = 0; n < F::kUnits; ++n)
-      x[n] = __builtin_amdgcn_raw_buffer_load_b128(hbuf, whole || k0 + 8 * n < p.inter ? from + 16 * n : kPast, 0, 0);
+      x[0][n] = __builtin_amdgcn_raw_buffer_load_b128(hbuf, whole || k0 + 8 * n < p.inter ? from + 16 * n : kPast, 0, 0);
     next(x_at);
     return mask;
   };
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  auto step = [&](const u32x4 (&x)[F::kUnits], uint32_t mask, u32x4 (&ahead)[F::kUnits]) __attribute__((always_inline)) {
+  f32x4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
+  auto step = [&](const u32x4 (&x)[1][F::kUnits], uint32_t mask, u32x4 (&ahead)[1][F::kUnits]) __attribute__((always_inline)) {
     // Behind the copies of this stage went those of kDownRing - 2 more, and as many stages of x.
     wait_vm<(kDownRing - 2) * (F::kCopies + F::kUnits)>();
     const uint32_t mask_ahead = load_x(ahead);
@@ -636,12 +650,12 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
       const int64_t block = int64_t(entry(at.u)[0]) * fp8::blocks_of(p.hidden) + column / fp8::kBlock;
       scale = sload(p.down_s8 + block * blocks, at.s);
     }
-    contract<kType, true>(ring_at + out * F::kSlot, x, scale, mask, acc);
+    contract<kType, 1, true>(ring_at + out * F::kSlot, x, scale, mask, acc);
     out = out + 1 == kDownRing ? 0 : out + 1;
     next(at);
     return mask_ahead;
   };
-  u32x4 x0[F::kUnits], x1[F::kUnits];
+  u32x4 x0[1][F::kUnits], x1[1][F::kUnits];
   if (wave < total) {
     // (x behind all copies but the last, as in every step: what the compiler waits for before x is the same then.)
     for (int n = 0; n < kDownRing - 2; ++n) copy_next();
@@ -656,7 +670,7 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
       mask = step(x1, mask, x0);
     }
   }
-  lds_write16(red_at + wave * 1024 + c * 64 + q * 16, acc);
+  lds_write16(red_at + wave * 1024 + c * 64 + q * 16, acc[0]);
   wait_vm<0>();
   lds_barrier();
   if (threadIdx.x < 16 * kMostTokens) {
@@ -680,21 +694,28 @@ int launch(K kernel, unsigned grid, unsigned threads, unsigned lds, const MlpPar
   return kOk;
 }
 
-template <int kType, int kStages>
+template <int kType, int kT, int kStages>
 int launch_gate_up(const MlpParams& p, hipStream_t stream) {
-  using G = GateUp<kType, kStages>;
-  return launch(gate_up_kernel<kType, kStages>, G::kTwo ? 512 : 256, kThreads, G::kLds, p, stream);
+  using G = GateUp<kType, kT, kStages>;
+  return launch(gate_up_kernel<kType, kT, kStages>, G::kTwo ? 512 : 256, kThreads, G::kLds, p, stream);
 }
 
 // Registers of x: 32, 64 or (one workgroup a CU) all of 128.
-template <int kType>
+template <int kType, int kT>
 int launch_gate_up(const MlpParams& p, hipStream_t stream) {
   const int per_wave = int(((Format<kType>::row_bytes(p.hidden) + 127) / 128 + kWaves - 1) / kWaves);
-  constexpr int kAll = 32 / Format<kType>::kUnits;
+  constexpr int kAll = 32 / (kT * Format<kType>::kUnits);
   if constexpr (kAll >= 8)
-    if (per_wave <= kAll / 4) return launch_gate_up<kType, kAll / 4>(p, stream);
-  if (per_wave <= kAll / 2) return launch_gate_up<kType, kAll / 2>(p, stream);
-  return launch_gate_up<kType, kAll>(p, stream);
+    if (per_wave <= kAll / 4) return launch_gate_up<kType, kT, kAll / 4>(p, stream);
+  if (per_wave <= kAll / 2) return launch_gate_up<kType, kT, kAll / 2>(p, stream);
+  return launch_gate_up<kType, kT, kAll>(p, stream);
+}
+
+template <int kType>
+int launch_gate_up(const MlpParams& p, hipStream_t stream) {
+  if constexpr (kType != kMxfp4)
+    if (p.tokens > 16) return launch_gate_up<kType, 2>(p, stream);
+  return launch_gate_up<kType, 1>(p, stream);
 }
 
 template <int kType>
@@ -712,10 +733,11 @@ int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
 
 // What the first kernel takes, and (up to kMostTokens) the second.
 bool first_fits(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
-  if (tokens > kMostFirst || experts > kMostExperts || top > kMostTop) return false;
+  if (tokens > kMostFirst || experts > kMostExperts || top > kMostTop || tokens * top > kMostChoices) return false;
+  if (tokens > 16 && (type == LF_EXPERT_MXFP4 || (type == LF_EXPERT_FP8 && hidden <= 2048))) return false;
   if (type == LF_EXPERT_MXFP4 && (hidden % 128 || inter % 128)) return false;
   // x of a wave's stages in 128 registers; an expert's weights within 31 bits.
-  return hidden <= 8192 && inter <= (int64_t(1) << 20) && (hidden + 16) * (inter + 16) * 2 < (int64_t(1) << 31);
+  return hidden <= (tokens <= 16 ? 8192 : 4096) && inter <= (int64_t(1) << 20) && (hidden + 16) * (inter + 16) * 2 < (int64_t(1) << 31);
 }
 
 bool fused_fits(int64_t tokens, int32_t experts, int32_t top, int64_t hidden, int64_t inter, int32_t type) {
