@@ -62,6 +62,7 @@ constexpr int kFewTokens = 2;        // routed by ranks
 constexpr int kMostExperts = 256;
 constexpr int kMostTop = 16;
 constexpr int kMostChoices = 256;
+constexpr int kTable = kMostTokens * kMostTop;  // chosen experts of two launches
 constexpr int kSlotWeights = 16 * 128;
 constexpr uint32_t kPast = 0x80000000u;  // past the end of every buffer here
 
@@ -610,7 +611,7 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
     if (a.s >= per) a.s -= per, ++a.u;
   };
   // (Past the last one whatever is there: copies and rows of x are zeros then. So no entry waits for their number.)
-  auto entry = [&](int u) { return sload(reinterpret_cast<const i32x4*>(p.table), 1 + min(u, kMostChoices - 1)); };
+  auto entry = [&](int u) { return sload(reinterpret_cast<const i32x4*>(p.table), 1 + min(u, kTable - 1)); };
   At to{wave, wave / per, wave % per}, x_at = to, at = to;
   int in = 0, out = 0;
   auto copy_next = [&]() __attribute__((always_inline)) {
@@ -871,7 +872,7 @@ extern "C" int64_t lf_expert_mlp_workspace_size(int64_t tokens, int32_t experts,
   const int64_t unit = type == LF_EXPERT_BF16 ? 8 : type == LF_EXPERT_FP8 ? 16 : 32;
   if (hidden < 1 || inter < 1 || hidden % unit || inter % unit || (type == LF_EXPERT_FP8 && inter % lf::fp8::kBlock)) return -1;
   if (hidden >= (int64_t(1) << 24) || inter >= (int64_t(1) << 24)) return -1;
-  if (fused_fits(tokens, experts, top, hidden, inter, type)) return padded16(tokens * top * inter * 4) + 16 * (1 + kMostChoices);
+  if (fused_fits(tokens, experts, top, hidden, inter, type)) return padded16(tokens * top * inter * 4) + 16 * (1 + kTable);
   if (tokens > kMostEach * int64_t(experts) / top) return -1;
   return ChainSpace(tokens, experts, top, hidden, inter).bytes;
 }
