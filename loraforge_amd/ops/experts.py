@@ -185,7 +185,7 @@ def expert_mlp(x, logits, gate_up, down, top_k: int, *, renormalize: bool = True
     each 128 x 128 block); ``base`` bf16 ``[T, H]`` (a shared expert's output or the residual).
     ``out`` may be ``base``. A token that may choose no expert is left with ``base`` (or zeros).
     fp32 sums, rounded once to bf16; what lies between the products is held in 16 bits of mantissa where an expert
-    has 32 choices or fewer on average, in bf16 above.
+    has 32 choices or fewer on average and both weights are of one type, else in bf16, as ``expert_linear`` gives it.
     """
     import torch
 
