@@ -680,7 +680,7 @@ __global__ __launch_bounds__(64 * kW, 2) void down_kernel(MlpParams p) {
     const uint32_t high = red_at + threadIdx.x * 4, low = high + 16 * kMostTokens * 4;
     float sum = lds_sum8(high), rest = lds_sum8(low);
     if constexpr (kW == 16) sum += lds_sum8(high + 8 * 1024), rest += lds_sum8(low + 8 * 1024);
-    sum += rest;
+    sum = join_pair(sum, rest);
     if (p.base) sum += bf16_to_f32(p.base[token * p.base_stride + n]);
     p.y[token * p.y_stride + n] = uint16_t(f32_to_bf16(sum));
   }

@@ -123,6 +123,12 @@ __device__ __forceinline__ void split_pair(float v, uint16_t& high, uint16_t& lo
   low = (high & 0x7f80u) == 0x7f80u ? uint16_t(0) : uint16_t(f32_to_bf16(rest));
 }
 
+// A product of a pair from those of its halves. Where the high half's is not finite it stands for both: beside an infinite
+// weight the low half's is NaN or of either sign.
+__device__ __forceinline__ float join_pair(float high, float low) {
+  return __builtin_fabsf(high) < __builtin_huge_valf() ? high + low : high;
+}
+
 // `part`: rows per workgroup (16, 32 or 64); `groups`: 16-row groups of weight rows (1 or 2).
 int launch_stream(const Params& p, int part, int groups, hipStream_t stream);
 int launch_rows(const Params& p, hipStream_t stream);

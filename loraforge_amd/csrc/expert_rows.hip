@@ -255,7 +255,7 @@ struct Rows {
     barrier_only();
     if (p.pair == kJoin) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] += __shfl_xor(out[e], 1, 64);
+      for (int e = 0; e < 4; ++e) out[e] = join_pair(out[e], __shfl_xor(out[e], 1, 64));  // (stored by the lane of the high half)
       if (c >= count || (c & 1)) return;
       float* y = reinterpret_cast<float*>(p.y) + int64_t((first + c) >> 1) * p.y_stride + column;
       if (p.y_vec && column + 4 <= p.width) {

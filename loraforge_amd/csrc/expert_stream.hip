@@ -199,7 +199,7 @@ __device__ __forceinline__ void stream_rows(const Params& p, const Segment& seg,
     const int n = block * columns + r;
     if (first + row >= seg.end || n >= p.width) continue;
     if (p.pair == kJoin) {  // (a pair's rows are in one pass)
-      if (!(row & 1)) reinterpret_cast<float*>(p.y)[int64_t((first + row) >> 1) * p.y_stride + n] = total(r, row) + total(r, row + 1);
+      if (!(row & 1)) reinterpret_cast<float*>(p.y)[int64_t((first + row) >> 1) * p.y_stride + n] = join_pair(total(r, row), total(r, row + 1));
       continue;
     }
     const float v = p.swiglu ? silu_mul_f32(total(r, row), total(r + 8 * kF, row)) : total(r, row);

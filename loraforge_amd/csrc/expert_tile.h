@@ -182,14 +182,16 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
         if (p.pair == kJoin) {  // (a pair's rows are in one tile, one behind the other)
           float low[8];
           values(r + 1, low);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = join_pair(v[e], low[e]);
           float* y = reinterpret_cast<float*>(p.y) + (row >> 1) * p.y_stride + col;
           if (vec) {
-            reinterpret_cast<f32x4*>(y)[0] = f32x4{v[0] + low[0], v[1] + low[1], v[2] + low[2], v[3] + low[3]};
-            reinterpret_cast<f32x4*>(y)[1] = f32x4{v[4] + low[4], v[5] + low[5], v[6] + low[6], v[7] + low[7]};
+            reinterpret_cast<f32x4*>(y)[0] = f32x4{v[0], v[1], v[2], v[3]};
+            reinterpret_cast<f32x4*>(y)[1] = f32x4{v[4], v[5], v[6], v[7]};
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (col + e < p.width) y[e] = v[e] + low[e];
+              if (col + e < p.width) y[e] = v[e];
           }
           continue;
         }

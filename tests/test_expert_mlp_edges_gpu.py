@@ -1,0 +1,91 @@
+"""Edges of the whole expert MLP (``expert_mlp``): weights that are not finite, and what the layout of its inputs may not change.
+
+Infinite values follow the formula: a product of an infinite weight and a value that is not
+zero is infinite with their sign, so a sum that holds one is, and every other output keeps its bits.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from loraforge_amd.ops import expert_mlp
+from oracle import experts as ox
+from oracle import fp8 as of
+from tests.test_expert_mlp_gpu import case, values
+
+pytestmark = pytest.mark.gpu
+
+# Two launches (16 and 8 waves in the second), the first one ahead of the operators, the operators alone; of
+# the down product the weight stream, a wave for 16 weight rows and row tiles.
+FORMS = [(1, 8, 8, 512, 256), (3, 8, 2, 512, 256), (8, 8, 2, 2688, 128), (9, 24, 4, 512, 256), (30, 8, 2, 2176, 256), (40, 8, 2, 512, 256),
+         (64, 24, 4, 1024, 1024), (128, 24, 4, 640, 512)]
+
+
+def activations(x, gate_up, expert):
+    """silu(gate) up of every token for one expert, in 64 bits."""
+    gu = values(gate_up if isinstance(gate_up, torch.Tensor) else type(gate_up)(gate_up.codes[expert : expert + 1], gate_up.scales[expert : expert + 1]))
+    return ox.product(x.double().cpu().numpy(), gu[expert if isinstance(gate_up, torch.Tensor) else 0], None, True)[0]
+
+
+def chosen_case(kind, tokens, experts, *sizes, device):
+    """``case`` with expert 1 among the first token's choices."""
+    x, logits, gate_up, down = case(kind, tokens, experts, *sizes, device, seed=tokens)
+    logits[0, 1] = 9.0
+    return x, logits, gate_up, down
+
+
+def hit_by(logits, top, expert):
+    _, chosen, *_ = ox.route(logits.double().cpu().numpy(), top)
+    return torch.from_numpy((chosen == expert).any(1))
+
+
+@pytest.mark.parametrize("tokens,experts,top,hidden,inter", FORMS)
+def test_infinite_down_weights(tokens, experts, top, hidden, inter, device):
+    x, logits, gate_up, down = chosen_case("bf16", tokens, experts, hidden, inter, device=device)
+    clean = expert_mlp(x, logits, gate_up, down, top)
+    down[1, 3, 5], down[1, 140, inter - 1] = float("inf"), float("-inf")
+    y = expert_mlp(x, logits, gate_up, down, top).cpu()
+    h, hit = activations(x, gate_up, 1), hit_by(logits, top, 1)
+    want = clean.cpu().clone()
+    want[:, 3] = torch.where(hit, torch.from_numpy(h[:, 5] * np.inf).bfloat16(), want[:, 3])
+    want[:, 140] = torch.where(hit, torch.from_numpy(h[:, inter - 1] * -np.inf).bfloat16(), want[:, 140])
+    assert (np.abs(h[:, [5, inter - 1]]) > 1e-5).all()  # (a sign that fp32 sums do not change)
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("tokens,experts,top,hidden,inter", FORMS)
+def test_infinite_scale_of_a_down_block(tokens, experts, top, hidden, inter, device):
+    """A block's products are summed, then scaled: infinite with the sum's sign."""
+    x, logits, gate_up, down = chosen_case("fp8", tokens, experts, hidden, inter, device=device)
+    clean = expert_mlp(x, logits, gate_up, down, top).cpu()
+    down.scales[1, 1, 0] = float("inf")
+    y = expert_mlp(x, logits, gate_up, down, top).cpu()
+    h, hit = activations(x, gate_up, 1), hit_by(logits, top, 1)
+    codes = of.values(down.codes[1].view(torch.uint8).cpu().numpy(), np.ones(down.scales.shape[1:], np.float32))
+    part = codes[128:256, :128]
+    sums, size = h[:, :128] @ part.T, np.abs(h[:, :128]) @ np.abs(part).T
+    clear = torch.from_numpy(np.abs(sums) > 2.0**-12 * size) & hit[:, None]
+    assert clear.sum() >= 0.9 * 128 * hit.sum()
+    want = clean.clone()
+    want[:, 128:256] = torch.where(hit[:, None], torch.from_numpy(sums * np.inf).bfloat16(), want[:, 128:256])
+    got = y.clone()
+    got[:, 128:256] = torch.where(hit[:, None] & ~clear, want[:, 128:256], got[:, 128:256])
+    assert torch.equal(got, want)
+    assert not torch.isfinite(y[hit][:, 128:256]).any()
+
+
+@pytest.mark.parametrize("tokens,experts,top,hidden,inter", FORMS)
+def test_infinite_gate_and_up_weights(tokens, experts, top, hidden, inter, device):
+    """silu(gate) times an infinite up is infinite, so are all outputs of its token with the signs of the down weights."""
+    x, logits, gate_up, down = chosen_case("bf16", tokens, experts, hidden, inter, device=device)
+    clean = expert_mlp(x, logits, gate_up, down, top)
+    h, hit = activations(x, gate_up, 1), hit_by(logits, top, 1)
+    gate_up[1, inter + 7, 11] = float("inf")
+    y = expert_mlp(x, logits, gate_up, down, top).cpu()
+    gate = x.double().cpu().numpy() @ gate_up[1, 7].double().cpu().numpy()
+    sign = np.sign(gate) * np.sign(x[:, 11].double().cpu().numpy())
+    want = clean.cpu().clone()
+    with np.errstate(invalid="ignore"):  # (infinity times a weight of zero)
+        want[hit] = torch.from_numpy((sign[:, None] * np.inf) * down[1, :, 7].double().cpu().numpy()[None])[hit].bfloat16()
+    assert (np.abs(gate) > 1e-4).all() and (sign != 0).all()
+    assert torch.equal(y[~hit], want[~hit]) and np.array_equal(y.float().numpy(), want.float().numpy(), equal_nan=True)
