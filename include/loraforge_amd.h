@@ -428,8 +428,8 @@ int lf_combine_experts(const uint16_t* rows, int64_t num_rows, int64_t rows_stri
  * 2 inter, hidden] (gate rows, then up rows), down [experts, hidden, inter], both of `type`, with the scales of
  * lf_expert_linear (MXFP4 bytes, 4-byte aligned; FP8 floats); base bf16 [tokens, hidden] or NULL (y may be base). Sums in
  * fp32; silu(gate) * up is held in 16 bits of mantissa (a pair of bf16), y rounded once.
- * Up to 8 tokens, 256 experts, top 16 and hidden 8192 (widths multiples of 128 for MXFP4) run in two launches (x rows within
- * 2 GiB), up to 32 in three (MXFP4 16; 256 choices, hidden 4096 from 17 on and with FP8 weights above 2048), else four.
+ * Up to 8 tokens, 256 experts, top 16 and hidden 8192 (widths multiples of 128 for MXFP4) run in two launches (x rows have to lie
+ * within 2 GiB, or are refused), up to 32 in three (MXFP4 16; 256 choices, hidden 4096 from 17 on and with FP8 weights above 2048), else four.
  * lf_expert_mlp_workspace_size: bytes (16-byte aligned, need not be cleared, not shared by calls that overlap), or -1 for
  * sizes that it does not take: more than 32 choices for each expert on average (tokens * top against experts; there the
  * products are bound by their matrix instructions, and lf_route_experts, lf_expert_linear and lf_combine_experts hold what lies between them in

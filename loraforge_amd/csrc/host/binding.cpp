@@ -1039,12 +1039,17 @@ PyObject* mlp(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (need < 0) return decline();
   void* stream;
   if (!current(dev, &stream)) return decline();
+  at::Tensor rows = *x;  // (the two launches, of up to 8 tokens, take offsets of 31 bits)
+  if (count > 1 && count <= 8 && a.x_stride >= ((int64_t(1) << 30) - hidden) / (count - 1)) {
+    rows = x->contiguous();
+    a.x_stride = hidden;
+  }
   Output out(args[7], count, hidden, dev);
   const bool onto = base && out.given && ptr<uint16_t>(out.given) == ptr<uint16_t>(base) && out.stride == a.base_stride;
   if (!out.ok({x, logits, gate_up.w, gate_up.scales, down.w, down.scales, onto ? nullptr : base})) return decline();
   const at::Tensor scratch = at::empty({need}, x->options().dtype(at::kByte));
   if (!on_gpu(scratch)) return decline();
-  a.x = x->data_ptr();
+  a.x = rows.data_ptr();
   a.logits = logits->data_ptr();
   a.logits_stride = stride(*logits, experts);
   a.fp32 = logits->scalar_type() == at::kFloat;

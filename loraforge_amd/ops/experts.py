@@ -185,7 +185,9 @@ def expert_mlp(x, logits, gate_up, down, top_k: int, *, renormalize: bool = True
     each 128 x 128 block); ``base`` bf16 ``[T, H]`` (a shared expert's output or the residual).
     ``out`` may be ``base``. A token that may choose no expert is left with ``base`` (or zeros).
     fp32 sums, rounded once to bf16; what lies between the products is held in 16 bits of mantissa where an expert
-    has 32 choices or fewer on average and both weights are of one type, else in bf16, as ``expert_linear`` gives it.
+    has 32 choices or fewer on average and both weights are of one type, else in bf16, as ``expert_linear`` gives it
+    (so also where the address of MXFP4 scales is no multiple of 4). Rows of ``x`` of up to 8 tokens that span 2 GiB are
+    gathered first.
     """
     import torch
 
@@ -261,8 +263,8 @@ def _expert_mlp(x, logits, gate_up, down, top_k, renormalize, base, out) -> bool
     parts = _parts(gate_up), _parts(down)
     if size < 0 or any(t.data_ptr() % 4 for part in parts for t in part[1:]):
         return False
-    if 1 < count <= 8 and x.stride(0) >= (2**30 - hidden) // (count - 1):  # (32-bit offsets)
-        return False
+    if 1 < count <= 8 and x.stride(0) >= (2**30 - hidden) // (count - 1):
+        x = x.contiguous()  # (the two launches take offsets of 31 bits)
     a = _lib.ExpertMlp()
     a.x, a.logits, a.y = x.data_ptr(), logits.data_ptr(), out.data_ptr()
     a.x_stride, a.logits_stride, a.y_stride = (t.stride(0) if count > 1 else t.shape[1] for t in (x, logits, out))

@@ -11,7 +11,8 @@ import torch
 from loraforge_amd.ops import expert_mlp
 from oracle import experts as ox
 from oracle import fp8 as of
-from tests.test_expert_mlp_gpu import case, values
+from tests.test_expert_mlp_gpu import KINDS, case, values
+from tests.test_native_calls_gpu import both
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +90,17 @@ def test_infinite_gate_and_up_weights(tokens, experts, top, hidden, inter, devic
         want[hit] = torch.from_numpy((sign[:, None] * np.inf) * down[1, :, 7].double().cpu().numpy()[None])[hit].bfloat16()
     assert (np.abs(gate) > 1e-4).all() and (sign != 0).all()
     assert torch.equal(y[~hit], want[~hit]) and np.array_equal(y.float().numpy(), want.float().numpy(), equal_nan=True)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens,experts", [(2, 8), (3, 8), (8, 8), (8, 300), (9, 8)])
+def test_rows_of_x_that_span_2_gib(kind, tokens, experts, device, monkeypatch):
+    """Bit for bit the result of the same rows beside each other, on the native path and in Python."""
+    x, logits, gate_up, down = case(kind, tokens, experts, 256, 128, device)
+    base = x.flip(0)
+    want = expert_mlp(x, logits, gate_up, down, 2, base=base)
+    span = 2**30 // (tokens - 1) // 8 * 8 + 64
+    far = torch.empty((tokens - 1) * span + 256, dtype=torch.bfloat16, device=device).as_strided((tokens, 256), (span, 1))
+    far.copy_(x)
+    taken, python = both(monkeypatch, lambda: expert_mlp(far, logits, gate_up, down, 2, base=base))
+    assert torch.equal(taken, want) and torch.equal(python, want)
