@@ -266,8 +266,10 @@ __device__ __forceinline__ void load_row(const float* src, float (&v)[kVec]) {
   }
 }
 
-// Eight columns per thread (16-byte accesses), or one.
-template <class Row, int kVec>
+// Eight columns per thread (16-byte accesses), or one. Rows are asked for kTogether at a time (one behind the other,
+// their latency was most of a few tokens' time): one and two where a token has no more, since each that it lacks costs
+// loads and additions all the same (8191 tokens of 4096 columns: one row 21 us, asked for as four 28).
+template <class Row, int kVec, int kTogether>
 __global__ __launch_bounds__(kCombineThreads) void combine_kernel(CombineParams p) {
   const int64_t chunks = p.n / kVec, total = p.tokens * chunks;
   for (int64_t i = int64_t(blockIdx.x) * kCombineThreads + threadIdx.x; i < total; i += int64_t(gridDim.x) * kCombineThreads) {
@@ -275,8 +277,6 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(CombineParams 
     float sum[kVec];
 #pragma unroll
     for (int k = 0; k < kVec; ++k) sum[k] = 0.0f;
-    // (Rows are asked for four at a time: one behind the other, their latency was most of a few tokens' time.)
-    constexpr int kTogether = 4;
     if (p.base) {
       float v[kVec];
       load_row<kVec>(p.base + t * p.base_stride + c, v);
@@ -320,10 +320,13 @@ int launch_combine(const Row* rows, int64_t num_rows, int64_t rows_stride, const
   const CombineParams p{rows, rows_stride, num_rows, positions, weights, base, base_stride, y, y_stride, tokens, top, n};
   const int64_t want = (tokens * (vec ? n / 8 : n) + kCombineThreads - 1) / kCombineThreads;
   const dim3 grid(unsigned(want < 65536 ? want : 65536)), threads(kCombineThreads);
+  auto run = [&](void (*one)(CombineParams), void (*two)(CombineParams), void (*more)(CombineParams)) {
+    hipLaunchKernelGGL(top == 1 ? one : top == 2 ? two : more, grid, threads, 0, s, p);
+  };
   if (vec)
-    hipLaunchKernelGGL((combine_kernel<Row, 8>), grid, threads, 0, s, p);
+    run(combine_kernel<Row, 8, 1>, combine_kernel<Row, 8, 2>, combine_kernel<Row, 8, 4>);
   else
-    hipLaunchKernelGGL((combine_kernel<Row, 1>), grid, threads, 0, s, p);
+    run(combine_kernel<Row, 1, 1>, combine_kernel<Row, 1, 2>, combine_kernel<Row, 1, 4>);
   LF_HIP(hipGetLastError());
   return kOk;
 }
