@@ -18,8 +18,8 @@ namespace expert {
 // result keeps them into the next one. Row r of such an x is rows 2 r and 2 r + 1, two rows of the product.
 enum Pair : int {
   kSingle,  // y bf16
-  kSplit,   // y: bf16 pairs, rows 2 r and 2 r + 1 of y
-  kJoin,    // x: pairs (`rows` and `x_rows` count both), y: fp32, one row for each pair
+  kSplit,   // y: bf16 pairs, rows 2 r and 2 r + 1 of y (of a product with SwiGLU)
+  kJoin,    // x: pairs (`rows` and `x_rows` count both), y: fp32, one row for each pair (without)
 };
 
 // Types of an operand.

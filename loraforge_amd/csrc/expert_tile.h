@@ -92,8 +92,11 @@ __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 // row c of fragment row i and weight row 8 g + 4 h + e of fragment j, and in LDS a
 // row's columns follow each other, so that eight lanes or more store whole cache
 // lines and the code is short (an unrolled epilogue straight from the
-// registers took longer to fetch than to run).
-template <int kI, int kJ, bool kSwiglu>
+// registers took longer to fetch than to run). For the same reason kPair (a Pair, or kAnyPair: as p.pair says) is a
+// parameter: with the stores of its three forms beside each other 1024 rows of 11008 x 4096, MXFP4 both, took 41 us, and
+// 33 without (rows of the last columns' tiles are stored a value at a time, and these tiles end last).
+constexpr int kAnyPair = -1;
+template <int kI, int kJ, bool kSwiglu, int kPair>
 __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][kJ], char* lds, int expert, int first, int count,
                                        int nt) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -121,7 +124,8 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
     }
   }
   const bool vec = p.y_vec && col + 8 <= p.width;
-  const bool all_vec = p.pair == kSingle && __ballot(!vec) == 0;
+  const int pair = kPair == kAnyPair ? p.pair : kPair;
+  const bool all_vec = pair == kSingle && __ballot(!vec) == 0;
   // Eight output columns of staged row r.
   auto values = [&](int r, float (&out)[8]) {
     const f32x4* v = reinterpret_cast<const f32x4*>(mine + r * kRowBytes + local * 4);
@@ -145,20 +149,20 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
     return u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
   };
 #pragma unroll
-  for (int pair = 0; pair < (kI + 1) / 2; ++pair) {
+  for (int two = 0; two < (kI + 1) / 2; ++two) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < kJ; ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          if (2 * pair + i < kI) {
-            const f32x16& a = acc[2 * pair + i][j];
+          if (2 * two + i < kI) {
+            const f32x16& a = acc[2 * two + i][j];
             *reinterpret_cast<f32x4*>(mine + (32 * i + c) * kRowBytes + (32 * j + 8 * g + 4 * h) * 4) =
                 f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
           }
-    const int staged = min(2, kI - 2 * pair) * 32;
-    auto place = [&](int r) { return (2 * pair + (r >> 5)) * 64 + 32 * wm + (r & 31); };
+    const int staged = min(2, kI - 2 * two) * 32;
+    auto place = [&](int r) { return (2 * two + (r >> 5)) * 64 + 32 * wm + (r & 31); };
     if (all_vec) {
       constexpr int kTogether = 32 / kRows < 4 ? 32 / kRows : 4;  // rows whose reads go out together
 #pragma unroll 1
@@ -175,11 +179,20 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
     } else {
 #pragma unroll 1
       for (int r = in_row; r < staged; r += kRows) {
+        if (pair == kSingle) {
+          const u32x4 o = output(r);
+          uint16_t* y = p.y + int64_t(first + place(r)) * p.y_stride + col;
+          if (place(r) >= count || idle) continue;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e < p.width) y[e] = uint16_t(o[e >> 1] >> (16 * (e & 1)));
+          continue;
+        }
         const int64_t row = first + place(r);
-        if (place(r) >= count || idle || (p.pair == kJoin && (r & 1))) continue;
+        if (place(r) >= count || idle || (pair == kJoin && (r & 1))) continue;
         float v[8];
         values(r, v);
-        if (p.pair == kJoin) {  // (a pair's rows are in one tile, one behind the other)
+        if (pair == kJoin) {  // (a pair's rows are in one tile, one behind the other)
           float low[8];
           values(r + 1, low);
 #pragma unroll
@@ -198,8 +211,8 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
         uint16_t high[8], low[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) split_pair(v[e], high[e], low[e]);
-        uint16_t* y = p.y + (p.pair == kSplit ? 2 * row : row) * p.y_stride + col;
-        if (vec && p.pair == kSplit) {
+        uint16_t* y = p.y + 2 * row * p.y_stride + col;
+        if (vec) {
           *reinterpret_cast<u32x4*>(y) = __builtin_bit_cast(u32x4, high);
           *reinterpret_cast<u32x4*>(y + p.y_stride) = __builtin_bit_cast(u32x4, low);
         } else {
@@ -207,7 +220,7 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
           for (int e = 0; e < 8; ++e)
             if (col + e < p.width) {
               y[e] = high[e];
-              if (p.pair == kSplit) y[p.y_stride + e] = low[e];
+              y[p.y_stride + e] = low[e];
             }
         }
       }
@@ -215,7 +228,7 @@ __device__ __forceinline__ void finish(const Params& p, const f32x16 (&acc)[kI][
   }
 }
 
-template <bool kXMx, bool kWMx, int kI, int kJ>
+template <bool kXMx, bool kWMx, int kI, int kJ, int kPair>
 struct Body {
   using S = Shape<kXMx, kWMx, kI, kJ>;
   const Params& p;
@@ -613,10 +626,10 @@ struct Body {
     // waves read their last operands.
     wait_vm<0>();
     lds_barrier();
-    if (p.swiglu)
-      finish<kI, kJ, true>(p, acc, lds, seg.expert, first, count, nt);
+    if (kPair == kSplit || (kPair == kSingle && p.swiglu))
+      finish<kI, kJ, true, kPair>(p, acc, lds, seg.expert, first, count, nt);
     else
-      finish<kI, kJ, false>(p, acc, lds, seg.expert, first, count, nt);
+      finish<kI, kJ, false, kPair>(p, acc, lds, seg.expert, first, count, nt);
   }
 };
 
@@ -706,16 +719,16 @@ __device__ __forceinline__ Place locate(const Params& p, int cap, int column_til
   return {seg, first, min(64 * (each + (mt < more)), seg.end - first), nt};
 }
 
-template <bool kXMx, bool kWMx, int kJ>
+template <bool kXMx, bool kWMx, int kJ, int kPair>
 __global__ __launch_bounds__(kThreads, 1) void tile_kernel(Params p, int cap, int column_tiles) {
   extern __shared__ char lds[];
   const auto [seg, first, count, nt] = locate(p, cap, column_tiles);
   if (count <= 0) return;
   switch ((count + 63) / 64) {
-    case 1: Body<kXMx, kWMx, 1, kJ>(p).run(lds, seg, first, count, nt); break;
-    case 2: Body<kXMx, kWMx, 2, kJ>(p).run(lds, seg, first, count, nt); break;
-    case 3: Body<kXMx, kWMx, 3, kJ>(p).run(lds, seg, first, count, nt); break;
-    default: Body<kXMx, kWMx, 4, kJ>(p).run(lds, seg, first, count, nt); break;
+    case 1: Body<kXMx, kWMx, 1, kJ, kPair>(p).run(lds, seg, first, count, nt); break;
+    case 2: Body<kXMx, kWMx, 2, kJ, kPair>(p).run(lds, seg, first, count, nt); break;
+    case 3: Body<kXMx, kWMx, 3, kJ, kPair>(p).run(lds, seg, first, count, nt); break;
+    default: Body<kXMx, kWMx, 4, kJ, kPair>(p).run(lds, seg, first, count, nt); break;
   }
 }
 
@@ -735,7 +748,11 @@ int launch_kernel(void (*kernel)(Params, int, int), const Params& p, int cap, hi
 }
 template <bool kXMx, bool kWMx, int kJ>
 int launch(const Params& p, int cap, hipStream_t stream) {
-  return launch_kernel<kJ>(tile_kernel<kXMx, kWMx, kJ>, p, cap, stream);
+  if constexpr (!kXMx) {
+    if (p.pair == kSplit) return launch_kernel<kJ>(tile_kernel<kXMx, kWMx, kJ, kSplit>, p, cap, stream);
+    if (p.pair == kJoin) return launch_kernel<kJ>(tile_kernel<kXMx, kWMx, kJ, kJoin>, p, cap, stream);
+  }
+  return launch_kernel<kJ>(tile_kernel<kXMx, kWMx, kJ, kSingle>, p, cap, stream);
 }
 
 }  // namespace tile

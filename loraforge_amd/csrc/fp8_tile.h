@@ -101,6 +101,8 @@ struct Body {
   // block of 128 each (all widths but 192), else of a fragment's. x rows' scales, in scale[i][0] until they are
   // multiplied with the weights'.
   static constexpr bool kOneBlock = kJ != 3;
+  // (One kernel for all of bf16 x: the compiler finds no registers for 192 rows x 128 weight rows that store pairs alone.)
+  static constexpr int kPair = kX8 ? kSingle : tile::kAnyPair;
   float sw[2][2], scale[kI][2];
   f32x16 t[2];
   float due[2];  // scales of the pair whose products wait in T
@@ -386,9 +388,9 @@ struct Body {
     wait_vm<0>();
     lds_barrier();
     if (p.swiglu)
-      tile::finish<kI, kJ, true>(p, acc, lds, seg.expert, first, count, nt);
+      tile::finish<kI, kJ, true, kPair>(p, acc, lds, seg.expert, first, count, nt);
     else
-      tile::finish<kI, kJ, false>(p, acc, lds, seg.expert, first, count, nt);
+      tile::finish<kI, kJ, false, kPair>(p, acc, lds, seg.expert, first, count, nt);
   }
 };
 
