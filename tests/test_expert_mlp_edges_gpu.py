@@ -1,4 +1,5 @@
-"""Edges of the whole expert MLP (``expert_mlp``): weights that are not finite, and what the layout of its inputs may not change.
+"""Edges of the whole expert MLP (``expert_mlp``): weights that are not finite, what the layout of its inputs may not change, and
+the sizes at which each variant of its kernels runs.
 
 Infinite values follow the formula: a product of an infinite weight and a value that is not
 zero is infinite with their sign, so a sum that holds one is, and every other output keeps its bits.
@@ -11,7 +12,7 @@ import torch
 from loraforge_amd.ops import expert_mlp
 from oracle import experts as ox
 from oracle import fp8 as of
-from tests.test_expert_mlp_gpu import KINDS, case, values
+from tests.test_expert_mlp_gpu import KINDS, case, close, expected, values
 from tests.test_native_calls_gpu import both
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +105,82 @@ def test_rows_of_x_that_span_2_gib(kind, tokens, experts, device, monkeypatch):
     far.copy_(x)
     taken, python = both(monkeypatch, lambda: expert_mlp(far, logits, gate_up, down, 2, base=base))
     assert torch.equal(taken, want) and torch.equal(python, want)
+
+
+# --------------------------------------------------------------------------
+# Sizes at which another variant of a kernel runs, at 16 bits between the products
+# --------------------------------------------------------------------------
+
+PAIRS = 2.0**-16 + 2.0**-20  # a pair of bf16 is off by 2^-8 of 2^-8 of the value, the fp32 activation by 2^-20
+
+
+def check(y, x, logits, gate_up, down, top, **options):
+    """Within the bound of pairs; of many outputs the deviation is that of their own rounding.
+
+    An error uniform within half a step has 2^-7 / sqrt(12) of the power of two below the value in the root
+    mean square, 0.00166 of values that are spread smoothly; rounding the intermediate to bf16 would make it 0.0024.
+    """
+    want, bound = expected(x, logits, gate_up, down, top, between=PAIRS, **options)
+    close(y, (want, bound))
+    if want.size >= 4096:
+        assert (y.double().cpu().numpy() - want).std() <= 2.0**-9 * want.std()
+
+
+def few(x, logits, tokens):
+    return x[:tokens], logits[:tokens]
+
+
+@pytest.mark.parametrize("kind,hidden", [("bf16", 4104), ("bf16", 8192), ("fp8", 4112), ("fp8", 8192), ("mxfp4", 4224), ("mxfp4", 8192)])
+def test_wide_hidden(kind, hidden, device):
+    """All registers of x: through LDS while it fits, else by loads (MXFP4, FP8: exchanged between the quarters of a wave)."""
+    x, logits, gate_up, down = case(kind, 16, 6, hidden, 128, device, seed=hidden)
+    for tokens in (1, 2, 6, 7, 8, 9, 16):
+        xs, ls = few(x, logits, tokens)
+        check(expert_mlp(xs, ls, gate_up, down, 2), xs, ls, gate_up, down, 2)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hidden", [2176, 3200, 4096])
+def test_x_past_what_lds_holds(kind, hidden, device):
+    """9 to 16 tokens whose x does not fit LDS beside two workgroups of a CU."""
+    x, logits, gate_up, down = case(kind, 16, 6, hidden, 128, device, seed=hidden)
+    for tokens in (9, 12, 16):
+        xs, ls = few(x, logits, tokens)
+        check(expert_mlp(xs, ls, gate_up, down, 2), xs, ls, gate_up, down, 2)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("experts,top", [(65, 1), (100, 8), (128, 16), (129, 16), (130, 8), (200, 1), (256, 16), (257, 3)])
+def test_many_experts(kind, experts, top, device):
+    """Routing in the first launch by ranks (1 and 2 tokens) and in rounds, of up to 128 and up to 256 experts."""
+    x, logits, gate_up, down = case(kind, 20, experts, 256, 128, device, seed=experts)
+    tied = torch.round(logits)
+    masked = logits.clone()
+    masked[torch.rand(masked.shape, generator=torch.Generator().manual_seed(top)) < 0.95] = -np.inf
+    masked[1], masked[:, experts - 1] = -np.inf, 0.5
+    masked[3] = -np.inf
+    for tokens in (1, 2, 5, 20):
+        for all_logits, renormalize in ((logits, True), (tied, False), (masked, True), (tied.bfloat16(), True)):
+            xs, ls = few(x, all_logits, tokens)
+            y = expert_mlp(xs, ls, gate_up, down, top, renormalize=renormalize)
+            check(y, xs, ls, gate_up, down, top, renormalize=renormalize)
+
+
+@pytest.mark.parametrize("kind,hidden,inter", [("bf16", 136, 72), ("bf16", 520, 264), ("bf16", 24, 8), ("bf16", 1032, 328), ("fp8", 144, 128),
+                                               ("fp8", 528, 256), ("fp8", 1040, 384), ("mxfp4", 96, 32), ("mxfp4", 544, 288), ("mxfp4", 384, 640)])
+def test_widths_with_a_remainder(kind, hidden, inter, device):
+    """Remainders of every loop and tile, with a base, of 1 to 160 tokens (routed by ranks, in rounds, in a chain; in row tiles)."""
+    x, logits, gate_up, down = case(kind, 160, 15, hidden, inter, device, seed=hidden)
+    base = x.flip(0)
+    for tokens in (1, 2, 5, 8, 16, 20, 40, 160):
+        (xs, ls), bs = few(x, logits, tokens), base[:tokens]
+        for b in (None, bs):
+            check(expert_mlp(xs, ls, gate_up, down, 3, base=b), xs, ls, gate_up, down, 3, base=b)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_pairs_in_row_tiles(kind, device):
+    """The down product of many rows: tiles of up to 256 rows, experts past the 64th among them."""
+    for tokens, experts, top, hidden, inter in ((128, 24, 4, 640, 512), (200, 70, 8, 512, 256), (256, 130, 8, 264 if kind == "bf16" else 640, 256)):
+        x, logits, gate_up, down = case(kind, tokens, experts, hidden, inter, device, seed=experts)
+        check(expert_mlp(x, logits, gate_up, down, top), x, logits, gate_up, down, top)
