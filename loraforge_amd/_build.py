@@ -52,7 +52,8 @@ NO_SCRATCH = {"expert_mlp.hip", "expert_stream.hip", "expert_rows.hip", "nf4_gem
 
 # The FP8 tiles scale a block's products by vector instructions, so their matrix instructions have to
 # leave results in registers that those reach (by default the compiler gives them the others of the
-# 512 and copies each value over: 16 more instructions a pair of fragments).
+# 512 and copies each value over: 16 more instructions a pair of fragments, and scratch in a kernel beside bf16 x). It is an
+# option of the compiler's back end, which no document promises: a compiler without it ends the build with its name.
 EXTRA_FLAGS = {f"fp8_tile_{types}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for types in ("fp8", "w8")}
 
 

@@ -15,7 +15,8 @@
 // scale is that of a whole step: a step's products are summed from zero and added
 // to the sums times x's and the weight's scale, in fp32.
 // The waves' partial sums meet in LDS, in a fixed order.
-// FP8 weights: a row of 4096 x 4096 5.8 us (16.8 MB, 2.9 TB/s: a launch, one load's latency, the join); 24 tokens over 64
+// FP8 weights: a row of 4096 x 4096 5.8 us (16.8 MB, 2.9 TB/s: a launch, two loads' latency, as a wave asks for its four
+// steps in pairs, the join); 24 tokens over 64
 // experts, top 4, 4096 x 4096 with SwiGLU 136-149 (727 MB fetched, 4.9-5.3 TB/s; a wave for 16 weight rows 158).
 #include "expert_params.h"
 

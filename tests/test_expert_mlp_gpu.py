@@ -1,9 +1,11 @@
 """The whole mixture-of-experts MLP (``expert_mlp``) against the 64-bit oracle.
 
-With a = silu(gate) up of an expert in 64 bits, the kernels hold a (or a times its routing
-weight) in bf16: off by 2^-8 of it (half a step; a second 2^-9 for a weight's or the fp32
+With a = silu(gate) up of an expert in 64 bits, a call of more than 32 choices an expert holds a in bf16: off by
+2^-8 of it (half a step; a second 2^-9 for a weight's or the fp32
 sums' share), so an output by (2^-8 + 2^-9) of the sum of magnitudes of its down terms, plus the fp32
-bound of both products, plus half a bf16 step of itself.
+bound of both products, plus half a bf16 step of itself. All others hold a (or a times its routing weight) as a pair of bf16,
+off by 2^-16: they are within that bound too, and at 2^-16 + 2^-20 in
+``test_keeps_16_bits_between_the_products`` and in ``test_expert_mlp_edges_gpu.py``.
 """
 
 import numpy as np
